@@ -5,11 +5,10 @@
 // that nothing is shared between CTAs.  16 heads of 64 x 32: 6 + 13 us, with one CTA for 64 rows of everything 7 + 17.
 // Bound by latency: eight warps an SM, a shared-memory load for every four to eight FMAs.
 #pragma once
+#include "attention_fma.cuh"
 #include "gemm.cuh"
 
 namespace gcb {
-
-constexpr int AS_OWN = 32, AS_T = 64;
 
 struct SmallAttn {
     const float *q, *k, *v, *g, *o;
@@ -18,91 +17,6 @@ struct SmallAttn {
     int T, D, H;
     float scale;
 };
-
-// ROWS rows of D columns from row r0 into [row][D + 4], asynchronously; rows beyond T are zero
-template <int ROWS>
-__device__ __forceinline__ void as_load(float* sm, const float* p, int64_t ld, int r0, int T, int D) {
-    const int d4 = D >> 2;
-    for (int i = threadIdx.x; i < ROWS * d4; i += 256) {
-        const int r = i / d4, c = (i - r * d4) * 4;
-        const bool live = r0 + r < T;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(sm + r * (D + 4) + c)), "l"(live ? p + (r0 + r) * ld + c : p), "r"(live ? 16 : 0) : "memory");
-    }
-}
-__device__ __forceinline__ void as_landed() {
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    __syncthreads();
-}
-// c[i][j] = a[ty + 16 i] . b[tx + 16 j]
-template <int R, int C>
-__device__ __forceinline__ void as_abt(float (&c)[R][C], const float* a, const float* b, int D, int ty, int tx) {
-#pragma unroll
-    for (int i = 0; i < R; ++i)
-#pragma unroll
-        for (int j = 0; j < C; ++j) c[i][j] = 0.0f;
-    const int P = D + 4;
-#pragma unroll 4
-    for (int d = 0; d < D; d += 4) {
-        float4 x[R], y[C];
-#pragma unroll
-        for (int i = 0; i < R; ++i) x[i] = ld4(a + (ty + 16 * i) * P + d);
-#pragma unroll
-        for (int j = 0; j < C; ++j) y[j] = ld4(b + (tx + 16 * j) * P + d);
-#pragma unroll
-        for (int i = 0; i < R; ++i)
-#pragma unroll
-            for (int j = 0; j < C; ++j) c[i][j] = fmaf(x[i].x, y[j].x, fmaf(x[i].y, y[j].y, fmaf(x[i].z, y[j].z, fmaf(x[i].w, y[j].w, c[i][j]))));
-    }
-}
-// acc[i][4 n + e] += sum_k p[ty + 16 i][k] b[k][64 n + 4 tx + e], k < 64
-template <int NC>
-__device__ __forceinline__ void as_ab(float (&acc)[2][4 * NC], const float* p, const float* b, int D, int ty, int tx) {
-    const int P = D + 4;
-#pragma unroll 4
-    for (int k = 0; k < AS_T; k += 4) {
-        float a[2][4];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) { const float4 x = ld4(p + (ty + 16 * i) * (AS_T + 4) + k); a[i][0] = x.x; a[i][1] = x.y; a[i][2] = x.z; a[i][3] = x.w; }
-#pragma unroll
-        for (int n = 0; n < NC; ++n) {
-            const int c = 64 * n + 4 * tx;
-            if (c >= D) break;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const float4 y = ld4(b + (k + q) * P + c);
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    acc[i][4 * n] = fmaf(a[i][q], y.x, acc[i][4 * n]); acc[i][4 * n + 1] = fmaf(a[i][q], y.y, acc[i][4 * n + 1]);
-                    acc[i][4 * n + 2] = fmaf(a[i][q], y.z, acc[i][4 * n + 2]); acc[i][4 * n + 3] = fmaf(a[i][q], y.w, acc[i][4 * n + 3]);
-                }
-            }
-        }
-    }
-}
-// acc[i][4 n + e] += sum_r p[r][2 ty + i] b[r][64 n + 4 tx + e], r < 64
-template <int NC>
-__device__ __forceinline__ void as_atb(float (&acc)[2][4 * NC], const float* p, const float* b, int D, int ty, int tx) {
-    const int P = D + 4;
-#pragma unroll 8
-    for (int r = 0; r < AS_T; ++r) {
-        const float2 a = *reinterpret_cast<const float2*>(p + r * (AS_OWN + 4) + 2 * ty);
-#pragma unroll
-        for (int n = 0; n < NC; ++n) {
-            const int c = 64 * n + 4 * tx;
-            if (c >= D) break;
-            const float4 y = ld4(b + r * P + c);
-            acc[0][4 * n] = fmaf(a.x, y.x, acc[0][4 * n]); acc[0][4 * n + 1] = fmaf(a.x, y.y, acc[0][4 * n + 1]);
-            acc[0][4 * n + 2] = fmaf(a.x, y.z, acc[0][4 * n + 2]); acc[0][4 * n + 3] = fmaf(a.x, y.w, acc[0][4 * n + 3]);
-            acc[1][4 * n] = fmaf(a.y, y.x, acc[1][4 * n]); acc[1][4 * n + 1] = fmaf(a.y, y.y, acc[1][4 * n + 1]);
-            acc[1][4 * n + 2] = fmaf(a.y, y.z, acc[1][4 * n + 2]); acc[1][4 * n + 3] = fmaf(a.y, y.w, acc[1][4 * n + 3]);
-        }
-    }
-}
-__device__ __forceinline__ float as_row(float v, bool is_max) {  // over the 16 threads of a row
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) { const float w = __shfl_xor_sync(0xffffffffu, v, o); v = is_max ? fmaxf(v, w) : v + w; }
-    return v;
-}
 
 // floats of shared memory: the 32-row tiles, the 64-row tiles and `blocks` blocks of scores
 static size_t as_floats(int own, int other, int blocks, int64_t D) { return (size_t)(own * AS_OWN + other * AS_T) * (D + 4) + (size_t)blocks * AS_T * (AS_OWN + 4); }

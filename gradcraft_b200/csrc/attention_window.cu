@@ -1,0 +1,636 @@
+// Causal attention under a visibility rule: a sliding window, a few first positions that stay visible (sinks), a learned bias by distance
+// bucket.  Forward, backward with the bias table's gradient, and the form for one new position per sequence over a cache.  The reference
+// has the causal form alone (frontend/tensor_other.hpp:53-93).
+//
+// This file holds the entry points, the fp32 FMA kernels, which take any strides and heads of up to 128 columns, and the kernel for single
+// positions.
+#include <algorithm>
+
+#include "attention_fma.cuh"
+#include "attention_window.cuh"
+
+namespace gcb {
+
+// ---- fp32 FMA kernels ----------------------------------------------------------------------------------------------------------
+// A CTA owns 32 queries (forward, dQ) or 32 keys (dK, dV) of a head and walks over tiles of 64 of the other side, skipping those that the
+// rule hides as a whole.  The bias of a tile is looked up once per distance (95 of them) and read from shared memory.
+constexpr int AW_DIAG = AS_OWN + AS_T - 1;
+
+// ROWS rows of D columns from row r0 into [row][Dp + 4], zero beyond T and D.  VEC: rows start on 16 bytes and D is a multiple of four.
+template <int ROWS, bool VEC>
+__device__ __forceinline__ void aw_load(float* sm, const float* p, int64_t ld, int r0, int T, int D, int Dp) {
+    if (VEC) { as_load<ROWS>(sm, p, ld, r0, T, D); return; }
+    for (int i = threadIdx.x; i < ROWS * Dp; i += 256) {
+        const int r = i / Dp, c = i - r * Dp;
+        sm[r * (Dp + 4) + c] = r0 + r < T && c < D ? p[(r0 + r) * ld + c] : 0.0f;
+    }
+}
+template <bool VEC>
+__device__ __forceinline__ float4 aw_ld4(const float* p, int c, int D) {
+    if (VEC) return c < D ? ld4(p + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+    return make_float4(c < D ? p[c] : 0.0f, c + 1 < D ? p[c + 1] : 0.0f, c + 2 < D ? p[c + 2] : 0.0f, c + 3 < D ? p[c + 3] : 0.0f);
+}
+template <bool VEC>
+__device__ __forceinline__ void aw_st4(float* p, int c, int D, float4 x) {
+    if (VEC) { if (c < D) st4(p + c, x); return; }
+    if (c < D) p[c] = x.x;
+    if (c + 1 < D) p[c + 1] = x.y;
+    if (c + 2 < D) p[c + 2] = x.z;
+    if (c + 3 < D) p[c + 3] = x.w;
+}
+// bias of the distances d0 .. d0 + 94 of a tile
+__device__ __forceinline__ void aw_tab(float* tab, const WindowRule& r, int h, int d0) {
+    if (r.bias == nullptr) return;
+    const int t = threadIdx.x;
+    if (t < AW_DIAG) tab[t] = d0 + t >= 0 ? r.bias[(int64_t)h * r.buckets + r.bucket(d0 + t)] : 0.0f;
+}
+// the tile of keys after k0 that queries q0 .. q0 + 31 look at
+__device__ __forceinline__ int aw_first_tile(const WindowRule& r, int q0) { return r.S > 0 ? 0 : r.window_first(q0) / AS_T * AS_T; }
+__device__ __forceinline__ int aw_next_tile(const WindowRule& r, int q0, int k0) {
+    const int k1 = k0 + AS_T, lo = r.window_first(q0) / AS_T * AS_T;
+    return k1 >= r.S && k1 < lo ? lo : k1;
+}
+static size_t aw_floats(int own, int other, int blocks, int64_t Dp) { return (size_t)(own * AS_OWN + other * AS_T) * (Dp + 4) + (size_t)blocks * AS_T * (AS_OWN + 4) + 2 * (AW_DIAG + 1); }
+
+template <int NC, bool VEC>
+__global__ void __launch_bounds__(256) window_attention_fwd_kernel(const __grid_constant__ WindowAttn p) {
+    extern __shared__ __align__(16) float aw_sm[];
+    pdl_trigger();
+    pdl_wait();
+    const int D = p.D, Dp = (D + 3) / 4 * 4, tx = threadIdx.x & 15, ty = threadIdx.x >> 4, head = blockIdx.x / p.tiles, q0 = (blockIdx.x - head * p.tiles) * AS_OWN, last = min(q0 + AS_OWN, p.T);
+    const int64_t b = head / p.H, h = head - b * p.H;
+    float *sq = aw_sm, *sk = sq + AS_OWN * (Dp + 4), *sv = sk + AS_T * (Dp + 4), *sp = sv + AS_T * (Dp + 4), *tab = sp + AS_T * (AS_OWN + 4);
+    const float *k = p.k + b * p.k_so + h * p.k_si, *v = p.v + b * p.v_so + h * p.v_si;
+    aw_load<AS_OWN, VEC>(sq, p.q + b * p.q_so + h * p.q_si, p.q_ld, q0, p.T, D, Dp);
+    float acc[2][4 * NC] = {}, m[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+    for (int k0 = aw_first_tile(p.rule, q0); k0 < last; k0 = aw_next_tile(p.rule, q0, k0)) {
+        __syncthreads();
+        aw_load<AS_T, VEC>(sk, k, p.k_ld, k0, p.T, D, Dp);
+        aw_load<AS_T, VEC>(sv, v, p.v_ld, k0, p.T, D, Dp);
+        aw_tab(tab, p.rule, (int)h, q0 - k0 - (AS_T - 1));
+        as_landed();
+        float s[2][4];
+        as_abt(s, sq, sk, Dp, ty, tx);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int row = q0 + ty + 16 * i;
+            float mx = m[i];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float z = p.rule.bias ? fmaf(s[i][j], p.scale, tab[ty + 16 * i - (tx + 16 * j) + AS_T - 1]) : s[i][j] * p.scale;
+                s[i][j] = p.rule.sees(row, k0 + tx + 16 * j) ? z : -INFINITY;
+                mx = fmaxf(mx, s[i][j]);
+            }
+            mx = as_row(mx, true);
+            const float rel = mx == -INFINITY ? 0.0f : mx, f = __expf(m[i] - rel);  // nothing seen yet: every term below is exp(-inf)
+            m[i] = mx;
+            float part = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { const float e = __expf(s[i][j] - rel); part += e; sp[(ty + 16 * i) * (AS_T + 4) + tx + 16 * j] = e; }
+            sum[i] = sum[i] * f + as_row(part, false);
+#pragma unroll
+            for (int e = 0; e < 4 * NC; ++e) acc[i][e] *= f;
+        }
+        __syncthreads();
+        as_ab<NC>(acc, sp, sv, Dp, ty, tx);
+    }
+    float* out = p.out + b * p.o_so + h * p.o_si;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int row = q0 + ty + 16 * i;
+        if (row >= p.T) continue;
+        const bool empty = m[i] == -INFINITY;
+        const float inv = empty ? 0.0f : 1.0f / sum[i];
+#pragma unroll
+        for (int n = 0; n < NC; ++n)
+            aw_st4<VEC>(out + row * p.o_ld, 64 * n + 4 * tx, D, make_float4(acc[i][4 * n] * inv, acc[i][4 * n + 1] * inv, acc[i][4 * n + 2] * inv, acc[i][4 * n + 3] * inv));
+        if (tx == 0) { p.row_max[head * p.Tp + row] = empty ? 0.0f : m[i]; p.row_inv[head * p.Tp + row] = inv; }
+    }
+}
+
+// dO . O and the statistics of this thread's rows ty + 16 i of a query tile (dO in shared memory, O requested before it has landed)
+template <int R, int NC, bool VEC>
+struct AwRows {
+    float delta[R], m[R], inv[R];
+    float4 y[R][NC];
+    __device__ __forceinline__ void request(const WindowAttn& p, int head, const float* o, int r0, int ty, int tx) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int row = r0 + ty + 16 * i;
+            const bool live = row < p.T;
+            m[i] = live ? p.row_max[head * p.Tp + row] : 0.0f;
+            inv[i] = live ? p.row_inv[head * p.Tp + row] : 0.0f;
+#pragma unroll
+            for (int n = 0; n < NC; ++n) y[i][n] = live ? aw_ld4<VEC>(o + row * p.o_ld, 64 * n + 4 * tx, p.D) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+    }
+    __device__ __forceinline__ void finish(const float* sg, int Dp, int ty, int tx) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            float d = 0.0f;
+#pragma unroll
+            for (int n = 0; n < NC; ++n)
+                if (64 * n + 4 * tx < Dp) {
+                    const float4 x = ld4(sg + (ty + 16 * i) * (Dp + 4) + 64 * n + 4 * tx);
+                    d = fmaf(x.x, y[i][n].x, fmaf(x.y, y[i][n].y, fmaf(x.z, y[i][n].z, fmaf(x.w, y[i][n].w, d))));
+                }
+            delta[i] = as_row(d, false);
+        }
+    }
+};
+
+// dQ of 32 queries; with a bias table also its gradient over them: thread n < buckets keeps bucket n, dbias_part is [head][tile][buckets].
+// Sums of a bucket go along the tile's diagonals, in a fixed order.
+template <int NC, bool VEC>
+__global__ void __launch_bounds__(256) window_attention_dq_kernel(const __grid_constant__ WindowAttn p) {
+    extern __shared__ __align__(16) float aw_sm[];
+    pdl_trigger();
+    pdl_wait();
+    const int D = p.D, Dp = (D + 3) / 4 * 4, tx = threadIdx.x & 15, ty = threadIdx.x >> 4, head = blockIdx.x / p.tiles, tile = blockIdx.x - head * p.tiles, q0 = tile * AS_OWN;
+    const int64_t b = head / p.H, h = head - b * p.H;
+    float *s0 = aw_sm, *s1 = s0 + AS_OWN * (Dp + 4), *s2 = s1 + AS_OWN * (Dp + 4), *s3 = s2 + AS_T * (Dp + 4), *ss = s3 + AS_T * (Dp + 4), *tab = ss + AS_T * (AS_OWN + 4), *diag = tab + AW_DIAG + 1;
+    const float *k = p.k + b * p.k_so + h * p.k_si, *v = p.v + b * p.v_so + h * p.v_si;
+    float dq[2][4 * NC] = {}, db = 0.0f;
+    AwRows<2, NC, VEC> rows;
+    aw_load<AS_OWN, VEC>(s0, p.q + b * p.q_so + h * p.q_si, p.q_ld, q0, p.T, D, Dp);
+    aw_load<AS_OWN, VEC>(s1, p.g + b * p.g_so + h * p.g_si, p.g_ld, q0, p.T, D, Dp);
+    rows.request(p, head, p.o + b * p.o_so + h * p.o_si, q0, ty, tx);
+    bool first = true;
+    for (int k0 = aw_first_tile(p.rule, q0); k0 < min(q0 + AS_OWN, p.T); k0 = aw_next_tile(p.rule, q0, k0)) {
+        const int d0 = q0 - k0 - (AS_T - 1);
+        __syncthreads();
+        aw_load<AS_T, VEC>(s2, k, p.k_ld, k0, p.T, D, Dp);
+        aw_load<AS_T, VEC>(s3, v, p.v_ld, k0, p.T, D, Dp);
+        aw_tab(tab, p.rule, (int)h, d0);
+        as_landed();
+        if (first) rows.finish(s1, Dp, ty, tx);
+        first = false;
+        float s[2][4], dp[2][4];
+        as_abt(s, s0, s2, Dp, ty, tx);
+        as_abt(dp, s1, s3, Dp, ty, tx);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int r = ty + 16 * i, c = tx + 16 * j;
+                const float z = p.rule.bias ? fmaf(s[i][j], p.scale, tab[r - c + AS_T - 1]) : s[i][j] * p.scale;
+                const float pr = p.rule.sees(q0 + r, k0 + c) ? __expf(z - rows.m[i]) * rows.inv[i] : 0.0f;
+                ss[r * (AS_T + 4) + c] = pr * (dp[i][j] - rows.delta[i]);
+            }
+        __syncthreads();
+        as_ab<NC>(dq, ss, s2, Dp, ty, tx);
+        if (p.dbias_part) {
+            const int t = threadIdx.x;
+            if (t < AW_DIAG) {
+                float a = 0.0f;
+                for (int r = max(0, t - (AS_T - 1)); r <= min(AS_OWN - 1, t); ++r) a += ss[r * (AS_T + 4) + r - t + AS_T - 1];
+                diag[t] = a;
+            }
+            __syncthreads();
+            if (t < p.rule.buckets) {
+                const int end = t + 1 < p.rule.buckets ? p.rule.starts[t + 1] - d0 : AW_DIAG;
+                float a = 0.0f;
+                for (int i = max(0, p.rule.starts[t] - d0); i < min(end, AW_DIAG); ++i) a += diag[i];
+                db += a;
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int r = q0 + ty + 16 * i;
+        if (r >= p.T) continue;
+#pragma unroll
+        for (int n = 0; n < NC; ++n)
+            aw_st4<VEC>(p.dq + b * p.d_so + h * p.d_si + r * p.d_ld, 64 * n + 4 * tx, D,
+                        make_float4(p.scale * dq[i][4 * n], p.scale * dq[i][4 * n + 1], p.scale * dq[i][4 * n + 2], p.scale * dq[i][4 * n + 3]));
+    }
+    if (p.dbias_part && threadIdx.x < p.rule.buckets) p.dbias_part[(int64_t)blockIdx.x * p.rule.buckets + threadIdx.x] = db;
+}
+
+// dK and dV of 32 keys from the queries that see them through the window.  FAR: from the queries beyond the window instead, which see the
+// first S keys only: a CTA takes 512 of them and leaves its sums in far_part, [head][key tile][chunk][dk, dv][32][Dp], so that the few
+// first keys of a long sequence are not one CTA's work.
+constexpr int AW_FAR = 512;
+template <int NC, bool VEC, bool FAR>
+__global__ void __launch_bounds__(256) window_attention_dkv_kernel(const __grid_constant__ WindowAttn p) {
+    extern __shared__ __align__(16) float aw_sm[];
+    pdl_trigger();
+    pdl_wait();
+    const int per_head = FAR ? (p.rule.S + AS_OWN - 1) / AS_OWN * p.far_chunks : p.tiles;
+    const int D = p.D, Dp = (D + 3) / 4 * 4, tx = threadIdx.x & 15, ty = threadIdx.x >> 4, head = blockIdx.x / per_head, item = blockIdx.x - head * per_head;
+    const int t0 = (FAR ? item / p.far_chunks : item) * AS_OWN, chunk = FAR ? item % p.far_chunks : 0;
+    const int64_t b = head / p.H, h = head - b * p.H;
+    float *s0 = aw_sm, *s1 = s0 + AS_OWN * (Dp + 4), *s2 = s1 + AS_OWN * (Dp + 4), *s3 = s2 + AS_T * (Dp + 4), *sp = s3 + AS_T * (Dp + 4), *ss = sp + AS_T * (AS_OWN + 4), *tab = ss + AS_T * (AS_OWN + 4);
+    const float *q = p.q + b * p.q_so + h * p.q_si, *g = p.g + b * p.g_so + h * p.g_si, *o = p.o + b * p.o_so + h * p.o_si;
+    float dk[2][4 * NC] = {}, dv[2][4 * NC] = {};
+    aw_load<AS_OWN, VEC>(s0, p.k + b * p.k_so + h * p.k_si, p.k_ld, t0, p.T, D, Dp);
+    aw_load<AS_OWN, VEC>(s1, p.v + b * p.v_so + h * p.v_si, p.v_ld, t0, p.T, D, Dp);
+    const int W = p.rule.W, keys_end = min(t0 + AS_OWN, p.T);
+    int r_begin, r_end;
+    if (FAR) {
+        r_begin = max(chunk * AW_FAR, (t0 + W) / AS_T * AS_T);
+        r_end = min(p.T, (chunk + 1) * AW_FAR);
+    } else {
+        r_begin = t0 / AS_T * AS_T;
+        r_end = W > 0 && W < p.T - keys_end ? keys_end - 1 + W : p.T;
+    }
+    for (int r0 = r_begin; r0 < r_end; r0 += AS_T) {
+        __syncthreads();
+        AwRows<4, NC, VEC> rows;
+        aw_load<AS_T, VEC>(s2, q, p.q_ld, r0, p.T, D, Dp);
+        aw_load<AS_T, VEC>(s3, g, p.g_ld, r0, p.T, D, Dp);
+        aw_tab(tab, p.rule, (int)h, r0 - t0 - (AS_OWN - 1));
+        rows.request(p, head, o, r0, ty, tx);
+        as_landed();
+        rows.finish(s3, Dp, ty, tx);
+        float s[4][2], dp[4][2];
+        as_abt(s, s2, s0, Dp, ty, tx);
+        as_abt(dp, s3, s1, Dp, ty, tx);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int r = ty + 16 * i, c = tx + 16 * j, d = r0 + r - (t0 + c);
+                const float z = p.rule.bias ? fmaf(s[i][j], p.scale, tab[r - c + AS_OWN - 1]) : s[i][j] * p.scale;
+                const bool seen = FAR ? d >= W && t0 + c < p.rule.S : d >= 0 && (W == 0 || d < W);
+                const float pr = seen ? __expf(z - rows.m[i]) * rows.inv[i] : 0.0f;
+                sp[r * (AS_OWN + 4) + c] = pr;
+                ss[r * (AS_OWN + 4) + c] = pr * (dp[i][j] - rows.delta[i]);
+            }
+        __syncthreads();
+        as_atb<NC>(dv, sp, s3, Dp, ty, tx);
+        as_atb<NC>(dk, ss, s2, Dp, ty, tx);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+            const int c = 64 * n + 4 * tx, r = t0 + 2 * ty + i;
+            const float4 a = make_float4(p.scale * dk[i][4 * n], p.scale * dk[i][4 * n + 1], p.scale * dk[i][4 * n + 2], p.scale * dk[i][4 * n + 3]);
+            const float4 e = make_float4(dv[i][4 * n], dv[i][4 * n + 1], dv[i][4 * n + 2], dv[i][4 * n + 3]);
+            if (FAR) {
+                if (c >= Dp) continue;
+                float* part = p.far_part + ((int64_t)blockIdx.x * 2 * AS_OWN + 2 * ty + i) * Dp + c;
+                st4(part, a);
+                st4(part + AS_OWN * Dp, e);
+            } else if (r < p.T) {
+                const int64_t at = b * p.d_so + h * p.d_si + r * p.d_ld;
+                aw_st4<VEC>(p.dk + at, c, D, a);
+                aw_st4<VEC>(p.dv + at, c, D, e);
+            }
+        }
+}
+// Adds the chunks of far_part, in their order, to dK and dV of the first S keys.  A block per (head, key), a thread per column.
+__global__ void __launch_bounds__(128) window_attention_far_kernel(const __grid_constant__ WindowAttn p, int keys) {
+    pdl_trigger();
+    pdl_wait();
+    const int head = blockIdx.x / keys, key = blockIdx.x - head * keys, c = threadIdx.x, Dp = (p.D + 3) / 4 * 4, key_tiles = (p.rule.S + AS_OWN - 1) / AS_OWN;
+    if (c >= p.D) return;
+    const int64_t b = head / p.H, h = head - b * p.H, stride = (int64_t)2 * AS_OWN * Dp;
+    const float* part = p.far_part + ((int64_t)head * key_tiles + key / AS_OWN) * p.far_chunks * stride + (key % AS_OWN) * Dp + c;
+    float dk = 0.0f, dv = 0.0f;
+#pragma unroll 4
+    for (int i = 0; i < p.far_chunks; ++i) { dk += part[i * stride]; dv += part[i * stride + AS_OWN * Dp]; }
+    const int64_t at = b * p.d_so + h * p.d_si + key * p.d_ld + c;
+    p.dk[at] += dk;
+    p.dv[at] += dv;
+}
+// dbias[h, n] (+)= the sum of dbias_part over sequences and tiles, a warp each, in a fixed order
+__global__ void __launch_bounds__(256) window_attention_dbias_kernel(float* __restrict__ dbias, const float* __restrict__ part, int H, int B, int tiles, int buckets, int accumulate) {
+    pdl_trigger();
+    pdl_wait();
+    const int w = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (w >= H * buckets) return;
+    const int h = w / buckets, n = w - h * buckets;
+    double a = 0.0;  // terms of both signs over the whole batch
+    for (int64_t i = lane; i < (int64_t)B * tiles; i += 32) { const int64_t b = i / tiles; a += part[((b * H + h) * tiles + i - b * tiles) * buckets + n]; }
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) a += __shfl_xor_sync(0xffffffffu, a, s);
+    if (lane == 0) dbias[w] = (accumulate ? dbias[w] : 0.0f) + (float)a;
+}
+
+// ---- one new position per sequence ----------------------------------------------------------------------------------------------
+// A cluster of up to eight CTAs takes one head of one sequence and cuts the keys it sees (the first S, then the window) into as many
+// stretches; each of a CTA's eight warps reads four groups of rows at a time, a lane four columns, with a running maximum per lane group.
+// The stretches are joined through distributed shared memory, in their order, by the first CTA.
+// Bound by memory: 8 D bytes a key and head.
+constexpr int ST_WARPS = 8, ST_MAX_SPLIT = 8;
+struct StepAttn {
+    const float *q, *k, *v;
+    float* out;
+    const int64_t* lengths;
+    int* status;
+    int64_t o_so, o_si, q_so, q_si, k_ld, k_so, k_si, v_ld, v_so, v_si, cache_len;
+    int D, H;
+    float scale;
+    WindowRule rule;
+};
+__device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ uint32_t cluster_size() { uint32_t r; asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ float peer_float(const float* p, uint32_t rank) {
+    uint32_t a = (uint32_t)__cvta_generic_to_shared(p), m;
+    float f;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(m) : "r"(a), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(m) : "memory");
+    return f;
+}
+
+template <int LPR, bool VEC>  // lanes a row: 8, 16 or 32 of four columns each
+__global__ void __launch_bounds__(32 * ST_WARPS) window_attention_step_kernel(const __grid_constant__ StepAttn p) {
+    constexpr int RPW = 32 / LPR, U = 4, GROUPS = ST_WARPS * RPW, STEP = GROUPS * U, DP = 4 * LPR;
+    __shared__ float g_m[GROUPS], g_sum[GROUPS], g_o[GROUPS][DP + 4], c_o[DP], c_m, c_sum;
+    pdl_trigger();
+    pdl_wait();
+    const int rank = (int)cluster_rank(), split = (int)cluster_size(), item = blockIdx.x / split, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t b = item / p.H, h = item - b * p.H;
+    const int D = p.D, col = 4 * (lane % LPR), group = warp * RPW + lane / LPR;
+    int64_t len = p.lengths[b];
+    if (len < 0 || len > p.cache_len) {  // reported, not read
+        if (threadIdx.x == 0 && rank == 0 && h == 0) { atomicExch(&p.status[0], 2); atomicExch(&p.status[1], (int)b); }
+        len = 0;
+    }
+    const int last = (int)len - 1, lo = p.rule.window_first(last), s0 = min(p.rule.S, lo), count = len > 0 ? s0 + (int)len - lo : 0;
+    const int per = (count + split - 1) / split, v0 = min(count, rank * per), v1 = min(count, v0 + per);
+    const float *kb = p.k + b * p.k_so + h * p.k_si, *vb = p.v + b * p.v_so + h * p.v_si;
+    float4 q = aw_ld4<VEC>(p.q + b * p.q_so + h * p.q_si, col, D), o = make_float4(0.f, 0.f, 0.f, 0.f);
+    q.x *= p.scale; q.y *= p.scale; q.z *= p.scale; q.w *= p.scale;
+    float m = -INFINITY, sum = 0.0f;
+    auto key_of = [&](int x) { return x < s0 ? x : lo + (x - s0); };
+    float4 kk[U], vv[U], kn[U], vn[U];  // rows in hand, and the next ones
+    auto rows = [&](int x, float4 (&kr)[U], float4 (&vr)[U]) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int y = x + u * GROUPS;
+            const bool live = y < v1;
+            const int64_t key = live ? key_of(y) : 0;
+            kr[u] = live ? aw_ld4<VEC>(kb + key * p.k_ld, col, D) : make_float4(0.f, 0.f, 0.f, 0.f);
+            vr[u] = live ? aw_ld4<VEC>(vb + key * p.v_ld, col, D) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+    };
+    rows(v0 + group, kk, vv);
+    for (int x0 = v0; x0 < v1; x0 += STEP) {  // the same trips for every lane
+        const int x = x0 + group;
+        rows(x + STEP, kn, vn);
+        float z[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) z[u] = fmaf(q.x, kk[u].x, fmaf(q.y, kk[u].y, fmaf(q.z, kk[u].z, q.w * kk[u].w)));
+#pragma unroll
+        for (int s = LPR / 2; s > 0; s >>= 1)
+#pragma unroll
+            for (int u = 0; u < U; ++u) z[u] += __shfl_xor_sync(0xffffffffu, z[u], s);
+        float mx = m;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int y = x + u * GROUPS;
+            if (p.rule.bias != nullptr && y < v1) z[u] += p.rule.bias[h * p.rule.buckets + p.rule.bucket(last - key_of(y))];
+            if (y >= v1) z[u] = -INFINITY;
+            mx = fmaxf(mx, z[u]);
+        }
+        const float rel = mx == -INFINITY ? 0.0f : mx, f = __expf(m - rel);
+        m = mx;
+        sum *= f;
+        o.x *= f; o.y *= f; o.z *= f; o.w *= f;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const float e = __expf(z[u] - rel);
+            sum += e;
+            o.x = fmaf(e, vv[u].x, o.x); o.y = fmaf(e, vv[u].y, o.y); o.z = fmaf(e, vv[u].z, o.z); o.w = fmaf(e, vv[u].w, o.w);
+            kk[u] = kn[u]; vv[u] = vn[u];
+        }
+    }
+    if (lane % LPR == 0) { g_m[group] = m; g_sum[group] = sum; }
+    st4(&g_o[group][col], o);
+    __syncthreads();
+    const int t = threadIdx.x;
+    if (t < DP) {  // this CTA's stretch: its groups in their order
+        float mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < GROUPS; ++i) mx = fmaxf(mx, g_m[i]);
+        const float rel = mx == -INFINITY ? 0.0f : mx;
+        float a = 0.0f, total = 0.0f;
+#pragma unroll
+        for (int i = 0; i < GROUPS; ++i) {
+            const float f = __expf(g_m[i] - rel);
+            a = fmaf(f, g_o[i][t], a);
+            total = fmaf(f, g_sum[i], total);
+        }
+        c_o[t] = a;
+        if (t == 0) { c_m = mx; c_sum = total; }
+    }
+    cluster_sync();
+    if (rank == 0 && t < D) {
+        float mx = -INFINITY;
+        for (int i = 0; i < split; ++i) mx = fmaxf(mx, peer_float(&c_m, i));
+        const float rel = mx == -INFINITY ? 0.0f : mx;
+        float a = 0.0f, total = 0.0f;
+        for (int i = 0; i < split; ++i) {
+            const float f = __expf(peer_float(&c_m, i) - rel);
+            a = fmaf(f, peer_float(c_o + t, i), a);
+            total = fmaf(f, peer_float(&c_sum, i), total);
+        }
+        p.out[b * p.o_so + h * p.o_si + t] = mx == -INFINITY ? 0.0f : a / total;
+    }
+    cluster_sync();  // nobody leaves while its shared memory is read
+}
+
+// ---- host side ----------------------------------------------------------------------------------------------------------------
+static bool vec_rows(const float* p, int64_t ld, int64_t so, int64_t si) { return aligned16(p) && ld % 4 == 0 && so % 4 == 0 && si % 4 == 0; }
+static bool own_rows(int64_t B, int64_t H, int64_t T, int64_t D, int64_t ld, int64_t so, int64_t si) { return (T <= 1 || ld >= D) && (H <= 1 || si > 0) && (B <= 1 || so > 0); }
+static size_t span_bytes(int64_t B, int64_t H, int64_t T, int64_t D, int64_t ld, int64_t so, int64_t si) { return sizeof(float) * (size_t)((B - 1) * so + (H - 1) * si + (T - 1) * ld + D); }
+constexpr int64_t AW_MAX_T = int64_t(1) << 24, AW_MAX_D = 128;
+
+template <class K>
+static int fma_launch(gcb_ctx* ctx, K kernel, bool* done, int64_t ctas, size_t floats, const WindowAttn& p) {
+    GCB_REQUIRE(ctas < (int64_t(1) << 31), "window attention: more tiles than a grid holds");
+    if (!done[ctx->device]) { GCB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448 - 1024)); done[ctx->device] = true; }
+    GCB_CHECK_CUDA(launch_next(ctx->stream, dim3((unsigned)ctas), 256, sizeof(float) * floats, kernel, p));
+    return GCB_OK;
+}
+template <int NC, bool VEC>
+static int fma_fwd(gcb_ctx* ctx, int64_t heads, const WindowAttn& p) {
+    static bool done[kMaxDevices] = {};
+    const int rc = fma_launch(ctx, window_attention_fwd_kernel<NC, VEC>, done, heads * p.tiles, aw_floats(1, 2, 1, (p.D + 3) / 4 * 4), p);
+    return rc ? rc : after_launch(ctx, "window_attention_fwd");
+}
+template <int NC, bool VEC>
+static int fma_bwd(gcb_ctx* ctx, int64_t heads, const WindowAttn& p) {
+    static bool done_q[kMaxDevices] = {}, done_kv[kMaxDevices] = {};
+    const int64_t Dp = (p.D + 3) / 4 * 4;
+    int rc = fma_launch(ctx, window_attention_dq_kernel<NC, VEC>, done_q, heads * p.tiles, aw_floats(2, 2, 1, Dp), p);
+    if (!rc) rc = after_launch(ctx, "window_attention_dq");
+    if (!rc) rc = fma_launch(ctx, window_attention_dkv_kernel<NC, VEC, false>, done_kv, heads * p.tiles, aw_floats(2, 2, 2, Dp), p);
+    return rc ? rc : after_launch(ctx, "window_attention_dkv");
+}
+// What queries beyond the window add to the first keys' gradients; after dK and dV have been written.
+template <int NC, bool VEC>
+static int fma_far(gcb_ctx* ctx, int64_t heads, const WindowAttn& p) {
+    static bool done[kMaxDevices] = {};
+    const int key_tiles = (p.rule.S + AS_OWN - 1) / AS_OWN, keys = std::min(p.rule.S, p.T);
+    int rc = fma_launch(ctx, window_attention_dkv_kernel<NC, VEC, true>, done, heads * key_tiles * p.far_chunks, aw_floats(2, 2, 2, (p.D + 3) / 4 * 4), p);
+    if (!rc) rc = after_launch(ctx, "window_attention_far");
+    if (rc) return rc;
+    GCB_CHECK_CUDA(launch_next(ctx->stream, dim3((unsigned)(heads * keys)), 128, 0, window_attention_far_kernel, p, keys));
+    return after_launch(ctx, "window_attention_far_sum");
+}
+
+}  // namespace gcb
+
+using namespace gcb;
+
+extern "C" {
+
+int gcb_relative_bucket_starts(int64_t buckets, int64_t reach, int64_t* starts) {
+    GCB_REQUIRE(buckets >= 1 && buckets <= AW_MAX_BUCKETS && reach >= 1 && reach < (int64_t(1) << 30) && starts, "gcb_relative_bucket_starts: 1 to %d buckets and a positive distance are needed", AW_MAX_BUCKETS);
+    // Bucket e + k of e + m starts at the least n with n^m e^k >= reach^k e^m: whole numbers of up to 64 factors of 30 bits, so that no
+    // border hangs on the rounding of a logarithm.
+    const int64_t e = std::max<int64_t>(1, buckets / 2), m = buckets - e, far = std::max(reach, e);
+    struct Big {
+        uint32_t w[128];
+        int n;
+    };
+    auto times = [](Big& x, uint64_t f, int64_t times) {
+        for (; times > 0; --times) {
+            uint64_t carry = 0;
+            for (int i = 0; i < x.n; ++i) { carry += x.w[i] * f; x.w[i] = (uint32_t)carry; carry >>= 32; }
+            if (carry) x.w[x.n++] = (uint32_t)carry;
+        }
+    };
+    auto less = [](const Big& a, const Big& b) {
+        if (a.n != b.n) return a.n < b.n;
+        for (int i = a.n - 1; i >= 0; --i) if (a.w[i] != b.w[i]) return a.w[i] < b.w[i];
+        return false;
+    };
+    for (int64_t n = 0; n < e; ++n) starts[n] = n;
+    for (int64_t k = 0; k < m; ++k) {
+        Big right = {{1}, 1};
+        times(right, (uint64_t)far, k);
+        times(right, (uint64_t)e, m);
+        int64_t lo = 0, hi = far;  // lo is too small, hi is not
+        while (hi - lo > 1) {
+            const int64_t mid = lo + (hi - lo) / 2;
+            Big left = {{1}, 1};
+            times(left, (uint64_t)mid, m);
+            times(left, (uint64_t)e, k);
+            (less(left, right) ? lo : hi) = mid;
+        }
+        starts[e + k] = hi;
+    }
+    return GCB_OK;
+}
+
+int gcb_window_attention_fwd_f32(gcb_ctx* ctx, int64_t B, int64_t H, int64_t T, int64_t D, float* out, int64_t o_ld, int64_t o_so, int64_t o_si, float* stats, const float* q, int64_t q_ld, int64_t q_so, int64_t q_si,
+                                 const float* k, int64_t k_ld, int64_t k_so, int64_t k_si, const float* v, int64_t v_ld, int64_t v_so, int64_t v_si, float scale, int64_t window, int64_t sinks, const float* bias,
+                                 int64_t buckets, const int64_t* bucket_starts) {
+    GCB_REQUIRE(ctx && B >= 0 && H >= 0 && T >= 0 && D >= 0, "gcb_window_attention_fwd_f32: bad arguments");
+    WindowAttn p = {};
+    int rc = make_rule(p.rule, "gcb_window_attention_fwd_f32", window, sinks, bias, buckets, bucket_starts);
+    if (rc) return rc;
+    if (B == 0 || H == 0 || T == 0 || D == 0) return GCB_OK;
+    if (D > AW_MAX_D || T > AW_MAX_T) { set_error("gcb_window_attention_fwd_f32: heads of up to %lld columns and sequences of up to %lld positions", (long long)AW_MAX_D, (long long)AW_MAX_T); return GCB_UNSUPPORTED; }
+    GCB_REQUIRE(out && stats && q && k && v && own_rows(B, H, T, D, o_ld, o_so, o_si), "gcb_window_attention_fwd_f32: NULL pointer, or output rows that overlap");
+    cudaSetDevice(ctx->device);
+    p.q = q; p.q_ld = q_ld; p.q_so = q_so; p.q_si = q_si;
+    p.k = k; p.k_ld = k_ld; p.k_so = k_so; p.k_si = k_si;
+    p.v = v; p.v_ld = v_ld; p.v_so = v_so; p.v_si = v_si;
+    p.out = out; p.o_ld = o_ld; p.o_so = o_so; p.o_si = o_si;
+    p.Tp = gcb_attention_stats_floats(1, 1, T) / 2; p.T = (int)T; p.D = (int)D; p.H = (int)H; p.scale = scale;
+    p.row_max = stats; p.row_inv = stats + B * H * p.Tp;
+    p.tiles = (int)((T + AS_OWN - 1) / AS_OWN);
+    const bool vec = D % 4 == 0 && vec_rows(q, q_ld, q_so, q_si) && vec_rows(k, k_ld, k_so, k_si) && vec_rows(v, v_ld, v_so, v_si) && vec_rows(out, o_ld, o_so, o_si);
+    rc = D <= 64 ? (vec ? fma_fwd<1, true>(ctx, B * H, p) : fma_fwd<1, false>(ctx, B * H, p)) : (vec ? fma_fwd<2, true>(ctx, B * H, p) : fma_fwd<2, false>(ctx, B * H, p));
+    if (rc) return rc;
+    note_write(ctx, out, span_bytes(B, H, T, D, o_ld, o_so, o_si));
+    return GCB_OK;
+}
+
+int gcb_window_attention_bwd_f32(gcb_ctx* ctx, int64_t B, int64_t H, int64_t T, int64_t D, float* dq, float* dk, float* dv, int64_t d_ld, int64_t d_so, int64_t d_si, float* dbias, int accumulate_dbias,
+                                 const float* dout, int64_t g_ld, int64_t g_so, int64_t g_si, const float* out, int64_t o_ld, int64_t o_so, int64_t o_si, const float* stats, const float* q, int64_t q_ld, int64_t q_so,
+                                 int64_t q_si, const float* k, int64_t k_ld, int64_t k_so, int64_t k_si, const float* v, int64_t v_ld, int64_t v_so, int64_t v_si, float scale, int64_t window, int64_t sinks,
+                                 const float* bias, int64_t buckets, const int64_t* bucket_starts) {
+    GCB_REQUIRE(ctx && B >= 0 && H >= 0 && T >= 0 && D >= 0, "gcb_window_attention_bwd_f32: bad arguments");
+    WindowAttn p = {};
+    int rc = make_rule(p.rule, "gcb_window_attention_bwd_f32", window, sinks, bias, buckets, bucket_starts);
+    if (rc) return rc;
+    GCB_REQUIRE(bias || !dbias, "gcb_window_attention_bwd_f32: a gradient of the bias without a bias");
+    if (B == 0 || H == 0 || T == 0 || D == 0) return dbias && !accumulate_dbias && H > 0 ? gcb_fill_f32(ctx, dbias, 0.0f, H * buckets) : GCB_OK;
+    if (D > AW_MAX_D || T > AW_MAX_T) { set_error("gcb_window_attention_bwd_f32: heads of up to %lld columns and sequences of up to %lld positions", (long long)AW_MAX_D, (long long)AW_MAX_T); return GCB_UNSUPPORTED; }
+    GCB_REQUIRE(dq && dk && dv && dout && out && stats && q && k && v && own_rows(B, H, T, D, d_ld, d_so, d_si), "gcb_window_attention_bwd_f32: NULL pointer, or gradient rows that overlap");
+    cudaSetDevice(ctx->device);
+    p.q = q; p.q_ld = q_ld; p.q_so = q_so; p.q_si = q_si;
+    p.k = k; p.k_ld = k_ld; p.k_so = k_so; p.k_si = k_si;
+    p.v = v; p.v_ld = v_ld; p.v_so = v_so; p.v_si = v_si;
+    p.g = dout; p.g_ld = g_ld; p.g_so = g_so; p.g_si = g_si;
+    p.o = out; p.o_ld = o_ld; p.o_so = o_so; p.o_si = o_si;
+    p.dq = dq; p.dk = dk; p.dv = dv; p.d_ld = d_ld; p.d_so = d_so; p.d_si = d_si;
+    p.Tp = gcb_attention_stats_floats(1, 1, T) / 2; p.T = (int)T; p.D = (int)D; p.H = (int)H; p.scale = scale;
+    p.row_max = const_cast<float*>(stats); p.row_inv = p.row_max + B * H * p.Tp;
+    p.tiles = (int)((T + AS_OWN - 1) / AS_OWN);
+    const int64_t Dp = (D + 3) / 4 * 4, heads = B * H;
+    const bool vec = D % 4 == 0 && vec_rows(q, q_ld, q_so, q_si) && vec_rows(k, k_ld, k_so, k_si) && vec_rows(v, v_ld, v_so, v_si) && vec_rows(dout, g_ld, g_so, g_si) && vec_rows(out, o_ld, o_so, o_si) &&
+                     vec_rows(dq, d_ld, d_so, d_si) && vec_rows(dk, d_ld, d_so, d_si) && vec_rows(dv, d_ld, d_so, d_si);
+    Scratch part(ctx), far(ctx);
+    if (dbias) {
+        if ((rc = part.get(sizeof(float) * (size_t)(heads * p.tiles * buckets)))) return rc;
+        p.dbias_part = part.as<float>();
+    }
+    rc = D <= 64 ? (vec ? fma_bwd<1, true>(ctx, heads, p) : fma_bwd<1, false>(ctx, heads, p)) : (vec ? fma_bwd<2, true>(ctx, heads, p) : fma_bwd<2, false>(ctx, heads, p));
+    if (rc) return rc;
+    if (p.rule.S > 0 && p.rule.W < T) {  // some query looks past its window
+        p.far_chunks = (int)((T + AW_FAR - 1) / AW_FAR);
+        if ((rc = far.get(sizeof(float) * (size_t)(heads * ((p.rule.S + AS_OWN - 1) / AS_OWN) * p.far_chunks * 2 * AS_OWN * Dp)))) return rc;
+        p.far_part = far.as<float>();
+        rc = D <= 64 ? (vec ? fma_far<1, true>(ctx, heads, p) : fma_far<1, false>(ctx, heads, p)) : (vec ? fma_far<2, true>(ctx, heads, p) : fma_far<2, false>(ctx, heads, p));
+        if (rc) return rc;
+    }
+    for (float* d : {dq, dk, dv}) note_write(ctx, d, span_bytes(B, H, T, D, d_ld, d_so, d_si));
+    if (dbias) {
+        GCB_CHECK_CUDA(launch_next(ctx->stream, dim3((unsigned)((H * buckets + 7) / 8)), 256, 0, window_attention_dbias_kernel, dbias, part.as<float>(), (int)H, (int)B, p.tiles, (int)buckets, accumulate_dbias));
+        note_write(ctx, dbias, sizeof(float) * (size_t)(H * buckets));
+        return after_launch(ctx, "window_attention_dbias");
+    }
+    return GCB_OK;
+}
+
+int gcb_window_attention_step_f32(gcb_ctx* ctx, int64_t n_seq, int64_t H, int64_t D, float* out, int64_t o_so, int64_t o_si, const float* q, int64_t q_so, int64_t q_si, const float* k, int64_t k_ld, int64_t k_so,
+                                  int64_t k_si, const float* v, int64_t v_ld, int64_t v_so, int64_t v_si, int64_t cache_len, const int64_t* lengths, float scale, int64_t window, int64_t sinks, const float* bias,
+                                  int64_t buckets, const int64_t* bucket_starts) {
+    GCB_REQUIRE(ctx && n_seq >= 0 && H >= 0 && D >= 0 && cache_len >= 0, "gcb_window_attention_step_f32: bad arguments");
+    StepAttn p = {};
+    int rc = make_rule(p.rule, "gcb_window_attention_step_f32", window, sinks, bias, buckets, bucket_starts);
+    if (rc) return rc;
+    if (n_seq == 0 || H == 0 || D == 0) return GCB_OK;
+    if (D > AW_MAX_D || cache_len >= (int64_t(1) << 30)) { set_error("gcb_window_attention_step_f32: heads of up to %lld columns and caches of less than 2^30 positions", (long long)AW_MAX_D); return GCB_UNSUPPORTED; }
+    GCB_REQUIRE(out && q && (cache_len == 0 || (k && v)) && lengths && own_rows(n_seq, H, 1, D, 0, o_so, o_si), "gcb_window_attention_step_f32: NULL pointer, or output rows that overlap");
+    cudaSetDevice(ctx->device);
+    p.q = q; p.q_so = q_so; p.q_si = q_si;
+    p.k = k; p.k_ld = k_ld; p.k_so = k_so; p.k_si = k_si;
+    p.v = v; p.v_ld = v_ld; p.v_so = v_so; p.v_si = v_si;
+    p.out = out; p.o_so = o_so; p.o_si = o_si;
+    p.lengths = lengths; p.status = ctx->d_status; p.cache_len = cache_len; p.D = (int)D; p.H = (int)H; p.scale = scale;
+    const bool vec = D % 4 == 0 && vec_rows(q, 0, q_so, q_si) && vec_rows(k, k_ld, k_so, k_si) && vec_rows(v, v_ld, v_so, v_si);
+    // As many stretches as fill the SMs about twice over, none shorter than 64 keys.
+    const int64_t seen = p.rule.W ? std::min<int64_t>(cache_len, (int64_t)p.rule.W + p.rule.S) : cache_len;
+    int64_t split = 1;
+    while (split < ST_MAX_SPLIT && n_seq * H * split < 2 * kSMs && seen / (2 * split) >= 64) split *= 2;
+    GCB_REQUIRE(n_seq * H * split < (int64_t(1) << 31), "gcb_window_attention_step_f32: more heads than a grid holds");
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(n_seq * H * split));
+    cfg.blockDim = dim3(32 * ST_WARPS);
+    cfg.stream = ctx->stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)split; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = n_seq * H * split <= kSMs ? 2 : 1;
+    auto run = [&](auto kernel) { return cudaLaunchKernelEx(&cfg, kernel, p); };
+    if (D <= 32) GCB_CHECK_CUDA(vec ? run(window_attention_step_kernel<8, true>) : run(window_attention_step_kernel<8, false>));
+    else if (D <= 64) GCB_CHECK_CUDA(vec ? run(window_attention_step_kernel<16, true>) : run(window_attention_step_kernel<16, false>));
+    else GCB_CHECK_CUDA(vec ? run(window_attention_step_kernel<32, true>) : run(window_attention_step_kernel<32, false>));
+    note_write(ctx, out, span_bytes(n_seq, H, 1, D, 0, o_so, o_si));
+    return after_launch(ctx, "window_attention_step");
+}
+
+}  // extern "C"

@@ -250,6 +250,42 @@ GCB_API int gcb_attention_bwd_f32(gcb_ctx* ctx, int64_t batch, int64_t heads, in
                           const float* q, int64_t q_ld, int64_t q_so, int64_t q_si, const float* k, int64_t k_ld, int64_t k_so, int64_t k_si,
                           const float* v, int64_t v_ld, int64_t v_so, int64_t v_si, float scale);
 
+/* Causal attention under a visibility rule, over batch x heads sequences of seq_len rows and head_dim columns (head_dim <= 128):
+ *   query i sees key j   <=>   j <= i and (window == 0 or i - j < window or j < sinks)          sinks <= 64
+ *   score(i, j) = scale q_i . k_j + bias[h, n],  n = the last bucket with bucket_starts[n] <= i - j
+ * bias (optional): device, heads x buckets; bucket_starts: host, `buckets` (<= 64) first distances, ascending from 0 (several buckets may
+ * start at one distance; the last of them counts).  A bias of -inf hides a bucket; a query that then sees nothing gets zeros and gives no gradient.
+ * q, k, v, out, dout and the gradients are addressed through row, sequence and head strides in elements, any strides for what is only read; columns
+ * are contiguous.  out and the gradients must not overlap their inputs.  stats: gcb_attention_stats_floats floats that the forward
+ * fills and the backward reads.  dq, dk and dv share one layout and are overwritten; dbias (optional, heads x buckets) is overwritten or added
+ * to.  Deterministic: every sum is taken in a fixed order.  The backward takes workspace from the arena while it runs.
+ * A value that is not finite in a row of k or v reaches, besides the queries that see it, others whose tile holds that row.
+ * The reference has the causal form (frontend/tensor_other.hpp:53-93). */
+GCB_API int gcb_window_attention_fwd_f32(gcb_ctx* ctx, int64_t batch, int64_t heads, int64_t seq_len, int64_t head_dim, float* out, int64_t o_ld, int64_t o_so, int64_t o_si, float* stats,
+                                 const float* q, int64_t q_ld, int64_t q_so, int64_t q_si, const float* k, int64_t k_ld, int64_t k_so, int64_t k_si,
+                                 const float* v, int64_t v_ld, int64_t v_so, int64_t v_si, float scale, int64_t window, int64_t sinks, const float* bias /*opt*/, int64_t buckets, const int64_t* bucket_starts);
+GCB_API int gcb_window_attention_bwd_f32(gcb_ctx* ctx, int64_t batch, int64_t heads, int64_t seq_len, int64_t head_dim, float* dq, float* dk, float* dv, int64_t d_ld, int64_t d_so, int64_t d_si,
+                                 float* dbias /*opt*/, int accumulate_dbias, const float* dout, int64_t g_ld, int64_t g_so, int64_t g_si, const float* out, int64_t o_ld, int64_t o_so, int64_t o_si, const float* stats,
+                                 const float* q, int64_t q_ld, int64_t q_so, int64_t q_si, const float* k, int64_t k_ld, int64_t k_so, int64_t k_si,
+                                 const float* v, int64_t v_ld, int64_t v_so, int64_t v_si, float scale, int64_t window, int64_t sinks, const float* bias /*opt*/, int64_t buckets, const int64_t* bucket_starts);
+/* The same for one new position of every sequence: q and out hold one row a head, k and v (caches of cache_len rows a sequence) the
+ * positions so far, the new one's among them; lengths (device, n_seq) says how many those are, and the query is at the last of them.  A
+ * length of 0 gives zeros; one outside 0 .. cache_len is reported like an index outside its table, and gives zeros.  Rows beyond a sequence's length,
+ * and rows the rule hides, are not read. */
+GCB_API int gcb_window_attention_step_f32(gcb_ctx* ctx, int64_t n_seq, int64_t heads, int64_t head_dim, float* out, int64_t o_so, int64_t o_si, const float* q, int64_t q_so, int64_t q_si,
+                                 const float* k, int64_t k_ld, int64_t k_so, int64_t k_si, const float* v, int64_t v_ld, int64_t v_so, int64_t v_si, int64_t cache_len, const int64_t* lengths,
+                                 float scale, int64_t window, int64_t sinks, const float* bias /*opt*/, int64_t buckets, const int64_t* bucket_starts);
+/* First distances of relative position buckets (host memory in and out): the first half of them hold one distance each, the others grow by a constant
+ * factor, such that `reach` would start the one after the last.  Exact in whole numbers. */
+GCB_API int gcb_relative_bucket_starts(int64_t buckets, int64_t reach, int64_t* starts);
+
+/* Dropout with a mask that is drawn again wherever it is needed: element i takes word i % 4 of Philox4x32-10 at counter offset + i / 4
+ * under the key seed (both as unsigned numbers), and is dropped when that word is below p 2^32 (p in 0 .. 1); what is kept is divided by 1 - p.
+ * fwd: out = residual + dropout(x), residual optional; out may be x or residual.  bwd: dx (+)= the same mask and factor on dy.  A call uses up
+ * (n + 3) / 4 counters: the next one with the same seed continues at offset + (n + 3) / 4.  A dropped value is not looked at. */
+GCB_API int gcb_dropout_fwd_f32(gcb_ctx* ctx, float* out, const float* x, const float* residual /*opt*/, int64_t n, float p, int64_t seed, int64_t offset);
+GCB_API int gcb_dropout_bwd_f32(gcb_ctx* ctx, float* dx, const float* dy, int64_t n, float p, int64_t seed, int64_t offset, int accumulate);
+
 /* Pre-split weights (no counterpart in the reference: cuBLAS in TF32 mode rounds operands on the fly, kernels_math.cu:27-36).
  * The split-fp32 GEMM needs two BF16 companions of every operand tile; for the B operand they are normally derived inside the
  * kernel, by every CTA that uses the tile.  A dense rows x cols matrix registered here keeps them in global memory in tile
