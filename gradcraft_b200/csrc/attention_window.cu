@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(256) window_attention_fwd_kernel(const __grid_
 #pragma unroll
         for (int n = 0; n < NC; ++n)
             aw_st4<VEC>(out + row * p.o_ld, 64 * n + 4 * tx, D, make_float4(acc[i][4 * n] * inv, acc[i][4 * n + 1] * inv, acc[i][4 * n + 2] * inv, acc[i][4 * n + 3] * inv));
-        if (tx == 0) { p.row_max[head * p.Tp + row] = empty ? 0.0f : m[i]; p.row_inv[head * p.Tp + row] = inv; }
+        if (tx == 0) { p.row_max[head * p.Tp + row] = empty ? INFINITY : m[i]; p.row_inv[head * p.Tp + row] = inv; }
     }
 }
 
@@ -118,7 +118,7 @@ struct AwRows {
         for (int i = 0; i < R; ++i) {
             const int row = r0 + ty + 16 * i;
             const bool live = row < p.T;
-            m[i] = live ? p.row_max[head * p.Tp + row] : 0.0f;
+            m[i] = live ? p.row_max[head * p.Tp + row] : INFINITY;
             inv[i] = live ? p.row_inv[head * p.Tp + row] : 0.0f;
 #pragma unroll
             for (int n = 0; n < NC; ++n) y[i][n] = live ? aw_ld4<VEC>(o + row * p.o_ld, 64 * n + 4 * tx, p.D) : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -538,7 +538,8 @@ int gcb_window_attention_fwd_f32(gcb_ctx* ctx, int64_t B, int64_t H, int64_t T, 
     p.row_max = stats; p.row_inv = stats + B * H * p.Tp;
     p.tiles = (int)((T + AS_OWN - 1) / AS_OWN);
     const bool vec = D % 4 == 0 && vec_rows(q, q_ld, q_so, q_si) && vec_rows(k, k_ld, k_so, k_si) && vec_rows(v, v_ld, v_so, v_si) && vec_rows(out, o_ld, o_so, o_si);
-    rc = D <= 64 ? (vec ? fma_fwd<1, true>(ctx, B * H, p) : fma_fwd<1, false>(ctx, B * H, p)) : (vec ? fma_fwd<2, true>(ctx, B * H, p) : fma_fwd<2, false>(ctx, B * H, p));
+    if (window_tc_takes(ctx, B, p)) rc = window_tc_fwd(ctx, B, p);
+    else rc = D <= 64 ? (vec ? fma_fwd<1, true>(ctx, B * H, p) : fma_fwd<1, false>(ctx, B * H, p)) : (vec ? fma_fwd<2, true>(ctx, B * H, p) : fma_fwd<2, false>(ctx, B * H, p));
     if (rc) return rc;
     note_write(ctx, out, span_bytes(B, H, T, D, o_ld, o_so, o_si));
     return GCB_OK;
@@ -569,12 +570,15 @@ int gcb_window_attention_bwd_f32(gcb_ctx* ctx, int64_t B, int64_t H, int64_t T, 
     const int64_t Dp = (D + 3) / 4 * 4, heads = B * H;
     const bool vec = D % 4 == 0 && vec_rows(q, q_ld, q_so, q_si) && vec_rows(k, k_ld, k_so, k_si) && vec_rows(v, v_ld, v_so, v_si) && vec_rows(dout, g_ld, g_so, g_si) && vec_rows(out, o_ld, o_so, o_si) &&
                      vec_rows(dq, d_ld, d_so, d_si) && vec_rows(dk, d_ld, d_so, d_si) && vec_rows(dv, d_ld, d_so, d_si);
+    const bool tc = window_tc_takes(ctx, B, p);
+    const int tiles = tc ? (int)((T + AW_TC_TILE - 1) / AW_TC_TILE) : p.tiles;
     Scratch part(ctx), far(ctx);
     if (dbias) {
-        if ((rc = part.get(sizeof(float) * (size_t)(heads * p.tiles * buckets)))) return rc;
+        if ((rc = part.get(sizeof(float) * (size_t)(heads * tiles * buckets)))) return rc;
         p.dbias_part = part.as<float>();
     }
-    rc = D <= 64 ? (vec ? fma_bwd<1, true>(ctx, heads, p) : fma_bwd<1, false>(ctx, heads, p)) : (vec ? fma_bwd<2, true>(ctx, heads, p) : fma_bwd<2, false>(ctx, heads, p));
+    if (tc) rc = window_tc_bwd(ctx, B, p);
+    else rc = D <= 64 ? (vec ? fma_bwd<1, true>(ctx, heads, p) : fma_bwd<1, false>(ctx, heads, p)) : (vec ? fma_bwd<2, true>(ctx, heads, p) : fma_bwd<2, false>(ctx, heads, p));
     if (rc) return rc;
     if (p.rule.S > 0 && p.rule.W < T) {  // some query looks past its window
         p.far_chunks = (int)((T + AW_FAR - 1) / AW_FAR);
@@ -585,7 +589,7 @@ int gcb_window_attention_bwd_f32(gcb_ctx* ctx, int64_t B, int64_t H, int64_t T, 
     }
     for (float* d : {dq, dk, dv}) note_write(ctx, d, span_bytes(B, H, T, D, d_ld, d_so, d_si));
     if (dbias) {
-        GCB_CHECK_CUDA(launch_next(ctx->stream, dim3((unsigned)((H * buckets + 7) / 8)), 256, 0, window_attention_dbias_kernel, dbias, part.as<float>(), (int)H, (int)B, p.tiles, (int)buckets, accumulate_dbias));
+        GCB_CHECK_CUDA(launch_next(ctx->stream, dim3((unsigned)((H * buckets + 7) / 8)), 256, 0, window_attention_dbias_kernel, dbias, part.as<float>(), (int)H, (int)B, tiles, (int)buckets, accumulate_dbias));
         note_write(ctx, dbias, sizeof(float) * (size_t)(H * buckets));
         return after_launch(ctx, "window_attention_dbias");
     }

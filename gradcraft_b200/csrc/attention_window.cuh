@@ -45,12 +45,18 @@ inline int make_rule(WindowRule& r, const char* who, int64_t window, int64_t sin
 
 struct WindowAttn {
     const float *q, *k, *v, *g, *o;
-    float *out, *dq, *dk, *dv, *row_max, *row_inv;  // statistics: per query the maximum score and 1 / sum (0 where nothing is seen), Tp a head
+    float *out, *dq, *dk, *dv, *row_max, *row_inv;  // statistics: per query the maximum score and 1 / sum (infinity and 0 where nothing is seen: P is then 0 whatever a score is), Tp a head
     float *dbias_part, *far_part;                   // backward: partial sums, see the kernels that fill them
     int64_t q_ld, q_so, q_si, k_ld, k_so, k_si, v_ld, v_so, v_si, g_ld, g_so, g_si, o_ld, o_so, o_si, d_ld, d_so, d_si, Tp;
     int T, D, H, tiles, far_chunks;
     float scale;
     WindowRule rule;
 };
+
+// The kernels of attention_window_tc.cu.
+bool window_tc_takes(gcb_ctx* ctx, int64_t B, const WindowAttn& a);
+int window_tc_fwd(gcb_ctx* ctx, int64_t B, const WindowAttn& a);
+int window_tc_bwd(gcb_ctx* ctx, int64_t B, const WindowAttn& a);
+constexpr int AW_TC_TILE = 128;  // queries of a tile there
 
 }  // namespace gcb

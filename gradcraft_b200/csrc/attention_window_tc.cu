@@ -1,0 +1,975 @@
+// Attention under a visibility rule (attention_window.cuh) on tcgen05 / TMEM, in the split-fp32 arithmetic of the GEMMs, for heads of up to 64
+// columns: the forward, dK and dV of 128 keys, dQ and the bias gradient of 128 queries, one kernel each.  Nothing T x T goes through
+// memory, and blocks that the rule hides as a whole are not visited, so that a sequence costs T (window + sinks).
+// Reference counterpart: the causal form alone (frontend/tensor_other.hpp:53-93).
+//
+// Tiles, roles and the order of products are those of attention.cu, with these differences:
+//   - a unit's key blocks are the blocks of the first S keys and those of its window; the two query tiles of a forward CTA share the union;
+//   - scores are masked only in blocks that a border of the rule passes through, a test per warp;
+//   - a bias is read from a table by distance (one launch makes it, as long as the distances it tells apart), 191 entries a block through
+//     shared memory, beyond its last distance from a register;
+//   - a query may see nothing of a block that its tile visits: a maximum of -inf stands for "nothing yet" until the first key;
+//   - dQ is a kernel of its own that forms P and dS again (three products a block), because dS of a long sequence is too much memory: five
+//     products and T^2 floats there, seven products here.
+// The gradients of the first S keys from queries beyond the window are left to the FMA kernel of attention_window.cu: 128-key tiles would
+// spend T / 64 blocks on a handful of keys.
+// Every wait is bounded, as in the GEMM kernels.
+#include "attention_tc.cuh"
+#include "attention_window.cuh"
+
+namespace gcb {
+
+constexpr int WT_DIAG = AT_ROWS + AT_KEYS - 1;  // distances in a block of scores
+constexpr int WT_TAB = 192;                     // their place in shared memory, in floats
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct WindowTc {
+    int64_t q_ld, q_so, q_si, k_ld, k_so, k_si, v_ld, v_so, v_si, g_ld, g_so, g_si, o_ld, o_so, o_si, d_ld, d_so, d_si;
+    const float *q, *k, *v, *g, *o;
+    float *out, *dq, *dk, *dv, *row_max, *row_inv, *delta, *dbias_part;
+    const float* tab;  // [H][tab_len]: bias by distance, the last one for all distances beyond; NULL: no bias
+    int tab_len;
+    int64_t Tp;
+    float scale;
+    int T, D, H, heads, units, group, tiles_per_unit;
+    int64_t items, loop_end;
+    int* status;
+    WindowRule rule;
+};
+
+__global__ void __launch_bounds__(256) window_attention_table_kernel(float* __restrict__ tab, int len, const __grid_constant__ WindowRule r) {
+    pdl_trigger();
+    pdl_wait();
+    const int d = blockIdx.x * 256 + threadIdx.x, h = blockIdx.y;
+    if (d < len) tab[(int64_t)h * len + d] = r.bias[(int64_t)h * r.buckets + r.bucket(d)];
+}
+__device__ __forceinline__ int clamp_distance(int d, int len) { return max(0, min(d, len - 1)); }
+
+// The key blocks that a 128-query tile from row r0 looks at: 0 .. sinks - 1, then first .. last.  None where r0 lies beyond the sequence.
+struct TileKeys {
+    int sinks, first, last;
+    __device__ __forceinline__ TileKeys(const WindowTc& p, int r0) {
+        const bool there = r0 < p.T;
+        first = p.rule.window_first(r0) / AT_KEYS;
+        last = there ? (min(p.T, r0 + AT_ROWS) - 1) / AT_KEYS : -1;
+        sinks = there ? min((p.rule.S + AT_KEYS - 1) / AT_KEYS, first) : 0;
+    }
+    __device__ __forceinline__ int count() const { return last < 0 ? 0 : sinks + last - first + 1; }
+    __device__ __forceinline__ int block(int j) const { return j < sinks ? j : first + j - sinks; }
+    __device__ __forceinline__ bool has(int b) const { return b < sinks || (b >= first && b <= last); }
+    __device__ __forceinline__ int begin() const { return sinks > 0 ? 0 : first; }
+};
+__device__ __forceinline__ bool all_any(bool x) {  // barrier of the 512 threads of the query warps, with the or of their x
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 512, p;\n\tselp.b32 %0, 1, 0, q;\n\t}" : "=r"(r) : "r"((uint32_t)x) : "memory");
+    return r != 0;
+}
+// Keeps score e of a row (query i against key j0 + e) or hides it; `room` = i - j0.
+__device__ __forceinline__ bool keeps(int e, int room, int window_from, int sinks_to) { return e <= room && (e >= window_from || e < sinks_to); }
+
+// ---- forward ------------------------------------------------------------------------------------------------------------------
+// Tensor memory of query tile q, from column 256 q: scores / t of P [0, 64), bf16(P) [64, 96), bf16(P - t) [96, 128), O [128, 192), t of q [192, 256).
+template <int DP, bool BIAS>
+__global__ void __launch_bounds__(AT_FWD_THREADS, 1) window_attention_tc_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ WindowTc p) {
+    using S = AttnSmem<DP>;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
+    const uint32_t bars = base + S::BAR_OFF;
+    auto full = [&](int b) { return bars + 8u * b; };        // blocks k0 k1 v0 v1: landed
+    auto conv = [&](int b) { return bars + 8u * (4 + b); };  // companions written
+    auto empty = [&](int b) { return bars + 8u * (8 + b); }; // products have read it
+    auto s_full = [&](int q) { return bars + 8u * (12 + q); };
+    auto p_ready = [&](int q) { return bars + 8u * (14 + q); };
+    auto o_full = [&](int q) { return bars + 8u * (16 + q); };
+    auto q_ready = [&](int q) { return bars + 8u * (18 + q); };
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int b = 0; b < 4; ++b) { mbar_init(full(b), 1); mbar_init(conv(b), 4); mbar_init(empty(b), 1); }
+        for (int q = 0; q < 2; ++q) { mbar_init(s_full(q), 1); mbar_init(p_ready(q), 8); mbar_init(o_full(q), 1); mbar_init(q_ready(q), 8); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    const uint32_t tmem = tmem_take(bars + 8u * 20, reinterpret_cast<volatile uint32_t*>(gen + S::BAR_OFF + 8 * 20), warp);
+    pdl_trigger();
+    pdl_wait();
+    auto tile_row = [&](const AttnItem& it, int q) { return q < p.tiles_per_unit ? (it.unit * p.tiles_per_unit + q) * AT_ROWS : p.T; };
+    // both tiles' blocks: those of tile 0 up to the end of tile 1's (the second tile's window begins before the first one's ends)
+    struct Union {
+        TileKeys a, b;
+        int blocks;
+        __device__ __forceinline__ Union(const TileKeys& x, const TileKeys& y) : a(x), b(y), blocks(x.sinks + max(x.last, y.last) - x.first + 1) {}
+        __device__ __forceinline__ int block(int n) const { return a.block(n); }
+    };
+    auto slot = [&](int kind, uint32_t n) { return (int)(2 * kind + (n & 1u)); };  // kind 0: k, 1: v; n: running block number
+
+    if (warp < 4) regs_give<56>();
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t n = 0;
+            bool ok = true;
+            for (int64_t w = blockIdx.x; w < p.loop_end && ok; w += gridDim.x) {
+                const AttnItem it = attn_item(p, w, false);
+                if (it.skip) continue;
+                const Union u(TileKeys(p, tile_row(it, 0)), TileKeys(p, tile_row(it, 1)));
+                for (int j = 0; j < u.blocks && ok; ++j, ++n) {
+                    const uint32_t ph = ((n >> 1) & 1u) ^ 1u;
+                    const int kb = slot(0, n), vb = slot(1, n), r0 = u.block(j) * AT_KEYS;
+                    ok = mbar_wait(empty(kb), ph, p.status, 41);
+                    if (!ok) break;
+                    load_k_major<DP>(base + S::BLOCKS_OFF + kb * S::BLOCK, &map_k, full(kb), r0, it.h, it.b);
+                    ok = mbar_wait(empty(vb), ph, p.status, 41);
+                    if (!ok) break;
+                    load_mn_major<DP>(base + S::BLOCKS_OFF + vb * S::BLOCK, &map_v, full(vb), r0, it.h, it.b);
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (elect_one()) {
+            const uint32_t base16 = base >> 4;
+            uint32_t n = 0, q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
+            bool ok = true;
+            for (int64_t w = blockIdx.x; w < p.loop_end && ok; w += gridDim.x) {
+                const AttnItem it = attn_item(p, w, false);
+                if (it.skip) continue;
+                const Union u(TileKeys(p, tile_row(it, 0)), TileKeys(p, tile_row(it, 1)));
+                const int blocks = u.blocks;
+                auto scores = [&](int q, int j) {
+                    issue_scores<DP>(tmem + 256 * q, tmem + 256 * q + 192, base16 + q * (S::TWIN / 16), base16 + S::BLOCKS_OFF / 16 + slot(0, n + j) * (S::BLOCK / 16));
+                    umma_commit(s_full(q));
+                };
+                auto k_landed = [&](int j) {
+                    const bool r = mbar_wait(conv(slot(0, n + j)), ((n + j) >> 1) & 1u, p.status, 42);
+                    after_sync();
+                    return r;
+                };
+#pragma unroll
+                for (int q = 0; q < 2; ++q)
+                    if (ok && (q ? u.b : u.a).last >= 0) { ok = mbar_wait(q_ready(q), q_phase[q] & 1u, p.status, 43); ++q_phase[q]; }
+                if (ok) ok = k_landed(0);
+                if (!ok) break;
+#pragma unroll
+                for (int q = 0; q < 2; ++q)
+                    if ((q ? u.b : u.a).has(u.block(0))) scores(q, 0);
+                umma_commit(empty(slot(0, n)));
+                for (int j = 0; j < blocks && ok; ++j) {
+                    const int vb = slot(1, n + j), now = u.block(j), next = u.block(j + 1);
+                    const uint32_t v_raw = base16 + S::BLOCKS_OFF / 16 + vb * (S::BLOCK / 16);
+                    ok = mbar_wait(conv(vb), ((n + j) >> 1) & 1u, p.status, 44);
+                    bool k_here = false;
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        const TileKeys& t = q ? u.b : u.a;
+                        if (ok && t.has(now)) {
+                            ok = mbar_wait(p_ready(q), p_phase[q] & 1u, p.status, 45);
+                            ++p_phase[q];
+                            if (ok) {
+                                after_sync();
+                                const uint32_t t0 = tmem + 256 * q;
+                                issue_values<DP>(t0 + 128, t0, t0 + 64, t0 + 96, v_raw, now != t.begin());
+                                if (now == t.last) umma_commit(o_full(q));
+                            }
+                        }
+                        if (ok && j + 1 < blocks && t.has(next)) {
+                            if (!k_here) { ok = k_landed(j + 1); k_here = true; }
+                            if (ok) scores(q, j + 1);
+                        }
+                    }
+                    if (!ok) break;
+                    umma_commit(empty(vb));
+                    if (j + 1 < blocks) umma_commit(empty(slot(0, n + j + 1)));
+                }
+                n += blocks;
+            }
+        }
+    } else if (warp >= 4 && warp < 8) {
+        regs_give<72>();
+        const int t = threadIdx.x - 128;
+        uint32_t n = 0;
+        bool ok = true;
+        for (int64_t w = blockIdx.x; w < p.loop_end && ok; w += gridDim.x) {
+            const AttnItem it = attn_item(p, w, false);
+            if (it.skip) continue;
+            const Union u(TileKeys(p, tile_row(it, 0)), TileKeys(p, tile_row(it, 1)));
+            for (int j = 0; j < u.blocks && ok; ++j, ++n) {
+#pragma unroll
+                for (int kind = 0; kind < 2; ++kind) {
+                    const int b = slot(kind, n);
+                    ok = warp_wait(full(b), (n >> 1) & 1u, p.status, 46);
+                    if (!ok) break;
+                    uint8_t* raw = gen + S::BLOCKS_OFF + b * S::BLOCK;
+                    if (kind == 0) split_k_major<DP>(raw, t);
+                    else split_mn_major<DP>(raw, raw + S::RAW, t);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(conv(b));
+                }
+            }
+        }
+    } else if (warp >= 8) {
+        regs_take<88>();
+        // two threads a query: each has 32 of a block's 64 keys, and half of the columns of q and O
+        const int q = (warp - 8) >> 3, half = ((warp - 8) >> 2) & 1, row = 32 * (warp & 3) + lane, bar = 1 + q, at_tile = (threadIdx.x - 256) & 255;
+        const uint32_t t0 = tmem + 256 * q + ((uint32_t)(32 * (warp & 3)) << 16);
+        float* xch = reinterpret_cast<float*>(gen + S::STAGE_OFF) + q * 256;  // [half][row]
+        float* tabs = reinterpret_cast<float*>(gen + S::STAGE_OFF + 2048) + q * 2 * WT_TAB;
+        constexpr int OC = DP / 2;
+        const float c = BIAS ? kLog2e : p.scale * kLog2e;  // scores, or scores before the scale, to log2 units
+        uint32_t s_phase = 0, o_phase = 0;
+        bool ok = true;
+        for (int64_t w = blockIdx.x; w < p.loop_end && ok; w += gridDim.x) {
+            const AttnItem it = attn_item(p, w, false);
+            if (it.skip) continue;
+            const int r0 = tile_row(it, q);
+            const TileKeys keys(p, r0);
+            const int blocks = keys.count();
+            if (!blocks) continue;
+            const int r = r0 + row;
+            const bool live = r < p.T;
+            {
+                float x[OC];
+                load_row<DP / 32>(x, p.q + it.b * p.q_so + it.h * p.q_si + r * p.q_ld + half * OC, live, p.D - half * OC);
+                place_row<DP / 32>(x, t0 + 192 + half * OC, gen + q * S::TWIN + half * (OC / 16) * 8192, row);
+            }
+            tmem_stores_done();
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_ready(q));
+            // the bias of a block's 191 distances: requested a block ahead, in shared memory before the barrier of the block in front
+            const float* tab = BIAS ? p.tab + (int64_t)it.h * p.tab_len : nullptr;
+            const float beyond = BIAS ? __ldg(tab + p.tab_len - 1) : 0.0f;
+            auto distance = [&](int b) { return r0 - (b + 1) * AT_KEYS + 1; };  // the smallest one of a block
+            auto request = [&](int b) { return at_tile < WT_DIAG ? __ldg(tab + clamp_distance(distance(b) + at_tile, p.tab_len)) : 0.0f; };
+            if (BIAS) {
+                if (at_tile < WT_DIAG) tabs[at_tile] = request(keys.begin());
+                pair_sync(bar);
+            }
+            float m = -INFINITY, sum = 0.0f;  // m: the maximum the probabilities are relative to
+            bool good = true;
+            for (int j = 0; j < blocks; ++j) {
+                const int b = keys.block(j);
+                float ahead = 0.0f;
+                if (BIAS && j + 1 < blocks) ahead = request(keys.block(j + 1));
+                good = good && warp_wait(s_full(q), s_phase & 1u, p.status, 47);  // every thread keeps step with the barriers below, whatever a wait says
+                ++s_phase;
+                after_sync();
+                float v[32];
+                tmem_ld32(t0 + 32 * half, v);
+                const int j0 = b * AT_KEYS + 32 * half, room = r - j0;
+                if (BIAS) {
+                    if (distance(b) >= p.tab_len - 1) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) v[e] = fmaf(v[e], p.scale, beyond);
+                    } else {
+                        const float* mine = tabs + (j & 1) * WT_TAB + row - 32 * half + AT_KEYS - 1;
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) v[e] = fmaf(v[e], p.scale, mine[-e]);
+                    }
+                    if (j + 1 < blocks && at_tile < WT_DIAG) tabs[((j + 1) & 1) * WT_TAB + at_tile] = ahead;
+                }
+                // a border passes through where the warp's first query does not see its last key or its last query not the first one
+                if (room - lane < 31 || (p.rule.W > 0 && room - lane + 31 >= p.rule.W && j0 + 31 >= p.rule.S)) {
+                    const int from = p.rule.W > 0 ? room - p.rule.W + 1 : 0, to = p.rule.S - j0;
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) v[e] = keeps(e, room, from, to) ? v[e] : -INFINITY;
+                }
+                float mx = max32(v);
+                if (pair_any(bar, j == 0 || (mx - m) * c > 8.0f)) {  // almost only in the first block
+                    xch[half * 128 + row] = mx;
+                    pair_sync(bar);
+                    mx = fmaxf(mx, xch[(half ^ 1) * 128 + row]);
+                    if (j == 0) {
+                        m = mx;
+                    } else {  // O holds the previous blocks' sums: their products came before these scores
+                        const float f = mx > m ? ex2((m - mx) * c) : 1.0f;
+                        m = fmaxf(m, mx);
+                        sum *= f;
+#pragma unroll
+                        for (int g = 0; g < OC / 16; ++g) {
+                            uint32_t x[16];
+                            tmem_ld16(t0 + 128 + half * OC + 16 * g, x);
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * f);
+                            tmem_st16(t0 + 128 + half * OC + 16 * g, x);
+                        }
+                    }
+                    pair_sync(bar);  // both have read before either writes again
+                }
+                const float rel = m == -INFINITY ? 0.0f : m, m2 = rel * c;  // nothing seen yet: every score is -inf
+                float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                    v[e] = BIAS ? ex2((v[e] - rel) * c) : ex2(fmaf(v[e], c, -m2));  // a bias may be the type's lowest value, which log2 units cannot hold
+                    acc[e & 3] += v[e];
+                }
+                sum += (acc[0] + acc[1]) + (acc[2] + acc[3]);
+                place_parts(v, t0 + 32 * half, t0 + 64 + 16 * half, t0 + 96 + 16 * half);
+                tmem_stores_done();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_ready(q));
+            }
+            good = good && warp_wait(o_full(q), o_phase & 1u, p.status, 48);
+            ++o_phase;
+            after_sync();
+            xch[half * 128 + row] = sum;
+            ok = !pair_any(bar, !good);  // all of a tile's threads leave together
+            const bool empty_row = m == -INFINITY;
+            const float inv = empty_row ? 0.0f : 1.0f / (sum + xch[(half ^ 1) * 128 + row]);
+            pair_sync(bar);
+            if (!ok) break;
+            float* dst = p.out + it.b * p.o_so + it.h * p.o_si + r * p.o_ld;
+#pragma unroll
+            for (int g = 0; g < OC / 16; ++g) {
+                uint32_t x[16];
+                tmem_ld16(t0 + 128 + half * OC + 16 * g, x);
+                if (live)
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4)
+                        if (half * OC + 16 * g + e < p.D)
+                            st4(dst + half * OC + 16 * g + e, make_float4(__uint_as_float(x[e]) * inv, __uint_as_float(x[e + 1]) * inv, __uint_as_float(x[e + 2]) * inv, __uint_as_float(x[e + 3]) * inv));
+            }
+            if (half == 0 && live) {
+                const int64_t at = ((int64_t)it.b * p.H + it.h) * p.Tp + r;
+                p.row_max[at] = empty_row ? INFINITY : BIAS ? m : m * p.scale;
+                p.row_inv[at] = inv;
+            }
+        }
+    }
+    tmem_give(tmem, warp);
+}
+
+// ---- dK and dV ----------------------------------------------------------------------------------------------------------------
+// As the backward kernel of attention.cu: a thread owns a key and sixteen of a block's queries, everything transposed; queries from the
+// diagonal to the window's end.
+// Tensor memory: S^T / t of P^T [0, 64), dP^T / t of dS^T [64, 128), P^T companions [128, 192), dS^T companions [192, 256), dV [256, 320), dK [320, 384),
+// t of k [384, 448), t of v [448, 512).
+template <int DP, bool BIAS>
+__global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_kernel(const __grid_constant__ CUtensorMap map_qk, const __grid_constant__ CUtensorMap map_qn, const __grid_constant__ CUtensorMap map_ok,
+                                                                                const __grid_constant__ CUtensorMap map_on, const __grid_constant__ WindowTc p) {
+    using S = AttnSmem<DP>;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
+    const uint32_t bars = base + S::BAR_OFF;
+    enum { QK = 0, OK = 1, ON = 2, QN = 3 };  // blocks: q and dO K-major for the scores and dP, dO and q MN-major for dV and dK
+    auto full = [&](int b) { return bars + 8u * b; };
+    auto conv = [&](int b) { return bars + 8u * (4 + b); };
+    auto empty = [&](int b) { return bars + 8u * (8 + b); };
+    const uint32_t s_full = bars + 8u * 12, dp_full = bars + 8u * 13, p_ready = bars + 8u * 14, ds_ready = bars + 8u * 15, acc_full = bars + 8u * 16, kv_ready = bars + 8u * 17;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int b = 0; b < 4; ++b) { mbar_init(full(b), 1); mbar_init(conv(b), 4); mbar_init(empty(b), 1); }
+        mbar_init(s_full, 1); mbar_init(dp_full, 1); mbar_init(acc_full, 1);
+        mbar_init(p_ready, 16); mbar_init(ds_ready, 16); mbar_init(kv_ready, 16);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    const uint32_t tmem = tmem_take(bars + 8u * 20, reinterpret_cast<volatile uint32_t*>(gen + S::BAR_OFF + 8 * 20), warp);
+    pdl_trigger();
+    pdl_wait();
+    auto steps = [&](const AttnItem& it) {  // blocks of queries from the tile's first key to the last query that sees its last one
+        const int k0 = it.unit * AT_ROWS, k1 = min(p.T, k0 + AT_ROWS), end = p.rule.W > 0 && p.rule.W < p.T - k1 ? k1 - 1 + p.rule.W : p.T;
+        return (end - k0 + AT_KEYS - 1) / AT_KEYS;
+    };
+    // the order in which blocks are loaded, split and used within an item of n steps
+    auto sequence = [&](int n, auto&& f) -> bool {
+        if (!f((int)QK, 0) || !f((int)OK, 0)) return false;
+        for (int i = 0; i < n; ++i) {
+            if (!f((int)ON, i)) return false;
+            if (i + 1 < n && !f((int)QK, i + 1)) return false;
+            if (!f((int)QN, i)) return false;
+            if (i + 1 < n && !f((int)OK, i + 1)) return false;
+        }
+        return true;
+    };
+    float* tabs = reinterpret_cast<float*>(gen + S::STAGE_OFF);  // bias of a block's distances, two blocks
+
+    if (warp < 4) regs_give<64>();
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t n0 = 0;
+            bool ok = true;
+            for (int64_t w = blockIdx.x; w < p.loop_end && ok; w += gridDim.x) {
+                const AttnItem it = attn_item(p, w, true);
+                if (it.skip) continue;
+                const int n = steps(it);
+                ok = sequence(n, [&](int b, int i) {
+                    if (!mbar_wait(empty(b), ((n0 + i) & 1u) ^ 1u, p.status, 51)) return false;
+                    const uint32_t dst = base + S::BLOCKS_OFF + b * S::BLOCK;
+                    const int r0 = it.unit * AT_ROWS + i * AT_KEYS;
+                    if (b == QK) load_k_major<DP>(dst, &map_qk, full(b), r0, it.h, it.b);
+                    else if (b == OK) load_k_major<DP>(dst, &map_ok, full(b), r0, it.h, it.b);
+                    else load_mn_major<DP>(dst, b == ON ? &map_on : &map_qn, full(b), r0, it.h, it.b);
+                    return true;
+                });
+                n0 += n;
+            }
+        }
+    } else if (warp == 1) {
+        if (elect_one()) {
+            const uint32_t base16 = base >> 4;
+            uint32_t n0 = 0, items = 0;
+            bool ok = true;
+            for (int64_t w = blockIdx.x; w < p.loop_end && ok; w += gridDim.x, ++items) {
+                const AttnItem it = attn_item(p, w, true);
+                if (it.skip) break;  // only the last round has items left out
+                const int n = steps(it);
+                auto landed = [&](int b, int i) {
+                    const bool r = mbar_wait(conv(b), (n0 + i) & 1u, p.status, 52);
+                    after_sync();
+                    return r;
+                };
+                ok = mbar_wait(kv_ready, items & 1u, p.status, 53);
+                if (!ok) break;
+                ok = sequence(n, [&](int b, int i) {
+                    const uint32_t blk = base16 + S::BLOCKS_OFF / 16 + b * (S::BLOCK / 16), ph = (n0 + i) & 1u;
+                    if (b == ON && !mbar_wait(p_ready, ph, p.status, 54)) return false;
+                    if (b == QN && !mbar_wait(ds_ready, ph, p.status, 55)) return false;
+                    if (!landed(b, i)) return false;
+                    if (b == QK) issue_scores<DP>(tmem, tmem + 384, base16, blk);
+                    else if (b == OK) issue_scores<DP>(tmem + 64, tmem + 448, base16 + S::TWIN / 16, blk);
+                    else if (b == ON) issue_values<DP>(tmem + 256, tmem, tmem + 128, tmem + 160, blk, i > 0);
+                    else issue_values<DP>(tmem + 320, tmem + 64, tmem + 192, tmem + 224, blk, i > 0);
+                    umma_commit(empty(b));
+                    if (b == QK) umma_commit(s_full);
+                    else if (b == OK) umma_commit(dp_full);
+                    return true;
+                });
+                if (!ok) break;
+                umma_commit(acc_full);
+                n0 += n;
+            }
+        }
+    } else if (warp >= 4 && warp < 12) {
+        regs_give<56>();
+        // warps 4..7: the K-major blocks, the query statistics and the bias; warps 8..11: the MN-major blocks
+        const int t = threadIdx.x & 127;
+        const bool k_major = warp < 8;
+        float* stats_sm = reinterpret_cast<float*>(gen + S::STATS_OFF);
+        uint32_t n0 = 0;
+        bool ok = true;
+        for (int64_t w = blockIdx.x; w < p.loop_end && ok; w += gridDim.x) {
+            const AttnItem it = attn_item(p, w, true);
+            if (it.skip) continue;
+            const int n = steps(it), q_at = it.unit * AT_ROWS + t;
+            const int64_t at = ((int64_t)it.b * p.H + it.h) * p.Tp;
+            const float* tab = BIAS ? p.tab + (int64_t)it.h * p.tab_len : nullptr;
+            float nm = 0.f, ni = 0.f, nd = 0.f, nb0 = 0.f, nb1 = 0.f;  // the next block's, loaded a block ahead
+            const bool mine = k_major && t < AT_KEYS;
+            // statistics of queries beyond the sequence are not there: P is then zero
+            auto stats = [&](int i) {
+                const int q = q_at + i * AT_KEYS;
+                const bool live = mine && q < p.T;
+                nm = live ? __ldg(p.row_max + at + q) : INFINITY;
+                ni = live ? __ldg(p.row_inv + at + q) : 0.0f;
+            };
+            auto term = [&](int i) { nd = mine && q_at + i * AT_KEYS < p.T ? __ldg(p.delta + at + q_at + i * AT_KEYS) : 0.0f; };
+            auto bias = [&](int i) {
+                if (!BIAS || !k_major) return;
+                const int d0 = i * AT_KEYS - (AT_ROWS - 1);
+                nb0 = __ldg(tab + clamp_distance(d0 + t, p.tab_len));
+                nb1 = __ldg(tab + clamp_distance(d0 + t + 128, p.tab_len));
+            };
+            stats(0); term(0); bias(0);
+            ok = sequence(n, [&](int b, int i) {
+                if (k_major != (b <= OK)) return true;
+                if (!warp_wait(full(b), (n0 + i) & 1u, p.status, 56)) return false;
+                uint8_t* raw = gen + S::BLOCKS_OFF + b * S::BLOCK;
+                // Two slots, by the running number of the block: the one before last has been used (its products preceded the last one's, which
+                // this block's copy waited for), also where the last one belongs to the item before.
+                if (k_major) {
+                    float* slot = stats_sm + ((n0 + i) & 1u) * 3 * AT_KEYS + t;
+                    if (b == QK) {
+                        if (mine) { slot[0] = BIAS ? nm : nm * kLog2e; slot[AT_KEYS] = ni; }
+                        if (BIAS) {
+                            float* tb = tabs + ((n0 + i) & 1u) * WT_TAB + t;
+                            tb[0] = nb0;
+                            if (t < WT_TAB - 128) tb[128] = nb1;
+                        }
+                        if (i + 1 < n) { stats(i + 1); bias(i + 1); }
+                    } else {
+                        if (mine) slot[2 * AT_KEYS] = nd;
+                        if (i + 1 < n) term(i + 1);
+                    }
+                }
+                if (k_major) split_k_major<DP>(raw, t);
+                else split_mn_major<DP>(raw, raw + S::RAW, t);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(conv(b));
+                return true;
+            });
+            n0 += n;
+        }
+    } else if (warp >= 12) {
+        regs_take<80>();
+        const int part = (warp - 12) >> 2, row = 32 * (warp & 3) + lane;  // this warp: 32 keys x 16 of the block's 64 queries
+        constexpr int OC = DP / 2;                                       // and half of the columns of k (parts 0, 1) or v (2, 3)
+        const int half = part & 1;
+        const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+        const float c = p.scale * kLog2e;
+        uint32_t n = 0, items = 0;
+        bool ok = true;
+        for (int64_t w = blockIdx.x; w < p.loop_end && ok; w += gridDim.x, ++items) {
+            const AttnItem it = attn_item(p, w, true);
+            if (it.skip) break;
+            const int key = it.unit * AT_ROWS + row;
+            const bool live = key < p.T;
+            {
+                float x[OC];
+                load_row<DP / 32>(x, (part < 2 ? p.k + it.b * p.k_so + it.h * p.k_si + key * p.k_ld : p.v + it.b * p.v_so + it.h * p.v_si + key * p.v_ld) + half * OC, live, p.D - half * OC);
+                place_row<DP / 32>(x, lanes + (part < 2 ? 384 : 448) + half * OC, gen + (part >> 1) * S::TWIN + half * (OC / 16) * 8192, row);
+            }
+            tmem_stores_done();
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(kv_ready);
+            const int cnt = steps(it);
+#pragma unroll 1
+            for (int i = 0; i < cnt; ++i, ++n) {
+                const float4* mp = reinterpret_cast<const float4*>(gen + S::STATS_OFF + (n & 1u) * 3 * AT_KEYS * 4) + 4 * part;
+                const float4 *ip = mp + AT_KEYS / 4, *dp = ip + AT_KEYS / 4;
+                ok = warp_wait(s_full, n & 1u, p.status, 57);
+                if (!ok) break;
+                after_sync();
+                uint32_t u[16];
+                float pr[16];
+                tmem_ld16(lanes + 16 * part, u);
+                const int first = row - i * AT_KEYS - 16 * part;  // queries from here on look at this key, as many as the window is long
+                const float* bias = tabs + (n & 1u) * WT_TAB + (AT_ROWS - 1) + 16 * part - row;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float4 m = mp[e], iv = ip[e];
+                    const float mm[4] = {m.x, m.y, m.z, m.w}, ii[4] = {iv.x, iv.y, iv.z, iv.w};
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const float s = __uint_as_float(u[4 * e + x]);
+                        pr[4 * e + x] = (BIAS ? ex2((fmaf(s, p.scale, bias[4 * e + x]) - mm[x]) * kLog2e) : ex2(fmaf(s, c, -mm[x]))) * ii[x];
+                    }
+                }
+                if (i < 2 || (p.rule.W > 0 && (i + 1) * AT_KEYS > p.rule.W)) {  // the diagonal block, and those the window ends in
+                    const int end = p.rule.W > 0 ? min(16, first + p.rule.W) : 16;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) pr[e] = e >= first && e < end ? pr[e] : 0.0f;
+                }
+                place_parts16(pr, lanes + 16 * part, lanes + 128 + 8 * part, lanes + 160 + 8 * part);
+                tmem_stores_done();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_ready);
+                ok = warp_wait(dp_full, n & 1u, p.status, 58);
+                if (!ok) break;
+                after_sync();
+                tmem_ld16(lanes + 64 + 16 * part, u);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {  // dS = scale P (dP - dO . O); a masked P is zero whatever dP holds
+                    const float4 d = dp[e];
+                    const float dd[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) pr[4 * e + x] = pr[4 * e + x] * p.scale * (__uint_as_float(u[4 * e + x]) - dd[x]);
+                }
+                place_parts16(pr, lanes + 64 + 16 * part, lanes + 192 + 8 * part, lanes + 224 + 8 * part);
+                tmem_stores_done();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(ds_ready);
+            }
+            if (!ok) break;
+            ok = warp_wait(acc_full, items & 1u, p.status, 59);
+            if (!ok) break;
+            after_sync();
+            float* dst = (part < 2 ? p.dk : p.dv) + it.b * p.d_so + it.h * p.d_si + key * p.d_ld + half * OC;
+#pragma unroll
+            for (int g = 0; g < OC / 16; ++g) {
+                uint32_t x[16];
+                tmem_ld16(lanes + (part < 2 ? 320 : 256) + half * OC + 16 * g, x);
+                if (live)
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4)
+                        if (half * OC + 16 * g + e < p.D) st4(dst + 16 * g + e, make_float4(__uint_as_float(x[e]), __uint_as_float(x[e + 1]), __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3])));
+            }
+        }
+    }
+    tmem_give(tmem, warp);
+}
+
+// ---- dQ and the bias gradient ---------------------------------------------------------------------------------------------------
+// A CTA takes 128 queries and walks over their keys: S = q k^T and dP = dO v^T of one block while dQ += dS k of the block before passes.  Four
+// threads a query, sixteen of a block's keys each.  dO . O is formed here, from the rows that are loaded anyway, and kept for dK.
+// Scores and dP alternate between two places, x = 0 and 1; dS takes the place of both, a thread's columns where it has read them.
+// Tensor memory: S / companions of dS [128 x, + 64) (of 16 keys: 8 columns bf16(dS), 8 bf16(dS - t)), dP / t of dS [128 x + 64, + 64), dQ [256, 320), t of q [320, 384), t of dO [384, 448).
+// Bias gradient: a warp adds up the dS of its 32 x 16 block along the diagonals, 47 of them, through shared memory, and lane n those
+// that belong to buckets n and n + 32; a block that lies in one bucket as a whole is added up row by row in registers instead.
+template <int DP, bool BIAS>
+__global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kernel(const __grid_constant__ CUtensorMap map_kk, const __grid_constant__ CUtensorMap map_vk, const __grid_constant__ CUtensorMap map_kn,
+                                                                               const __grid_constant__ WindowTc p) {
+    using S = AttnSmem<DP>;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
+    const uint32_t bars = base + S::BAR_OFF;
+    enum { KK = 0, VK = 1, KN = 2 };  // blocks: k and v K-major for the scores and dP, k MN-major for dQ
+    constexpr int DIAG_OFF = S::BLOCKS_OFF + 3 * S::BLOCK, DIAG_WARP = 32 * 17 * 4;  // the fourth block's place and the staging area behind it
+    static_assert(DIAG_OFF + 16 * DIAG_WARP + 3 * WT_TAB * 4 + (16 * AW_MAX_BUCKETS + 2 * AT_ROWS) * 4 <= S::BAR_OFF, "shared memory");
+    auto full = [&](int b) { return bars + 8u * b; };
+    auto conv = [&](int b) { return bars + 8u * (3 + b); };
+    auto empty = [&](int b) { return bars + 8u * (6 + b); };
+    auto s_full = [&](uint32_t n) { return bars + 8u * (9 + (n & 1u)); };
+    auto dp_full = [&](uint32_t n) { return bars + 8u * (11 + (n & 1u)); };
+    auto ds_ready = [&](uint32_t n) { return bars + 8u * (13 + (n & 1u)); };
+    const uint32_t acc_full = bars + 8u * 15, q_ready = bars + 8u * 16;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int b = 0; b < 3; ++b) { mbar_init(full(b), 1); mbar_init(conv(b), 4); mbar_init(empty(b), 1); }
+        for (int x = 0; x < 2; ++x) { mbar_init(s_full(x), 1); mbar_init(dp_full(x), 1); mbar_init(ds_ready(x), 16); }
+        mbar_init(acc_full, 1); mbar_init(q_ready, 16);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    const uint32_t tmem = tmem_take(bars + 8u * 20, reinterpret_cast<volatile uint32_t*>(gen + S::BAR_OFF + 8 * 20), warp);
+    pdl_trigger();
+    pdl_wait();
+    // the order in which blocks are loaded, split and used within an item of n steps
+    auto sequence = [&](int n, auto&& f) -> bool {
+        if (!f((int)KK, 0) || !f((int)VK, 0)) return false;
+        for (int i = 0; i < n; ++i) {
+            if (i + 1 < n && (!f((int)KK, i + 1) || !f((int)VK, i + 1))) return false;
+            if (!f((int)KN, i)) return false;
+        }
+        return true;
+    };
+    float* tabs = reinterpret_cast<float*>(gen + DIAG_OFF + 16 * DIAG_WARP);  // bias of a block's distances, three blocks
+    float* sums = tabs + 3 * WT_TAB;                                          // [warp][bucket] at an item's end
+    float* xch = sums + 16 * AW_MAX_BUCKETS;                                  // [half][row]: dO . O
+
+    if (warp < 4) regs_give<64>();
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t n0 = 0;
+            bool ok = true;
+            for (int64_t w = blockIdx.x; w < p.loop_end && ok; w += gridDim.x) {
+                const AttnItem it = attn_item(p, w, false);
+                if (it.skip) continue;
+                const TileKeys keys(p, it.unit * AT_ROWS);
+                ok = sequence(keys.count(), [&](int b, int i) {
+                    if (!mbar_wait(empty(b), ((n0 + i) & 1u) ^ 1u, p.status, 61)) return false;
+                    const uint32_t dst = base + S::BLOCKS_OFF + b * S::BLOCK;
+                    const int r0 = keys.block(i) * AT_KEYS;
+                    if (b == KN) load_mn_major<DP>(dst, &map_kn, full(b), r0, it.h, it.b);
+                    else load_k_major<DP>(dst, b == KK ? &map_kk : &map_vk, full(b), r0, it.h, it.b);
+                    return true;
+                });
+                n0 += keys.count();
+            }
+        }
+    } else if (warp == 1) {
+        if (elect_one()) {
+            const uint32_t base16 = base >> 4;
+            uint32_t n0 = 0, items = 0;
+            bool ok = true;
+            for (int64_t w = blockIdx.x; w < p.loop_end && ok; w += gridDim.x, ++items) {
+                const AttnItem it = attn_item(p, w, false);
+                if (it.skip) break;  // only the last round has items left out
+                const int n = TileKeys(p, it.unit * AT_ROWS).count();
+                ok = mbar_wait(q_ready, items & 1u, p.status, 62);
+                if (!ok) break;
+                ok = sequence(n, [&](int b, int i) {
+                    const uint32_t blk = base16 + S::BLOCKS_OFF / 16 + b * (S::BLOCK / 16), at = n0 + i, place = tmem + 128 * (at & 1u);
+                    if (b == KN && !mbar_wait(ds_ready(at), (at >> 1) & 1u, p.status, 63)) return false;
+                    if (!mbar_wait(conv(b), at & 1u, p.status, 64)) return false;
+                    after_sync();
+                    if (b == KK) issue_scores<DP>(place, tmem + 320, base16, blk);
+                    else if (b == VK) issue_scores<DP>(place + 64, tmem + 384, base16 + S::TWIN / 16, blk);
+                    else issue_values<DP, 16>(tmem + 256, place + 64, place, place + 8, blk, i > 0);
+                    umma_commit(empty(b));
+                    if (b == KK) umma_commit(s_full(at));
+                    else if (b == VK) umma_commit(dp_full(at));
+                    return true;
+                });
+                if (!ok) break;
+                umma_commit(acc_full);
+                n0 += n;
+            }
+        }
+    } else if (warp >= 4 && warp < 12) {
+        regs_give<56>();
+        // warps 4..7: the K-major blocks and the bias; warps 8..11: the MN-major blocks
+        const int t = threadIdx.x & 127;
+        const bool k_major = warp < 8;
+        uint32_t n0 = 0;
+        bool ok = true;
+        for (int64_t w = blockIdx.x; w < p.loop_end && ok; w += gridDim.x) {
+            const AttnItem it = attn_item(p, w, false);
+            if (it.skip) continue;
+            const TileKeys keys(p, it.unit * AT_ROWS);
+            const int n = keys.count();
+            const float* tab = BIAS ? p.tab + (int64_t)it.h * p.tab_len : nullptr;
+            float nb0 = 0.f, nb1 = 0.f;  // the next block's, loaded a block ahead
+            auto bias = [&](int i) {
+                if (!BIAS || !k_major) return;
+                const int d0 = it.unit * AT_ROWS - (keys.block(i) + 1) * AT_KEYS + 1;
+                nb0 = __ldg(tab + clamp_distance(d0 + t, p.tab_len));
+                nb1 = __ldg(tab + clamp_distance(d0 + t + 128, p.tab_len));
+            };
+            bias(0);
+            ok = sequence(n, [&](int b, int i) {
+                if (k_major != (b <= VK)) return true;
+                if (!warp_wait(full(b), (n0 + i) & 1u, p.status, 65)) return false;
+                if (BIAS && b == KK) {
+                    // Three slots, by the running number of the block: this copy waited for the scores of the last block, which were asked for after
+                    // the dS of the third last had been made.
+                    float* tb = tabs + (n0 + i) % 3u * WT_TAB + t;
+                    tb[0] = nb0;
+                    if (t < WT_TAB - 128) tb[128] = nb1;
+                    if (i + 1 < n) bias(i + 1);
+                }
+                uint8_t* raw = gen + S::BLOCKS_OFF + b * S::BLOCK;
+                if (k_major) split_k_major<DP>(raw, t);
+                else split_mn_major<DP>(raw, raw + S::RAW, t);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(conv(b));
+                return true;
+            });
+            n0 += n;
+        }
+    } else if (warp >= 12) {
+        regs_take<80>();
+        const int part = (warp - 12) >> 2, row = 32 * (warp & 3) + lane;  // this warp: 32 queries x 16 of the block's 64 keys
+        constexpr int OC = DP / 2;                                       // and half of the columns of q (parts 0, 1) or dO (2, 3)
+        const int half = part & 1;
+        const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+        float* diag = reinterpret_cast<float*>(gen + DIAG_OFF + (warp - 12) * DIAG_WARP);
+        const float c = p.scale * kLog2e;
+        const bool wants_dbias = BIAS && p.dbias_part != nullptr;
+        uint32_t n = 0, items = 0;
+        bool good = true;
+        for (int64_t w = blockIdx.x; w < p.loop_end; w += gridDim.x, ++items) {
+            const AttnItem it = attn_item(p, w, false);
+            if (it.skip) break;
+            const int r0 = it.unit * AT_ROWS, r = r0 + row;
+            const bool live = r < p.T;
+            const int64_t at = ((int64_t)it.b * p.H + it.h) * p.Tp + r;
+            {
+                float x[OC];
+                load_row<DP / 32>(x, (part < 2 ? p.q + it.b * p.q_so + it.h * p.q_si + r * p.q_ld : p.g + it.b * p.g_so + it.h * p.g_si + r * p.g_ld) + half * OC, live, p.D - half * OC);
+                place_row<DP / 32>(x, lanes + (part < 2 ? 320 : 384) + half * OC, gen + (part >> 1) * S::TWIN + half * (OC / 16) * 8192, row);
+                if (part >= 2) {
+                    float a = 0.0f;
+                    const float* o = p.o + it.b * p.o_so + it.h * p.o_si + r * p.o_ld + half * OC;
+#pragma unroll
+                    for (int e = 0; e < OC; e += 4)
+                        if (live && half * OC + e < p.D) { const float4 y = ld4(o + e); a = fmaf(x[e], y.x, fmaf(x[e + 1], y.y, fmaf(x[e + 2], y.z, fmaf(x[e + 3], y.w, a)))); }
+                    xch[half * AT_ROWS + row] = a;
+                }
+            }
+            tmem_stores_done();
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_ready);
+            all_any(false);
+            const float delta = xch[row] + xch[AT_ROWS + row];
+            if (part == 0 && live) p.delta[at] = delta;
+            const float inv = live ? p.row_inv[at] : 0.0f, m = live ? p.row_max[at] * (BIAS ? 1.0f : kLog2e) : INFINITY;
+            const float* tab = BIAS ? p.tab + (int64_t)it.h * p.tab_len : nullptr;
+            const float beyond = BIAS ? __ldg(tab + p.tab_len - 1) : 0.0f;
+            const TileKeys keys(p, r0);
+            const int cnt = keys.count();
+            // bias gradient: this lane's buckets, and what belongs to bucket `run_of` as a whole; buckets only go down along the walk
+            float sum0 = 0.0f, sum1 = 0.0f, run = 0.0f;
+            int run_of = p.rule.buckets - 1, near_of = run_of, far_of = run_of;
+            auto settle = [&]() {
+                const float a = warp_sum(run);
+                if (lane == (run_of & 31)) { if (run_of < 32) sum0 += a; else sum1 += a; }
+                run = 0.0f;
+            };
+#pragma unroll 1
+            for (int i = 0; i < cnt; ++i, ++n) {
+                const uint32_t place = lanes + 128 * (n & 1u);
+                const int b = keys.block(i), j0 = b * AT_KEYS + 16 * part, room = r - j0;
+                good = good && warp_wait(s_full(n), (n >> 1) & 1u, p.status, 66);  // every thread keeps step with the barriers of the items, whatever a wait says
+                after_sync();
+                uint32_t u[16];
+                float pr[16];
+                tmem_ld16(place + 16 * part, u);
+                if (BIAS) {
+                    if (r0 - (b + 1) * AT_KEYS + 1 >= p.tab_len - 1) {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) pr[e] = ex2((fmaf(__uint_as_float(u[e]), p.scale, beyond) - m) * kLog2e) * inv;
+                    } else {
+                        const float* mine = tabs + n % 3u * WT_TAB + row - 16 * part + AT_KEYS - 1;
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) pr[e] = ex2((fmaf(__uint_as_float(u[e]), p.scale, mine[-e]) - m) * kLog2e) * inv;
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) pr[e] = ex2(fmaf(__uint_as_float(u[e]), c, -m)) * inv;
+                }
+                if (room - lane < 15 || (p.rule.W > 0 && room - lane + 31 >= p.rule.W && j0 + 15 >= p.rule.S)) {
+                    const int from = p.rule.W > 0 ? room - p.rule.W + 1 : 0, to = p.rule.S - j0;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) pr[e] = keeps(e, room, from, to) ? pr[e] : 0.0f;
+                }
+                good = good && warp_wait(dp_full(n), (n >> 1) & 1u, p.status, 67);
+                after_sync();
+                tmem_ld16(place + 64 + 16 * part, u);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) pr[e] *= __uint_as_float(u[e]) - delta;  // a masked P is zero whatever dP holds
+                place_parts16(pr, place + 64 + 16 * part, place + 16 * part, place + 16 * part + 8);
+                tmem_stores_done();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(ds_ready(n));
+                const int d1 = room - lane + 31, d0 = room - lane - 15;  // largest and smallest distance of the warp's 32 x 16 block
+                if (wants_dbias && d1 >= 0) {
+                    while (p.rule.starts[far_of] > d1) --far_of;
+                    while (p.rule.starts[near_of] > max(d0, 0)) --near_of;
+                    if (near_of == far_of) {
+                        if (run_of != near_of) { settle(); run_of = near_of; }
+                        float a[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) a[e & 3] += pr[e];
+                        run += (a[0] + a[1]) + (a[2] + a[3]);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) diag[lane * 17 + e] = pr[e];
+                        __syncwarp();
+                        float a = 0.0f, a2 = 0.0f;  // diagonals `lane` and `lane` + 32: distances d0 + lane, d0 + lane + 32
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const int l = lane - 15 + e;
+                            if (l >= 0) a += diag[(l & 31) * 17 + e];
+                            if (l + 32 < 32) a2 += diag[((l + 32) & 31) * 17 + e];
+                        }
+                        __syncwarp();
+                        diag[lane] = a;
+                        diag[32 + lane] = a2;
+                        __syncwarp();
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            const int bucket = lane + 32 * k;
+                            if (bucket > far_of || bucket < near_of) continue;
+                            const int from = max(0, p.rule.starts[bucket] - d0), to = bucket + 1 < p.rule.buckets ? min(47, p.rule.starts[bucket + 1] - d0) : 47;
+                            float t = 0.0f;
+                            for (int x = from; x < to; ++x) t += diag[x];
+                            (k ? sum1 : sum0) += t;
+                        }
+                        __syncwarp();
+                    }
+                }
+            }
+            good = good && warp_wait(acc_full, items & 1u, p.status, 68);
+            after_sync();
+            if (wants_dbias) {
+                settle();
+                sums[(warp - 12) * AW_MAX_BUCKETS + lane] = sum0;
+                sums[(warp - 12) * AW_MAX_BUCKETS + 32 + lane] = sum1;
+            }
+            if (all_any(!good)) break;  // all of them leave together
+            const int t = threadIdx.x - 384;
+            if (wants_dbias && t < p.rule.buckets) {
+                float a = 0.0f;
+#pragma unroll
+                for (int x = 0; x < 16; ++x) a += sums[x * AW_MAX_BUCKETS + t];
+                p.dbias_part[(((int64_t)it.b * p.H + it.h) * p.units + it.unit) * p.rule.buckets + t] = a;
+            }
+            if (16 * part < DP) {
+                float* dst = p.dq + it.b * p.d_so + it.h * p.d_si + r * p.d_ld + 16 * part;
+                uint32_t x[16];
+                tmem_ld16(lanes + 256 + 16 * part, x);
+                if (live)
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4)
+                        if (16 * part + e < p.D)
+                            st4(dst + e, make_float4(p.scale * __uint_as_float(x[e]), p.scale * __uint_as_float(x[e + 1]), p.scale * __uint_as_float(x[e + 2]), p.scale * __uint_as_float(x[e + 3])));
+            }
+        }
+    }
+    tmem_give(tmem, warp);
+}
+
+// ---- host side ----------------------------------------------------------------------------------------------------------------
+static WindowTc operands(gcb_ctx* ctx, int64_t B, const WindowAttn& a, int tiles_per_unit) {
+    WindowTc p = {};
+    p.q = a.q; p.q_ld = a.q_ld; p.q_so = a.q_so; p.q_si = a.q_si;
+    p.k = a.k; p.k_ld = a.k_ld; p.k_so = a.k_so; p.k_si = a.k_si;
+    p.v = a.v; p.v_ld = a.v_ld; p.v_so = a.v_so; p.v_si = a.v_si;
+    p.g = a.g; p.g_ld = a.g_ld; p.g_so = a.g_so; p.g_si = a.g_si;
+    p.o = a.o; p.o_ld = a.o_ld; p.o_so = a.o_so; p.o_si = a.o_si;
+    p.dq = a.dq; p.dk = a.dk; p.dv = a.dv; p.d_ld = a.d_ld; p.d_so = a.d_so; p.d_si = a.d_si;
+    p.out = a.out; p.row_max = a.row_max; p.row_inv = a.row_inv; p.dbias_part = a.dbias_part;
+    p.scale = a.scale; p.T = a.T; p.D = a.D; p.rule = a.rule; p.status = ctx->d_status;
+    plan(p, B, a.H, a.T, tiles_per_unit);
+    return p;
+}
+// The bias by distance of every head, up to the first distance of the last bucket.
+static int make_table(gcb_ctx* ctx, WindowTc& p, Scratch& mem) {
+    if (p.rule.bias == nullptr) return GCB_OK;
+    p.tab_len = std::min(p.T, p.rule.starts[p.rule.buckets - 1] + 1);
+    const int rc = mem.get(sizeof(float) * (size_t)p.H * p.tab_len);
+    if (rc) return rc;
+    p.tab = mem.as<float>();
+    GCB_CHECK_CUDA(launch_next(ctx->stream, dim3((unsigned)((p.tab_len + 255) / 256), (unsigned)p.H), 256, 0, window_attention_table_kernel, mem.as<float>(), p.tab_len, p.rule));
+    return after_launch(ctx, "window_attention_table");
+}
+template <class K, class... Maps>
+static int tc_launch(gcb_ctx* ctx, K kernel, bool* done, unsigned threads, size_t smem, const WindowTc& p, const Maps&... maps) {
+    if (!done[ctx->device]) { GCB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)); done[ctx->device] = true; }
+    GCB_CHECK_CUDA(launch_chained(ctx->stream, dim3((unsigned)std::min<int64_t>(p.items, kSMs)), threads, smem, kernel, maps..., p));
+    return GCB_OK;
+}
+template <int DP, bool BIAS>
+static int run_fwd(gcb_ctx* ctx, const WindowTc& p, const CUtensorMap& k, const CUtensorMap& v) {
+    static bool done[kMaxDevices] = {};
+    return tc_launch(ctx, window_attention_tc_fwd_kernel<DP, BIAS>, done, AT_FWD_THREADS, AttnSmem<DP>::TOTAL, p, k, v);
+}
+template <int DP, bool BIAS>
+static int run_bwd(gcb_ctx* ctx, const WindowTc& p, const CUtensorMap& kk, const CUtensorMap& vk, const CUtensorMap& kn, const CUtensorMap& qk, const CUtensorMap& qn, const CUtensorMap& ok, const CUtensorMap& on) {
+    static bool done_q[kMaxDevices] = {}, done_kv[kMaxDevices] = {};
+    int rc = tc_launch(ctx, window_attention_tc_dq_kernel<DP, BIAS>, done_q, AT_BWD_THREADS, AttnSmem<DP>::TOTAL, p, kk, vk, kn);
+    if (!rc) rc = after_launch(ctx, "window_attention_tc_dq");
+    if (!rc) rc = tc_launch(ctx, window_attention_tc_dkv_kernel<DP, BIAS>, done_kv, AT_BWD_THREADS, AttnSmem<DP>::TOTAL, p, qk, qn, ok, on);
+    return rc ? rc : after_launch(ctx, "window_attention_tc_dkv");
+}
+
+// Heads of up to 64 columns (tensor memory holds two query tiles of that width), the split arithmetic of mode 2, rows that TMA can address.
+bool window_tc_takes(gcb_ctx* ctx, int64_t B, const WindowAttn& a) {
+    if (ctx->gemm_engine == 1 || ctx->gemm_split_mode != 2 || a.D > 64 || a.D % 4 != 0 || !(a.scale > 0.0f) || a.scale > 1e30f) return false;
+    if (!rows_ok(a.q, a.q_ld, a.q_so, a.q_si, B, a.H) || !rows_ok(a.k, a.k_ld, a.k_so, a.k_si, B, a.H) || !rows_ok(a.v, a.v_ld, a.v_so, a.v_si, B, a.H)) return false;
+    if (a.out && !rows_ok(a.out, a.o_ld, a.o_so, a.o_si, B, a.H)) return false;
+    if (a.g && (!rows_ok(a.g, a.g_ld, a.g_so, a.g_si, B, a.H) || !rows_ok(a.o, a.o_ld, a.o_so, a.o_si, B, a.H) || !rows_ok(a.dq, a.d_ld, a.d_so, a.d_si, B, a.H) || !rows_ok(a.dk, a.d_ld, a.d_so, a.d_si, B, a.H) ||
+                !rows_ok(a.dv, a.d_ld, a.d_so, a.d_si, B, a.H)))
+        return false;
+    return B * a.H * ((a.T + 127) / 128) < (int64_t(1) << 30) && a.H <= 65535 && tma_encode(ctx) != nullptr;
+}
+
+int window_tc_fwd(gcb_ctx* ctx, int64_t B, const WindowAttn& a) {
+    TmaEncodeFn enc = tma_encode(ctx);
+    // two query tiles share their key blocks; one tile a CTA where pairs would leave SMs idle
+    WindowTc p = operands(ctx, B, a, B * a.H * ((a.T + 255) / 256) < kSMs ? 1 : 2);
+    Scratch tab(ctx);
+    int rc = make_table(ctx, p, tab);
+    if (rc) return rc;
+    CUtensorMap k, v;
+    GCB_REQUIRE(encode_rows(enc, &k, a.k, a.D, a.T, a.k_ld, a.k_si, a.k_so, a.H, B, 16, AT_KEYS, CU_TENSOR_MAP_SWIZZLE_64B) &&
+                    encode_rows(enc, &v, a.v, a.D, a.T, a.v_ld, a.v_si, a.v_so, a.H, B, 32, AT_KEYS, CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B),
+                "window attention: strides beyond what TMA can address");
+    rc = p.tab ? (a.D <= 32 ? run_fwd<32, true>(ctx, p, k, v) : run_fwd<64, true>(ctx, p, k, v)) : (a.D <= 32 ? run_fwd<32, false>(ctx, p, k, v) : run_fwd<64, false>(ctx, p, k, v));
+    return rc ? rc : after_launch(ctx, "window_attention_tc_fwd");
+}
+
+// a.dbias_part: [head][tile of 128 queries][bucket], or NULL.
+int window_tc_bwd(gcb_ctx* ctx, int64_t B, const WindowAttn& a) {
+    TmaEncodeFn enc = tma_encode(ctx);
+    WindowTc p = operands(ctx, B, a, 1);
+    Scratch tab(ctx), delta(ctx);
+    int rc = make_table(ctx, p, tab);
+    if (!rc) rc = delta.get(sizeof(float) * (size_t)(p.heads * p.Tp));
+    if (rc) return rc;
+    p.delta = delta.as<float>();
+    CUtensorMap kk, vk, kn, qk, qn, ok, on;
+    auto rows = [&](CUtensorMap* map, const float* x, int64_t ld, int64_t so, int64_t si, bool k_major) {
+        return encode_rows(enc, map, x, a.D, a.T, ld, si, so, a.H, B, k_major ? 16 : 32, AT_KEYS, k_major ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B);
+    };
+    GCB_REQUIRE(rows(&kk, a.k, a.k_ld, a.k_so, a.k_si, true) && rows(&kn, a.k, a.k_ld, a.k_so, a.k_si, false) && rows(&vk, a.v, a.v_ld, a.v_so, a.v_si, true) && rows(&qk, a.q, a.q_ld, a.q_so, a.q_si, true) &&
+                    rows(&qn, a.q, a.q_ld, a.q_so, a.q_si, false) && rows(&ok, a.g, a.g_ld, a.g_so, a.g_si, true) && rows(&on, a.g, a.g_ld, a.g_so, a.g_si, false),
+                "window attention: strides beyond what TMA can address");
+    if (p.tab) return a.D <= 32 ? run_bwd<32, true>(ctx, p, kk, vk, kn, qk, qn, ok, on) : run_bwd<64, true>(ctx, p, kk, vk, kn, qk, qn, ok, on);
+    return a.D <= 32 ? run_bwd<32, false>(ctx, p, kk, vk, kn, qk, qn, ok, on) : run_bwd<64, false>(ctx, p, kk, vk, kn, qk, qn, ok, on);
+}
+
+}  // namespace gcb
