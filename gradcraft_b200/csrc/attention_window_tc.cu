@@ -19,6 +19,7 @@
 
 namespace gcb {
 
+constexpr int WT_FLUSH = 8;                     // blocks whose products are added up in tensor memory before the sum moves on
 constexpr int WT_DIAG = AT_ROWS + AT_KEYS - 1;  // distances in a block of scores
 constexpr int WT_TAB = 192;                     // their place in shared memory, in floats
 constexpr float kLog2e = 1.4426950408889634f;
@@ -66,6 +67,92 @@ __device__ __forceinline__ bool all_any(bool x) {  // barrier of the 512 threads
 }
 // Keeps score e of a row (query i against key j0 + e) or hides it; `room` = i - j0.
 __device__ __forceinline__ bool keeps(int e, int room, int window_from, int sinks_to) { return e <= room && (e >= window_from || e < sinks_to); }
+
+// Blocks of the 64-row side: raw tiles from TMA, 32 columns of 64 rows a copy (rows of 128 bytes, 128-byte swizzle: K-major; in 32-byte units:
+// MN-major), and BF16 companions, bf16(x) then bf16(x - t), as 8 x 8 core matrices in rows of DP / 8.  A core matrix holds 8 rows of 8 columns either
+// way, so one set of companions serves a product over the columns (K-major: scores, dP) and one over the rows (MN-major: values).
+template <int DP>
+struct WinTile {
+    static constexpr int RAW = AT_KEYS * DP * 4, TWIN = RAW, SMALL = RAW / 2, ROWS8 = DP * 16;
+};
+template <int DP>
+__device__ __forceinline__ void win_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int r0, int h, int b) {
+    mbar_expect_tx(bar, WinTile<DP>::RAW);
+#pragma unroll
+    for (int c = 0; c < DP / 32; ++c) tma_load_4d(dst + c * 8192, map, bar, 32 * c, r0, h, b);
+}
+// Companions of a raw tile; 128 threads, a core-matrix row (8 columns) at a time, all loads first.
+template <int DP, bool MN>
+__device__ __forceinline__ void win_split(const uint8_t* raw, uint8_t* twin, int t) {
+    constexpr int U = DP / 16;
+    float4 x[U][2];
+#pragma unroll
+    for (int v = 0; v < U; ++v) {
+        const int u = t + 128 * v, r = u & 7, j = (u >> 3) % (DP / 8), row = u / DP * 8 + r;
+        const uint8_t* at = raw + (j >> 2) * 8192 + row * 128;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int half = MN ? e ^ (r >> 2) : e;  // rows four apart have their unit in the same place: they take its halves in turn
+            x[v][e] = *reinterpret_cast<const float4*>(at + (MN ? ((((j & 3) ^ (r & 3)) << 5) | (half << 4)) : (((2 * (j & 3) + e) ^ r) << 4)));
+        }
+    }
+#pragma unroll
+    for (int v = 0; v < U; ++v) {
+        const int u = t + 128 * v, r = u & 7, j = (u >> 3) % (DP / 8);
+        const bool swap = MN && (r >> 2);
+        const float4 a = swap ? x[v][1] : x[v][0], b = swap ? x[v][0] : x[v][1];
+        uint8_t* at = twin + u / DP * WinTile<DP>::ROWS8 + j * 128 + r * 16;
+        *reinterpret_cast<uint4*>(at) = make_uint4(pack_bf16(a.x, a.y), pack_bf16(a.z, a.w), pack_bf16(b.x, b.y), pack_bf16(b.z, b.w));
+        *reinterpret_cast<uint4*>(at + WinTile<DP>::SMALL) = make_uint4(pack_bf16(a.x - trunc_tf32(a.x), a.y - trunc_tf32(a.y)), pack_bf16(a.z - trunc_tf32(a.z), a.w - trunc_tf32(a.w)),
+                                                                        pack_bf16(b.x - trunc_tf32(b.x), b.y - trunc_tf32(b.y)), pack_bf16(b.z - trunc_tf32(b.z), b.w - trunc_tf32(b.w)));
+    }
+}
+// D[128 x 64] = A[128 x DP] B[64 x DP]^T.  A: t in tensor memory, companions in shared memory (place_row); B: K-major raw tile and companions (addresses in 16-byte units).
+template <int DP>
+__device__ __forceinline__ void win_scores(uint32_t d, uint32_t a_t, uint32_t a_twin, uint32_t b_raw, uint32_t b_twin) {
+    constexpr uint32_t idesc = (1u << 4) | (2u << 7) | (2u << 10) | ((uint32_t)(AT_KEYS >> 3) << 17) | ((uint32_t)(AT_ROWS >> 4) << 24);
+    constexpr uint32_t idesc_bf = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(AT_KEYS >> 3) << 17) | ((uint32_t)(AT_ROWS >> 4) << 24);
+    constexpr uint32_t small = WinTile<DP>::SMALL / 16;
+    asm volatile("" : "+r"(a_t), "+r"(a_twin), "+r"(b_raw), "+r"(b_twin));  // descriptors are made here, one addition each: kept across the loop they are spilled
+#pragma unroll
+    for (int kb = 0; kb < DP / 16; ++kb) {
+        const uint32_t b = b_raw + (kb >> 1) * 512 + (kb & 1) * 4, tw = b_twin + kb * 16, a = a_twin + kb * 512;
+        umma_tf32_ts(d, a_t + 16 * kb, tile_desc<16, 1024, 2>(b), idesc, kb > 0 ? 1u : 0u);
+        umma_tf32_ts(d, a_t + 16 * kb + 8, tile_desc<16, 1024, 2>(b + 2), idesc, 1u);
+        umma_bf16(d, tile_desc<128, 256, 0>(a + 256), tile_desc<128, WinTile<DP>::ROWS8, 0>(tw), idesc_bf, 1u);
+        umma_bf16(d, tile_desc<128, 256, 0>(a), tile_desc<128, WinTile<DP>::ROWS8, 0>(tw + small), idesc_bf, 1u);
+    }
+}
+// D[128 x DP] (+)= A[128 x 64] B[64 x DP].  A: its three parts in tensor memory, the companions of 16 columns STEP apart; B: MN-major raw tile and companions.
+template <int DP, int STEP>
+__device__ __forceinline__ void win_values(uint32_t d, uint32_t a_t, uint32_t a_big, uint32_t a_sml, uint32_t b_raw, uint32_t b_twin, bool accumulate) {
+    constexpr uint32_t idesc = (1u << 4) | (2u << 7) | (2u << 10) | (1u << 16) | ((uint32_t)(DP >> 3) << 17) | ((uint32_t)(AT_ROWS >> 4) << 24);
+    constexpr uint32_t idesc_bf = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(DP >> 3) << 17) | ((uint32_t)(AT_ROWS >> 4) << 24);
+    constexpr uint32_t small = WinTile<DP>::SMALL / 16;
+    asm volatile("" : "+r"(a_t), "+r"(a_big), "+r"(a_sml), "+r"(b_raw), "+r"(b_twin));
+#pragma unroll
+    for (int kb = 0; kb < AT_KEYS / 16; ++kb) {
+        const uint32_t b = b_raw + kb * 128, tw = b_twin + kb * 2 * (WinTile<DP>::ROWS8 / 16);
+        umma_tf32_ts(d, a_t + 16 * kb, tile_desc<8192, 512, 1>(b), idesc, (kb > 0 || accumulate) ? 1u : 0u);
+        umma_tf32_ts(d, a_t + 16 * kb + 8, tile_desc<8192, 512, 1>(b + 64), idesc, 1u);
+        umma_bf16_ts(d, a_sml + STEP * kb, tile_desc<WinTile<DP>::ROWS8, 128, 0>(tw), idesc_bf, 1u);
+        umma_bf16_ts(d, a_big + STEP * kb, tile_desc<WinTile<DP>::ROWS8, 128, 0>(tw + small), idesc_bf, 1u);
+    }
+}
+// Moves 16 columns of a sum out of tensor memory: dst = (there ? dst * f : 0) + sum, columns up to `cols`.
+// The tensor core truncates when it adds, so that a sum over hundreds of instructions comes out too small by half a unit for each (8192 keys in one
+// sum: 6e-5 of the result); one of WT_FLUSH blocks, 128 instructions, is off by 3e-6, and these are added here with rounding.
+__device__ __forceinline__ void move_sum(uint32_t taddr, float* dst, int cols, bool live, bool there, float f) {
+    uint32_t x[16];
+    tmem_ld16(taddr, x);
+    if (!live) return;
+#pragma unroll
+    for (int e = 0; e < 16; e += 4)
+        if (e < cols) {
+            const float4 o = there ? ld4(dst + e) : make_float4(0.f, 0.f, 0.f, 0.f);
+            st4(dst + e, make_float4(fmaf(o.x, f, __uint_as_float(x[e])), fmaf(o.y, f, __uint_as_float(x[e + 1])), fmaf(o.z, f, __uint_as_float(x[e + 2])), fmaf(o.w, f, __uint_as_float(x[e + 3]))));
+        }
+}
 
 // ---- forward ------------------------------------------------------------------------------------------------------------------
 // Tensor memory of query tile q, from column 256 q: scores / t of P [0, 64), bf16(P) [64, 96), bf16(P - t) [96, 128), O [128, 192), t of q [192, 256).
@@ -116,10 +203,10 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 1) window_attention_tc_fwd_ker
                     const int kb = slot(0, n), vb = slot(1, n), r0 = u.block(j) * AT_KEYS;
                     ok = mbar_wait(empty(kb), ph, p.status, 41);
                     if (!ok) break;
-                    load_k_major<DP>(base + S::BLOCKS_OFF + kb * S::BLOCK, &map_k, full(kb), r0, it.h, it.b);
+                    win_load<DP>(base + S::BLOCKS_OFF + kb * S::BLOCK, &map_k, full(kb), r0, it.h, it.b);
                     ok = mbar_wait(empty(vb), ph, p.status, 41);
                     if (!ok) break;
-                    load_mn_major<DP>(base + S::BLOCKS_OFF + vb * S::BLOCK, &map_v, full(vb), r0, it.h, it.b);
+                    win_load<DP>(base + S::BLOCKS_OFF + vb * S::BLOCK, &map_v, full(vb), r0, it.h, it.b);
                 }
             }
         }
@@ -133,8 +220,10 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 1) window_attention_tc_fwd_ker
                 if (it.skip) continue;
                 const Union u(TileKeys(p, tile_row(it, 0)), TileKeys(p, tile_row(it, 1)));
                 const int blocks = u.blocks;
+                int done[2] = {0, 0};  // blocks of each tile
                 auto scores = [&](int q, int j) {
-                    issue_scores<DP>(tmem + 256 * q, tmem + 256 * q + 192, base16 + q * (S::TWIN / 16), base16 + S::BLOCKS_OFF / 16 + slot(0, n + j) * (S::BLOCK / 16));
+                    const uint32_t raw = base16 + S::BLOCKS_OFF / 16 + slot(0, n + j) * (S::BLOCK / 16);
+                    win_scores<DP>(tmem + 256 * q, tmem + 256 * q + 192, base16 + q * (S::TWIN / 16), raw, raw + S::RAW / 16);
                     umma_commit(s_full(q));
                 };
                 auto k_landed = [&](int j) {
@@ -165,7 +254,7 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 1) window_attention_tc_fwd_ker
                             if (ok) {
                                 after_sync();
                                 const uint32_t t0 = tmem + 256 * q;
-                                issue_values<DP>(t0 + 128, t0, t0 + 64, t0 + 96, v_raw, now != t.begin());
+                                win_values<DP, 8>(t0 + 128, t0, t0 + 64, t0 + 96, v_raw, v_raw + S::RAW / 16, (done[q]++ % WT_FLUSH) != 0);
                                 if (now == t.last) umma_commit(o_full(q));
                             }
                         }
@@ -197,8 +286,8 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 1) window_attention_tc_fwd_ker
                     ok = warp_wait(full(b), (n >> 1) & 1u, p.status, 46);
                     if (!ok) break;
                     uint8_t* raw = gen + S::BLOCKS_OFF + b * S::BLOCK;
-                    if (kind == 0) split_k_major<DP>(raw, t);
-                    else split_mn_major<DP>(raw, raw + S::RAW, t);
+                    if (kind == 0) win_split<DP, false>(raw, raw + S::RAW, t);
+                    else win_split<DP, true>(raw, raw + S::RAW, t);
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
                     if (lane == 0) mbar_arrive(conv(b));
@@ -243,7 +332,8 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 1) window_attention_tc_fwd_ker
                 if (at_tile < WT_DIAG) tabs[at_tile] = request(keys.begin());
                 pair_sync(bar);
             }
-            float m = -INFINITY, sum = 0.0f;  // m: the maximum the probabilities are relative to
+            float* dst = p.out + it.b * p.o_so + it.h * p.o_si + r * p.o_ld + half * OC;
+            float m = -INFINITY, sum = 0.0f, m_out = -INFINITY;  // m: the maximum the probabilities are relative to; m_out: the one what has moved to `out` is
             bool good = true;
             for (int j = 0; j < blocks; ++j) {
                 const int b = keys.block(j);
@@ -252,6 +342,12 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 1) window_attention_tc_fwd_ker
                 good = good && warp_wait(s_full(q), s_phase & 1u, p.status, 47);  // every thread keeps step with the barriers below, whatever a wait says
                 ++s_phase;
                 after_sync();
+                if (j > 0 && j % WT_FLUSH == 0) {  // the products of the blocks before came before these scores
+                    const float f = m_out == m ? 1.0f : ex2((m_out - m) * c);
+#pragma unroll
+                    for (int g = 0; g < OC / 16; ++g) move_sum(t0 + 128 + half * OC + 16 * g, dst + 16 * g, p.D - half * OC - 16 * g, live, j > WT_FLUSH, f);
+                    m_out = m;
+                }
                 float v[32];
                 tmem_ld32(t0 + 32 * half, v);
                 const int j0 = b * AT_KEYS + 32 * half, room = r - j0;
@@ -316,7 +412,8 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 1) window_attention_tc_fwd_ker
             const float inv = empty_row ? 0.0f : 1.0f / (sum + xch[(half ^ 1) * 128 + row]);
             pair_sync(bar);
             if (!ok) break;
-            float* dst = p.out + it.b * p.o_so + it.h * p.o_si + r * p.o_ld;
+            const bool there = blocks > WT_FLUSH;
+            const float fo = inv * (m_out == m ? 1.0f : ex2((m_out - m) * c));
 #pragma unroll
             for (int g = 0; g < OC / 16; ++g) {
                 uint32_t x[16];
@@ -324,8 +421,11 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 1) window_attention_tc_fwd_ker
                 if (live)
 #pragma unroll
                     for (int e = 0; e < 16; e += 4)
-                        if (half * OC + 16 * g + e < p.D)
-                            st4(dst + half * OC + 16 * g + e, make_float4(__uint_as_float(x[e]) * inv, __uint_as_float(x[e + 1]) * inv, __uint_as_float(x[e + 2]) * inv, __uint_as_float(x[e + 3]) * inv));
+                        if (half * OC + 16 * g + e < p.D) {
+                            const float4 o = there ? ld4(dst + 16 * g + e) : make_float4(0.f, 0.f, 0.f, 0.f);
+                            st4(dst + 16 * g + e, make_float4(fmaf(o.x, fo, __uint_as_float(x[e]) * inv), fmaf(o.y, fo, __uint_as_float(x[e + 1]) * inv), fmaf(o.z, fo, __uint_as_float(x[e + 2]) * inv),
+                                                              fmaf(o.w, fo, __uint_as_float(x[e + 3]) * inv)));
+                        }
             }
             if (half == 0 && live) {
                 const int64_t at = ((int64_t)it.b * p.H + it.h) * p.Tp + r;
@@ -338,49 +438,57 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 1) window_attention_tc_fwd_ker
 }
 
 // ---- dK and dV ----------------------------------------------------------------------------------------------------------------
-// As the backward kernel of attention.cu: a thread owns a key and sixteen of a block's queries, everything transposed; queries from the
-// diagonal to the window's end.
+// A thread owns a key and sixteen of a block's queries, everything transposed: S^T = k q^T, dP^T = v dO^T, dV += P^T dO, dK += dS^T q, for the
+// queries from the diagonal to the window's end.  Products are ordered so that the tensor core has dV(i), S(i+1) to do while dS(i) is made
+// and dK(i), dP(i+1) while P(i+1) is.
+//   warp 0       TMA producer        warp 1       MMA issuer
+//   warps 4..7   companions of q, the statistics of its rows and the bias        warps 8..11  companions of dO        warps 12..27  four threads a key
+// A tile of q arrives K-major, a block ahead, and once more MN-major; so does dO.  Companions stay until the tile's second product has read them.
 // Tensor memory: S^T / t of P^T [0, 64), dP^T / t of dS^T [64, 128), P^T companions [128, 192), dS^T companions [192, 256), dV [256, 320), dK [320, 384),
 // t of k [384, 448), t of v [448, 512).
+template <int DP>
+struct DkvSmem {
+    using T = WinTile<DP>;
+    static constexpr int OWN = AT_ROWS * DP * 4;  // companions of a 128-row operand
+    static constexpr int Q_RAW = 2 * OWN, O_RAW = Q_RAW + 2 * T::RAW, Q_MN = O_RAW + T::RAW, O_MN = Q_MN + T::RAW, Q_TWIN = O_MN + T::RAW, O_TWIN = Q_TWIN + 2 * T::TWIN;
+    static constexpr int STATS = O_TWIN + 2 * T::TWIN;  // row maximum, 1 / sum and dO . O of a block's queries, two blocks; then the bias of its distances, two blocks
+    static constexpr int TABS = STATS + 2 * 3 * AT_KEYS * 4, BAR = TABS + 2 * WT_TAB * 4, TOTAL = BAR + 256 + 1024;
+    static_assert(TOTAL <= 232448, "shared memory");
+};
 template <int DP, bool BIAS>
 __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_kernel(const __grid_constant__ CUtensorMap map_qk, const __grid_constant__ CUtensorMap map_qn, const __grid_constant__ CUtensorMap map_ok,
                                                                                 const __grid_constant__ CUtensorMap map_on, const __grid_constant__ WindowTc p) {
-    using S = AttnSmem<DP>;
+    using S = DkvSmem<DP>;
+    using T = WinTile<DP>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
-    const uint32_t bars = base + S::BAR_OFF;
-    enum { QK = 0, OK = 1, ON = 2, QN = 3 };  // blocks: q and dO K-major for the scores and dP, dO and q MN-major for dV and dK
-    auto full = [&](int b) { return bars + 8u * b; };
-    auto conv = [&](int b) { return bars + 8u * (4 + b); };
-    auto empty = [&](int b) { return bars + 8u * (8 + b); };
-    const uint32_t s_full = bars + 8u * 12, dp_full = bars + 8u * 13, p_ready = bars + 8u * 14, ds_ready = bars + 8u * 15, acc_full = bars + 8u * 16, kv_ready = bars + 8u * 17;
+    const uint32_t bars = base + S::BAR;
+    enum { QK = 0, OK = 1, ON = 2, QN = 3 };  // tiles: q and dO K-major for the scores and dP, dO and q MN-major for dV and dK
+    auto bar = [&](int i) { return bars + 8u * i; };
+    // n: running number of a block; parities of what has two places and of what has one
+    auto two = [](uint32_t n) { return (n >> 1) & 1u; };
+    auto one = [](uint32_t n) { return n & 1u; };
+    auto q_full = [&](uint32_t n) { return bar(0 + (n & 1u)); };
+    auto q_empty = [&](uint32_t n) { return bar(2 + (n & 1u)); };
+    auto q_conv = [&](uint32_t n) { return bar(4 + (n & 1u)); };
+    auto q_free = [&](uint32_t n) { return bar(6 + (n & 1u)); };   // companions: dK has read them
+    auto o_conv = [&](uint32_t n) { return bar(8 + (n & 1u)); };
+    auto o_free = [&](uint32_t n) { return bar(10 + (n & 1u)); };  // dV has read them
+    const uint32_t o_full = bar(12), o_empty = bar(13), on_full = bar(14), on_empty = bar(15), qn_full = bar(16), qn_empty = bar(17);
+    const uint32_t s_full = bar(18), dp_full = bar(19), p_ready = bar(20), ds_ready = bar(21), acc_full = bar(22), kv_ready = bar(23);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int b = 0; b < 4; ++b) { mbar_init(full(b), 1); mbar_init(conv(b), 4); mbar_init(empty(b), 1); }
-        mbar_init(s_full, 1); mbar_init(dp_full, 1); mbar_init(acc_full, 1);
-        mbar_init(p_ready, 16); mbar_init(ds_ready, 16); mbar_init(kv_ready, 16);
+        for (int i = 0; i < 24; ++i) mbar_init(bar(i), i == 4 || i == 5 || i == 8 || i == 9 ? 4 : i == 20 || i == 21 || i == 23 ? 16 : 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    const uint32_t tmem = tmem_take(bars + 8u * 20, reinterpret_cast<volatile uint32_t*>(gen + S::BAR_OFF + 8 * 20), warp);
+    const uint32_t tmem = tmem_take(bars + 8u * 24, reinterpret_cast<volatile uint32_t*>(gen + S::BAR + 8 * 24), warp);
     pdl_trigger();
     pdl_wait();
     auto steps = [&](const AttnItem& it) {  // blocks of queries from the tile's first key to the last query that sees its last one
         const int k0 = it.unit * AT_ROWS, k1 = min(p.T, k0 + AT_ROWS), end = p.rule.W > 0 && p.rule.W < p.T - k1 ? k1 - 1 + p.rule.W : p.T;
         return (end - k0 + AT_KEYS - 1) / AT_KEYS;
     };
-    // the order in which blocks are loaded, split and used within an item of n steps
-    auto sequence = [&](int n, auto&& f) -> bool {
-        if (!f((int)QK, 0) || !f((int)OK, 0)) return false;
-        for (int i = 0; i < n; ++i) {
-            if (!f((int)ON, i)) return false;
-            if (i + 1 < n && !f((int)QK, i + 1)) return false;
-            if (!f((int)QN, i)) return false;
-            if (i + 1 < n && !f((int)OK, i + 1)) return false;
-        }
-        return true;
-    };
-    float* tabs = reinterpret_cast<float*>(gen + S::STAGE_OFF);  // bias of a block's distances, two blocks
 
     if (warp < 4) regs_give<64>();
     if (warp == 0) {
@@ -391,15 +499,18 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
                 const AttnItem it = attn_item(p, w, true);
                 if (it.skip) continue;
                 const int n = steps(it);
-                ok = sequence(n, [&](int b, int i) {
-                    if (!mbar_wait(empty(b), ((n0 + i) & 1u) ^ 1u, p.status, 51)) return false;
-                    const uint32_t dst = base + S::BLOCKS_OFF + b * S::BLOCK;
-                    const int r0 = it.unit * AT_ROWS + i * AT_KEYS;
-                    if (b == QK) load_k_major<DP>(dst, &map_qk, full(b), r0, it.h, it.b);
-                    else if (b == OK) load_k_major<DP>(dst, &map_ok, full(b), r0, it.h, it.b);
-                    else load_mn_major<DP>(dst, b == ON ? &map_on : &map_qn, full(b), r0, it.h, it.b);
+                auto load = [&](int kind, int i) {
+                    if (i >= n) return true;
+                    const uint32_t at = n0 + i;
+                    const uint32_t e = kind == QK ? q_empty(at) : kind == OK ? o_empty : kind == ON ? on_empty : qn_empty, f = kind == QK ? q_full(at) : kind == OK ? o_full : kind == ON ? on_full : qn_full;
+                    const uint32_t dst = base + (kind == QK ? S::Q_RAW + (at & 1u) * T::RAW : kind == OK ? S::O_RAW : kind == ON ? S::O_MN : S::Q_MN);
+                    if (!mbar_wait(e, (kind == QK ? two(at) : one(at)) ^ 1u, p.status, 51)) return false;
+                    win_load<DP>(dst, kind == QK ? &map_qk : kind == OK ? &map_ok : kind == ON ? &map_on : &map_qn, f, it.unit * AT_ROWS + i * AT_KEYS, it.h, it.b);
                     return true;
-                });
+                };
+                ok = load(QK, 0) && load(OK, 0) && load(QK, 1);
+                // in the order in which places become free: dV(i - 1), S(i), dK(i - 1), dP(i)
+                for (int i = 0; i < n && ok; ++i) ok = load(ON, i) && load(QK, i + 2) && load(QN, i) && load(OK, i + 1);
                 n0 += n;
             }
         }
@@ -412,27 +523,46 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
                 const AttnItem it = attn_item(p, w, true);
                 if (it.skip) break;  // only the last round has items left out
                 const int n = steps(it);
-                auto landed = [&](int b, int i) {
-                    const bool r = mbar_wait(conv(b), (n0 + i) & 1u, p.status, 52);
+                auto landed = [&](uint32_t b, uint32_t parity) {
+                    const bool r = mbar_wait(b, parity, p.status, 52);
                     after_sync();
                     return r;
                 };
+                auto scores = [&](int i) {
+                    const uint32_t at = n0 + i;
+                    if (i >= n) return true;
+                    if (!landed(q_conv(at), two(at))) return false;
+                    win_scores<DP>(tmem, tmem + 384, base16, base16 + (S::Q_RAW + (at & 1u) * T::RAW) / 16, base16 + (S::Q_TWIN + (at & 1u) * T::TWIN) / 16);
+                    umma_commit(q_empty(at));
+                    umma_commit(s_full);
+                    return true;
+                };
+                auto dprobs = [&](int i) {
+                    const uint32_t at = n0 + i;
+                    if (i >= n) return true;
+                    if (!landed(o_conv(at), two(at))) return false;
+                    win_scores<DP>(tmem + 64, tmem + 448, base16 + S::OWN / 16, base16 + S::O_RAW / 16, base16 + (S::O_TWIN + (at & 1u) * T::TWIN) / 16);
+                    umma_commit(o_empty);
+                    umma_commit(dp_full);
+                    return true;
+                };
                 ok = mbar_wait(kv_ready, items & 1u, p.status, 53);
                 if (!ok) break;
-                ok = sequence(n, [&](int b, int i) {
-                    const uint32_t blk = base16 + S::BLOCKS_OFF / 16 + b * (S::BLOCK / 16), ph = (n0 + i) & 1u;
-                    if (b == ON && !mbar_wait(p_ready, ph, p.status, 54)) return false;
-                    if (b == QN && !mbar_wait(ds_ready, ph, p.status, 55)) return false;
-                    if (!landed(b, i)) return false;
-                    if (b == QK) issue_scores<DP>(tmem, tmem + 384, base16, blk);
-                    else if (b == OK) issue_scores<DP>(tmem + 64, tmem + 448, base16 + S::TWIN / 16, blk);
-                    else if (b == ON) issue_values<DP>(tmem + 256, tmem, tmem + 128, tmem + 160, blk, i > 0);
-                    else issue_values<DP>(tmem + 320, tmem + 64, tmem + 192, tmem + 224, blk, i > 0);
-                    umma_commit(empty(b));
-                    if (b == QK) umma_commit(s_full);
-                    else if (b == OK) umma_commit(dp_full);
-                    return true;
-                });
+                ok = scores(0) && dprobs(0);
+                for (int i = 0; i < n && ok; ++i) {
+                    const uint32_t at = n0 + i;
+                    ok = mbar_wait(on_full, one(at), p.status, 54) && landed(p_ready, one(at));
+                    if (!ok) break;
+                    win_values<DP, 8>(tmem + 256, tmem, tmem + 128, tmem + 160, base16 + S::O_MN / 16, base16 + (S::O_TWIN + (at & 1u) * T::TWIN) / 16, i % WT_FLUSH != 0);
+                    umma_commit(on_empty);
+                    umma_commit(o_free(at));
+                    ok = scores(i + 1) && mbar_wait(qn_full, one(at), p.status, 55) && landed(ds_ready, one(at));
+                    if (!ok) break;
+                    win_values<DP, 8>(tmem + 320, tmem + 64, tmem + 192, tmem + 224, base16 + S::Q_MN / 16, base16 + (S::Q_TWIN + (at & 1u) * T::TWIN) / 16, i % WT_FLUSH != 0);
+                    umma_commit(qn_empty);
+                    umma_commit(q_free(at));
+                    ok = dprobs(i + 1);
+                }
                 if (!ok) break;
                 umma_commit(acc_full);
                 n0 += n;
@@ -440,69 +570,57 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
         }
     } else if (warp >= 4 && warp < 12) {
         regs_give<56>();
-        // warps 4..7: the K-major blocks, the query statistics and the bias; warps 8..11: the MN-major blocks
         const int t = threadIdx.x & 127;
-        const bool k_major = warp < 8;
-        float* stats_sm = reinterpret_cast<float*>(gen + S::STATS_OFF);
+        const bool of_q = warp < 8;
         uint32_t n0 = 0;
         bool ok = true;
         for (int64_t w = blockIdx.x; w < p.loop_end && ok; w += gridDim.x) {
             const AttnItem it = attn_item(p, w, true);
             if (it.skip) continue;
             const int n = steps(it), q_at = it.unit * AT_ROWS + t;
-            const int64_t at = ((int64_t)it.b * p.H + it.h) * p.Tp;
+            const int64_t at_head = ((int64_t)it.b * p.H + it.h) * p.Tp;
             const float* tab = BIAS ? p.tab + (int64_t)it.h * p.tab_len : nullptr;
             float nm = 0.f, ni = 0.f, nd = 0.f, nb0 = 0.f, nb1 = 0.f;  // the next block's, loaded a block ahead
-            const bool mine = k_major && t < AT_KEYS;
-            // statistics of queries beyond the sequence are not there: P is then zero
-            auto stats = [&](int i) {
-                const int q = q_at + i * AT_KEYS;
-                const bool live = mine && q < p.T;
-                nm = live ? __ldg(p.row_max + at + q) : INFINITY;
-                ni = live ? __ldg(p.row_inv + at + q) : 0.0f;
-            };
-            auto term = [&](int i) { nd = mine && q_at + i * AT_KEYS < p.T ? __ldg(p.delta + at + q_at + i * AT_KEYS) : 0.0f; };
-            auto bias = [&](int i) {
-                if (!BIAS || !k_major) return;
-                const int d0 = i * AT_KEYS - (AT_ROWS - 1);
-                nb0 = __ldg(tab + clamp_distance(d0 + t, p.tab_len));
-                nb1 = __ldg(tab + clamp_distance(d0 + t + 128, p.tab_len));
-            };
-            stats(0); term(0); bias(0);
-            ok = sequence(n, [&](int b, int i) {
-                if (k_major != (b <= OK)) return true;
-                if (!warp_wait(full(b), (n0 + i) & 1u, p.status, 56)) return false;
-                uint8_t* raw = gen + S::BLOCKS_OFF + b * S::BLOCK;
-                // Two slots, by the running number of the block: the one before last has been used (its products preceded the last one's, which
-                // this block's copy waited for), also where the last one belongs to the item before.
-                if (k_major) {
-                    float* slot = stats_sm + ((n0 + i) & 1u) * 3 * AT_KEYS + t;
-                    if (b == QK) {
-                        if (mine) { slot[0] = BIAS ? nm : nm * kLog2e; slot[AT_KEYS] = ni; }
-                        if (BIAS) {
-                            float* tb = tabs + ((n0 + i) & 1u) * WT_TAB + t;
-                            tb[0] = nb0;
-                            if (t < WT_TAB - 128) tb[128] = nb1;
-                        }
-                        if (i + 1 < n) { stats(i + 1); bias(i + 1); }
-                    } else {
-                        if (mine) slot[2 * AT_KEYS] = nd;
-                        if (i + 1 < n) term(i + 1);
-                    }
+            auto request = [&](int i) {
+                const int q = q_at + i * AT_KEYS, d0 = i * AT_KEYS - (AT_ROWS - 1);
+                const bool live = t < AT_KEYS && q < p.T;  // queries beyond the sequence have no statistics: P is then zero
+                nm = live ? __ldg(p.row_max + at_head + q) : INFINITY;
+                ni = live ? __ldg(p.row_inv + at_head + q) : 0.0f;
+                nd = live ? __ldg(p.delta + at_head + q) : 0.0f;
+                if (BIAS) {
+                    nb0 = __ldg(tab + clamp_distance(d0 + t, p.tab_len));
+                    nb1 = __ldg(tab + clamp_distance(d0 + t + 128, p.tab_len));
                 }
-                if (k_major) split_k_major<DP>(raw, t);
-                else split_mn_major<DP>(raw, raw + S::RAW, t);
+            };
+            if (of_q) request(0);
+            for (int i = 0; i < n && ok; ++i) {
+                const uint32_t at = n0 + i;
+                ok = warp_wait(of_q ? q_full(at) : o_full, of_q ? two(at) : one(at), p.status, 56);
+                if (!ok) break;
+                // the place is free once the second product of the block before last has read it; its statistics were used before that
+                ok = warp_wait(of_q ? q_free(at) : o_free(at), two(at) ^ 1u, p.status, 56);
+                if (!ok) break;
+                if (of_q) {
+                    float* slot = reinterpret_cast<float*>(gen + S::STATS) + (at & 1u) * 3 * AT_KEYS + t;
+                    if (t < AT_KEYS) { slot[0] = BIAS ? nm : nm * kLog2e; slot[AT_KEYS] = ni; slot[2 * AT_KEYS] = nd; }
+                    if (BIAS) {
+                        float* tb = reinterpret_cast<float*>(gen + S::TABS) + (at & 1u) * WT_TAB + t;
+                        tb[0] = nb0;
+                        if (t < WT_TAB - 128) tb[128] = nb1;
+                    }
+                    if (i + 1 < n) request(i + 1);
+                }
+                win_split<DP, false>(gen + (of_q ? S::Q_RAW + (at & 1u) * T::RAW : S::O_RAW), gen + (of_q ? S::Q_TWIN : S::O_TWIN) + (at & 1u) * T::TWIN, t);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(conv(b));
-                return true;
-            });
+                if (lane == 0) mbar_arrive(of_q ? q_conv(at) : o_conv(at));
+            }
             n0 += n;
         }
     } else if (warp >= 12) {
         regs_take<80>();
         const int part = (warp - 12) >> 2, row = 32 * (warp & 3) + lane;  // this warp: 32 keys x 16 of the block's 64 queries
-        constexpr int OC = DP / 2;                                       // and half of the columns of k (parts 0, 1) or v (2, 3)
+        constexpr int OC = DP / 2;                                       // and half of the columns of k and dK (parts 0, 1) or v and dV (2, 3)
         const int half = part & 1;
         const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
         const float c = p.scale * kLog2e;
@@ -516,25 +634,31 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
             {
                 float x[OC];
                 load_row<DP / 32>(x, (part < 2 ? p.k + it.b * p.k_so + it.h * p.k_si + key * p.k_ld : p.v + it.b * p.v_so + it.h * p.v_si + key * p.v_ld) + half * OC, live, p.D - half * OC);
-                place_row<DP / 32>(x, lanes + (part < 2 ? 384 : 448) + half * OC, gen + (part >> 1) * S::TWIN + half * (OC / 16) * 8192, row);
+                place_row<DP / 32>(x, lanes + (part < 2 ? 384 : 448) + half * OC, gen + (part >> 1) * S::OWN + half * (OC / 16) * 8192, row);
             }
             tmem_stores_done();
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(kv_ready);
             const int cnt = steps(it);
+            float* dst = (part < 2 ? p.dk : p.dv) + it.b * p.d_so + it.h * p.d_si + key * p.d_ld + half * OC;
+            auto move = [&](bool there) {
+#pragma unroll
+                for (int g = 0; g < OC / 16; ++g) move_sum(lanes + (part < 2 ? 320 : 256) + half * OC + 16 * g, dst + 16 * g, p.D - half * OC - 16 * g, live, there, 1.0f);
+            };
 #pragma unroll 1
             for (int i = 0; i < cnt; ++i, ++n) {
-                const float4* mp = reinterpret_cast<const float4*>(gen + S::STATS_OFF + (n & 1u) * 3 * AT_KEYS * 4) + 4 * part;
+                const float4* mp = reinterpret_cast<const float4*>(gen + S::STATS + (n & 1u) * 3 * AT_KEYS * 4) + 4 * part;
                 const float4 *ip = mp + AT_KEYS / 4, *dp = ip + AT_KEYS / 4;
                 ok = warp_wait(s_full, n & 1u, p.status, 57);
                 if (!ok) break;
                 after_sync();
+                if (part >= 2 && i > 0 && i % WT_FLUSH == 0) move(i > WT_FLUSH);  // dV of the blocks before came before these scores
                 uint32_t u[16];
                 float pr[16];
                 tmem_ld16(lanes + 16 * part, u);
                 const int first = row - i * AT_KEYS - 16 * part;  // queries from here on look at this key, as many as the window is long
-                const float* bias = tabs + (n & 1u) * WT_TAB + (AT_ROWS - 1) + 16 * part - row;
+                const float* bias = reinterpret_cast<const float*>(gen + S::TABS) + (n & 1u) * WT_TAB + (AT_ROWS - 1) + 16 * part - row;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float4 m = mp[e], iv = ip[e];
@@ -566,6 +690,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
                     for (int x = 0; x < 4; ++x) pr[4 * e + x] = pr[4 * e + x] * p.scale * (__uint_as_float(u[4 * e + x]) - dd[x]);
                 }
                 place_parts16(pr, lanes + 64 + 16 * part, lanes + 192 + 8 * part, lanes + 224 + 8 * part);
+                if (part < 2 && i > 0 && i % WT_FLUSH == 0) move(i > WT_FLUSH);  // dK of the blocks before came before this dP
                 tmem_stores_done();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(ds_ready);
@@ -574,16 +699,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
             ok = warp_wait(acc_full, items & 1u, p.status, 59);
             if (!ok) break;
             after_sync();
-            float* dst = (part < 2 ? p.dk : p.dv) + it.b * p.d_so + it.h * p.d_si + key * p.d_ld + half * OC;
-#pragma unroll
-            for (int g = 0; g < OC / 16; ++g) {
-                uint32_t x[16];
-                tmem_ld16(lanes + (part < 2 ? 320 : 256) + half * OC + 16 * g, x);
-                if (live)
-#pragma unroll
-                    for (int e = 0; e < 16; e += 4)
-                        if (half * OC + 16 * g + e < p.D) st4(dst + 16 * g + e, make_float4(__uint_as_float(x[e]), __uint_as_float(x[e + 1]), __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3])));
-            }
+            move(cnt > WT_FLUSH);
         }
     }
     tmem_give(tmem, warp);
@@ -592,50 +708,52 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
 // ---- dQ and the bias gradient ---------------------------------------------------------------------------------------------------
 // A CTA takes 128 queries and walks over their keys: S = q k^T and dP = dO v^T of one block while dQ += dS k of the block before passes.  Four
 // threads a query, sixteen of a block's keys each.  dO . O is formed here, from the rows that are loaded anyway, and kept for dK.
+// Roles as above, the companions of k and the bias by warps 4..7, those of v by warps 8..11.  K-major tiles arrive up to two blocks ahead.
 // Scores and dP alternate between two places, x = 0 and 1; dS takes the place of both, a thread's columns where it has read them.
 // Tensor memory: S / companions of dS [128 x, + 64) (of 16 keys: 8 columns bf16(dS), 8 bf16(dS - t)), dP / t of dS [128 x + 64, + 64), dQ [256, 320), t of q [320, 384), t of dO [384, 448).
-// Bias gradient: a warp adds up the dS of its 32 x 16 block along the diagonals, 47 of them, through shared memory, and lane n those
+// Bias gradient: a warp adds up the dS of its 32 x 16 block along the diagonals, 47 of them, in sixteen shuffles, and lane n those
 // that belong to buckets n and n + 32; a block that lies in one bucket as a whole is added up row by row in registers instead.
+template <int DP>
+struct DqSmem {
+    using T = WinTile<DP>;
+    static constexpr int OWN = AT_ROWS * DP * 4;
+    static constexpr int K_RAW = 2 * OWN, V_RAW = K_RAW + 2 * T::RAW, K_MN = V_RAW + 2 * T::RAW, K_TWIN = K_MN + T::RAW, V_TWIN = K_TWIN + 2 * T::TWIN;
+    static constexpr int TABS = V_TWIN + 2 * T::TWIN, DIAG = TABS + 2 * WT_TAB * 4;  // bias of a block's distances, two blocks; [warp][64]: sums by diagonal, at an item's end by bucket
+    static constexpr int XCH = DIAG + 16 * 64 * 4, BAR = XCH + 2 * AT_ROWS * 4, TOTAL = BAR + 256 + 1024;
+    static_assert(TOTAL <= 232448 && AW_MAX_BUCKETS == 64, "shared memory");
+};
 template <int DP, bool BIAS>
 __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kernel(const __grid_constant__ CUtensorMap map_kk, const __grid_constant__ CUtensorMap map_vk, const __grid_constant__ CUtensorMap map_kn,
                                                                                const __grid_constant__ WindowTc p) {
-    using S = AttnSmem<DP>;
+    using S = DqSmem<DP>;
+    using T = WinTile<DP>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
-    const uint32_t bars = base + S::BAR_OFF;
-    enum { KK = 0, VK = 1, KN = 2 };  // blocks: k and v K-major for the scores and dP, k MN-major for dQ
-    constexpr int DIAG_OFF = S::BLOCKS_OFF + 3 * S::BLOCK, DIAG_WARP = 32 * 17 * 4;  // the fourth block's place and the staging area behind it
-    static_assert(DIAG_OFF + 16 * DIAG_WARP + 3 * WT_TAB * 4 + (16 * AW_MAX_BUCKETS + 2 * AT_ROWS) * 4 <= S::BAR_OFF, "shared memory");
-    auto full = [&](int b) { return bars + 8u * b; };
-    auto conv = [&](int b) { return bars + 8u * (3 + b); };
-    auto empty = [&](int b) { return bars + 8u * (6 + b); };
-    auto s_full = [&](uint32_t n) { return bars + 8u * (9 + (n & 1u)); };
-    auto dp_full = [&](uint32_t n) { return bars + 8u * (11 + (n & 1u)); };
-    auto ds_ready = [&](uint32_t n) { return bars + 8u * (13 + (n & 1u)); };
-    const uint32_t acc_full = bars + 8u * 15, q_ready = bars + 8u * 16;
+    const uint32_t bars = base + S::BAR;
+    enum { KK = 0, VK = 1, KN = 2 };  // tiles: k and v K-major for the scores and dP, k MN-major for dQ
+    auto bar = [&](int i) { return bars + 8u * i; };
+    auto two = [](uint32_t n) { return (n >> 1) & 1u; };
+    auto one = [](uint32_t n) { return n & 1u; };
+    auto k_full = [&](uint32_t n) { return bar(0 + (n & 1u)); };
+    auto k_empty = [&](uint32_t n) { return bar(2 + (n & 1u)); };
+    auto k_conv = [&](uint32_t n) { return bar(4 + (n & 1u)); };
+    auto k_free = [&](uint32_t n) { return bar(6 + (n & 1u)); };  // companions: dQ has read them
+    auto v_full = [&](uint32_t n) { return bar(8 + (n & 1u)); };
+    auto v_empty = [&](uint32_t n) { return bar(10 + (n & 1u)); };  // tile and companions
+    auto v_conv = [&](uint32_t n) { return bar(12 + (n & 1u)); };
+    auto s_full = [&](uint32_t n) { return bar(14 + (n & 1u)); };
+    auto dp_full = [&](uint32_t n) { return bar(16 + (n & 1u)); };
+    auto ds_ready = [&](uint32_t n) { return bar(18 + (n & 1u)); };
+    const uint32_t kn_full = bar(20), kn_empty = bar(21), acc_full = bar(22), q_ready = bar(23);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int b = 0; b < 3; ++b) { mbar_init(full(b), 1); mbar_init(conv(b), 4); mbar_init(empty(b), 1); }
-        for (int x = 0; x < 2; ++x) { mbar_init(s_full(x), 1); mbar_init(dp_full(x), 1); mbar_init(ds_ready(x), 16); }
-        mbar_init(acc_full, 1); mbar_init(q_ready, 16);
+        for (int i = 0; i < 24; ++i) mbar_init(bar(i), i == 4 || i == 5 || i == 12 || i == 13 ? 4 : i == 18 || i == 19 || i == 23 ? 16 : 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    const uint32_t tmem = tmem_take(bars + 8u * 20, reinterpret_cast<volatile uint32_t*>(gen + S::BAR_OFF + 8 * 20), warp);
+    const uint32_t tmem = tmem_take(bars + 8u * 24, reinterpret_cast<volatile uint32_t*>(gen + S::BAR + 8 * 24), warp);
     pdl_trigger();
     pdl_wait();
-    // the order in which blocks are loaded, split and used within an item of n steps
-    auto sequence = [&](int n, auto&& f) -> bool {
-        if (!f((int)KK, 0) || !f((int)VK, 0)) return false;
-        for (int i = 0; i < n; ++i) {
-            if (i + 1 < n && (!f((int)KK, i + 1) || !f((int)VK, i + 1))) return false;
-            if (!f((int)KN, i)) return false;
-        }
-        return true;
-    };
-    float* tabs = reinterpret_cast<float*>(gen + DIAG_OFF + 16 * DIAG_WARP);  // bias of a block's distances, three blocks
-    float* sums = tabs + 3 * WT_TAB;                                          // [warp][bucket] at an item's end
-    float* xch = sums + 16 * AW_MAX_BUCKETS;                                  // [half][row]: dO . O
 
     if (warp < 4) regs_give<64>();
     if (warp == 0) {
@@ -646,15 +764,20 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
                 const AttnItem it = attn_item(p, w, false);
                 if (it.skip) continue;
                 const TileKeys keys(p, it.unit * AT_ROWS);
-                ok = sequence(keys.count(), [&](int b, int i) {
-                    if (!mbar_wait(empty(b), ((n0 + i) & 1u) ^ 1u, p.status, 61)) return false;
-                    const uint32_t dst = base + S::BLOCKS_OFF + b * S::BLOCK;
-                    const int r0 = keys.block(i) * AT_KEYS;
-                    if (b == KN) load_mn_major<DP>(dst, &map_kn, full(b), r0, it.h, it.b);
-                    else load_k_major<DP>(dst, b == KK ? &map_kk : &map_vk, full(b), r0, it.h, it.b);
+                const int n = keys.count();
+                auto load = [&](int kind, int i) {
+                    if (i >= n) return true;
+                    const uint32_t at = n0 + i;
+                    const uint32_t e = kind == KK ? k_empty(at) : kind == VK ? v_empty(at) : kn_empty, f = kind == KK ? k_full(at) : kind == VK ? v_full(at) : kn_full;
+                    const uint32_t dst = base + (kind == KN ? S::K_MN : (kind == KK ? S::K_RAW : S::V_RAW) + (at & 1u) * T::RAW);
+                    if (!mbar_wait(e, (kind == KN ? one(at) : two(at)) ^ 1u, p.status, 61)) return false;
+                    win_load<DP>(dst, kind == KK ? &map_kk : kind == VK ? &map_vk : &map_kn, f, keys.block(i) * AT_KEYS, it.h, it.b);
                     return true;
-                });
-                n0 += keys.count();
+                };
+                ok = load(KK, 0) && load(VK, 0) && load(KK, 1) && load(VK, 1);
+                // in the order in which places become free: S(i), dP(i), dQ(i - 1)
+                for (int i = 0; i < n && ok; ++i) ok = load(KN, i) && load(KK, i + 2) && load(VK, i + 2);
+                n0 += n;
             }
         }
     } else if (warp == 1) {
@@ -666,31 +789,44 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
                 const AttnItem it = attn_item(p, w, false);
                 if (it.skip) break;  // only the last round has items left out
                 const int n = TileKeys(p, it.unit * AT_ROWS).count();
-                ok = mbar_wait(q_ready, items & 1u, p.status, 62);
-                if (!ok) break;
-                ok = sequence(n, [&](int b, int i) {
-                    const uint32_t blk = base16 + S::BLOCKS_OFF / 16 + b * (S::BLOCK / 16), at = n0 + i, place = tmem + 128 * (at & 1u);
-                    if (b == KN && !mbar_wait(ds_ready(at), (at >> 1) & 1u, p.status, 63)) return false;
-                    if (!mbar_wait(conv(b), at & 1u, p.status, 64)) return false;
+                auto landed = [&](uint32_t b, uint32_t parity) {
+                    const bool r = mbar_wait(b, parity, p.status, 62);
                     after_sync();
-                    if (b == KK) issue_scores<DP>(place, tmem + 320, base16, blk);
-                    else if (b == VK) issue_scores<DP>(place + 64, tmem + 384, base16 + S::TWIN / 16, blk);
-                    else issue_values<DP, 16>(tmem + 256, place + 64, place, place + 8, blk, i > 0);
-                    umma_commit(empty(b));
-                    if (b == KK) umma_commit(s_full(at));
-                    else if (b == VK) umma_commit(dp_full(at));
+                    return r;
+                };
+                auto products = [&](int i) {  // S and dP of block i
+                    const uint32_t at = n0 + i, place = tmem + 128 * (at & 1u), raw = (at & 1u) * (T::RAW / 16), twin = (at & 1u) * (T::TWIN / 16);
+                    if (i >= n) return true;
+                    if (!landed(k_conv(at), two(at))) return false;
+                    win_scores<DP>(place, tmem + 320, base16, base16 + S::K_RAW / 16 + raw, base16 + S::K_TWIN / 16 + twin);
+                    umma_commit(k_empty(at));
+                    umma_commit(s_full(at));
+                    if (!landed(v_conv(at), two(at))) return false;
+                    win_scores<DP>(place + 64, tmem + 384, base16 + S::OWN / 16, base16 + S::V_RAW / 16 + raw, base16 + S::V_TWIN / 16 + twin);
+                    umma_commit(v_empty(at));
+                    umma_commit(dp_full(at));
                     return true;
-                });
+                };
+                ok = mbar_wait(q_ready, items & 1u, p.status, 63);
                 if (!ok) break;
-                umma_commit(acc_full);
+                ok = products(0);
+                for (int i = 0; i < n && ok; ++i) {
+                    const uint32_t at = n0 + i, place = tmem + 128 * (at & 1u);
+                    ok = products(i + 1) && mbar_wait(kn_full, one(at), p.status, 64) && landed(ds_ready(at), two(at));
+                    if (!ok) break;
+                    win_values<DP, 16>(tmem + 256, place + 64, place, place + 8, base16 + S::K_MN / 16, base16 + (S::K_TWIN + (at & 1u) * T::TWIN) / 16, i % WT_FLUSH != 0);
+                    umma_commit(kn_empty);
+                    umma_commit(k_free(at));
+                    if (i + 1 == n || (i + 1) % WT_FLUSH == 0) umma_commit(acc_full);
+                }
+                if (!ok) break;
                 n0 += n;
             }
         }
     } else if (warp >= 4 && warp < 12) {
         regs_give<56>();
-        // warps 4..7: the K-major blocks and the bias; warps 8..11: the MN-major blocks
         const int t = threadIdx.x & 127;
-        const bool k_major = warp < 8;
+        const bool of_k = warp < 8;
         uint32_t n0 = 0;
         bool ok = true;
         for (int64_t w = blockIdx.x; w < p.loop_end && ok; w += gridDim.x) {
@@ -700,32 +836,31 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
             const int n = keys.count();
             const float* tab = BIAS ? p.tab + (int64_t)it.h * p.tab_len : nullptr;
             float nb0 = 0.f, nb1 = 0.f;  // the next block's, loaded a block ahead
-            auto bias = [&](int i) {
-                if (!BIAS || !k_major) return;
+            auto request = [&](int i) {
                 const int d0 = it.unit * AT_ROWS - (keys.block(i) + 1) * AT_KEYS + 1;
                 nb0 = __ldg(tab + clamp_distance(d0 + t, p.tab_len));
                 nb1 = __ldg(tab + clamp_distance(d0 + t + 128, p.tab_len));
             };
-            bias(0);
-            ok = sequence(n, [&](int b, int i) {
-                if (k_major != (b <= VK)) return true;
-                if (!warp_wait(full(b), (n0 + i) & 1u, p.status, 65)) return false;
-                if (BIAS && b == KK) {
-                    // Three slots, by the running number of the block: this copy waited for the scores of the last block, which were asked for after
-                    // the dS of the third last had been made.
-                    float* tb = tabs + (n0 + i) % 3u * WT_TAB + t;
-                    tb[0] = nb0;
-                    if (t < WT_TAB - 128) tb[128] = nb1;
-                    if (i + 1 < n) bias(i + 1);
+            if (BIAS && of_k) request(0);
+            for (int i = 0; i < n && ok; ++i) {
+                const uint32_t at = n0 + i;
+                ok = warp_wait(of_k ? k_full(at) : v_full(at), two(at), p.status, 65);
+                if (!ok) break;
+                if (of_k) {  // the place is free once dQ of the block before last has read it; its bias was used before that
+                    ok = warp_wait(k_free(at), two(at) ^ 1u, p.status, 65);
+                    if (!ok) break;
+                    if (BIAS) {
+                        float* tb = reinterpret_cast<float*>(gen + S::TABS) + (at & 1u) * WT_TAB + t;
+                        tb[0] = nb0;
+                        if (t < WT_TAB - 128) tb[128] = nb1;
+                        if (i + 1 < n) request(i + 1);
+                    }
                 }
-                uint8_t* raw = gen + S::BLOCKS_OFF + b * S::BLOCK;
-                if (k_major) split_k_major<DP>(raw, t);
-                else split_mn_major<DP>(raw, raw + S::RAW, t);
+                win_split<DP, false>(gen + (of_k ? S::K_RAW : S::V_RAW) + (at & 1u) * T::RAW, gen + (of_k ? S::K_TWIN : S::V_TWIN) + (at & 1u) * T::TWIN, t);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(conv(b));
-                return true;
-            });
+                if (lane == 0) mbar_arrive(of_k ? k_conv(at) : v_conv(at));
+            }
             n0 += n;
         }
     } else if (warp >= 12) {
@@ -734,12 +869,14 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
         constexpr int OC = DP / 2;                                       // and half of the columns of q (parts 0, 1) or dO (2, 3)
         const int half = part & 1;
         const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
-        float* diag = reinterpret_cast<float*>(gen + DIAG_OFF + (warp - 12) * DIAG_WARP);
+        float* sums = reinterpret_cast<float*>(gen + S::DIAG);  // [warp][64]
+        float* diag = sums + (warp - 12) * 64;
+        float* xch = reinterpret_cast<float*>(gen + S::XCH);  // [half][row]: dO . O
         const float c = p.scale * kLog2e;
         const bool wants_dbias = BIAS && p.dbias_part != nullptr;
-        uint32_t n = 0, items = 0;
+        uint32_t n = 0, moved = 0;
         bool good = true;
-        for (int64_t w = blockIdx.x; w < p.loop_end; w += gridDim.x, ++items) {
+        for (int64_t w = blockIdx.x; w < p.loop_end; w += gridDim.x) {
             const AttnItem it = attn_item(p, w, false);
             if (it.skip) break;
             const int r0 = it.unit * AT_ROWS, r = r0 + row;
@@ -748,7 +885,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
             {
                 float x[OC];
                 load_row<DP / 32>(x, (part < 2 ? p.q + it.b * p.q_so + it.h * p.q_si + r * p.q_ld : p.g + it.b * p.g_so + it.h * p.g_si + r * p.g_ld) + half * OC, live, p.D - half * OC);
-                place_row<DP / 32>(x, lanes + (part < 2 ? 320 : 384) + half * OC, gen + (part >> 1) * S::TWIN + half * (OC / 16) * 8192, row);
+                place_row<DP / 32>(x, lanes + (part < 2 ? 320 : 384) + half * OC, gen + (part >> 1) * S::OWN + half * (OC / 16) * 8192, row);
                 if (part >= 2) {
                     float a = 0.0f;
                     const float* o = p.o + it.b * p.o_so + it.h * p.o_si + r * p.o_ld + half * OC;
@@ -770,6 +907,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
             const float beyond = BIAS ? __ldg(tab + p.tab_len - 1) : 0.0f;
             const TileKeys keys(p, r0);
             const int cnt = keys.count();
+            float* dst = p.dq + it.b * p.d_so + it.h * p.d_si + r * p.d_ld + 16 * part;
             // bias gradient: this lane's buckets, and what belongs to bucket `run_of` as a whole; buckets only go down along the walk
             float sum0 = 0.0f, sum1 = 0.0f, run = 0.0f;
             int run_of = p.rule.buckets - 1, near_of = run_of, far_of = run_of;
@@ -792,7 +930,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
 #pragma unroll
                         for (int e = 0; e < 16; ++e) pr[e] = ex2((fmaf(__uint_as_float(u[e]), p.scale, beyond) - m) * kLog2e) * inv;
                     } else {
-                        const float* mine = tabs + n % 3u * WT_TAB + row - 16 * part + AT_KEYS - 1;
+                        const float* mine = reinterpret_cast<const float*>(gen + S::TABS) + (n & 1u) * WT_TAB + row - 16 * part + AT_KEYS - 1;
 #pragma unroll
                         for (int e = 0; e < 16; ++e) pr[e] = ex2((fmaf(__uint_as_float(u[e]), p.scale, mine[-e]) - m) * kLog2e) * inv;
                     }
@@ -811,6 +949,12 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
 #pragma unroll
                 for (int e = 0; e < 16; ++e) pr[e] *= __uint_as_float(u[e]) - delta;  // a masked P is zero whatever dP holds
                 place_parts16(pr, place + 64 + 16 * part, place + 16 * part, place + 16 * part + 8);
+                if (i > 0 && i % WT_FLUSH == 0) {
+                    good = good && warp_wait(acc_full, moved & 1u, p.status, 68);
+                    ++moved;
+                    after_sync();
+                    if (16 * part < DP) move_sum(lanes + 256 + 16 * part, dst, p.D - 16 * part, live, i > WT_FLUSH, 1.0f);
+                }
                 tmem_stores_done();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(ds_ready(n));
@@ -825,17 +969,13 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
                         for (int e = 0; e < 16; ++e) a[e & 3] += pr[e];
                         run += (a[0] + a[1]) + (a[2] + a[3]);
                     } else {
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) diag[lane * 17 + e] = pr[e];
-                        __syncwarp();
                         float a = 0.0f, a2 = 0.0f;  // diagonals `lane` and `lane` + 32: distances d0 + lane, d0 + lane + 32
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            const int l = lane - 15 + e;
-                            if (l >= 0) a += diag[(l & 31) * 17 + e];
-                            if (l + 32 < 32) a2 += diag[((l + 32) & 31) * 17 + e];
+                        for (int e = 0; e < 16; ++e) {  // key e meets diagonal t at query t - 15 + e, and diagonal t + 32 at the same lane's number modulo 32
+                            const float x = __shfl_sync(0xffffffffu, pr[e], (lane + 17 + e) & 31);
+                            if (lane - 15 + e >= 0) a += x;
+                            else a2 += x;
                         }
-                        __syncwarp();
                         diag[lane] = a;
                         diag[32 + lane] = a2;
                         __syncwarp();
@@ -852,30 +992,32 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
                     }
                 }
             }
-            good = good && warp_wait(acc_full, items & 1u, p.status, 68);
+            good = good && warp_wait(acc_full, moved & 1u, p.status, 68);
+            ++moved;
             after_sync();
             if (wants_dbias) {
                 settle();
-                sums[(warp - 12) * AW_MAX_BUCKETS + lane] = sum0;
-                sums[(warp - 12) * AW_MAX_BUCKETS + 32 + lane] = sum1;
+                diag[lane] = sum0;
+                diag[32 + lane] = sum1;
             }
             if (all_any(!good)) break;  // all of them leave together
             const int t = threadIdx.x - 384;
             if (wants_dbias && t < p.rule.buckets) {
                 float a = 0.0f;
 #pragma unroll
-                for (int x = 0; x < 16; ++x) a += sums[x * AW_MAX_BUCKETS + t];
+                for (int x = 0; x < 16; ++x) a += sums[x * 64 + t];
                 p.dbias_part[(((int64_t)it.b * p.H + it.h) * p.units + it.unit) * p.rule.buckets + t] = a;
             }
             if (16 * part < DP) {
-                float* dst = p.dq + it.b * p.d_so + it.h * p.d_si + r * p.d_ld + 16 * part;
                 uint32_t x[16];
                 tmem_ld16(lanes + 256 + 16 * part, x);
                 if (live)
 #pragma unroll
                     for (int e = 0; e < 16; e += 4)
-                        if (16 * part + e < p.D)
-                            st4(dst + e, make_float4(p.scale * __uint_as_float(x[e]), p.scale * __uint_as_float(x[e + 1]), p.scale * __uint_as_float(x[e + 2]), p.scale * __uint_as_float(x[e + 3])));
+                        if (16 * part + e < p.D) {
+                            const float4 o = cnt > WT_FLUSH ? ld4(dst + e) : make_float4(0.f, 0.f, 0.f, 0.f);
+                            st4(dst + e, make_float4(p.scale * (o.x + __uint_as_float(x[e])), p.scale * (o.y + __uint_as_float(x[e + 1])), p.scale * (o.z + __uint_as_float(x[e + 2])), p.scale * (o.w + __uint_as_float(x[e + 3]))));
+                        }
             }
         }
     }
@@ -920,9 +1062,9 @@ static int run_fwd(gcb_ctx* ctx, const WindowTc& p, const CUtensorMap& k, const 
 template <int DP, bool BIAS>
 static int run_bwd(gcb_ctx* ctx, const WindowTc& p, const CUtensorMap& kk, const CUtensorMap& vk, const CUtensorMap& kn, const CUtensorMap& qk, const CUtensorMap& qn, const CUtensorMap& ok, const CUtensorMap& on) {
     static bool done_q[kMaxDevices] = {}, done_kv[kMaxDevices] = {};
-    int rc = tc_launch(ctx, window_attention_tc_dq_kernel<DP, BIAS>, done_q, AT_BWD_THREADS, AttnSmem<DP>::TOTAL, p, kk, vk, kn);
+    int rc = tc_launch(ctx, window_attention_tc_dq_kernel<DP, BIAS>, done_q, AT_BWD_THREADS, DqSmem<DP>::TOTAL, p, kk, vk, kn);
     if (!rc) rc = after_launch(ctx, "window_attention_tc_dq");
-    if (!rc) rc = tc_launch(ctx, window_attention_tc_dkv_kernel<DP, BIAS>, done_kv, AT_BWD_THREADS, AttnSmem<DP>::TOTAL, p, qk, qn, ok, on);
+    if (!rc) rc = tc_launch(ctx, window_attention_tc_dkv_kernel<DP, BIAS>, done_kv, AT_BWD_THREADS, DkvSmem<DP>::TOTAL, p, qk, qn, ok, on);
     return rc ? rc : after_launch(ctx, "window_attention_tc_dkv");
 }
 
@@ -945,7 +1087,7 @@ int window_tc_fwd(gcb_ctx* ctx, int64_t B, const WindowAttn& a) {
     int rc = make_table(ctx, p, tab);
     if (rc) return rc;
     CUtensorMap k, v;
-    GCB_REQUIRE(encode_rows(enc, &k, a.k, a.D, a.T, a.k_ld, a.k_si, a.k_so, a.H, B, 16, AT_KEYS, CU_TENSOR_MAP_SWIZZLE_64B) &&
+    GCB_REQUIRE(encode_rows(enc, &k, a.k, a.D, a.T, a.k_ld, a.k_si, a.k_so, a.H, B, 32, AT_KEYS, CU_TENSOR_MAP_SWIZZLE_128B) &&
                     encode_rows(enc, &v, a.v, a.D, a.T, a.v_ld, a.v_si, a.v_so, a.H, B, 32, AT_KEYS, CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B),
                 "window attention: strides beyond what TMA can address");
     rc = p.tab ? (a.D <= 32 ? run_fwd<32, true>(ctx, p, k, v) : run_fwd<64, true>(ctx, p, k, v)) : (a.D <= 32 ? run_fwd<32, false>(ctx, p, k, v) : run_fwd<64, false>(ctx, p, k, v));
@@ -963,7 +1105,7 @@ int window_tc_bwd(gcb_ctx* ctx, int64_t B, const WindowAttn& a) {
     p.delta = delta.as<float>();
     CUtensorMap kk, vk, kn, qk, qn, ok, on;
     auto rows = [&](CUtensorMap* map, const float* x, int64_t ld, int64_t so, int64_t si, bool k_major) {
-        return encode_rows(enc, map, x, a.D, a.T, ld, si, so, a.H, B, k_major ? 16 : 32, AT_KEYS, k_major ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B);
+        return encode_rows(enc, map, x, a.D, a.T, ld, si, so, a.H, B, 32, AT_KEYS, k_major ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B);
     };
     GCB_REQUIRE(rows(&kk, a.k, a.k_ld, a.k_so, a.k_si, true) && rows(&kn, a.k, a.k_ld, a.k_so, a.k_si, false) && rows(&vk, a.v, a.v_ld, a.v_so, a.v_si, true) && rows(&qk, a.q, a.q_ld, a.q_so, a.q_si, true) &&
                     rows(&qn, a.q, a.q_ld, a.q_so, a.q_si, false) && rows(&ok, a.g, a.g_ld, a.g_so, a.g_si, true) && rows(&on, a.g, a.g_ld, a.g_so, a.g_si, false),
