@@ -28,6 +28,7 @@ struct WindowTc {
     int64_t q_ld, q_so, q_si, k_ld, k_so, k_si, v_ld, v_so, v_si, g_ld, g_so, g_si, o_ld, o_so, o_si, d_ld, d_so, d_si;
     const float *q, *k, *v, *g, *o;
     float *out, *dq, *dk, *dv, *row_max, *row_inv, *delta, *dbias_part;
+    float* moved;      // 64 KB a CTA, where an item may have more than WT_FLUSH blocks
     const float* tab;  // [H][tab_len]: bias by distance, the last one for all distances beyond; NULL: no bias
     int tab_len;
     int64_t Tp;
@@ -139,25 +140,65 @@ __device__ __forceinline__ void win_values(uint32_t d, uint32_t a_t, uint32_t a_
         umma_bf16_ts(d, a_big + STEP * kb, tile_desc<WinTile<DP>::ROWS8, 128, 0>(tw + small), idesc_bf, 1u);
     }
 }
-// Moves 16 columns of a sum out of tensor memory: dst = (there ? dst * f : 0) + sum, columns up to `cols`.
+// The 128 rows a CTA owns of an operand or of a result pass through shared memory, as TMA moves them: [32 columns][128 rows][128 bytes], 128-byte swizzle.
+// (Threads that load and store the row they own, 16 bytes of 32 different lines an instruction, took 20 000 cycles an item where this takes 4000.)
+// A loaded tile lies where its companions go: threads read their rows, wait for one another, and write the companions over it.
+template <int DP>
+__device__ __forceinline__ void own_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int r0, int h, int b) {
+    mbar_expect_tx(bar, AT_ROWS * DP * 4);
+#pragma unroll
+    for (int c = 0; c < DP / 32; ++c)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) tma_load_4d(dst + c * 16384 + x * 8192, map, bar, 32 * c, r0 + 64 * x, h, b);
+}
+template <int DP>
+__device__ __forceinline__ void own_store(const CUtensorMap* map, uint32_t src, const WindowTc& p, int r0, int h, int b) {
+#pragma unroll
+    for (int c = 0; c < DP / 32; ++c)
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+            if (32 * c < p.D && r0 + 64 * x < p.T) tma_store_4d(map, src + c * 16384 + x * 8192, 32 * c, r0 + 64 * x, h, b);
+}
+__device__ __forceinline__ float4* own_at(uint8_t* tile, int row, int col) { return reinterpret_cast<float4*>(tile + (col >> 5) * 16384 + row * 128 + ((((col & 31) >> 2) ^ (row & 7)) << 4)); }
+template <int N>
+__device__ __forceinline__ void own_read(float (&x)[N], uint8_t* tile, int row, int col) {
+#pragma unroll
+    for (int e = 0; e < N; e += 4) {
+        const float4 f = *own_at(tile, row, col + e);
+        x[e] = f.x; x[e + 1] = f.y; x[e + 2] = f.z; x[e + 3] = f.w;
+    }
+}
+// Moves 16 columns of a sum from tensor memory to a CTA's place in `moved`, [which][column / 4][row][4]: moved = (there ? moved * f : 0) + sum.
 // The tensor core truncates when it adds, so that a sum over hundreds of instructions comes out too small by half a unit for each (8192 keys in one
 // sum: 6e-5 of the result); one of WT_FLUSH blocks, 128 instructions, is off by 3e-6, and these are added here with rounding.
-__device__ __forceinline__ void move_sum(uint32_t taddr, float* dst, int cols, bool live, bool there, float f) {
+__device__ __forceinline__ void move_sum(uint32_t taddr, float* moved, bool there, float f) {
     uint32_t x[16];
     tmem_ld16(taddr, x);
-    if (!live) return;
 #pragma unroll
-    for (int e = 0; e < 16; e += 4)
-        if (e < cols) {
-            const float4 o = there ? ld4(dst + e) : make_float4(0.f, 0.f, 0.f, 0.f);
-            st4(dst + e, make_float4(fmaf(o.x, f, __uint_as_float(x[e])), fmaf(o.y, f, __uint_as_float(x[e + 1])), fmaf(o.z, f, __uint_as_float(x[e + 2])), fmaf(o.w, f, __uint_as_float(x[e + 3]))));
-        }
+    for (int e = 0; e < 4; ++e) {
+        float* at = moved + e * 4 * AT_ROWS;
+        const float4 o = there ? ld4(at) : make_float4(0.f, 0.f, 0.f, 0.f);
+        st4(at, make_float4(fmaf(o.x, f, __uint_as_float(x[4 * e])), fmaf(o.y, f, __uint_as_float(x[4 * e + 1])), fmaf(o.z, f, __uint_as_float(x[4 * e + 2])), fmaf(o.w, f, __uint_as_float(x[4 * e + 3]))));
+    }
 }
+// 16 columns of a result on their way out: a sum in tensor memory times f, plus what has moved times f_moved.
+__device__ __forceinline__ void place_result(uint8_t* tile, int row, int col, uint32_t taddr, const float* moved, bool there, float f, float f_moved) {
+    uint32_t x[16];
+    tmem_ld16(taddr, x);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float4 o = there ? ld4(moved + e * 4 * AT_ROWS) : make_float4(0.f, 0.f, 0.f, 0.f);
+        *own_at(tile, row, col + 4 * e) = make_float4(fmaf(o.x, f_moved, __uint_as_float(x[4 * e]) * f), fmaf(o.y, f_moved, __uint_as_float(x[4 * e + 1]) * f), fmaf(o.z, f_moved, __uint_as_float(x[4 * e + 2]) * f),
+                                                      fmaf(o.w, f_moved, __uint_as_float(x[4 * e + 3]) * f));
+    }
+}
+__device__ __forceinline__ float* moved_at(const WindowTc& p, int which, int col, int row) { return p.moved + ((int64_t)blockIdx.x * 2 + which) * 64 * AT_ROWS + (col * AT_ROWS + row * 4); }
 
 // ---- forward ------------------------------------------------------------------------------------------------------------------
 // Tensor memory of query tile q, from column 256 q: scores / t of P [0, 64), bf16(P) [64, 96), bf16(P - t) [96, 128), O [128, 192), t of q [192, 256).
 template <int DP, bool BIAS>
-__global__ void __launch_bounds__(AT_FWD_THREADS, 1) window_attention_tc_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ WindowTc p) {
+__global__ void __launch_bounds__(AT_FWD_THREADS, 1) window_attention_tc_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_q,
+                                                                                    const __grid_constant__ CUtensorMap map_o, const __grid_constant__ WindowTc p) {
     using S = AttnSmem<DP>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -170,13 +211,14 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 1) window_attention_tc_fwd_ker
     auto p_ready = [&](int q) { return bars + 8u * (14 + q); };
     auto o_full = [&](int q) { return bars + 8u * (16 + q); };
     auto q_ready = [&](int q) { return bars + 8u * (18 + q); };
+    auto own_full = [&](int q) { return bars + 8u * (20 + q); };
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int b = 0; b < 4; ++b) { mbar_init(full(b), 1); mbar_init(conv(b), 4); mbar_init(empty(b), 1); }
-        for (int q = 0; q < 2; ++q) { mbar_init(s_full(q), 1); mbar_init(p_ready(q), 8); mbar_init(o_full(q), 1); mbar_init(q_ready(q), 8); }
+        for (int q = 0; q < 2; ++q) { mbar_init(s_full(q), 1); mbar_init(p_ready(q), 8); mbar_init(o_full(q), 1); mbar_init(q_ready(q), 8); mbar_init(own_full(q), 1); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    const uint32_t tmem = tmem_take(bars + 8u * 20, reinterpret_cast<volatile uint32_t*>(gen + S::BAR_OFF + 8 * 20), warp);
+    const uint32_t tmem = tmem_take(bars + 8u * 24, reinterpret_cast<volatile uint32_t*>(gen + S::BAR_OFF + 8 * 24), warp);
     pdl_trigger();
     pdl_wait();
     auto tile_row = [&](const AttnItem& it, int q) { return q < p.tiles_per_unit ? (it.unit * p.tiles_per_unit + q) * AT_ROWS : p.T; };
@@ -303,8 +345,19 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 1) window_attention_tc_fwd_ker
         float* tabs = reinterpret_cast<float*>(gen + S::STAGE_OFF + 2048) + q * 2 * WT_TAB;
         constexpr int OC = DP / 2;
         const float c = BIAS ? kLog2e : p.scale * kLog2e;  // scores, or scores before the scale, to log2 units
-        uint32_t s_phase = 0, o_phase = 0;
+        uint32_t s_phase = 0, o_phase = 0, items = 0;
         bool ok = true;
+        uint8_t* own = gen + q * S::TWIN;
+        // this tile's rows of the item at w or the next one that has any
+        auto fetch = [&](int64_t w) {
+            for (; w < p.loop_end; w += gridDim.x) {
+                const AttnItem it = attn_item(p, w, false);
+                if (it.skip || tile_row(it, q) >= p.T) continue;
+                own_load<DP>(base + q * S::TWIN, &map_q, own_full(q), tile_row(it, q), it.h, it.b);
+                break;
+            }
+        };
+        if (at_tile == 0) fetch(blockIdx.x);
         for (int64_t w = blockIdx.x; w < p.loop_end && ok; w += gridDim.x) {
             const AttnItem it = attn_item(p, w, false);
             if (it.skip) continue;
@@ -314,9 +367,12 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 1) window_attention_tc_fwd_ker
             if (!blocks) continue;
             const int r = r0 + row;
             const bool live = r < p.T;
+            bool good = warp_wait(own_full(q), items & 1u, p.status, 49);  // every thread keeps step with the barriers below, whatever a wait says
+            ++items;
             {
                 float x[OC];
-                load_row<DP / 32>(x, p.q + it.b * p.q_so + it.h * p.q_si + r * p.q_ld + half * OC, live, p.D - half * OC);
+                own_read(x, own, row, half * OC);
+                pair_sync(bar);
                 place_row<DP / 32>(x, t0 + 192 + half * OC, gen + q * S::TWIN + half * (OC / 16) * 8192, row);
             }
             tmem_stores_done();
@@ -332,20 +388,19 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 1) window_attention_tc_fwd_ker
                 if (at_tile < WT_DIAG) tabs[at_tile] = request(keys.begin());
                 pair_sync(bar);
             }
-            float* dst = p.out + it.b * p.o_so + it.h * p.o_si + r * p.o_ld + half * OC;
+            float* moved = moved_at(p, q, half * OC, row);
             float m = -INFINITY, sum = 0.0f, m_out = -INFINITY;  // m: the maximum the probabilities are relative to; m_out: the one what has moved to `out` is
-            bool good = true;
             for (int j = 0; j < blocks; ++j) {
                 const int b = keys.block(j);
                 float ahead = 0.0f;
                 if (BIAS && j + 1 < blocks) ahead = request(keys.block(j + 1));
-                good = good && warp_wait(s_full(q), s_phase & 1u, p.status, 47);  // every thread keeps step with the barriers below, whatever a wait says
+                good = good && warp_wait(s_full(q), s_phase & 1u, p.status, 47);
                 ++s_phase;
                 after_sync();
                 if (j > 0 && j % WT_FLUSH == 0) {  // the products of the blocks before came before these scores
                     const float f = m_out == m ? 1.0f : ex2((m_out - m) * c);
 #pragma unroll
-                    for (int g = 0; g < OC / 16; ++g) move_sum(t0 + 128 + half * OC + 16 * g, dst + 16 * g, p.D - half * OC - 16 * g, live, j > WT_FLUSH, f);
+                    for (int g = 0; g < OC / 16; ++g) move_sum(t0 + 128 + half * OC + 16 * g, moved + 16 * g * AT_ROWS, j > WT_FLUSH, f);
                     m_out = m;
                 }
                 float v[32];
@@ -412,20 +467,16 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 1) window_attention_tc_fwd_ker
             const float inv = empty_row ? 0.0f : 1.0f / (sum + xch[(half ^ 1) * 128 + row]);
             pair_sync(bar);
             if (!ok) break;
-            const bool there = blocks > WT_FLUSH;
-            const float fo = inv * (m_out == m ? 1.0f : ex2((m_out - m) * c));
+            const float inv_moved = inv * (m_out == m ? 1.0f : ex2((m_out - m) * c));
 #pragma unroll
-            for (int g = 0; g < OC / 16; ++g) {
-                uint32_t x[16];
-                tmem_ld16(t0 + 128 + half * OC + 16 * g, x);
-                if (live)
-#pragma unroll
-                    for (int e = 0; e < 16; e += 4)
-                        if (half * OC + 16 * g + e < p.D) {
-                            const float4 o = there ? ld4(dst + 16 * g + e) : make_float4(0.f, 0.f, 0.f, 0.f);
-                            st4(dst + 16 * g + e, make_float4(fmaf(o.x, fo, __uint_as_float(x[e]) * inv), fmaf(o.y, fo, __uint_as_float(x[e + 1]) * inv), fmaf(o.z, fo, __uint_as_float(x[e + 2]) * inv),
-                                                              fmaf(o.w, fo, __uint_as_float(x[e + 3]) * inv)));
-                        }
+            for (int g = 0; g < OC / 16; ++g) place_result(own, row, half * OC + 16 * g, t0 + 128 + half * OC + 16 * g, moved + 16 * g * AT_ROWS, blocks > WT_FLUSH, inv, inv_moved);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            pair_sync(bar);
+            if (at_tile == 0) {
+                own_store<DP>(&map_o, base + q * S::TWIN, p, r0, it.h, it.b);
+                tma_store_commit();
+                tma_store_wait_read<0>();
+                fetch(w + gridDim.x);
             }
             if (half == 0 && live) {
                 const int64_t at = ((int64_t)it.b * p.H + it.h) * p.Tp + r;
@@ -433,6 +484,7 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 1) window_attention_tc_fwd_ker
                 p.row_inv[at] = inv;
             }
         }
+        if (at_tile == 0) tma_store_wait_all();
     }
     tmem_give(tmem, warp);
 }
@@ -443,21 +495,23 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 1) window_attention_tc_fwd_ker
 // and dK(i), dP(i+1) while P(i+1) is.
 //   warp 0       TMA producer        warp 1       MMA issuer
 //   warps 4..7   companions of q, the statistics of its rows and the bias        warps 8..11  companions of dO        warps 12..27  four threads a key
-// A tile of q arrives K-major, a block ahead, and once more MN-major; so does dO.  Companions stay until the tile's second product has read them.
+// A tile of q arrives K-major and once more MN-major; so does dO.  Companions stay until the tile's second product has read them: three places for
+// those of q, so that a block's scores do not wait for dK of the block before.
 // Tensor memory: S^T / t of P^T [0, 64), dP^T / t of dS^T [64, 128), P^T companions [128, 192), dS^T companions [192, 256), dV [256, 320), dK [320, 384),
 // t of k [384, 448), t of v [448, 512).
 template <int DP>
 struct DkvSmem {
     using T = WinTile<DP>;
     static constexpr int OWN = AT_ROWS * DP * 4;  // companions of a 128-row operand
-    static constexpr int Q_RAW = 2 * OWN, O_RAW = Q_RAW + 2 * T::RAW, Q_MN = O_RAW + T::RAW, O_MN = Q_MN + T::RAW, Q_TWIN = O_MN + T::RAW, O_TWIN = Q_TWIN + 2 * T::TWIN;
-    static constexpr int STATS = O_TWIN + 2 * T::TWIN;  // row maximum, 1 / sum and dO . O of a block's queries, two blocks; then the bias of its distances, two blocks
-    static constexpr int TABS = STATS + 2 * 3 * AT_KEYS * 4, BAR = TABS + 2 * WT_TAB * 4, TOTAL = BAR + 256 + 1024;
+    static constexpr int Q_RAW = 2 * OWN, O_RAW = Q_RAW + T::RAW, Q_MN = O_RAW + T::RAW, O_MN = Q_MN + T::RAW, Q_TWIN = O_MN + T::RAW, O_TWIN = Q_TWIN + 3 * T::TWIN;
+    static constexpr int STATS = O_TWIN + 2 * T::TWIN;  // row maximum, 1 / sum and dO . O of a block's queries, three blocks; then the bias of its distances, three blocks
+    static constexpr int TABS = STATS + 3 * 3 * AT_KEYS * 4, BAR = TABS + 3 * WT_TAB * 4, TOTAL = BAR + 256 + 1024;
     static_assert(TOTAL <= 232448, "shared memory");
 };
 template <int DP, bool BIAS>
 __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_kernel(const __grid_constant__ CUtensorMap map_qk, const __grid_constant__ CUtensorMap map_qn, const __grid_constant__ CUtensorMap map_ok,
-                                                                                const __grid_constant__ CUtensorMap map_on, const __grid_constant__ WindowTc p) {
+                                                                                const __grid_constant__ CUtensorMap map_on, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                                                                                const __grid_constant__ CUtensorMap map_dk, const __grid_constant__ CUtensorMap map_dv, const __grid_constant__ WindowTc p) {
     using S = DkvSmem<DP>;
     using T = WinTile<DP>;
     extern __shared__ uint8_t smem_raw[];
@@ -469,20 +523,19 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
     // n: running number of a block; parities of what has two places and of what has one
     auto two = [](uint32_t n) { return (n >> 1) & 1u; };
     auto one = [](uint32_t n) { return n & 1u; };
-    auto q_full = [&](uint32_t n) { return bar(0 + (n & 1u)); };
-    auto q_empty = [&](uint32_t n) { return bar(2 + (n & 1u)); };
-    auto q_conv = [&](uint32_t n) { return bar(4 + (n & 1u)); };
-    auto q_free = [&](uint32_t n) { return bar(6 + (n & 1u)); };   // companions: dK has read them
-    auto o_conv = [&](uint32_t n) { return bar(8 + (n & 1u)); };
-    auto o_free = [&](uint32_t n) { return bar(10 + (n & 1u)); };  // dV has read them
-    const uint32_t o_full = bar(12), o_empty = bar(13), on_full = bar(14), on_empty = bar(15), qn_full = bar(16), qn_empty = bar(17);
-    const uint32_t s_full = bar(18), dp_full = bar(19), p_ready = bar(20), ds_ready = bar(21), acc_full = bar(22), kv_ready = bar(23);
+    auto three = [](uint32_t n) { return (n / 3u) & 1u; };
+    auto q_conv = [&](uint32_t n) { return bar(0 + n % 3u); };
+    auto q_free = [&](uint32_t n) { return bar(3 + n % 3u); };    // companions: dK has read them
+    auto o_conv = [&](uint32_t n) { return bar(6 + (n & 1u)); };
+    auto o_free = [&](uint32_t n) { return bar(8 + (n & 1u)); };  // dV has read them
+    const uint32_t q_full = bar(10), q_empty = bar(11), o_full = bar(12), o_empty = bar(13), on_full = bar(14), on_empty = bar(15), qn_full = bar(16), qn_empty = bar(17);
+    const uint32_t s_full = bar(18), dp_full = bar(19), p_ready = bar(20), ds_ready = bar(21), acc_full = bar(22), kv_ready = bar(23), own_full = bar(24);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 24; ++i) mbar_init(bar(i), i == 4 || i == 5 || i == 8 || i == 9 ? 4 : i == 20 || i == 21 || i == 23 ? 16 : 1);
+        for (int i = 0; i < 25; ++i) mbar_init(bar(i), i < 3 || i == 6 || i == 7 ? 4 : i == 20 || i == 21 || i == 23 ? 16 : i == 24 ? 2 : 1);  // own_full: two tiles
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    const uint32_t tmem = tmem_take(bars + 8u * 24, reinterpret_cast<volatile uint32_t*>(gen + S::BAR + 8 * 24), warp);
+    const uint32_t tmem = tmem_take(bars + 8u * 28, reinterpret_cast<volatile uint32_t*>(gen + S::BAR + 8 * 28), warp);
     pdl_trigger();
     pdl_wait();
     auto steps = [&](const AttnItem& it) {  // blocks of queries from the tile's first key to the last query that sees its last one
@@ -502,15 +555,15 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
                 auto load = [&](int kind, int i) {
                     if (i >= n) return true;
                     const uint32_t at = n0 + i;
-                    const uint32_t e = kind == QK ? q_empty(at) : kind == OK ? o_empty : kind == ON ? on_empty : qn_empty, f = kind == QK ? q_full(at) : kind == OK ? o_full : kind == ON ? on_full : qn_full;
-                    const uint32_t dst = base + (kind == QK ? S::Q_RAW + (at & 1u) * T::RAW : kind == OK ? S::O_RAW : kind == ON ? S::O_MN : S::Q_MN);
-                    if (!mbar_wait(e, (kind == QK ? two(at) : one(at)) ^ 1u, p.status, 51)) return false;
+                    const uint32_t e = kind == QK ? q_empty : kind == OK ? o_empty : kind == ON ? on_empty : qn_empty, f = kind == QK ? q_full : kind == OK ? o_full : kind == ON ? on_full : qn_full;
+                    const uint32_t dst = base + (kind == QK ? S::Q_RAW : kind == OK ? S::O_RAW : kind == ON ? S::O_MN : S::Q_MN);
+                    if (!mbar_wait(e, one(at) ^ 1u, p.status, 51)) return false;
                     win_load<DP>(dst, kind == QK ? &map_qk : kind == OK ? &map_ok : kind == ON ? &map_on : &map_qn, f, it.unit * AT_ROWS + i * AT_KEYS, it.h, it.b);
                     return true;
                 };
-                ok = load(QK, 0) && load(OK, 0) && load(QK, 1);
-                // in the order in which places become free: dV(i - 1), S(i), dK(i - 1), dP(i)
-                for (int i = 0; i < n && ok; ++i) ok = load(ON, i) && load(QK, i + 2) && load(QN, i) && load(OK, i + 1);
+                ok = load(QK, 0) && load(OK, 0);
+                // in the order in which places become free: S(i), dV(i - 1), dP(i), dK(i - 1)
+                for (int i = 0; i < n && ok; ++i) ok = load(QK, i + 1) && load(ON, i) && load(OK, i + 1) && load(QN, i);
                 n0 += n;
             }
         }
@@ -531,9 +584,9 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
                 auto scores = [&](int i) {
                     const uint32_t at = n0 + i;
                     if (i >= n) return true;
-                    if (!landed(q_conv(at), two(at))) return false;
-                    win_scores<DP>(tmem, tmem + 384, base16, base16 + (S::Q_RAW + (at & 1u) * T::RAW) / 16, base16 + (S::Q_TWIN + (at & 1u) * T::TWIN) / 16);
-                    umma_commit(q_empty(at));
+                    if (!landed(q_conv(at), three(at))) return false;
+                    win_scores<DP>(tmem, tmem + 384, base16, base16 + S::Q_RAW / 16, base16 + (S::Q_TWIN + at % 3u * T::TWIN) / 16);
+                    umma_commit(q_empty);
                     umma_commit(s_full);
                     return true;
                 };
@@ -558,7 +611,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
                     umma_commit(o_free(at));
                     ok = scores(i + 1) && mbar_wait(qn_full, one(at), p.status, 55) && landed(ds_ready, one(at));
                     if (!ok) break;
-                    win_values<DP, 8>(tmem + 320, tmem + 64, tmem + 192, tmem + 224, base16 + S::Q_MN / 16, base16 + (S::Q_TWIN + (at & 1u) * T::TWIN) / 16, i % WT_FLUSH != 0);
+                    win_values<DP, 8>(tmem + 320, tmem + 64, tmem + 192, tmem + 224, base16 + S::Q_MN / 16, base16 + (S::Q_TWIN + at % 3u * T::TWIN) / 16, i % WT_FLUSH != 0);
                     umma_commit(qn_empty);
                     umma_commit(q_free(at));
                     ok = dprobs(i + 1);
@@ -595,22 +648,22 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
             if (of_q) request(0);
             for (int i = 0; i < n && ok; ++i) {
                 const uint32_t at = n0 + i;
-                ok = warp_wait(of_q ? q_full(at) : o_full, of_q ? two(at) : one(at), p.status, 56);
+                ok = warp_wait(of_q ? q_full : o_full, one(at), p.status, 56);
                 if (!ok) break;
-                // the place is free once the second product of the block before last has read it; its statistics were used before that
-                ok = warp_wait(of_q ? q_free(at) : o_free(at), two(at) ^ 1u, p.status, 56);
+                ok = warp_wait(of_q ? q_free(at) : o_free(at), (of_q ? three(at) : two(at)) ^ 1u, p.status, 56);  // the second product that read what is there
                 if (!ok) break;
                 if (of_q) {
-                    float* slot = reinterpret_cast<float*>(gen + S::STATS) + (at & 1u) * 3 * AT_KEYS + t;
-                    if (t < AT_KEYS) { slot[0] = BIAS ? nm : nm * kLog2e; slot[AT_KEYS] = ni; slot[2 * AT_KEYS] = nd; }
+                    // in three places as well: what was there has been used by the block whose companions these replace
+                    float* slot = reinterpret_cast<float*>(gen + S::STATS) + at % 3u * 3 * AT_KEYS + t;
+                    if (t < AT_KEYS) { slot[0] = BIAS ? nm : nm * kLog2e - log2f(ni); slot[AT_KEYS] = ni; slot[2 * AT_KEYS] = nd; }
                     if (BIAS) {
-                        float* tb = reinterpret_cast<float*>(gen + S::TABS) + (at & 1u) * WT_TAB + t;
+                        float* tb = reinterpret_cast<float*>(gen + S::TABS) + at % 3u * WT_TAB + t;
                         tb[0] = nb0;
                         if (t < WT_TAB - 128) tb[128] = nb1;
                     }
                     if (i + 1 < n) request(i + 1);
                 }
-                win_split<DP, false>(gen + (of_q ? S::Q_RAW + (at & 1u) * T::RAW : S::O_RAW), gen + (of_q ? S::Q_TWIN : S::O_TWIN) + (at & 1u) * T::TWIN, t);
+                win_split<DP, false>(gen + (of_q ? S::Q_RAW : S::O_RAW), gen + (of_q ? S::Q_TWIN + at % 3u * T::TWIN : S::O_TWIN + (at & 1u) * T::TWIN), t);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(of_q ? q_conv(at) : o_conv(at));
@@ -625,48 +678,60 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
         const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
         const float c = p.scale * kLog2e;
         uint32_t n = 0, items = 0;
-        bool ok = true;
-        for (int64_t w = blockIdx.x; w < p.loop_end && ok; w += gridDim.x, ++items) {
+        bool good = true;
+        uint8_t* own = gen + (part >> 1) * S::OWN;
+        auto fetch = [&](int64_t w) {  // the rows of the item at w
+            if (w >= p.loop_end) return;
+            const AttnItem it = attn_item(p, w, true);
+            if (it.skip) return;
+            own_load<DP>(base, &map_k, own_full, it.unit * AT_ROWS, it.h, it.b);
+            own_load<DP>(base + S::OWN, &map_v, own_full, it.unit * AT_ROWS, it.h, it.b);
+        };
+        if (threadIdx.x == 384) fetch(blockIdx.x);
+        for (int64_t w = blockIdx.x; w < p.loop_end; w += gridDim.x, ++items) {
             const AttnItem it = attn_item(p, w, true);
             if (it.skip) break;
-            const int key = it.unit * AT_ROWS + row;
-            const bool live = key < p.T;
+            good = good && warp_wait(own_full, items & 1u, p.status, 50);  // every thread keeps step with the barriers of the items, whatever a wait says
             {
                 float x[OC];
-                load_row<DP / 32>(x, (part < 2 ? p.k + it.b * p.k_so + it.h * p.k_si + key * p.k_ld : p.v + it.b * p.v_so + it.h * p.v_si + key * p.v_ld) + half * OC, live, p.D - half * OC);
-                place_row<DP / 32>(x, lanes + (part < 2 ? 384 : 448) + half * OC, gen + (part >> 1) * S::OWN + half * (OC / 16) * 8192, row);
+                own_read(x, own, row, half * OC);
+                all_any(false);
+                place_row<DP / 32>(x, lanes + (part < 2 ? 384 : 448) + half * OC, own + half * (OC / 16) * 8192, row);
             }
             tmem_stores_done();
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(kv_ready);
             const int cnt = steps(it);
-            float* dst = (part < 2 ? p.dk : p.dv) + it.b * p.d_so + it.h * p.d_si + key * p.d_ld + half * OC;
+            float* moved = moved_at(p, part >> 1, half * OC, row);
             auto move = [&](bool there) {
 #pragma unroll
-                for (int g = 0; g < OC / 16; ++g) move_sum(lanes + (part < 2 ? 320 : 256) + half * OC + 16 * g, dst + 16 * g, p.D - half * OC - 16 * g, live, there, 1.0f);
+                for (int g = 0; g < OC / 16; ++g) move_sum(lanes + (part < 2 ? 320 : 256) + half * OC + 16 * g, moved + 16 * g * AT_ROWS, there, 1.0f);
             };
 #pragma unroll 1
             for (int i = 0; i < cnt; ++i, ++n) {
-                const float4* mp = reinterpret_cast<const float4*>(gen + S::STATS + (n & 1u) * 3 * AT_KEYS * 4) + 4 * part;
+                const float4* mp = reinterpret_cast<const float4*>(gen + S::STATS + n % 3u * 3 * AT_KEYS * 4) + 4 * part;
                 const float4 *ip = mp + AT_KEYS / 4, *dp = ip + AT_KEYS / 4;
-                ok = warp_wait(s_full, n & 1u, p.status, 57);
-                if (!ok) break;
+                good = good && warp_wait(s_full, n & 1u, p.status, 57);
                 after_sync();
                 if (part >= 2 && i > 0 && i % WT_FLUSH == 0) move(i > WT_FLUSH);  // dV of the blocks before came before these scores
                 uint32_t u[16];
                 float pr[16];
                 tmem_ld16(lanes + 16 * part, u);
                 const int first = row - i * AT_KEYS - 16 * part;  // queries from here on look at this key, as many as the window is long
-                const float* bias = reinterpret_cast<const float*>(gen + S::TABS) + (n & 1u) * WT_TAB + (AT_ROWS - 1) + 16 * part - row;
+                const float* bias = reinterpret_cast<const float*>(gen + S::TABS) + n % 3u * WT_TAB + (AT_ROWS - 1) + 16 * part - row;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float4 m = mp[e], iv = ip[e];
-                    const float mm[4] = {m.x, m.y, m.z, m.w}, ii[4] = {iv.x, iv.y, iv.z, iv.w};
+                    const float4 m = mp[e];
+                    const float mm[4] = {m.x, m.y, m.z, m.w};
+                    if (BIAS) {
+                        const float4 iv = ip[e];
+                        const float ii[4] = {iv.x, iv.y, iv.z, iv.w};
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        const float s = __uint_as_float(u[4 * e + x]);
-                        pr[4 * e + x] = (BIAS ? ex2((fmaf(s, p.scale, bias[4 * e + x]) - mm[x]) * kLog2e) : ex2(fmaf(s, c, -mm[x]))) * ii[x];
+                        for (int x = 0; x < 4; ++x) pr[4 * e + x] = ex2((fmaf(__uint_as_float(u[4 * e + x]), p.scale, bias[4 * e + x]) - mm[x]) * kLog2e) * ii[x];
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) pr[4 * e + x] = ex2(fmaf(__uint_as_float(u[4 * e + x]), c, -mm[x]));
                     }
                 }
                 if (i < 2 || (p.rule.W > 0 && (i + 1) * AT_KEYS > p.rule.W)) {  // the diagonal block, and those the window ends in
@@ -678,16 +743,15 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
                 tmem_stores_done();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_ready);
-                ok = warp_wait(dp_full, n & 1u, p.status, 58);
-                if (!ok) break;
+                good = good && warp_wait(dp_full, n & 1u, p.status, 58);
                 after_sync();
                 tmem_ld16(lanes + 64 + 16 * part, u);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {  // dS = scale P (dP - dO . O); a masked P is zero whatever dP holds
+                for (int e = 0; e < 4; ++e) {  // a masked P is zero whatever dP holds; the scale comes last
                     const float4 d = dp[e];
                     const float dd[4] = {d.x, d.y, d.z, d.w};
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) pr[4 * e + x] = pr[4 * e + x] * p.scale * (__uint_as_float(u[4 * e + x]) - dd[x]);
+                    for (int x = 0; x < 4; ++x) pr[4 * e + x] *= __uint_as_float(u[4 * e + x]) - dd[x];
                 }
                 place_parts16(pr, lanes + 64 + 16 * part, lanes + 192 + 8 * part, lanes + 224 + 8 * part);
                 if (part < 2 && i > 0 && i % WT_FLUSH == 0) move(i > WT_FLUSH);  // dK of the blocks before came before this dP
@@ -695,12 +759,22 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
                 __syncwarp();
                 if (lane == 0) mbar_arrive(ds_ready);
             }
-            if (!ok) break;
-            ok = warp_wait(acc_full, items & 1u, p.status, 59);
-            if (!ok) break;
+            good = good && warp_wait(acc_full, items & 1u, p.status, 59);
             after_sync();
-            move(cnt > WT_FLUSH);
+            const float f = part < 2 ? p.scale : 1.0f;
+#pragma unroll
+            for (int g = 0; g < OC / 16; ++g) place_result(own, row, half * OC + 16 * g, lanes + (part < 2 ? 320 : 256) + half * OC + 16 * g, moved + 16 * g * AT_ROWS, cnt > WT_FLUSH, f, f);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            if (all_any(!good)) break;  // all of them leave together
+            if (threadIdx.x == 384) {
+                own_store<DP>(&map_dk, base, p, it.unit * AT_ROWS, it.h, it.b);
+                own_store<DP>(&map_dv, base + S::OWN, p, it.unit * AT_ROWS, it.h, it.b);
+                tma_store_commit();
+                tma_store_wait_read<0>();
+                fetch(w + gridDim.x);
+            }
         }
+        if (threadIdx.x == 384) tma_store_wait_all();
     }
     tmem_give(tmem, warp);
 }
@@ -717,13 +791,14 @@ template <int DP>
 struct DqSmem {
     using T = WinTile<DP>;
     static constexpr int OWN = AT_ROWS * DP * 4;
-    static constexpr int K_RAW = 2 * OWN, V_RAW = K_RAW + 2 * T::RAW, K_MN = V_RAW + 2 * T::RAW, K_TWIN = K_MN + T::RAW, V_TWIN = K_TWIN + 2 * T::TWIN;
-    static constexpr int TABS = V_TWIN + 2 * T::TWIN, DIAG = TABS + 2 * WT_TAB * 4;  // bias of a block's distances, two blocks; [warp][64]: sums by diagonal, at an item's end by bucket
-    static constexpr int XCH = DIAG + 16 * 64 * 4, BAR = XCH + 2 * AT_ROWS * 4, TOTAL = BAR + 256 + 1024;
+    static constexpr int K_RAW = 2 * OWN, V_RAW = K_RAW + 2 * T::RAW, K_MN = V_RAW + 2 * T::RAW, K_TWIN = K_MN + T::RAW, V_TWIN = K_TWIN + 3 * T::TWIN;
+    static constexpr int TABS = V_TWIN + T::TWIN, DIAG = TABS + 3 * WT_TAB * 4;  // bias of a block's distances, three blocks; [warp][64]: sums by diagonal, at an item's end by bucket
+    static constexpr int XCH = DIAG + 16 * 64 * 4, BAR = XCH + AT_ROWS * 4, TOTAL = BAR + 256 + 1024;
     static_assert(TOTAL <= 232448 && AW_MAX_BUCKETS == 64, "shared memory");
 };
 template <int DP, bool BIAS>
-__global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kernel(const __grid_constant__ CUtensorMap map_kk, const __grid_constant__ CUtensorMap map_vk, const __grid_constant__ CUtensorMap map_kn,
+__global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kernel(const __grid_constant__ CUtensorMap map_kk, const __grid_constant__ CUtensorMap map_vk, const __grid_constant__ CUtensorMap map_kn, const __grid_constant__ CUtensorMap map_q,
+                                                                               const __grid_constant__ CUtensorMap map_do, const __grid_constant__ CUtensorMap map_dq,
                                                                                const __grid_constant__ WindowTc p) {
     using S = DqSmem<DP>;
     using T = WinTile<DP>;
@@ -737,21 +812,21 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
     auto one = [](uint32_t n) { return n & 1u; };
     auto k_full = [&](uint32_t n) { return bar(0 + (n & 1u)); };
     auto k_empty = [&](uint32_t n) { return bar(2 + (n & 1u)); };
-    auto k_conv = [&](uint32_t n) { return bar(4 + (n & 1u)); };
-    auto k_free = [&](uint32_t n) { return bar(6 + (n & 1u)); };  // companions: dQ has read them
-    auto v_full = [&](uint32_t n) { return bar(8 + (n & 1u)); };
-    auto v_empty = [&](uint32_t n) { return bar(10 + (n & 1u)); };  // tile and companions
-    auto v_conv = [&](uint32_t n) { return bar(12 + (n & 1u)); };
+    auto three = [](uint32_t n) { return (n / 3u) & 1u; };
+    auto k_conv = [&](uint32_t n) { return bar(4 + n % 3u); };
+    auto k_free = [&](uint32_t n) { return bar(7 + n % 3u); };  // companions: dQ has read them
+    auto v_full = [&](uint32_t n) { return bar(10 + (n & 1u)); };
+    auto v_empty = [&](uint32_t n) { return bar(12 + (n & 1u)); };
     auto s_full = [&](uint32_t n) { return bar(14 + (n & 1u)); };
     auto dp_full = [&](uint32_t n) { return bar(16 + (n & 1u)); };
     auto ds_ready = [&](uint32_t n) { return bar(18 + (n & 1u)); };
-    const uint32_t kn_full = bar(20), kn_empty = bar(21), acc_full = bar(22), q_ready = bar(23);
+    const uint32_t kn_full = bar(20), kn_empty = bar(21), acc_full = bar(22), q_ready = bar(23), v_conv = bar(24), v_free = bar(25), own_full = bar(26);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 24; ++i) mbar_init(bar(i), i == 4 || i == 5 || i == 12 || i == 13 ? 4 : i == 18 || i == 19 || i == 23 ? 16 : 1);
+        for (int i = 0; i < 27; ++i) mbar_init(bar(i), (i >= 4 && i < 7) || i == 24 ? 4 : i == 18 || i == 19 || i == 23 ? 16 : i == 26 ? 2 : 1);  // own_full: two tiles
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    const uint32_t tmem = tmem_take(bars + 8u * 24, reinterpret_cast<volatile uint32_t*>(gen + S::BAR + 8 * 24), warp);
+    const uint32_t tmem = tmem_take(bars + 8u * 28, reinterpret_cast<volatile uint32_t*>(gen + S::BAR + 8 * 28), warp);
     pdl_trigger();
     pdl_wait();
 
@@ -795,15 +870,16 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
                     return r;
                 };
                 auto products = [&](int i) {  // S and dP of block i
-                    const uint32_t at = n0 + i, place = tmem + 128 * (at & 1u), raw = (at & 1u) * (T::RAW / 16), twin = (at & 1u) * (T::TWIN / 16);
+                    const uint32_t at = n0 + i, place = tmem + 128 * (at & 1u), raw = (at & 1u) * (T::RAW / 16);
                     if (i >= n) return true;
-                    if (!landed(k_conv(at), two(at))) return false;
-                    win_scores<DP>(place, tmem + 320, base16, base16 + S::K_RAW / 16 + raw, base16 + S::K_TWIN / 16 + twin);
+                    if (!landed(k_conv(at), three(at))) return false;
+                    win_scores<DP>(place, tmem + 320, base16, base16 + S::K_RAW / 16 + raw, base16 + (S::K_TWIN + at % 3u * T::TWIN) / 16);
                     umma_commit(k_empty(at));
                     umma_commit(s_full(at));
-                    if (!landed(v_conv(at), two(at))) return false;
-                    win_scores<DP>(place + 64, tmem + 384, base16 + S::OWN / 16, base16 + S::V_RAW / 16 + raw, base16 + S::V_TWIN / 16 + twin);
+                    if (!landed(v_conv, one(at))) return false;
+                    win_scores<DP>(place + 64, tmem + 384, base16 + S::OWN / 16, base16 + S::V_RAW / 16 + raw, base16 + S::V_TWIN / 16);
                     umma_commit(v_empty(at));
+                    umma_commit(v_free);
                     umma_commit(dp_full(at));
                     return true;
                 };
@@ -814,7 +890,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
                     const uint32_t at = n0 + i, place = tmem + 128 * (at & 1u);
                     ok = products(i + 1) && mbar_wait(kn_full, one(at), p.status, 64) && landed(ds_ready(at), two(at));
                     if (!ok) break;
-                    win_values<DP, 16>(tmem + 256, place + 64, place, place + 8, base16 + S::K_MN / 16, base16 + (S::K_TWIN + (at & 1u) * T::TWIN) / 16, i % WT_FLUSH != 0);
+                    win_values<DP, 16>(tmem + 256, place + 64, place, place + 8, base16 + S::K_MN / 16, base16 + (S::K_TWIN + at % 3u * T::TWIN) / 16, i % WT_FLUSH != 0);
                     umma_commit(kn_empty);
                     umma_commit(k_free(at));
                     if (i + 1 == n || (i + 1) % WT_FLUSH == 0) umma_commit(acc_full);
@@ -846,20 +922,18 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
                 const uint32_t at = n0 + i;
                 ok = warp_wait(of_k ? k_full(at) : v_full(at), two(at), p.status, 65);
                 if (!ok) break;
-                if (of_k) {  // the place is free once dQ of the block before last has read it; its bias was used before that
-                    ok = warp_wait(k_free(at), two(at) ^ 1u, p.status, 65);
-                    if (!ok) break;
-                    if (BIAS) {
-                        float* tb = reinterpret_cast<float*>(gen + S::TABS) + (at & 1u) * WT_TAB + t;
-                        tb[0] = nb0;
-                        if (t < WT_TAB - 128) tb[128] = nb1;
-                        if (i + 1 < n) request(i + 1);
-                    }
+                ok = warp_wait(of_k ? k_free(at) : v_free, (of_k ? three(at) : one(at)) ^ 1u, p.status, 65);  // the last product that read what is there
+                if (!ok) break;
+                if (BIAS && of_k) {  // in three places as well: what was there has been used by the block whose companions these replace
+                    float* tb = reinterpret_cast<float*>(gen + S::TABS) + at % 3u * WT_TAB + t;
+                    tb[0] = nb0;
+                    if (t < WT_TAB - 128) tb[128] = nb1;
+                    if (i + 1 < n) request(i + 1);
                 }
-                win_split<DP, false>(gen + (of_k ? S::K_RAW : S::V_RAW) + (at & 1u) * T::RAW, gen + (of_k ? S::K_TWIN : S::V_TWIN) + (at & 1u) * T::TWIN, t);
+                win_split<DP, false>(gen + (of_k ? S::K_RAW : S::V_RAW) + (at & 1u) * T::RAW, gen + (of_k ? S::K_TWIN + at % 3u * T::TWIN : S::V_TWIN), t);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(of_k ? k_conv(at) : v_conv(at));
+                if (lane == 0) mbar_arrive(of_k ? k_conv(at) : v_conv);
             }
             n0 += n;
         }
@@ -871,43 +945,63 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
         const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
         float* sums = reinterpret_cast<float*>(gen + S::DIAG);  // [warp][64]
         float* diag = sums + (warp - 12) * 64;
-        float* xch = reinterpret_cast<float*>(gen + S::XCH);  // [half][row]: dO . O
+        float* xch = reinterpret_cast<float*>(gen + S::XCH);  // dO . O of every row
         const float c = p.scale * kLog2e;
         const bool wants_dbias = BIAS && p.dbias_part != nullptr;
-        uint32_t n = 0, moved = 0;
+        uint32_t n = 0, sums_out = 0, items = 0;
         bool good = true;
-        for (int64_t w = blockIdx.x; w < p.loop_end; w += gridDim.x) {
+        uint8_t* own = gen + (part >> 1) * S::OWN;
+        auto fetch = [&](int64_t w) {  // the rows of the item at w
+            if (w >= p.loop_end) return;
+            const AttnItem it = attn_item(p, w, false);
+            if (it.skip) return;
+            own_load<DP>(base, &map_q, own_full, it.unit * AT_ROWS, it.h, it.b);
+            own_load<DP>(base + S::OWN, &map_do, own_full, it.unit * AT_ROWS, it.h, it.b);
+        };
+        if (threadIdx.x == 384) fetch(blockIdx.x);
+        for (int64_t w = blockIdx.x; w < p.loop_end; w += gridDim.x, ++items) {
             const AttnItem it = attn_item(p, w, false);
             if (it.skip) break;
             const int r0 = it.unit * AT_ROWS, r = r0 + row;
             const bool live = r < p.T;
             const int64_t at = ((int64_t)it.b * p.H + it.h) * p.Tp + r;
+            // dO . O: a warp's eight rows, DP / 4 lanes each, while the tiles arrive
+            constexpr int LANES = DP / 4, STEP = 32 / LANES;
+            float a[8 / STEP];
+#pragma unroll
+            for (int x = 0; x < 8 / STEP; ++x) {
+                const int rr = r0 + 8 * (warp - 12) + x * STEP + lane / LANES, col = 4 * (lane % LANES);
+                const bool in = rr < p.T && col < p.D;
+                const float4 u = in ? ld4(p.g + it.b * p.g_so + it.h * p.g_si + rr * p.g_ld + col) : make_float4(0.f, 0.f, 0.f, 0.f);
+                const float4 y = in ? ld4(p.o + it.b * p.o_so + it.h * p.o_si + rr * p.o_ld + col) : make_float4(0.f, 0.f, 0.f, 0.f);
+                a[x] = fmaf(u.x, y.x, fmaf(u.y, y.y, fmaf(u.z, y.z, u.w * y.w)));
+            }
+#pragma unroll
+            for (int s = LANES / 2; s > 0; s >>= 1)
+#pragma unroll
+                for (int x = 0; x < 8 / STEP; ++x) a[x] += __shfl_xor_sync(0xffffffffu, a[x], s);
+            if (lane % LANES == 0)
+#pragma unroll
+                for (int x = 0; x < 8 / STEP; ++x) xch[8 * (warp - 12) + x * STEP + lane / LANES] = a[x];
+            good = good && warp_wait(own_full, items & 1u, p.status, 60);  // every thread keeps step with the barriers of the items, whatever a wait says
             {
                 float x[OC];
-                load_row<DP / 32>(x, (part < 2 ? p.q + it.b * p.q_so + it.h * p.q_si + r * p.q_ld : p.g + it.b * p.g_so + it.h * p.g_si + r * p.g_ld) + half * OC, live, p.D - half * OC);
-                place_row<DP / 32>(x, lanes + (part < 2 ? 320 : 384) + half * OC, gen + (part >> 1) * S::OWN + half * (OC / 16) * 8192, row);
-                if (part >= 2) {
-                    float a = 0.0f;
-                    const float* o = p.o + it.b * p.o_so + it.h * p.o_si + r * p.o_ld + half * OC;
-#pragma unroll
-                    for (int e = 0; e < OC; e += 4)
-                        if (live && half * OC + e < p.D) { const float4 y = ld4(o + e); a = fmaf(x[e], y.x, fmaf(x[e + 1], y.y, fmaf(x[e + 2], y.z, fmaf(x[e + 3], y.w, a)))); }
-                    xch[half * AT_ROWS + row] = a;
-                }
+                own_read(x, own, row, half * OC);
+                all_any(false);
+                place_row<DP / 32>(x, lanes + (part < 2 ? 320 : 384) + half * OC, own + half * (OC / 16) * 8192, row);
             }
             tmem_stores_done();
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(q_ready);
-            all_any(false);
-            const float delta = xch[row] + xch[AT_ROWS + row];
+            const float delta = xch[row];
             if (part == 0 && live) p.delta[at] = delta;
-            const float inv = live ? p.row_inv[at] : 0.0f, m = live ? p.row_max[at] * (BIAS ? 1.0f : kLog2e) : INFINITY;
+            const float inv = live ? p.row_inv[at] : 0.0f, m = !live ? INFINITY : BIAS ? p.row_max[at] : p.row_max[at] * kLog2e - log2f(inv);
             const float* tab = BIAS ? p.tab + (int64_t)it.h * p.tab_len : nullptr;
             const float beyond = BIAS ? __ldg(tab + p.tab_len - 1) : 0.0f;
             const TileKeys keys(p, r0);
             const int cnt = keys.count();
-            float* dst = p.dq + it.b * p.d_so + it.h * p.d_si + r * p.d_ld + 16 * part;
+            float* moved = moved_at(p, 0, 16 * part, row);
             // bias gradient: this lane's buckets, and what belongs to bucket `run_of` as a whole; buckets only go down along the walk
             float sum0 = 0.0f, sum1 = 0.0f, run = 0.0f;
             int run_of = p.rule.buckets - 1, near_of = run_of, far_of = run_of;
@@ -920,7 +1014,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
             for (int i = 0; i < cnt; ++i, ++n) {
                 const uint32_t place = lanes + 128 * (n & 1u);
                 const int b = keys.block(i), j0 = b * AT_KEYS + 16 * part, room = r - j0;
-                good = good && warp_wait(s_full(n), (n >> 1) & 1u, p.status, 66);  // every thread keeps step with the barriers of the items, whatever a wait says
+                good = good && warp_wait(s_full(n), (n >> 1) & 1u, p.status, 66);
                 after_sync();
                 uint32_t u[16];
                 float pr[16];
@@ -930,13 +1024,13 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
 #pragma unroll
                         for (int e = 0; e < 16; ++e) pr[e] = ex2((fmaf(__uint_as_float(u[e]), p.scale, beyond) - m) * kLog2e) * inv;
                     } else {
-                        const float* mine = reinterpret_cast<const float*>(gen + S::TABS) + (n & 1u) * WT_TAB + row - 16 * part + AT_KEYS - 1;
+                        const float* mine = reinterpret_cast<const float*>(gen + S::TABS) + n % 3u * WT_TAB + row - 16 * part + AT_KEYS - 1;
 #pragma unroll
                         for (int e = 0; e < 16; ++e) pr[e] = ex2((fmaf(__uint_as_float(u[e]), p.scale, mine[-e]) - m) * kLog2e) * inv;
                     }
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) pr[e] = ex2(fmaf(__uint_as_float(u[e]), c, -m)) * inv;
+                    for (int e = 0; e < 16; ++e) pr[e] = ex2(fmaf(__uint_as_float(u[e]), c, -m));
                 }
                 if (room - lane < 15 || (p.rule.W > 0 && room - lane + 31 >= p.rule.W && j0 + 15 >= p.rule.S)) {
                     const int from = p.rule.W > 0 ? room - p.rule.W + 1 : 0, to = p.rule.S - j0;
@@ -950,10 +1044,10 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
                 for (int e = 0; e < 16; ++e) pr[e] *= __uint_as_float(u[e]) - delta;  // a masked P is zero whatever dP holds
                 place_parts16(pr, place + 64 + 16 * part, place + 16 * part, place + 16 * part + 8);
                 if (i > 0 && i % WT_FLUSH == 0) {
-                    good = good && warp_wait(acc_full, moved & 1u, p.status, 68);
-                    ++moved;
+                    good = good && warp_wait(acc_full, sums_out & 1u, p.status, 68);
+                    ++sums_out;
                     after_sync();
-                    if (16 * part < DP) move_sum(lanes + 256 + 16 * part, dst, p.D - 16 * part, live, i > WT_FLUSH, 1.0f);
+                    if (16 * part < DP) move_sum(lanes + 256 + 16 * part, moved, i > WT_FLUSH, 1.0f);
                 }
                 tmem_stores_done();
                 __syncwarp();
@@ -992,15 +1086,23 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
                     }
                 }
             }
-            good = good && warp_wait(acc_full, moved & 1u, p.status, 68);
-            ++moved;
+            good = good && warp_wait(acc_full, sums_out & 1u, p.status, 68);
+            ++sums_out;
             after_sync();
             if (wants_dbias) {
                 settle();
                 diag[lane] = sum0;
                 diag[32 + lane] = sum1;
             }
+            if (16 * part < DP) place_result(gen, row, 16 * part, lanes + 256 + 16 * part, moved, cnt > WT_FLUSH, p.scale, p.scale);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             if (all_any(!good)) break;  // all of them leave together
+            if (threadIdx.x == 384) {
+                own_store<DP>(&map_dq, base, p, r0, it.h, it.b);
+                tma_store_commit();
+                tma_store_wait_read<0>();
+                fetch(w + gridDim.x);
+            }
             const int t = threadIdx.x - 384;
             if (wants_dbias && t < p.rule.buckets) {
                 float a = 0.0f;
@@ -1008,18 +1110,8 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
                 for (int x = 0; x < 16; ++x) a += sums[x * 64 + t];
                 p.dbias_part[(((int64_t)it.b * p.H + it.h) * p.units + it.unit) * p.rule.buckets + t] = a;
             }
-            if (16 * part < DP) {
-                uint32_t x[16];
-                tmem_ld16(lanes + 256 + 16 * part, x);
-                if (live)
-#pragma unroll
-                    for (int e = 0; e < 16; e += 4)
-                        if (16 * part + e < p.D) {
-                            const float4 o = cnt > WT_FLUSH ? ld4(dst + e) : make_float4(0.f, 0.f, 0.f, 0.f);
-                            st4(dst + e, make_float4(p.scale * (o.x + __uint_as_float(x[e])), p.scale * (o.y + __uint_as_float(x[e + 1])), p.scale * (o.z + __uint_as_float(x[e + 2])), p.scale * (o.w + __uint_as_float(x[e + 3]))));
-                        }
-            }
         }
+        if (threadIdx.x == 384) tma_store_wait_all();
     }
     tmem_give(tmem, warp);
 }
@@ -1055,17 +1147,27 @@ static int tc_launch(gcb_ctx* ctx, K kernel, bool* done, unsigned threads, size_
     return GCB_OK;
 }
 template <int DP, bool BIAS>
-static int run_fwd(gcb_ctx* ctx, const WindowTc& p, const CUtensorMap& k, const CUtensorMap& v) {
+static int run_fwd(gcb_ctx* ctx, const WindowTc& p, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& q, const CUtensorMap& o) {
     static bool done[kMaxDevices] = {};
-    return tc_launch(ctx, window_attention_tc_fwd_kernel<DP, BIAS>, done, AT_FWD_THREADS, AttnSmem<DP>::TOTAL, p, k, v);
+    return tc_launch(ctx, window_attention_tc_fwd_kernel<DP, BIAS>, done, AT_FWD_THREADS, AttnSmem<DP>::TOTAL, p, k, v, q, o);
 }
+struct BwdMaps {
+    CUtensorMap kk, vk, kn, qk, qn, ok, on, dq, dk, dv;
+};
 template <int DP, bool BIAS>
-static int run_bwd(gcb_ctx* ctx, const WindowTc& p, const CUtensorMap& kk, const CUtensorMap& vk, const CUtensorMap& kn, const CUtensorMap& qk, const CUtensorMap& qn, const CUtensorMap& ok, const CUtensorMap& on) {
+static int run_bwd(gcb_ctx* ctx, const WindowTc& p, const BwdMaps& m) {
     static bool done_q[kMaxDevices] = {}, done_kv[kMaxDevices] = {};
-    int rc = tc_launch(ctx, window_attention_tc_dq_kernel<DP, BIAS>, done_q, AT_BWD_THREADS, DqSmem<DP>::TOTAL, p, kk, vk, kn);
+    int rc = tc_launch(ctx, window_attention_tc_dq_kernel<DP, BIAS>, done_q, AT_BWD_THREADS, DqSmem<DP>::TOTAL, p, m.kk, m.vk, m.kn, m.qk, m.ok, m.dq);
     if (!rc) rc = after_launch(ctx, "window_attention_tc_dq");
-    if (!rc) rc = tc_launch(ctx, window_attention_tc_dkv_kernel<DP, BIAS>, done_kv, AT_BWD_THREADS, DkvSmem<DP>::TOTAL, p, qk, qn, ok, on);
+    if (!rc) rc = tc_launch(ctx, window_attention_tc_dkv_kernel<DP, BIAS>, done_kv, AT_BWD_THREADS, DkvSmem<DP>::TOTAL, p, m.qk, m.qn, m.ok, m.on, m.kk, m.vk, m.dk, m.dv);
     return rc ? rc : after_launch(ctx, "window_attention_tc_dkv");
+}
+// Room for the sums that leave tensor memory before an item's end.
+static int make_moved(WindowTc& p, Scratch& mem) {
+    if (p.T <= WT_FLUSH * AT_KEYS) return GCB_OK;
+    const int rc = mem.get((size_t)std::min<int64_t>(p.items, kSMs) * 2 * 64 * AT_ROWS * sizeof(float));
+    p.moved = mem.as<float>();
+    return rc;
 }
 
 // Heads of up to 64 columns (tensor memory holds two query tiles of that width), the split arithmetic of mode 2, rows that TMA can address.
@@ -1083,14 +1185,17 @@ int window_tc_fwd(gcb_ctx* ctx, int64_t B, const WindowAttn& a) {
     TmaEncodeFn enc = tma_encode(ctx);
     // two query tiles share their key blocks; one tile a CTA where pairs would leave SMs idle
     WindowTc p = operands(ctx, B, a, B * a.H * ((a.T + 255) / 256) < kSMs ? 1 : 2);
-    Scratch tab(ctx);
+    Scratch tab(ctx), moved(ctx);
     int rc = make_table(ctx, p, tab);
+    if (!rc) rc = make_moved(p, moved);
     if (rc) return rc;
-    CUtensorMap k, v;
+    CUtensorMap k, v, q, o;
     GCB_REQUIRE(encode_rows(enc, &k, a.k, a.D, a.T, a.k_ld, a.k_si, a.k_so, a.H, B, 32, AT_KEYS, CU_TENSOR_MAP_SWIZZLE_128B) &&
+                    encode_rows(enc, &q, a.q, a.D, a.T, a.q_ld, a.q_si, a.q_so, a.H, B, 32, AT_KEYS, CU_TENSOR_MAP_SWIZZLE_128B) &&
+                    encode_rows(enc, &o, a.out, a.D, a.T, a.o_ld, a.o_si, a.o_so, a.H, B, 32, AT_KEYS, CU_TENSOR_MAP_SWIZZLE_128B) &&
                     encode_rows(enc, &v, a.v, a.D, a.T, a.v_ld, a.v_si, a.v_so, a.H, B, 32, AT_KEYS, CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B),
                 "window attention: strides beyond what TMA can address");
-    rc = p.tab ? (a.D <= 32 ? run_fwd<32, true>(ctx, p, k, v) : run_fwd<64, true>(ctx, p, k, v)) : (a.D <= 32 ? run_fwd<32, false>(ctx, p, k, v) : run_fwd<64, false>(ctx, p, k, v));
+    rc = p.tab ? (a.D <= 32 ? run_fwd<32, true>(ctx, p, k, v, q, o) : run_fwd<64, true>(ctx, p, k, v, q, o)) : (a.D <= 32 ? run_fwd<32, false>(ctx, p, k, v, q, o) : run_fwd<64, false>(ctx, p, k, v, q, o));
     return rc ? rc : after_launch(ctx, "window_attention_tc_fwd");
 }
 
@@ -1098,20 +1203,22 @@ int window_tc_fwd(gcb_ctx* ctx, int64_t B, const WindowAttn& a) {
 int window_tc_bwd(gcb_ctx* ctx, int64_t B, const WindowAttn& a) {
     TmaEncodeFn enc = tma_encode(ctx);
     WindowTc p = operands(ctx, B, a, 1);
-    Scratch tab(ctx), delta(ctx);
+    Scratch tab(ctx), delta(ctx), moved(ctx);
     int rc = make_table(ctx, p, tab);
+    if (!rc) rc = make_moved(p, moved);
     if (!rc) rc = delta.get(sizeof(float) * (size_t)(p.heads * p.Tp));
     if (rc) return rc;
     p.delta = delta.as<float>();
-    CUtensorMap kk, vk, kn, qk, qn, ok, on;
-    auto rows = [&](CUtensorMap* map, const float* x, int64_t ld, int64_t so, int64_t si, bool k_major) {
-        return encode_rows(enc, map, x, a.D, a.T, ld, si, so, a.H, B, 32, AT_KEYS, k_major ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B);
+    BwdMaps m;
+    auto rows = [&](CUtensorMap& map, const float* x, int64_t ld, int64_t so, int64_t si, bool k_major) {
+        return encode_rows(enc, &map, x, a.D, a.T, ld, si, so, a.H, B, 32, AT_KEYS, k_major ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B);
     };
-    GCB_REQUIRE(rows(&kk, a.k, a.k_ld, a.k_so, a.k_si, true) && rows(&kn, a.k, a.k_ld, a.k_so, a.k_si, false) && rows(&vk, a.v, a.v_ld, a.v_so, a.v_si, true) && rows(&qk, a.q, a.q_ld, a.q_so, a.q_si, true) &&
-                    rows(&qn, a.q, a.q_ld, a.q_so, a.q_si, false) && rows(&ok, a.g, a.g_ld, a.g_so, a.g_si, true) && rows(&on, a.g, a.g_ld, a.g_so, a.g_si, false),
+    GCB_REQUIRE(rows(m.kk, a.k, a.k_ld, a.k_so, a.k_si, true) && rows(m.kn, a.k, a.k_ld, a.k_so, a.k_si, false) && rows(m.vk, a.v, a.v_ld, a.v_so, a.v_si, true) && rows(m.qk, a.q, a.q_ld, a.q_so, a.q_si, true) &&
+                    rows(m.qn, a.q, a.q_ld, a.q_so, a.q_si, false) && rows(m.ok, a.g, a.g_ld, a.g_so, a.g_si, true) && rows(m.on, a.g, a.g_ld, a.g_so, a.g_si, false) &&
+                    rows(m.dq, a.dq, a.d_ld, a.d_so, a.d_si, true) && rows(m.dk, a.dk, a.d_ld, a.d_so, a.d_si, true) && rows(m.dv, a.dv, a.d_ld, a.d_so, a.d_si, true),
                 "window attention: strides beyond what TMA can address");
-    if (p.tab) return a.D <= 32 ? run_bwd<32, true>(ctx, p, kk, vk, kn, qk, qn, ok, on) : run_bwd<64, true>(ctx, p, kk, vk, kn, qk, qn, ok, on);
-    return a.D <= 32 ? run_bwd<32, false>(ctx, p, kk, vk, kn, qk, qn, ok, on) : run_bwd<64, false>(ctx, p, kk, vk, kn, qk, qn, ok, on);
+    if (p.tab) return a.D <= 32 ? run_bwd<32, true>(ctx, p, m) : run_bwd<64, true>(ctx, p, m);
+    return a.D <= 32 ? run_bwd<32, false>(ctx, p, m) : run_bwd<64, false>(ctx, p, m);
 }
 
 }  // namespace gcb
