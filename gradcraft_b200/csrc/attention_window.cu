@@ -39,10 +39,8 @@ __device__ __forceinline__ void aw_st4(float* p, int c, int D, float4 x) {
     if (c + 3 < D) p[c + 3] = x.w;
 }
 // bias of the distances d0 .. d0 + 94 of a tile
-__device__ __forceinline__ void aw_tab(float* tab, const WindowRule& r, int h, int d0) {
-    if (r.bias == nullptr) return;
-    const int t = threadIdx.x;
-    if (t < AW_DIAG) tab[t] = d0 + t >= 0 ? r.bias[(int64_t)h * r.buckets + r.bucket(d0 + t)] : 0.0f;
+__device__ __forceinline__ void aw_tab(float* sm, const WindowAttn& p, int64_t h, int d0) {
+    if (p.tab != nullptr && threadIdx.x < AW_DIAG) sm[threadIdx.x] = p.tab[h * p.tab_len + clamp_distance(d0 + (int)threadIdx.x, p.tab_len)];
 }
 // the tile of keys after k0 that queries q0 .. q0 + 31 look at
 __device__ __forceinline__ int aw_first_tile(const WindowRule& r, int q0) { return r.S > 0 ? 0 : r.window_first(q0) / AS_T * AS_T; }
@@ -67,7 +65,7 @@ __global__ void __launch_bounds__(256) window_attention_fwd_kernel(const __grid_
         __syncthreads();
         aw_load<AS_T, VEC>(sk, k, p.k_ld, k0, p.T, D, Dp);
         aw_load<AS_T, VEC>(sv, v, p.v_ld, k0, p.T, D, Dp);
-        aw_tab(tab, p.rule, (int)h, q0 - k0 - (AS_T - 1));
+        aw_tab(tab, p, h, q0 - k0 - (AS_T - 1));
         as_landed();
         float s[2][4];
         as_abt(s, sq, sk, Dp, ty, tx);
@@ -77,7 +75,7 @@ __global__ void __launch_bounds__(256) window_attention_fwd_kernel(const __grid_
             float mx = m[i];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float z = p.rule.bias ? fmaf(s[i][j], p.scale, tab[ty + 16 * i - (tx + 16 * j) + AS_T - 1]) : s[i][j] * p.scale;
+                const float z = p.tab ? fmaf(s[i][j], p.scale, tab[ty + 16 * i - (tx + 16 * j) + AS_T - 1]) : s[i][j] * p.scale;
                 s[i][j] = p.rule.sees(row, k0 + tx + 16 * j) ? z : -INFINITY;
                 mx = fmaxf(mx, s[i][j]);
             }
@@ -161,9 +159,14 @@ __global__ void __launch_bounds__(256) window_attention_dq_kernel(const __grid_c
         __syncthreads();
         aw_load<AS_T, VEC>(s2, k, p.k_ld, k0, p.T, D, Dp);
         aw_load<AS_T, VEC>(s3, v, p.v_ld, k0, p.T, D, Dp);
-        aw_tab(tab, p.rule, (int)h, d0);
+        aw_tab(tab, p, h, d0);
         as_landed();
-        if (first) rows.finish(s1, Dp, ty, tx);
+        if (first) {
+            rows.finish(s1, Dp, ty, tx);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                if (tx == 0 && q0 + ty + 16 * i < p.T) p.delta[head * p.Tp + q0 + ty + 16 * i] = rows.delta[i];
+        }
         first = false;
         float s[2][4], dp[2][4];
         as_abt(s, s0, s2, Dp, ty, tx);
@@ -173,7 +176,7 @@ __global__ void __launch_bounds__(256) window_attention_dq_kernel(const __grid_c
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const int r = ty + 16 * i, c = tx + 16 * j;
-                const float z = p.rule.bias ? fmaf(s[i][j], p.scale, tab[r - c + AS_T - 1]) : s[i][j] * p.scale;
+                const float z = p.tab ? fmaf(s[i][j], p.scale, tab[r - c + AS_T - 1]) : s[i][j] * p.scale;
                 const float pr = p.rule.sees(q0 + r, k0 + c) ? __expf(z - rows.m[i]) * rows.inv[i] : 0.0f;
                 ss[r * (AS_T + 4) + c] = pr * (dp[i][j] - rows.delta[i]);
             }
@@ -207,18 +210,13 @@ __global__ void __launch_bounds__(256) window_attention_dq_kernel(const __grid_c
     if (p.dbias_part && threadIdx.x < p.rule.buckets) p.dbias_part[(int64_t)blockIdx.x * p.rule.buckets + threadIdx.x] = db;
 }
 
-// dK and dV of 32 keys from the queries that see them through the window.  FAR: from the queries beyond the window instead, which see the
-// first S keys only: a CTA takes 512 of them and leaves its sums in far_part, [head][key tile][chunk][dk, dv][32][Dp], so that the few
-// first keys of a long sequence are not one CTA's work.
-constexpr int AW_FAR = 512;
-template <int NC, bool VEC, bool FAR>
+// dK and dV of 32 keys from the queries that see them through the window.
+template <int NC, bool VEC>
 __global__ void __launch_bounds__(256) window_attention_dkv_kernel(const __grid_constant__ WindowAttn p) {
     extern __shared__ __align__(16) float aw_sm[];
     pdl_trigger();
     pdl_wait();
-    const int per_head = FAR ? (p.rule.S + AS_OWN - 1) / AS_OWN * p.far_chunks : p.tiles;
-    const int D = p.D, Dp = (D + 3) / 4 * 4, tx = threadIdx.x & 15, ty = threadIdx.x >> 4, head = blockIdx.x / per_head, item = blockIdx.x - head * per_head;
-    const int t0 = (FAR ? item / p.far_chunks : item) * AS_OWN, chunk = FAR ? item % p.far_chunks : 0;
+    const int D = p.D, Dp = (D + 3) / 4 * 4, tx = threadIdx.x & 15, ty = threadIdx.x >> 4, head = blockIdx.x / p.tiles, t0 = (blockIdx.x - head * p.tiles) * AS_OWN;
     const int64_t b = head / p.H, h = head - b * p.H;
     float *s0 = aw_sm, *s1 = s0 + AS_OWN * (Dp + 4), *s2 = s1 + AS_OWN * (Dp + 4), *s3 = s2 + AS_T * (Dp + 4), *sp = s3 + AS_T * (Dp + 4), *ss = sp + AS_T * (AS_OWN + 4), *tab = ss + AS_T * (AS_OWN + 4);
     const float *q = p.q + b * p.q_so + h * p.q_si, *g = p.g + b * p.g_so + h * p.g_si, *o = p.o + b * p.o_so + h * p.o_si;
@@ -226,20 +224,13 @@ __global__ void __launch_bounds__(256) window_attention_dkv_kernel(const __grid_
     aw_load<AS_OWN, VEC>(s0, p.k + b * p.k_so + h * p.k_si, p.k_ld, t0, p.T, D, Dp);
     aw_load<AS_OWN, VEC>(s1, p.v + b * p.v_so + h * p.v_si, p.v_ld, t0, p.T, D, Dp);
     const int W = p.rule.W, keys_end = min(t0 + AS_OWN, p.T);
-    int r_begin, r_end;
-    if (FAR) {
-        r_begin = max(chunk * AW_FAR, (t0 + W) / AS_T * AS_T);
-        r_end = min(p.T, (chunk + 1) * AW_FAR);
-    } else {
-        r_begin = t0 / AS_T * AS_T;
-        r_end = W > 0 && W < p.T - keys_end ? keys_end - 1 + W : p.T;
-    }
-    for (int r0 = r_begin; r0 < r_end; r0 += AS_T) {
+    const int r_end = W > 0 && W < p.T - keys_end ? keys_end - 1 + W : p.T;
+    for (int r0 = t0 / AS_T * AS_T; r0 < r_end; r0 += AS_T) {
         __syncthreads();
         AwRows<4, NC, VEC> rows;
         aw_load<AS_T, VEC>(s2, q, p.q_ld, r0, p.T, D, Dp);
         aw_load<AS_T, VEC>(s3, g, p.g_ld, r0, p.T, D, Dp);
-        aw_tab(tab, p.rule, (int)h, r0 - t0 - (AS_OWN - 1));
+        aw_tab(tab, p, h, r0 - t0 - (AS_OWN - 1));
         rows.request(p, head, o, r0, ty, tx);
         as_landed();
         rows.finish(s3, Dp, ty, tx);
@@ -251,8 +242,8 @@ __global__ void __launch_bounds__(256) window_attention_dkv_kernel(const __grid_
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const int r = ty + 16 * i, c = tx + 16 * j, d = r0 + r - (t0 + c);
-                const float z = p.rule.bias ? fmaf(s[i][j], p.scale, tab[r - c + AS_OWN - 1]) : s[i][j] * p.scale;
-                const bool seen = FAR ? d >= W && t0 + c < p.rule.S : d >= 0 && (W == 0 || d < W);
+                const float z = p.tab ? fmaf(s[i][j], p.scale, tab[r - c + AS_OWN - 1]) : s[i][j] * p.scale;
+                const bool seen = d >= 0 && (W == 0 || d < W);
                 const float pr = seen ? __expf(z - rows.m[i]) * rows.inv[i] : 0.0f;
                 sp[r * (AS_OWN + 4) + c] = pr;
                 ss[r * (AS_OWN + 4) + c] = pr * (dp[i][j] - rows.delta[i]);
@@ -268,29 +259,118 @@ __global__ void __launch_bounds__(256) window_attention_dkv_kernel(const __grid_
             const int c = 64 * n + 4 * tx, r = t0 + 2 * ty + i;
             const float4 a = make_float4(p.scale * dk[i][4 * n], p.scale * dk[i][4 * n + 1], p.scale * dk[i][4 * n + 2], p.scale * dk[i][4 * n + 3]);
             const float4 e = make_float4(dv[i][4 * n], dv[i][4 * n + 1], dv[i][4 * n + 2], dv[i][4 * n + 3]);
-            if (FAR) {
-                if (c >= Dp) continue;
-                float* part = p.far_part + ((int64_t)blockIdx.x * 2 * AS_OWN + 2 * ty + i) * Dp + c;
-                st4(part, a);
-                st4(part + AS_OWN * Dp, e);
-            } else if (r < p.T) {
+            if (r < p.T) {
                 const int64_t at = b * p.d_so + h * p.d_si + r * p.d_ld;
                 aw_st4<VEC>(p.dk + at, c, D, a);
                 aw_st4<VEC>(p.dv + at, c, D, e);
             }
         }
 }
-// Adds the chunks of far_part, in their order, to dK and dV of the first S keys.  A block per (head, key), a thread per column.
-__global__ void __launch_bounds__(128) window_attention_far_kernel(const __grid_constant__ WindowAttn p, int keys) {
+// What the queries beyond the window, which see the first S keys alone, add to those keys' gradients.  Tiles of keys would spend most of their work on
+// keys that are not seen: here four keys lie in registers, a column quadruple a lane, and a warp passes over the rows of q and dO, 32 / LPR at a time.
+// A CTA takes far_rows queries of a head and four of the keys, and leaves its sums in far_part, [head][chunk][S][dk, dv][Dp].
+// Bound by memory (q and dO once for every four keys) and, about as much, by the eight sums over a row's lanes.
+// 256 heads of 768 queries beyond a window, four keys: 228 us as tiles of 32 keys.
+constexpr int AW_KEYS = 4;
+template <int LPR>
+__device__ __forceinline__ void sum_eight(float (&v)[8], int lane) {  // every lane gets all eight sums over its LPR lanes: halves change hands until each lane has one
+    const bool b0 = lane & (LPR / 2), b1 = lane & (LPR / 4), b2 = lane & (LPR / 8);
+    float w[4], x[2], y;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = (b0 ? v[4 + i] : v[i]) + __shfl_xor_sync(0xffffffffu, b0 ? v[i] : v[4 + i], LPR / 2);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) x[i] = (b1 ? w[2 + i] : w[i]) + __shfl_xor_sync(0xffffffffu, b1 ? w[i] : w[2 + i], LPR / 4);
+    y = (b2 ? x[1] : x[0]) + __shfl_xor_sync(0xffffffffu, b2 ? x[0] : x[1], LPR / 8);
+#pragma unroll
+    for (int s = LPR / 16; s > 0; s >>= 1) y += __shfl_xor_sync(0xffffffffu, y, s);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __shfl_sync(0xffffffffu, y, (lane & ~(LPR - 1)) | ((i & 4) ? LPR / 2 : 0) | ((i & 2) ? LPR / 4 : 0) | ((i & 1) ? LPR / 8 : 0));
+}
+template <int LPR, bool VEC>
+__global__ void __launch_bounds__(256, 2) window_attention_far_kernel(const __grid_constant__ WindowAttn p) {
+    constexpr int RPW = 32 / LPR, U = 2, DP = 4 * LPR, STEP = 8 * RPW;
+    __shared__ float sums[8][2 * AW_KEYS][DP];
     pdl_trigger();
     pdl_wait();
-    const int head = blockIdx.x / keys, key = blockIdx.x - head * keys, c = threadIdx.x, Dp = (p.D + 3) / 4 * 4, key_tiles = (p.rule.S + AS_OWN - 1) / AS_OWN;
+    const int groups = (p.rule.S + AW_KEYS - 1) / AW_KEYS, per_head = groups * p.far_chunks, head = blockIdx.x / per_head, item = blockIdx.x - head * per_head, j0 = item / p.far_chunks * AW_KEYS, chunk = item % p.far_chunks;
+    const int64_t b = head / p.H, h = head - b * p.H;
+    const int D = p.D, W = p.rule.W, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = 4 * (lane % LPR), r_end = min(p.T, W + (chunk + 1) * p.far_rows);
+    const float *qb = p.q + b * p.q_so + h * p.q_si, *gb = p.g + b * p.g_so + h * p.g_si, *tab = p.tab ? p.tab + h * p.tab_len : nullptr;
+    float4 k[AW_KEYS], v[AW_KEYS], dk[AW_KEYS] = {}, dv[AW_KEYS] = {};
+    const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int x = 0; x < AW_KEYS; ++x) {
+        const bool there = j0 + x < min(p.rule.S, p.T);
+        k[x] = there ? aw_ld4<VEC>(p.k + b * p.k_so + h * p.k_si + (j0 + x) * p.k_ld, col, D) : zero;
+        v[x] = there ? aw_ld4<VEC>(p.v + b * p.v_so + h * p.v_si + (j0 + x) * p.v_ld, col, D) : zero;
+    }
+    for (int r0 = W + chunk * p.far_rows + warp * RPW; r0 < r_end; r0 += U * STEP) {
+        float4 q[U], g[U];
+        float m[U], inv[U], delta[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int r = r0 + u * STEP + lane / LPR;
+            const bool live = r < r_end;
+            q[u] = live ? aw_ld4<VEC>(qb + r * p.q_ld, col, D) : zero;
+            g[u] = live ? aw_ld4<VEC>(gb + r * p.g_ld, col, D) : zero;
+            m[u] = live ? p.row_max[head * p.Tp + r] : INFINITY;
+            inv[u] = live ? p.row_inv[head * p.Tp + r] : 0.0f;
+            delta[u] = live ? p.delta[head * p.Tp + r] : 0.0f;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int r = r0 + u * STEP + lane / LPR;
+            float s[2 * AW_KEYS];
+#pragma unroll
+            for (int x = 0; x < AW_KEYS; ++x) {
+                s[x] = fmaf(q[u].x, k[x].x, fmaf(q[u].y, k[x].y, fmaf(q[u].z, k[x].z, q[u].w * k[x].w)));
+                s[AW_KEYS + x] = fmaf(g[u].x, v[x].x, fmaf(g[u].y, v[x].y, fmaf(g[u].z, v[x].z, g[u].w * v[x].w)));
+            }
+            sum_eight<LPR>(s, lane);
+#pragma unroll
+            for (int x = 0; x < AW_KEYS; ++x) {
+                const int d = r - j0 - x;
+                const float z = tab ? fmaf(s[x], p.scale, tab[clamp_distance(d, p.tab_len)]) : s[x] * p.scale;
+                const float pr = d >= W && j0 + x < p.rule.S ? __expf(z - m[u]) * inv[u] : 0.0f, ds = pr * (s[AW_KEYS + x] - delta[u]);
+                dk[x].x = fmaf(ds, q[u].x, dk[x].x); dk[x].y = fmaf(ds, q[u].y, dk[x].y); dk[x].z = fmaf(ds, q[u].z, dk[x].z); dk[x].w = fmaf(ds, q[u].w, dk[x].w);
+                dv[x].x = fmaf(pr, g[u].x, dv[x].x); dv[x].y = fmaf(pr, g[u].y, dv[x].y); dv[x].z = fmaf(pr, g[u].z, dv[x].z); dv[x].w = fmaf(pr, g[u].w, dv[x].w);
+            }
+        }
+    }
+#pragma unroll
+    for (int x = 0; x < AW_KEYS; ++x) {
+        float e[8] = {p.scale * dk[x].x, p.scale * dk[x].y, p.scale * dk[x].z, p.scale * dk[x].w, dv[x].x, dv[x].y, dv[x].z, dv[x].w};
+#pragma unroll
+        for (int s = LPR; s < 32; s <<= 1)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) e[i] += __shfl_xor_sync(0xffffffffu, e[i], s);
+        if (lane < LPR) {
+            st4(&sums[warp][2 * x][col], make_float4(e[0], e[1], e[2], e[3]));
+            st4(&sums[warp][2 * x + 1][col], make_float4(e[4], e[5], e[6], e[7]));
+        }
+    }
+    __syncthreads();
+    const int Dp = (D + 3) / 4 * 4;
+    for (int i = threadIdx.x; i < 2 * AW_KEYS * DP; i += 256) {
+        const int x = i / DP, c = i - x * DP, key = j0 + x / 2;
+        if (c >= Dp || key >= p.rule.S) continue;
+        float a = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) a += sums[w][x][c];
+        p.far_part[((((int64_t)head * p.far_chunks + chunk) * p.rule.S + key) * 2 + (x & 1)) * Dp + c] = a;
+    }
+}
+// Adds the chunks of far_part, in their order, to dK and dV of the first keys.  A block per (head, key), a thread per column.
+__global__ void __launch_bounds__(128) window_attention_far_sum_kernel(const __grid_constant__ WindowAttn p, int keys) {
+    pdl_trigger();
+    pdl_wait();
+    const int head = blockIdx.x / keys, key = blockIdx.x - head * keys, c = threadIdx.x, Dp = (p.D + 3) / 4 * 4;
     if (c >= p.D) return;
-    const int64_t b = head / p.H, h = head - b * p.H, stride = (int64_t)2 * AS_OWN * Dp;
-    const float* part = p.far_part + ((int64_t)head * key_tiles + key / AS_OWN) * p.far_chunks * stride + (key % AS_OWN) * Dp + c;
+    const int64_t b = head / p.H, h = head - b * p.H, stride = (int64_t)p.rule.S * 2 * Dp;
+    const float* part = p.far_part + (int64_t)head * p.far_chunks * stride + key * 2 * Dp + c;
     float dk = 0.0f, dv = 0.0f;
-#pragma unroll 4
-    for (int i = 0; i < p.far_chunks; ++i) { dk += part[i * stride]; dv += part[i * stride + AS_OWN * Dp]; }
+#pragma unroll 8
+    for (int i = 0; i < p.far_chunks; ++i) { dk += part[i * stride]; dv += part[i * stride + Dp]; }
     const int64_t at = b * p.d_so + h * p.d_si + key * p.d_ld + c;
     p.dk[at] += dk;
     p.dv[at] += dv;
@@ -438,7 +518,7 @@ __global__ void __launch_bounds__(32 * ST_WARPS) window_attention_step_kernel(co
 static bool vec_rows(const float* p, int64_t ld, int64_t so, int64_t si) { return aligned16(p) && ld % 4 == 0 && so % 4 == 0 && si % 4 == 0; }
 static bool own_rows(int64_t B, int64_t H, int64_t T, int64_t D, int64_t ld, int64_t so, int64_t si) { return (T <= 1 || ld >= D) && (H <= 1 || si > 0) && (B <= 1 || so > 0); }
 static size_t span_bytes(int64_t B, int64_t H, int64_t T, int64_t D, int64_t ld, int64_t so, int64_t si) { return sizeof(float) * (size_t)((B - 1) * so + (H - 1) * si + (T - 1) * ld + D); }
-constexpr int64_t AW_MAX_T = int64_t(1) << 24, AW_MAX_D = 128;
+constexpr int64_t AW_MAX_T = int64_t(1) << 24, AW_MAX_D = 128, AW_MAX_H = 65535;
 
 template <class K>
 static int fma_launch(gcb_ctx* ctx, K kernel, bool* done, int64_t ctas, size_t floats, const WindowAttn& p) {
@@ -459,19 +539,44 @@ static int fma_bwd(gcb_ctx* ctx, int64_t heads, const WindowAttn& p) {
     const int64_t Dp = (p.D + 3) / 4 * 4;
     int rc = fma_launch(ctx, window_attention_dq_kernel<NC, VEC>, done_q, heads * p.tiles, aw_floats(2, 2, 1, Dp), p);
     if (!rc) rc = after_launch(ctx, "window_attention_dq");
-    if (!rc) rc = fma_launch(ctx, window_attention_dkv_kernel<NC, VEC, false>, done_kv, heads * p.tiles, aw_floats(2, 2, 2, Dp), p);
+    if (!rc) rc = fma_launch(ctx, window_attention_dkv_kernel<NC, VEC>, done_kv, heads * p.tiles, aw_floats(2, 2, 2, Dp), p);
     return rc ? rc : after_launch(ctx, "window_attention_dkv");
 }
-// What queries beyond the window add to the first keys' gradients; after dK and dV have been written.
-template <int NC, bool VEC>
-static int fma_far(gcb_ctx* ctx, int64_t heads, const WindowAttn& p) {
-    static bool done[kMaxDevices] = {};
-    const int key_tiles = (p.rule.S + AS_OWN - 1) / AS_OWN, keys = std::min(p.rule.S, p.T);
-    int rc = fma_launch(ctx, window_attention_dkv_kernel<NC, VEC, true>, done, heads * key_tiles * p.far_chunks, aw_floats(2, 2, 2, (p.D + 3) / 4 * 4), p);
-    if (!rc) rc = after_launch(ctx, "window_attention_far");
+// What queries beyond the window add to the first keys' gradients; after dK and dV have been written, and delta.
+static int far_gradients(gcb_ctx* ctx, int64_t heads, WindowAttn& p, bool vec, Scratch& mem) {
+    const int Dp = (p.D + 3) / 4 * 4, groups = (p.rule.S + AW_KEYS - 1) / AW_KEYS, keys = std::min(p.rule.S, p.T);
+    // 256 queries a CTA, and where that leaves SMs idle 64
+    p.far_rows = heads * groups * ((p.T - p.rule.W + 255) / 256) >= 2 * kSMs ? 256 : 64;
+    p.far_chunks = (p.T - p.rule.W + p.far_rows - 1) / p.far_rows;
+    const int64_t ctas = heads * groups * p.far_chunks;
+    GCB_REQUIRE(ctas < (int64_t(1) << 31) && heads * keys < (int64_t(1) << 31), "window attention: more tiles than a grid holds");
+    const int rc = mem.get(sizeof(float) * (size_t)(heads * p.far_chunks * p.rule.S * 2 * Dp));
     if (rc) return rc;
-    GCB_CHECK_CUDA(launch_next(ctx->stream, dim3((unsigned)(heads * keys)), 128, 0, window_attention_far_kernel, p, keys));
+    p.far_part = mem.as<float>();
+    auto run = [&](auto kernel) { return launch_next(ctx->stream, dim3((unsigned)ctas), 256, 0, kernel, p); };
+    if (p.D <= 32) GCB_CHECK_CUDA(vec ? run(window_attention_far_kernel<8, true>) : run(window_attention_far_kernel<8, false>));
+    else if (p.D <= 64) GCB_CHECK_CUDA(vec ? run(window_attention_far_kernel<16, true>) : run(window_attention_far_kernel<16, false>));
+    else GCB_CHECK_CUDA(vec ? run(window_attention_far_kernel<32, true>) : run(window_attention_far_kernel<32, false>));
+    const int launched = after_launch(ctx, "window_attention_far");
+    if (launched) return launched;
+    GCB_CHECK_CUDA(launch_next(ctx->stream, dim3((unsigned)(heads * keys)), 128, 0, window_attention_far_sum_kernel, p, keys));
     return after_launch(ctx, "window_attention_far_sum");
+}
+// The bias by distance of every head, up to the first distance of the last bucket, which holds for all beyond.
+__global__ void __launch_bounds__(256) window_attention_table_kernel(float* __restrict__ tab, int len, const __grid_constant__ WindowRule r) {
+    pdl_trigger();
+    pdl_wait();
+    const int d = blockIdx.x * 256 + threadIdx.x, h = blockIdx.y;
+    if (d < len) tab[(int64_t)h * len + d] = r.bias[(int64_t)h * r.buckets + r.bucket(d)];
+}
+static int make_table(gcb_ctx* ctx, WindowAttn& p, Scratch& mem) {
+    if (p.rule.bias == nullptr) return GCB_OK;
+    p.tab_len = std::min(p.T, p.rule.starts[p.rule.buckets - 1] + 1);
+    const int rc = mem.get(sizeof(float) * (size_t)p.H * p.tab_len);
+    if (rc) return rc;
+    p.tab = mem.as<float>();
+    GCB_CHECK_CUDA(launch_next(ctx->stream, dim3((unsigned)((p.tab_len + 255) / 256), (unsigned)p.H), 256, 0, window_attention_table_kernel, mem.as<float>(), p.tab_len, p.rule));
+    return after_launch(ctx, "window_attention_table");
 }
 
 }  // namespace gcb
@@ -527,7 +632,7 @@ int gcb_window_attention_fwd_f32(gcb_ctx* ctx, int64_t B, int64_t H, int64_t T, 
     int rc = make_rule(p.rule, "gcb_window_attention_fwd_f32", window, sinks, bias, buckets, bucket_starts);
     if (rc) return rc;
     if (B == 0 || H == 0 || T == 0 || D == 0) return GCB_OK;
-    if (D > AW_MAX_D || T > AW_MAX_T) { set_error("gcb_window_attention_fwd_f32: heads of up to %lld columns and sequences of up to %lld positions", (long long)AW_MAX_D, (long long)AW_MAX_T); return GCB_UNSUPPORTED; }
+    if (D > AW_MAX_D || T > AW_MAX_T || H > AW_MAX_H) { set_error("gcb_window_attention_fwd_f32: at most %lld heads of %lld columns and sequences of %lld positions", (long long)AW_MAX_H, (long long)AW_MAX_D, (long long)AW_MAX_T); return GCB_UNSUPPORTED; }
     GCB_REQUIRE(out && stats && q && k && v && own_rows(B, H, T, D, o_ld, o_so, o_si), "gcb_window_attention_fwd_f32: NULL pointer, or output rows that overlap");
     cudaSetDevice(ctx->device);
     p.q = q; p.q_ld = q_ld; p.q_so = q_so; p.q_si = q_si;
@@ -538,6 +643,8 @@ int gcb_window_attention_fwd_f32(gcb_ctx* ctx, int64_t B, int64_t H, int64_t T, 
     p.row_max = stats; p.row_inv = stats + B * H * p.Tp;
     p.tiles = (int)((T + AS_OWN - 1) / AS_OWN);
     const bool vec = D % 4 == 0 && vec_rows(q, q_ld, q_so, q_si) && vec_rows(k, k_ld, k_so, k_si) && vec_rows(v, v_ld, v_so, v_si) && vec_rows(out, o_ld, o_so, o_si);
+    Scratch tab(ctx);
+    if ((rc = make_table(ctx, p, tab))) return rc;
     if (window_tc_takes(ctx, B, p)) rc = window_tc_fwd(ctx, B, p);
     else rc = D <= 64 ? (vec ? fma_fwd<1, true>(ctx, B * H, p) : fma_fwd<1, false>(ctx, B * H, p)) : (vec ? fma_fwd<2, true>(ctx, B * H, p) : fma_fwd<2, false>(ctx, B * H, p));
     if (rc) return rc;
@@ -555,7 +662,7 @@ int gcb_window_attention_bwd_f32(gcb_ctx* ctx, int64_t B, int64_t H, int64_t T, 
     if (rc) return rc;
     GCB_REQUIRE(bias || !dbias, "gcb_window_attention_bwd_f32: a gradient of the bias without a bias");
     if (B == 0 || H == 0 || T == 0 || D == 0) return dbias && !accumulate_dbias && H > 0 ? gcb_fill_f32(ctx, dbias, 0.0f, H * buckets) : GCB_OK;
-    if (D > AW_MAX_D || T > AW_MAX_T) { set_error("gcb_window_attention_bwd_f32: heads of up to %lld columns and sequences of up to %lld positions", (long long)AW_MAX_D, (long long)AW_MAX_T); return GCB_UNSUPPORTED; }
+    if (D > AW_MAX_D || T > AW_MAX_T || H > AW_MAX_H) { set_error("gcb_window_attention_bwd_f32: at most %lld heads of %lld columns and sequences of %lld positions", (long long)AW_MAX_H, (long long)AW_MAX_D, (long long)AW_MAX_T); return GCB_UNSUPPORTED; }
     GCB_REQUIRE(dq && dk && dv && dout && out && stats && q && k && v && own_rows(B, H, T, D, d_ld, d_so, d_si), "gcb_window_attention_bwd_f32: NULL pointer, or gradient rows that overlap");
     cudaSetDevice(ctx->device);
     p.q = q; p.q_ld = q_ld; p.q_so = q_so; p.q_si = q_si;
@@ -567,12 +674,14 @@ int gcb_window_attention_bwd_f32(gcb_ctx* ctx, int64_t B, int64_t H, int64_t T, 
     p.Tp = gcb_attention_stats_floats(1, 1, T) / 2; p.T = (int)T; p.D = (int)D; p.H = (int)H; p.scale = scale;
     p.row_max = const_cast<float*>(stats); p.row_inv = p.row_max + B * H * p.Tp;
     p.tiles = (int)((T + AS_OWN - 1) / AS_OWN);
-    const int64_t Dp = (D + 3) / 4 * 4, heads = B * H;
+    const int64_t heads = B * H;
     const bool vec = D % 4 == 0 && vec_rows(q, q_ld, q_so, q_si) && vec_rows(k, k_ld, k_so, k_si) && vec_rows(v, v_ld, v_so, v_si) && vec_rows(dout, g_ld, g_so, g_si) && vec_rows(out, o_ld, o_so, o_si) &&
                      vec_rows(dq, d_ld, d_so, d_si) && vec_rows(dk, d_ld, d_so, d_si) && vec_rows(dv, d_ld, d_so, d_si);
     const bool tc = window_tc_takes(ctx, B, p);
     const int tiles = tc ? (int)((T + AW_TC_TILE - 1) / AW_TC_TILE) : p.tiles;
-    Scratch part(ctx), far(ctx);
+    Scratch part(ctx), far(ctx), tab(ctx), delta(ctx);
+    if ((rc = make_table(ctx, p, tab)) || (rc = delta.get(sizeof(float) * (size_t)(heads * p.Tp)))) return rc;
+    p.delta = delta.as<float>();
     if (dbias) {
         if ((rc = part.get(sizeof(float) * (size_t)(heads * tiles * buckets)))) return rc;
         p.dbias_part = part.as<float>();
@@ -580,13 +689,7 @@ int gcb_window_attention_bwd_f32(gcb_ctx* ctx, int64_t B, int64_t H, int64_t T, 
     if (tc) rc = window_tc_bwd(ctx, B, p);
     else rc = D <= 64 ? (vec ? fma_bwd<1, true>(ctx, heads, p) : fma_bwd<1, false>(ctx, heads, p)) : (vec ? fma_bwd<2, true>(ctx, heads, p) : fma_bwd<2, false>(ctx, heads, p));
     if (rc) return rc;
-    if (p.rule.S > 0 && p.rule.W < T) {  // some query looks past its window
-        p.far_chunks = (int)((T + AW_FAR - 1) / AW_FAR);
-        if ((rc = far.get(sizeof(float) * (size_t)(heads * ((p.rule.S + AS_OWN - 1) / AS_OWN) * p.far_chunks * 2 * AS_OWN * Dp)))) return rc;
-        p.far_part = far.as<float>();
-        rc = D <= 64 ? (vec ? fma_far<1, true>(ctx, heads, p) : fma_far<1, false>(ctx, heads, p)) : (vec ? fma_far<2, true>(ctx, heads, p) : fma_far<2, false>(ctx, heads, p));
-        if (rc) return rc;
-    }
+    if (p.rule.S > 0 && p.rule.W < T && (rc = far_gradients(ctx, heads, p, vec, far))) return rc;  // some query looks past its window
     for (float* d : {dq, dk, dv}) note_write(ctx, d, span_bytes(B, H, T, D, d_ld, d_so, d_si));
     if (dbias) {
         GCB_CHECK_CUDA(launch_next(ctx->stream, dim3((unsigned)((H * buckets + 7) / 8)), 256, 0, window_attention_dbias_kernel, dbias, part.as<float>(), (int)H, (int)B, tiles, (int)buckets, accumulate_dbias));

@@ -24,6 +24,8 @@ struct WindowRule {
     }
 };
 
+__device__ __forceinline__ int clamp_distance(int d, int len) { return max(0, min(d, len - 1)); }
+
 // Checks and copies the rule of an entry point.
 inline int make_rule(WindowRule& r, const char* who, int64_t window, int64_t sinks, const float* bias, int64_t buckets, const int64_t* starts) {
     GCB_REQUIRE(window >= 0, "%s: the window must be a number of positions, or 0 for all of them", who);
@@ -47,8 +49,10 @@ struct WindowAttn {
     const float *q, *k, *v, *g, *o;
     float *out, *dq, *dk, *dv, *row_max, *row_inv;  // statistics: per query the maximum score and 1 / sum (infinity and 0 where nothing is seen: P is then 0 whatever a score is), Tp a head
     float *dbias_part, *far_part;                   // backward: partial sums, see the kernels that fill them
+    float* delta;                                   // backward: dO . O per query, Tp a head, written with dQ
+    const float* tab;                               // [H][tab_len]: bias by distance, the last one for all distances beyond; NULL: no bias
     int64_t q_ld, q_so, q_si, k_ld, k_so, k_si, v_ld, v_so, v_si, g_ld, g_so, g_si, o_ld, o_so, o_si, d_ld, d_so, d_si, Tp;
-    int T, D, H, tiles, far_chunks;
+    int T, D, H, tiles, tab_len, far_chunks, far_rows;
     float scale;
     WindowRule rule;
 };

@@ -6,7 +6,7 @@
 // Tiles, roles and the order of products are those of attention.cu, with these differences:
 //   - a unit's key blocks are the blocks of the first S keys and those of its window; the two query tiles of a forward CTA share the union;
 //   - scores are masked only in blocks that a border of the rule passes through, a test per warp;
-//   - a bias is read from a table by distance (one launch makes it, as long as the distances it tells apart), 191 entries a block through
+//   - a bias is read from a table by distance, 191 entries a block through
 //     shared memory, beyond its last distance from a register;
 //   - a query may see nothing of a block that its tile visits: a maximum of -inf stands for "nothing yet" until the first key;
 //   - dQ is a kernel of its own that forms P and dS again (three products a block), because dS of a long sequence is too much memory: five
@@ -38,14 +38,6 @@ struct WindowTc {
     int* status;
     WindowRule rule;
 };
-
-__global__ void __launch_bounds__(256) window_attention_table_kernel(float* __restrict__ tab, int len, const __grid_constant__ WindowRule r) {
-    pdl_trigger();
-    pdl_wait();
-    const int d = blockIdx.x * 256 + threadIdx.x, h = blockIdx.y;
-    if (d < len) tab[(int64_t)h * len + d] = r.bias[(int64_t)h * r.buckets + r.bucket(d)];
-}
-__device__ __forceinline__ int clamp_distance(int d, int len) { return max(0, min(d, len - 1)); }
 
 // The key blocks that a 128-query tile from row r0 looks at: 0 .. sinks - 1, then first .. last.  None where r0 lies beyond the sequence.
 struct TileKeys {
@@ -1126,19 +1118,9 @@ static WindowTc operands(gcb_ctx* ctx, int64_t B, const WindowAttn& a, int tiles
     p.o = a.o; p.o_ld = a.o_ld; p.o_so = a.o_so; p.o_si = a.o_si;
     p.dq = a.dq; p.dk = a.dk; p.dv = a.dv; p.d_ld = a.d_ld; p.d_so = a.d_so; p.d_si = a.d_si;
     p.out = a.out; p.row_max = a.row_max; p.row_inv = a.row_inv; p.dbias_part = a.dbias_part;
-    p.scale = a.scale; p.T = a.T; p.D = a.D; p.rule = a.rule; p.status = ctx->d_status;
+    p.delta = a.delta; p.tab = a.tab; p.tab_len = a.tab_len; p.scale = a.scale; p.T = a.T; p.D = a.D; p.rule = a.rule; p.status = ctx->d_status;
     plan(p, B, a.H, a.T, tiles_per_unit);
     return p;
-}
-// The bias by distance of every head, up to the first distance of the last bucket.
-static int make_table(gcb_ctx* ctx, WindowTc& p, Scratch& mem) {
-    if (p.rule.bias == nullptr) return GCB_OK;
-    p.tab_len = std::min(p.T, p.rule.starts[p.rule.buckets - 1] + 1);
-    const int rc = mem.get(sizeof(float) * (size_t)p.H * p.tab_len);
-    if (rc) return rc;
-    p.tab = mem.as<float>();
-    GCB_CHECK_CUDA(launch_next(ctx->stream, dim3((unsigned)((p.tab_len + 255) / 256), (unsigned)p.H), 256, 0, window_attention_table_kernel, mem.as<float>(), p.tab_len, p.rule));
-    return after_launch(ctx, "window_attention_table");
 }
 template <class K, class... Maps>
 static int tc_launch(gcb_ctx* ctx, K kernel, bool* done, unsigned threads, size_t smem, const WindowTc& p, const Maps&... maps) {
@@ -1178,16 +1160,15 @@ bool window_tc_takes(gcb_ctx* ctx, int64_t B, const WindowAttn& a) {
     if (a.g && (!rows_ok(a.g, a.g_ld, a.g_so, a.g_si, B, a.H) || !rows_ok(a.o, a.o_ld, a.o_so, a.o_si, B, a.H) || !rows_ok(a.dq, a.d_ld, a.d_so, a.d_si, B, a.H) || !rows_ok(a.dk, a.d_ld, a.d_so, a.d_si, B, a.H) ||
                 !rows_ok(a.dv, a.d_ld, a.d_so, a.d_si, B, a.H)))
         return false;
-    return B * a.H * ((a.T + 127) / 128) < (int64_t(1) << 30) && a.H <= 65535 && tma_encode(ctx) != nullptr;
+    return B * a.H * ((a.T + 127) / 128) < (int64_t(1) << 30) && tma_encode(ctx) != nullptr;
 }
 
 int window_tc_fwd(gcb_ctx* ctx, int64_t B, const WindowAttn& a) {
     TmaEncodeFn enc = tma_encode(ctx);
     // two query tiles share their key blocks; one tile a CTA where pairs would leave SMs idle
     WindowTc p = operands(ctx, B, a, B * a.H * ((a.T + 255) / 256) < kSMs ? 1 : 2);
-    Scratch tab(ctx), moved(ctx);
-    int rc = make_table(ctx, p, tab);
-    if (!rc) rc = make_moved(p, moved);
+    Scratch moved(ctx);
+    int rc = make_moved(p, moved);
     if (rc) return rc;
     CUtensorMap k, v, q, o;
     GCB_REQUIRE(encode_rows(enc, &k, a.k, a.D, a.T, a.k_ld, a.k_si, a.k_so, a.H, B, 32, AT_KEYS, CU_TENSOR_MAP_SWIZZLE_128B) &&
@@ -1203,12 +1184,9 @@ int window_tc_fwd(gcb_ctx* ctx, int64_t B, const WindowAttn& a) {
 int window_tc_bwd(gcb_ctx* ctx, int64_t B, const WindowAttn& a) {
     TmaEncodeFn enc = tma_encode(ctx);
     WindowTc p = operands(ctx, B, a, 1);
-    Scratch tab(ctx), delta(ctx), moved(ctx);
-    int rc = make_table(ctx, p, tab);
-    if (!rc) rc = make_moved(p, moved);
-    if (!rc) rc = delta.get(sizeof(float) * (size_t)(p.heads * p.Tp));
+    Scratch moved(ctx);
+    const int rc = make_moved(p, moved);
     if (rc) return rc;
-    p.delta = delta.as<float>();
     BwdMaps m;
     auto rows = [&](CUtensorMap& map, const float* x, int64_t ld, int64_t so, int64_t si, bool k_major) {
         return encode_rows(enc, &map, x, a.D, a.T, ld, si, so, a.H, B, 32, AT_KEYS, k_major ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B);
