@@ -74,14 +74,14 @@ __device__ __forceinline__ void win_load(uint32_t dst, const CUtensorMap* map, u
 #pragma unroll
     for (int c = 0; c < DP / 32; ++c) tma_load_4d(dst + c * 8192, map, bar, 32 * c, r0, h, b);
 }
-// Companions of a raw tile; 128 threads, a core-matrix row (8 columns) at a time, all loads first.
-template <int DP, bool MN>
+// Companions of a raw tile by THREADS threads, a core-matrix row (8 columns) at a time, all loads first.
+template <int DP, int THREADS, bool MN>
 __device__ __forceinline__ void win_split(const uint8_t* raw, uint8_t* twin, int t) {
-    constexpr int U = DP / 16;
+    constexpr int U = 8 * DP / THREADS;
     float4 x[U][2];
 #pragma unroll
     for (int v = 0; v < U; ++v) {
-        const int u = t + 128 * v, r = u & 7, j = (u >> 3) % (DP / 8), row = u / DP * 8 + r;
+        const int u = t + THREADS * v, r = u & 7, j = (u >> 3) % (DP / 8), row = u / DP * 8 + r;
         const uint8_t* at = raw + (j >> 2) * 8192 + row * 128;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
@@ -91,7 +91,7 @@ __device__ __forceinline__ void win_split(const uint8_t* raw, uint8_t* twin, int
     }
 #pragma unroll
     for (int v = 0; v < U; ++v) {
-        const int u = t + 128 * v, r = u & 7, j = (u >> 3) % (DP / 8);
+        const int u = t + THREADS * v, r = u & 7, j = (u >> 3) % (DP / 8);
         const bool swap = MN && (r >> 2);
         const float4 a = swap ? x[v][1] : x[v][0], b = swap ? x[v][0] : x[v][1];
         uint8_t* at = twin + u / DP * WinTile<DP>::ROWS8 + j * 128 + r * 16;
@@ -320,8 +320,8 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 1) window_attention_tc_fwd_ker
                     ok = warp_wait(full(b), (n >> 1) & 1u, p.status, 46);
                     if (!ok) break;
                     uint8_t* raw = gen + S::BLOCKS_OFF + b * S::BLOCK;
-                    if (kind == 0) win_split<DP, false>(raw, raw + S::RAW, t);
-                    else win_split<DP, true>(raw, raw + S::RAW, t);
+                    if (kind == 0) win_split<DP, 128, false>(raw, raw + S::RAW, t);
+                    else win_split<DP, 128, true>(raw, raw + S::RAW, t);
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
                     if (lane == 0) mbar_arrive(conv(b));
@@ -485,19 +485,18 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 1) window_attention_tc_fwd_ker
 // A thread owns a key and sixteen of a block's queries, everything transposed: S^T = k q^T, dP^T = v dO^T, dV += P^T dO, dK += dS^T q, for the
 // queries from the diagonal to the window's end.  Products are ordered so that the tensor core has dV(i), S(i+1) to do while dS(i) is made
 // and dK(i), dP(i+1) while P(i+1) is.
-//   warp 0       TMA producer        warp 1       MMA issuer
-//   warps 4..7   companions of q, the statistics of its rows and the bias        warps 8..11  companions of dO        warps 12..27  four threads a key
-// A tile of q arrives K-major and once more MN-major; so does dO.  Companions stay until the tile's second product has read them: three places for
-// those of q, so that a block's scores do not wait for dK of the block before.
+//   warps 0, 2   TMA producers: K-major tiles, MN-major tiles       warp 1  MMA issuer
+//   warps 4..11  companions, the statistics of a block's queries and its bias        warps 12..27  four threads a key
+// A tile of q arrives K-major and once more MN-major; so does dO.  Its companions serve both products and stay until the second has read them.
 // Tensor memory: S^T / t of P^T [0, 64), dP^T / t of dS^T [64, 128), P^T companions [128, 192), dS^T companions [192, 256), dV [256, 320), dK [320, 384),
 // t of k [384, 448), t of v [448, 512).
 template <int DP>
 struct DkvSmem {
     using T = WinTile<DP>;
     static constexpr int OWN = AT_ROWS * DP * 4;  // companions of a 128-row operand
-    static constexpr int Q_RAW = 2 * OWN, O_RAW = Q_RAW + T::RAW, Q_MN = O_RAW + T::RAW, O_MN = Q_MN + T::RAW, Q_TWIN = O_MN + T::RAW, O_TWIN = Q_TWIN + 3 * T::TWIN;
-    static constexpr int STATS = O_TWIN + 2 * T::TWIN;  // row maximum, 1 / sum and dO . O of a block's queries, three blocks; then the bias of its distances, three blocks
-    static constexpr int TABS = STATS + 3 * 3 * AT_KEYS * 4, BAR = TABS + 3 * WT_TAB * 4, TOTAL = BAR + 256 + 1024;
+    static constexpr int Q_RAW = 2 * OWN, O_RAW = Q_RAW + 2 * T::RAW, Q_MN = O_RAW + 2 * T::RAW, O_MN = Q_MN + T::RAW, Q_TWIN = O_MN + T::RAW, O_TWIN = Q_TWIN + 2 * T::TWIN;
+    static constexpr int STATS = O_TWIN + T::TWIN;  // row maximum, 1 / sum and dO . O of a block's queries, two blocks; then the bias of its distances, two blocks
+    static constexpr int TABS = STATS + 2 * 3 * AT_KEYS * 4, BAR = TABS + 2 * WT_TAB * 4, TOTAL = BAR + 256 + 1024;
     static_assert(TOTAL <= 232448, "shared memory");
 };
 template <int DP, bool BIAS>
@@ -510,21 +509,21 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
     const uint32_t bars = base + S::BAR;
-    enum { QK = 0, OK = 1, ON = 2, QN = 3 };  // tiles: q and dO K-major for the scores and dP, dO and q MN-major for dV and dK
     auto bar = [&](int i) { return bars + 8u * i; };
     // n: running number of a block; parities of what has two places and of what has one
     auto two = [](uint32_t n) { return (n >> 1) & 1u; };
     auto one = [](uint32_t n) { return n & 1u; };
-    auto three = [](uint32_t n) { return (n / 3u) & 1u; };
-    auto q_conv = [&](uint32_t n) { return bar(0 + n % 3u); };
-    auto q_free = [&](uint32_t n) { return bar(3 + n % 3u); };    // companions: dK has read them
-    auto o_conv = [&](uint32_t n) { return bar(6 + (n & 1u)); };
-    auto o_free = [&](uint32_t n) { return bar(8 + (n & 1u)); };  // dV has read them
-    const uint32_t q_full = bar(10), q_empty = bar(11), o_full = bar(12), o_empty = bar(13), on_full = bar(14), on_empty = bar(15), qn_full = bar(16), qn_empty = bar(17);
+    auto q_full = [&](uint32_t n) { return bar(0 + (n & 1u)); };
+    auto q_empty = [&](uint32_t n) { return bar(2 + (n & 1u)); };
+    auto q_conv = [&](uint32_t n) { return bar(4 + (n & 1u)); };
+    auto q_free = [&](uint32_t n) { return bar(6 + (n & 1u)); };  // companions: dK has read them
+    auto o_full = [&](uint32_t n) { return bar(8 + (n & 1u)); };
+    auto o_empty = [&](uint32_t n) { return bar(10 + (n & 1u)); };
+    const uint32_t o_conv = bar(12), o_free = bar(13), on_full = bar(14), on_empty = bar(15), qn_full = bar(16), qn_empty = bar(17);
     const uint32_t s_full = bar(18), dp_full = bar(19), p_ready = bar(20), ds_ready = bar(21), acc_full = bar(22), kv_ready = bar(23), own_full = bar(24);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 25; ++i) mbar_init(bar(i), i < 3 || i == 6 || i == 7 ? 4 : i == 20 || i == 21 || i == 23 ? 16 : i == 24 ? 2 : 1);  // own_full: two tiles
+        for (int i = 0; i < 25; ++i) mbar_init(bar(i), i == 4 || i == 5 || i == 12 ? 8 : i == 20 || i == 21 || i == 23 ? 16 : i == 24 ? 2 : 1);  // own_full: two tiles
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     const uint32_t tmem = tmem_take(bars + 8u * 28, reinterpret_cast<volatile uint32_t*>(gen + S::BAR + 8 * 28), warp);
@@ -536,7 +535,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
     };
 
     if (warp < 4) regs_give<64>();
-    if (warp == 0) {
+    if (warp == 0 || warp == 2) {  // K-major tiles by warp 0, up to two blocks ahead, MN-major ones by warp 2
         if (lane == 0) {
             uint32_t n0 = 0;
             bool ok = true;
@@ -544,18 +543,16 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
                 const AttnItem it = attn_item(p, w, true);
                 if (it.skip) continue;
                 const int n = steps(it);
-                auto load = [&](int kind, int i) {
-                    if (i >= n) return true;
-                    const uint32_t at = n0 + i;
-                    const uint32_t e = kind == QK ? q_empty : kind == OK ? o_empty : kind == ON ? on_empty : qn_empty, f = kind == QK ? q_full : kind == OK ? o_full : kind == ON ? on_full : qn_full;
-                    const uint32_t dst = base + (kind == QK ? S::Q_RAW : kind == OK ? S::O_RAW : kind == ON ? S::O_MN : S::Q_MN);
-                    if (!mbar_wait(e, one(at) ^ 1u, p.status, 51)) return false;
-                    win_load<DP>(dst, kind == QK ? &map_qk : kind == OK ? &map_ok : kind == ON ? &map_on : &map_qn, f, it.unit * AT_ROWS + i * AT_KEYS, it.h, it.b);
+                auto load = [&](uint32_t free, uint32_t parity, int dst, const CUtensorMap* map, uint32_t landed, int i) {
+                    if (!mbar_wait(free, parity ^ 1u, p.status, 51)) return false;
+                    win_load<DP>(base + dst, map, landed, it.unit * AT_ROWS + i * AT_KEYS, it.h, it.b);
                     return true;
                 };
-                ok = load(QK, 0) && load(OK, 0);
-                // in the order in which places become free: S(i), dV(i - 1), dP(i), dK(i - 1)
-                for (int i = 0; i < n && ok; ++i) ok = load(QK, i + 1) && load(ON, i) && load(OK, i + 1) && load(QN, i);
+                for (int i = 0; i < n && ok; ++i) {
+                    const uint32_t at = n0 + i, place = (at & 1u) * T::RAW;
+                    if (warp == 0) ok = load(q_empty(at), two(at), S::Q_RAW + place, &map_qk, q_full(at), i) && load(o_empty(at), two(at), S::O_RAW + place, &map_ok, o_full(at), i);
+                    else ok = load(on_empty, one(at), S::O_MN, &map_on, on_full, i) && load(qn_empty, one(at), S::Q_MN, &map_qn, qn_full, i);
+                }
                 n0 += n;
             }
         }
@@ -576,18 +573,18 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
                 auto scores = [&](int i) {
                     const uint32_t at = n0 + i;
                     if (i >= n) return true;
-                    if (!landed(q_conv(at), three(at))) return false;
-                    win_scores<DP>(tmem, tmem + 384, base16, base16 + S::Q_RAW / 16, base16 + (S::Q_TWIN + at % 3u * T::TWIN) / 16);
-                    umma_commit(q_empty);
+                    if (!landed(q_conv(at), two(at))) return false;
+                    win_scores<DP>(tmem, tmem + 384, base16, base16 + (S::Q_RAW + (at & 1u) * T::RAW) / 16, base16 + (S::Q_TWIN + (at & 1u) * T::TWIN) / 16);
+                    umma_commit(q_empty(at));
                     umma_commit(s_full);
                     return true;
                 };
                 auto dprobs = [&](int i) {
                     const uint32_t at = n0 + i;
                     if (i >= n) return true;
-                    if (!landed(o_conv(at), two(at))) return false;
-                    win_scores<DP>(tmem + 64, tmem + 448, base16 + S::OWN / 16, base16 + S::O_RAW / 16, base16 + (S::O_TWIN + (at & 1u) * T::TWIN) / 16);
-                    umma_commit(o_empty);
+                    if (!landed(o_conv, one(at))) return false;
+                    win_scores<DP>(tmem + 64, tmem + 448, base16 + S::OWN / 16, base16 + (S::O_RAW + (at & 1u) * T::RAW) / 16, base16 + S::O_TWIN / 16);
+                    umma_commit(o_empty(at));
                     umma_commit(dp_full);
                     return true;
                 };
@@ -598,12 +595,12 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
                     const uint32_t at = n0 + i;
                     ok = mbar_wait(on_full, one(at), p.status, 54) && landed(p_ready, one(at));
                     if (!ok) break;
-                    win_values<DP, 8>(tmem + 256, tmem, tmem + 128, tmem + 160, base16 + S::O_MN / 16, base16 + (S::O_TWIN + (at & 1u) * T::TWIN) / 16, i % WT_FLUSH != 0);
+                    win_values<DP, 8>(tmem + 256, tmem, tmem + 128, tmem + 160, base16 + S::O_MN / 16, base16 + S::O_TWIN / 16, i % WT_FLUSH != 0);
                     umma_commit(on_empty);
-                    umma_commit(o_free(at));
+                    umma_commit(o_free);
                     ok = scores(i + 1) && mbar_wait(qn_full, one(at), p.status, 55) && landed(ds_ready, one(at));
                     if (!ok) break;
-                    win_values<DP, 8>(tmem + 320, tmem + 64, tmem + 192, tmem + 224, base16 + S::Q_MN / 16, base16 + (S::Q_TWIN + at % 3u * T::TWIN) / 16, i % WT_FLUSH != 0);
+                    win_values<DP, 8>(tmem + 320, tmem + 64, tmem + 192, tmem + 224, base16 + S::Q_MN / 16, base16 + (S::Q_TWIN + (at & 1u) * T::TWIN) / 16, i % WT_FLUSH != 0);
                     umma_commit(qn_empty);
                     umma_commit(q_free(at));
                     ok = dprobs(i + 1);
@@ -615,8 +612,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
         }
     } else if (warp >= 4 && warp < 12) {
         regs_give<56>();
-        const int t = threadIdx.x & 127;
-        const bool of_q = warp < 8;
+        const int t = threadIdx.x - 128;
         uint32_t n0 = 0;
         bool ok = true;
         for (int64_t w = blockIdx.x; w < p.loop_end && ok; w += gridDim.x) {
@@ -625,40 +621,39 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
             const int n = steps(it), q_at = it.unit * AT_ROWS + t;
             const int64_t at_head = ((int64_t)it.b * p.H + it.h) * p.Tp;
             const float* tab = BIAS ? p.tab + (int64_t)it.h * p.tab_len : nullptr;
-            float nm = 0.f, ni = 0.f, nd = 0.f, nb0 = 0.f, nb1 = 0.f;  // the next block's, loaded a block ahead
+            float nm = 0.f, ni = 0.f, nd = 0.f, nb = 0.f;  // the next block's, loaded a block ahead
             auto request = [&](int i) {
                 const int q = q_at + i * AT_KEYS, d0 = i * AT_KEYS - (AT_ROWS - 1);
                 const bool live = t < AT_KEYS && q < p.T;  // queries beyond the sequence have no statistics: P is then zero
                 nm = live ? __ldg(p.row_max + at_head + q) : INFINITY;
                 ni = live ? __ldg(p.row_inv + at_head + q) : 0.0f;
                 nd = live ? __ldg(p.delta + at_head + q) : 0.0f;
-                if (BIAS) {
-                    nb0 = __ldg(tab + clamp_distance(d0 + t, p.tab_len));
-                    nb1 = __ldg(tab + clamp_distance(d0 + t + 128, p.tab_len));
-                }
+                if (BIAS) nb = __ldg(tab + clamp_distance(d0 + t, p.tab_len));
             };
-            if (of_q) request(0);
+            request(0);
             for (int i = 0; i < n && ok; ++i) {
-                const uint32_t at = n0 + i;
-                ok = warp_wait(of_q ? q_full : o_full, one(at), p.status, 56);
+                const uint32_t at = n0 + i, place = (at & 1u) * T::RAW;
+                // dK of the block before last has read the companions that these replace; its statistics were used before that
+                ok = warp_wait(q_full(at), two(at), p.status, 56) && warp_wait(q_free(at), two(at) ^ 1u, p.status, 56);
                 if (!ok) break;
-                ok = warp_wait(of_q ? q_free(at) : o_free(at), (of_q ? three(at) : two(at)) ^ 1u, p.status, 56);  // the second product that read what is there
-                if (!ok) break;
-                if (of_q) {
-                    // in three places as well: what was there has been used by the block whose companions these replace
-                    float* slot = reinterpret_cast<float*>(gen + S::STATS) + at % 3u * 3 * AT_KEYS + t;
-                    if (t < AT_KEYS) { slot[0] = BIAS ? nm : nm * kLog2e - log2f(ni); slot[AT_KEYS] = ni; slot[2 * AT_KEYS] = nd; }
-                    if (BIAS) {
-                        float* tb = reinterpret_cast<float*>(gen + S::TABS) + at % 3u * WT_TAB + t;
-                        tb[0] = nb0;
-                        if (t < WT_TAB - 128) tb[128] = nb1;
-                    }
-                    if (i + 1 < n) request(i + 1);
+                if (t < AT_KEYS) {
+                    float* slot = reinterpret_cast<float*>(gen + S::STATS) + (at & 1u) * 3 * AT_KEYS + t;
+                    slot[0] = BIAS ? nm : nm * kLog2e - log2f(ni);
+                    slot[AT_KEYS] = ni;
+                    slot[2 * AT_KEYS] = nd;
                 }
-                win_split<DP, false>(gen + (of_q ? S::Q_RAW : S::O_RAW), gen + (of_q ? S::Q_TWIN + at % 3u * T::TWIN : S::O_TWIN + (at & 1u) * T::TWIN), t);
+                if (BIAS && t < WT_TAB) reinterpret_cast<float*>(gen + S::TABS)[(at & 1u) * WT_TAB + t] = nb;
+                if (i + 1 < n) request(i + 1);
+                win_split<DP, 256, false>(gen + S::Q_RAW + place, gen + S::Q_TWIN + (at & 1u) * T::TWIN, t);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(of_q ? q_conv(at) : o_conv(at));
+                if (lane == 0) mbar_arrive(q_conv(at));
+                ok = warp_wait(o_full(at), two(at), p.status, 56) && warp_wait(o_free, one(at) ^ 1u, p.status, 56);
+                if (!ok) break;
+                win_split<DP, 256, false>(gen + S::O_RAW + place, gen + S::O_TWIN, t);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(o_conv);
             }
             n0 += n;
         }
@@ -702,7 +697,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
             };
 #pragma unroll 1
             for (int i = 0; i < cnt; ++i, ++n) {
-                const float4* mp = reinterpret_cast<const float4*>(gen + S::STATS + n % 3u * 3 * AT_KEYS * 4) + 4 * part;
+                const float4* mp = reinterpret_cast<const float4*>(gen + S::STATS + (n & 1u) * 3 * AT_KEYS * 4) + 4 * part;
                 const float4 *ip = mp + AT_KEYS / 4, *dp = ip + AT_KEYS / 4;
                 good = good && warp_wait(s_full, n & 1u, p.status, 57);
                 after_sync();
@@ -711,7 +706,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
                 float pr[16];
                 tmem_ld16(lanes + 16 * part, u);
                 const int first = row - i * AT_KEYS - 16 * part;  // queries from here on look at this key, as many as the window is long
-                const float* bias = reinterpret_cast<const float*>(gen + S::TABS) + n % 3u * WT_TAB + (AT_ROWS - 1) + 16 * part - row;
+                const float* bias = reinterpret_cast<const float*>(gen + S::TABS) + (n & 1u) * WT_TAB + (AT_ROWS - 1) + 16 * part - row;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float4 m = mp[e];
@@ -774,7 +769,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
 // ---- dQ and the bias gradient ---------------------------------------------------------------------------------------------------
 // A CTA takes 128 queries and walks over their keys: S = q k^T and dP = dO v^T of one block while dQ += dS k of the block before passes.  Four
 // threads a query, sixteen of a block's keys each.  dO . O is formed here, from the rows that are loaded anyway, and kept for dK.
-// Roles as above, the companions of k and the bias by warps 4..7, those of v by warps 8..11.  K-major tiles arrive up to two blocks ahead.
+// Roles as above.
 // Scores and dP alternate between two places, x = 0 and 1; dS takes the place of both, a thread's columns where it has read them.
 // Tensor memory: S / companions of dS [128 x, + 64) (of 16 keys: 8 columns bf16(dS), 8 bf16(dS - t)), dP / t of dS [128 x + 64, + 64), dQ [256, 320), t of q [320, 384), t of dO [384, 448).
 // Bias gradient: a warp adds up the dS of its 32 x 16 block along the diagonals, 47 of them, in sixteen shuffles, and lane n those
@@ -798,7 +793,6 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
     const uint32_t bars = base + S::BAR;
-    enum { KK = 0, VK = 1, KN = 2 };  // tiles: k and v K-major for the scores and dP, k MN-major for dQ
     auto bar = [&](int i) { return bars + 8u * i; };
     auto two = [](uint32_t n) { return (n >> 1) & 1u; };
     auto one = [](uint32_t n) { return n & 1u; };
@@ -815,7 +809,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
     const uint32_t kn_full = bar(20), kn_empty = bar(21), acc_full = bar(22), q_ready = bar(23), v_conv = bar(24), v_free = bar(25), own_full = bar(26);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 27; ++i) mbar_init(bar(i), (i >= 4 && i < 7) || i == 24 ? 4 : i == 18 || i == 19 || i == 23 ? 16 : i == 26 ? 2 : 1);  // own_full: two tiles
+        for (int i = 0; i < 27; ++i) mbar_init(bar(i), (i >= 4 && i < 7) || i == 24 ? 8 : i == 18 || i == 19 || i == 23 ? 16 : i == 26 ? 2 : 1);  // own_full: two tiles
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     const uint32_t tmem = tmem_take(bars + 8u * 28, reinterpret_cast<volatile uint32_t*>(gen + S::BAR + 8 * 28), warp);
@@ -823,7 +817,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
     pdl_wait();
 
     if (warp < 4) regs_give<64>();
-    if (warp == 0) {
+    if (warp == 0 || warp == 2) {  // K-major tiles by warp 0, up to two blocks ahead, MN-major ones by warp 2
         if (lane == 0) {
             uint32_t n0 = 0;
             bool ok = true;
@@ -832,18 +826,16 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
                 if (it.skip) continue;
                 const TileKeys keys(p, it.unit * AT_ROWS);
                 const int n = keys.count();
-                auto load = [&](int kind, int i) {
-                    if (i >= n) return true;
-                    const uint32_t at = n0 + i;
-                    const uint32_t e = kind == KK ? k_empty(at) : kind == VK ? v_empty(at) : kn_empty, f = kind == KK ? k_full(at) : kind == VK ? v_full(at) : kn_full;
-                    const uint32_t dst = base + (kind == KN ? S::K_MN : (kind == KK ? S::K_RAW : S::V_RAW) + (at & 1u) * T::RAW);
-                    if (!mbar_wait(e, (kind == KN ? one(at) : two(at)) ^ 1u, p.status, 61)) return false;
-                    win_load<DP>(dst, kind == KK ? &map_kk : kind == VK ? &map_vk : &map_kn, f, keys.block(i) * AT_KEYS, it.h, it.b);
+                auto load = [&](uint32_t free, uint32_t parity, int dst, const CUtensorMap* map, uint32_t landed, int i) {
+                    if (!mbar_wait(free, parity ^ 1u, p.status, 61)) return false;
+                    win_load<DP>(base + dst, map, landed, keys.block(i) * AT_KEYS, it.h, it.b);
                     return true;
                 };
-                ok = load(KK, 0) && load(VK, 0) && load(KK, 1) && load(VK, 1);
-                // in the order in which places become free: S(i), dP(i), dQ(i - 1)
-                for (int i = 0; i < n && ok; ++i) ok = load(KN, i) && load(KK, i + 2) && load(VK, i + 2);
+                for (int i = 0; i < n && ok; ++i) {
+                    const uint32_t at = n0 + i, place = (at & 1u) * T::RAW;
+                    if (warp == 0) ok = load(k_empty(at), two(at), S::K_RAW + place, &map_kk, k_full(at), i) && load(v_empty(at), two(at), S::V_RAW + place, &map_vk, v_full(at), i);
+                    else ok = load(kn_empty, one(at), S::K_MN, &map_kn, kn_full, i);
+                }
                 n0 += n;
             }
         }
@@ -893,8 +885,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
         }
     } else if (warp >= 4 && warp < 12) {
         regs_give<56>();
-        const int t = threadIdx.x & 127;
-        const bool of_k = warp < 8;
+        const int t = threadIdx.x - 128;
         uint32_t n0 = 0;
         bool ok = true;
         for (int64_t w = blockIdx.x; w < p.loop_end && ok; w += gridDim.x) {
@@ -903,29 +894,28 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
             const TileKeys keys(p, it.unit * AT_ROWS);
             const int n = keys.count();
             const float* tab = BIAS ? p.tab + (int64_t)it.h * p.tab_len : nullptr;
-            float nb0 = 0.f, nb1 = 0.f;  // the next block's, loaded a block ahead
-            auto request = [&](int i) {
-                const int d0 = it.unit * AT_ROWS - (keys.block(i) + 1) * AT_KEYS + 1;
-                nb0 = __ldg(tab + clamp_distance(d0 + t, p.tab_len));
-                nb1 = __ldg(tab + clamp_distance(d0 + t + 128, p.tab_len));
-            };
-            if (BIAS && of_k) request(0);
+            float nb = 0.f;  // the next block's, loaded a block ahead
+            auto request = [&](int i) { nb = __ldg(tab + clamp_distance(it.unit * AT_ROWS - (keys.block(i) + 1) * AT_KEYS + 1 + t, p.tab_len)); };
+            if (BIAS) request(0);
             for (int i = 0; i < n && ok; ++i) {
-                const uint32_t at = n0 + i;
-                ok = warp_wait(of_k ? k_full(at) : v_full(at), two(at), p.status, 65);
+                const uint32_t at = n0 + i, place = (at & 1u) * T::RAW;
+                // dQ of three blocks before has read the companions that these replace; its bias was used before that
+                ok = warp_wait(k_full(at), two(at), p.status, 65) && warp_wait(k_free(at), three(at) ^ 1u, p.status, 65);
                 if (!ok) break;
-                ok = warp_wait(of_k ? k_free(at) : v_free, (of_k ? three(at) : one(at)) ^ 1u, p.status, 65);  // the last product that read what is there
-                if (!ok) break;
-                if (BIAS && of_k) {  // in three places as well: what was there has been used by the block whose companions these replace
-                    float* tb = reinterpret_cast<float*>(gen + S::TABS) + at % 3u * WT_TAB + t;
-                    tb[0] = nb0;
-                    if (t < WT_TAB - 128) tb[128] = nb1;
+                if (BIAS) {
+                    if (t < WT_TAB) reinterpret_cast<float*>(gen + S::TABS)[at % 3u * WT_TAB + t] = nb;
                     if (i + 1 < n) request(i + 1);
                 }
-                win_split<DP, false>(gen + (of_k ? S::K_RAW : S::V_RAW) + (at & 1u) * T::RAW, gen + (of_k ? S::K_TWIN + at % 3u * T::TWIN : S::V_TWIN), t);
+                win_split<DP, 256, false>(gen + S::K_RAW + place, gen + S::K_TWIN + at % 3u * T::TWIN, t);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(of_k ? k_conv(at) : v_conv);
+                if (lane == 0) mbar_arrive(k_conv(at));
+                ok = warp_wait(v_full(at), two(at), p.status, 65) && warp_wait(v_free, one(at) ^ 1u, p.status, 65);
+                if (!ok) break;
+                win_split<DP, 256, false>(gen + S::V_RAW + place, gen + S::V_TWIN, t);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(v_conv);
             }
             n0 += n;
         }
