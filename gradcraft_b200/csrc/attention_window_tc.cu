@@ -490,20 +490,21 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 1) window_attention_tc_fwd_ker
 // A tile of q arrives K-major and once more MN-major; so does dO.  Its companions serve both products and stay until the second has read them.
 // Tensor memory: S^T / t of P^T [0, 64), dP^T / t of dS^T [64, 128), P^T companions [128, 192), dS^T companions [192, 256), dV [256, 320), dK [320, 384),
 // t of k [384, 448), t of v [448, 512).
-template <int DP>
+template <int DP, bool BIAS>
 struct DkvSmem {
     using T = WinTile<DP>;
     static constexpr int OWN = AT_ROWS * DP * 4;  // companions of a 128-row operand
-    static constexpr int Q_RAW = 2 * OWN, O_RAW = Q_RAW + 2 * T::RAW, Q_MN = O_RAW + 2 * T::RAW, O_MN = Q_MN + T::RAW, Q_TWIN = O_MN + T::RAW, O_TWIN = Q_TWIN + 2 * T::TWIN;
-    static constexpr int STATS = O_TWIN + T::TWIN;  // row maximum, 1 / sum and dO . O of a block's queries, two blocks; then the bias of its distances, two blocks
-    static constexpr int TABS = STATS + 2 * 3 * AT_KEYS * 4, BAR = TABS + 2 * WT_TAB * 4, TOTAL = BAR + 256 + 1024;
+    static constexpr int O_RAWS = BIAS ? 1 : 2;   // with a bias its table takes the place of the second one
+    static constexpr int Q_RAW = 2 * OWN, O_RAW = Q_RAW + 2 * T::RAW, Q_MN = O_RAW + O_RAWS * T::RAW, O_MN = Q_MN + T::RAW, Q_TWIN = O_MN + 2 * T::RAW, O_TWIN = Q_TWIN + 2 * T::TWIN;
+    static constexpr int STATS = O_TWIN + T::TWIN;  // row maximum, dO . O and (with a bias) 1 / sum of a block's queries, two blocks; then the bias of its distances, two blocks
+    static constexpr int STATS_BLOCK = (BIAS ? 3 : 2) * AT_KEYS * 4, TABS = STATS + 2 * STATS_BLOCK, BAR = TABS + (BIAS ? 2 * WT_TAB * 4 : 0), TOTAL = BAR + 256 + 1024;
     static_assert(TOTAL <= 232448, "shared memory");
 };
 template <int DP, bool BIAS>
 __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_kernel(const __grid_constant__ CUtensorMap map_qk, const __grid_constant__ CUtensorMap map_qn, const __grid_constant__ CUtensorMap map_ok,
                                                                                 const __grid_constant__ CUtensorMap map_on, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                                                                                 const __grid_constant__ CUtensorMap map_dk, const __grid_constant__ CUtensorMap map_dv, const __grid_constant__ WindowTc p) {
-    using S = DkvSmem<DP>;
+    using S = DkvSmem<DP, BIAS>;
     using T = WinTile<DP>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -517,13 +518,17 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
     auto q_empty = [&](uint32_t n) { return bar(2 + (n & 1u)); };
     auto q_conv = [&](uint32_t n) { return bar(4 + (n & 1u)); };
     auto q_free = [&](uint32_t n) { return bar(6 + (n & 1u)); };  // companions: dK has read them
-    auto o_full = [&](uint32_t n) { return bar(8 + (n & 1u)); };
-    auto o_empty = [&](uint32_t n) { return bar(10 + (n & 1u)); };
-    const uint32_t o_conv = bar(12), o_free = bar(13), on_full = bar(14), on_empty = bar(15), qn_full = bar(16), qn_empty = bar(17);
+    auto o_place = [](uint32_t n) { return S::O_RAWS == 2 ? n & 1u : 0u; };
+    auto o_parity = [](uint32_t n) { return S::O_RAWS == 2 ? (n >> 1) & 1u : n & 1u; };
+    auto o_full = [&](uint32_t n) { return bar(8 + o_place(n)); };
+    auto o_empty = [&](uint32_t n) { return bar(10 + o_place(n)); };
+    auto on_full = [&](uint32_t n) { return bar(14 + (n & 1u)); };
+    auto on_empty = [&](uint32_t n) { return bar(25 + (n & 1u)); };
+    const uint32_t o_conv = bar(12), o_free = bar(13), qn_full = bar(16), qn_empty = bar(17);
     const uint32_t s_full = bar(18), dp_full = bar(19), p_ready = bar(20), ds_ready = bar(21), acc_full = bar(22), kv_ready = bar(23), own_full = bar(24);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 25; ++i) mbar_init(bar(i), i == 4 || i == 5 || i == 12 ? 8 : i == 20 || i == 21 || i == 23 ? 16 : i == 24 ? 2 : 1);  // own_full: two tiles
+        for (int i = 0; i < 27; ++i) mbar_init(bar(i), i == 4 || i == 5 || i == 12 ? 8 : i == 20 || i == 21 || i == 23 ? 16 : i == 24 ? 2 : 1);  // own_full: two tiles
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     const uint32_t tmem = tmem_take(bars + 8u * 28, reinterpret_cast<volatile uint32_t*>(gen + S::BAR + 8 * 28), warp);
@@ -550,8 +555,8 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
                 };
                 for (int i = 0; i < n && ok; ++i) {
                     const uint32_t at = n0 + i, place = (at & 1u) * T::RAW;
-                    if (warp == 0) ok = load(q_empty(at), two(at), S::Q_RAW + place, &map_qk, q_full(at), i) && load(o_empty(at), two(at), S::O_RAW + place, &map_ok, o_full(at), i);
-                    else ok = load(on_empty, one(at), S::O_MN, &map_on, on_full, i) && load(qn_empty, one(at), S::Q_MN, &map_qn, qn_full, i);
+                    if (warp == 0) ok = load(q_empty(at), two(at), S::Q_RAW + place, &map_qk, q_full(at), i) && load(o_empty(at), o_parity(at), S::O_RAW + o_place(at) * T::RAW, &map_ok, o_full(at), i);
+                    else ok = load(on_empty(at), two(at), S::O_MN + place, &map_on, on_full(at), i) && load(qn_empty, one(at), S::Q_MN, &map_qn, qn_full, i);
                 }
                 n0 += n;
             }
@@ -583,7 +588,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
                     const uint32_t at = n0 + i;
                     if (i >= n) return true;
                     if (!landed(o_conv, one(at))) return false;
-                    win_scores<DP>(tmem + 64, tmem + 448, base16 + S::OWN / 16, base16 + (S::O_RAW + (at & 1u) * T::RAW) / 16, base16 + S::O_TWIN / 16);
+                    win_scores<DP>(tmem + 64, tmem + 448, base16 + S::OWN / 16, base16 + (S::O_RAW + o_place(at) * T::RAW) / 16, base16 + S::O_TWIN / 16);
                     umma_commit(o_empty(at));
                     umma_commit(dp_full);
                     return true;
@@ -593,10 +598,10 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
                 ok = scores(0) && dprobs(0);
                 for (int i = 0; i < n && ok; ++i) {
                     const uint32_t at = n0 + i;
-                    ok = mbar_wait(on_full, one(at), p.status, 54) && landed(p_ready, one(at));
+                    ok = mbar_wait(on_full(at), two(at), p.status, 54) && landed(p_ready, one(at));
                     if (!ok) break;
-                    win_values<DP, 8>(tmem + 256, tmem, tmem + 128, tmem + 160, base16 + S::O_MN / 16, base16 + S::O_TWIN / 16, i % WT_FLUSH != 0);
-                    umma_commit(on_empty);
+                    win_values<DP, 8>(tmem + 256, tmem, tmem + 128, tmem + 160, base16 + (S::O_MN + (at & 1u) * T::RAW) / 16, base16 + S::O_TWIN / 16, i % WT_FLUSH != 0);
+                    umma_commit(on_empty(at));
                     umma_commit(o_free);
                     ok = scores(i + 1) && mbar_wait(qn_full, one(at), p.status, 55) && landed(ds_ready, one(at));
                     if (!ok) break;
@@ -637,10 +642,10 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
                 ok = warp_wait(q_full(at), two(at), p.status, 56) && warp_wait(q_free(at), two(at) ^ 1u, p.status, 56);
                 if (!ok) break;
                 if (t < AT_KEYS) {
-                    float* slot = reinterpret_cast<float*>(gen + S::STATS) + (at & 1u) * 3 * AT_KEYS + t;
+                    float* slot = reinterpret_cast<float*>(gen + S::STATS + (at & 1u) * S::STATS_BLOCK) + t;
                     slot[0] = BIAS ? nm : nm * kLog2e - log2f(ni);
-                    slot[AT_KEYS] = ni;
-                    slot[2 * AT_KEYS] = nd;
+                    slot[AT_KEYS] = nd;
+                    if (BIAS) slot[2 * AT_KEYS] = ni;
                 }
                 if (BIAS && t < WT_TAB) reinterpret_cast<float*>(gen + S::TABS)[(at & 1u) * WT_TAB + t] = nb;
                 if (i + 1 < n) request(i + 1);
@@ -648,9 +653,9 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(q_conv(at));
-                ok = warp_wait(o_full(at), two(at), p.status, 56) && warp_wait(o_free, one(at) ^ 1u, p.status, 56);
+                ok = warp_wait(o_full(at), o_parity(at), p.status, 56) && warp_wait(o_free, one(at) ^ 1u, p.status, 56);
                 if (!ok) break;
-                win_split<DP, 256, false>(gen + S::O_RAW + place, gen + S::O_TWIN, t);
+                win_split<DP, 256, false>(gen + S::O_RAW + o_place(at) * T::RAW, gen + S::O_TWIN, t);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(o_conv);
@@ -697,8 +702,8 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
             };
 #pragma unroll 1
             for (int i = 0; i < cnt; ++i, ++n) {
-                const float4* mp = reinterpret_cast<const float4*>(gen + S::STATS + (n & 1u) * 3 * AT_KEYS * 4) + 4 * part;
-                const float4 *ip = mp + AT_KEYS / 4, *dp = ip + AT_KEYS / 4;
+                const float4* mp = reinterpret_cast<const float4*>(gen + S::STATS + (n & 1u) * S::STATS_BLOCK) + 4 * part;
+                const float4 *dp = mp + AT_KEYS / 4, *ip = dp + AT_KEYS / 4;
                 good = good && warp_wait(s_full, n & 1u, p.status, 57);
                 after_sync();
                 if (part >= 2 && i > 0 && i % WT_FLUSH == 0) move(i > WT_FLUSH);  // dV of the blocks before came before these scores
@@ -774,20 +779,22 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
 // Tensor memory: S / companions of dS [128 x, + 64) (of 16 keys: 8 columns bf16(dS), 8 bf16(dS - t)), dP / t of dS [128 x + 64, + 64), dQ [256, 320), t of q [320, 384), t of dO [384, 448).
 // Bias gradient: a warp adds up the dS of its 32 x 16 block along the diagonals, 47 of them, in sixteen shuffles, and lane n those
 // that belong to buckets n and n + 32; a block that lies in one bucket as a whole is added up row by row in registers instead.
-template <int DP>
+template <int DP, bool BIAS>
 struct DqSmem {
     using T = WinTile<DP>;
     static constexpr int OWN = AT_ROWS * DP * 4;
-    static constexpr int K_RAW = 2 * OWN, V_RAW = K_RAW + 2 * T::RAW, K_MN = V_RAW + 2 * T::RAW, K_TWIN = K_MN + T::RAW, V_TWIN = K_TWIN + 3 * T::TWIN;
-    static constexpr int TABS = V_TWIN + T::TWIN, DIAG = TABS + 3 * WT_TAB * 4;  // bias of a block's distances, three blocks; [warp][64]: sums by diagonal, at an item's end by bucket
-    static constexpr int XCH = DIAG + 16 * 64 * 4, BAR = XCH + AT_ROWS * 4, TOTAL = BAR + 256 + 1024;
+    static constexpr uint32_t TWINS = BIAS ? 2 : 3;  // with a bias its table and sums take the place of the third one
+    static constexpr int K_RAW = 2 * OWN, V_RAW = K_RAW + 2 * T::RAW, K_MN = V_RAW + 2 * T::RAW, K_TWIN = K_MN + 2 * T::RAW, V_TWIN = K_TWIN + TWINS * T::TWIN;
+    static constexpr int XCH = V_TWIN + T::TWIN, TABS = XCH + AT_ROWS * 4;                                 // dO . O of every row; bias of a block's distances, two blocks
+    static constexpr int DIAG = TABS + (BIAS ? 2 * WT_TAB * 4 : 0), BAR = DIAG + (BIAS ? 16 * 64 * 4 : 0);  // [warp][64]: sums by diagonal, at an item's end by bucket
+    static constexpr int TOTAL = BAR + 256 + 1024;
     static_assert(TOTAL <= 232448 && AW_MAX_BUCKETS == 64, "shared memory");
 };
 template <int DP, bool BIAS>
 __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kernel(const __grid_constant__ CUtensorMap map_kk, const __grid_constant__ CUtensorMap map_vk, const __grid_constant__ CUtensorMap map_kn, const __grid_constant__ CUtensorMap map_q,
                                                                                const __grid_constant__ CUtensorMap map_do, const __grid_constant__ CUtensorMap map_dq,
                                                                                const __grid_constant__ WindowTc p) {
-    using S = DqSmem<DP>;
+    using S = DqSmem<DP, BIAS>;
     using T = WinTile<DP>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -798,21 +805,24 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
     auto one = [](uint32_t n) { return n & 1u; };
     auto k_full = [&](uint32_t n) { return bar(0 + (n & 1u)); };
     auto k_empty = [&](uint32_t n) { return bar(2 + (n & 1u)); };
-    auto three = [](uint32_t n) { return (n / 3u) & 1u; };
-    auto k_conv = [&](uint32_t n) { return bar(4 + n % 3u); };
-    auto k_free = [&](uint32_t n) { return bar(7 + n % 3u); };  // companions: dQ has read them
+    auto twin = [](uint32_t n) { return n % S::TWINS; };
+    auto turn = [](uint32_t n) { return (n / S::TWINS) & 1u; };
+    auto k_conv = [&](uint32_t n) { return bar(4 + twin(n)); };
+    auto k_free = [&](uint32_t n) { return bar(7 + twin(n)); };  // companions: dQ has read them
     auto v_full = [&](uint32_t n) { return bar(10 + (n & 1u)); };
     auto v_empty = [&](uint32_t n) { return bar(12 + (n & 1u)); };
     auto s_full = [&](uint32_t n) { return bar(14 + (n & 1u)); };
     auto dp_full = [&](uint32_t n) { return bar(16 + (n & 1u)); };
     auto ds_ready = [&](uint32_t n) { return bar(18 + (n & 1u)); };
-    const uint32_t kn_full = bar(20), kn_empty = bar(21), acc_full = bar(22), q_ready = bar(23), v_conv = bar(24), v_free = bar(25), own_full = bar(26);
+    auto kn_full = [&](uint32_t n) { return bar(20 + (n & 1u)); };
+    auto kn_empty = [&](uint32_t n) { return bar(22 + (n & 1u)); };
+    const uint32_t v_conv = bar(24), v_free = bar(25), own_full = bar(26), q_ready = bar(27), acc_full = bar(28);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 27; ++i) mbar_init(bar(i), (i >= 4 && i < 7) || i == 24 ? 8 : i == 18 || i == 19 || i == 23 ? 16 : i == 26 ? 2 : 1);  // own_full: two tiles
+        for (int i = 0; i < 29; ++i) mbar_init(bar(i), (i >= 4 && i < 7) || i == 24 ? 8 : i == 18 || i == 19 || i == 27 ? 16 : i == 26 ? 2 : 1);  // own_full: two tiles
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    const uint32_t tmem = tmem_take(bars + 8u * 28, reinterpret_cast<volatile uint32_t*>(gen + S::BAR + 8 * 28), warp);
+    const uint32_t tmem = tmem_take(bars + 8u * 30, reinterpret_cast<volatile uint32_t*>(gen + S::BAR + 8 * 30), warp);
     pdl_trigger();
     pdl_wait();
 
@@ -834,7 +844,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
                 for (int i = 0; i < n && ok; ++i) {
                     const uint32_t at = n0 + i, place = (at & 1u) * T::RAW;
                     if (warp == 0) ok = load(k_empty(at), two(at), S::K_RAW + place, &map_kk, k_full(at), i) && load(v_empty(at), two(at), S::V_RAW + place, &map_vk, v_full(at), i);
-                    else ok = load(kn_empty, one(at), S::K_MN, &map_kn, kn_full, i);
+                    else ok = load(kn_empty(at), two(at), S::K_MN + place, &map_kn, kn_full(at), i);
                 }
                 n0 += n;
             }
@@ -856,8 +866,8 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
                 auto products = [&](int i) {  // S and dP of block i
                     const uint32_t at = n0 + i, place = tmem + 128 * (at & 1u), raw = (at & 1u) * (T::RAW / 16);
                     if (i >= n) return true;
-                    if (!landed(k_conv(at), three(at))) return false;
-                    win_scores<DP>(place, tmem + 320, base16, base16 + S::K_RAW / 16 + raw, base16 + (S::K_TWIN + at % 3u * T::TWIN) / 16);
+                    if (!landed(k_conv(at), turn(at))) return false;
+                    win_scores<DP>(place, tmem + 320, base16, base16 + S::K_RAW / 16 + raw, base16 + (S::K_TWIN + twin(at) * T::TWIN) / 16);
                     umma_commit(k_empty(at));
                     umma_commit(s_full(at));
                     if (!landed(v_conv, one(at))) return false;
@@ -872,10 +882,10 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
                 ok = products(0);
                 for (int i = 0; i < n && ok; ++i) {
                     const uint32_t at = n0 + i, place = tmem + 128 * (at & 1u);
-                    ok = products(i + 1) && mbar_wait(kn_full, one(at), p.status, 64) && landed(ds_ready(at), two(at));
+                    ok = products(i + 1) && mbar_wait(kn_full(at), two(at), p.status, 64) && landed(ds_ready(at), two(at));
                     if (!ok) break;
-                    win_values<DP, 16>(tmem + 256, place + 64, place, place + 8, base16 + S::K_MN / 16, base16 + (S::K_TWIN + at % 3u * T::TWIN) / 16, i % WT_FLUSH != 0);
-                    umma_commit(kn_empty);
+                    win_values<DP, 16>(tmem + 256, place + 64, place, place + 8, base16 + (S::K_MN + (at & 1u) * T::RAW) / 16, base16 + (S::K_TWIN + twin(at) * T::TWIN) / 16, i % WT_FLUSH != 0);
+                    umma_commit(kn_empty(at));
                     umma_commit(k_free(at));
                     if (i + 1 == n || (i + 1) % WT_FLUSH == 0) umma_commit(acc_full);
                 }
@@ -899,14 +909,14 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
             if (BIAS) request(0);
             for (int i = 0; i < n && ok; ++i) {
                 const uint32_t at = n0 + i, place = (at & 1u) * T::RAW;
-                // dQ of three blocks before has read the companions that these replace; its bias was used before that
-                ok = warp_wait(k_full(at), two(at), p.status, 65) && warp_wait(k_free(at), three(at) ^ 1u, p.status, 65);
+                // dQ has read the companions that these replace; that block's bias was used before
+                ok = warp_wait(k_full(at), two(at), p.status, 65) && warp_wait(k_free(at), turn(at) ^ 1u, p.status, 65);
                 if (!ok) break;
                 if (BIAS) {
-                    if (t < WT_TAB) reinterpret_cast<float*>(gen + S::TABS)[at % 3u * WT_TAB + t] = nb;
+                    if (t < WT_TAB) reinterpret_cast<float*>(gen + S::TABS)[(at & 1u) * WT_TAB + t] = nb;
                     if (i + 1 < n) request(i + 1);
                 }
-                win_split<DP, 256, false>(gen + S::K_RAW + place, gen + S::K_TWIN + at % 3u * T::TWIN, t);
+                win_split<DP, 256, false>(gen + S::K_RAW + place, gen + S::K_TWIN + twin(at) * T::TWIN, t);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(k_conv(at));
@@ -1006,7 +1016,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
 #pragma unroll
                         for (int e = 0; e < 16; ++e) pr[e] = ex2((fmaf(__uint_as_float(u[e]), p.scale, beyond) - m) * kLog2e) * inv;
                     } else {
-                        const float* mine = reinterpret_cast<const float*>(gen + S::TABS) + n % 3u * WT_TAB + row - 16 * part + AT_KEYS - 1;
+                        const float* mine = reinterpret_cast<const float*>(gen + S::TABS) + (n & 1u) * WT_TAB + row - 16 * part + AT_KEYS - 1;
 #pragma unroll
                         for (int e = 0; e < 16; ++e) pr[e] = ex2((fmaf(__uint_as_float(u[e]), p.scale, mine[-e]) - m) * kLog2e) * inv;
                     }
@@ -1129,9 +1139,9 @@ struct BwdMaps {
 template <int DP, bool BIAS>
 static int run_bwd(gcb_ctx* ctx, const WindowTc& p, const BwdMaps& m) {
     static bool done_q[kMaxDevices] = {}, done_kv[kMaxDevices] = {};
-    int rc = tc_launch(ctx, window_attention_tc_dq_kernel<DP, BIAS>, done_q, AT_BWD_THREADS, DqSmem<DP>::TOTAL, p, m.kk, m.vk, m.kn, m.qk, m.ok, m.dq);
+    int rc = tc_launch(ctx, window_attention_tc_dq_kernel<DP, BIAS>, done_q, AT_BWD_THREADS, DqSmem<DP, BIAS>::TOTAL, p, m.kk, m.vk, m.kn, m.qk, m.ok, m.dq);
     if (!rc) rc = after_launch(ctx, "window_attention_tc_dq");
-    if (!rc) rc = tc_launch(ctx, window_attention_tc_dkv_kernel<DP, BIAS>, done_kv, AT_BWD_THREADS, DkvSmem<DP>::TOTAL, p, m.qk, m.qn, m.ok, m.on, m.kk, m.vk, m.dk, m.dv);
+    if (!rc) rc = tc_launch(ctx, window_attention_tc_dkv_kernel<DP, BIAS>, done_kv, AT_BWD_THREADS, DkvSmem<DP, BIAS>::TOTAL, p, m.qk, m.qn, m.ok, m.on, m.kk, m.vk, m.dk, m.dv);
     return rc ? rc : after_launch(ctx, "window_attention_tc_dkv");
 }
 // Room for the sums that leave tensor memory before an item's end.
