@@ -514,21 +514,20 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
     // n: running number of a block; parities of what has two places and of what has one
     auto two = [](uint32_t n) { return (n >> 1) & 1u; };
     auto one = [](uint32_t n) { return n & 1u; };
-    auto q_full = [&](uint32_t n) { return bar(0 + (n & 1u)); };
-    auto q_empty = [&](uint32_t n) { return bar(2 + (n & 1u)); };
-    auto q_conv = [&](uint32_t n) { return bar(4 + (n & 1u)); };
-    auto q_free = [&](uint32_t n) { return bar(6 + (n & 1u)); };  // companions: dK has read them
     auto o_place = [](uint32_t n) { return S::O_RAWS == 2 ? n & 1u : 0u; };
-    auto o_parity = [](uint32_t n) { return S::O_RAWS == 2 ? (n >> 1) & 1u : n & 1u; };
-    auto o_full = [&](uint32_t n) { return bar(8 + o_place(n)); };
-    auto o_empty = [&](uint32_t n) { return bar(10 + o_place(n)); };
-    auto on_full = [&](uint32_t n) { return bar(14 + (n & 1u)); };
-    auto on_empty = [&](uint32_t n) { return bar(25 + (n & 1u)); };
-    const uint32_t o_conv = bar(12), o_free = bar(13), qn_full = bar(16), qn_empty = bar(17);
-    const uint32_t s_full = bar(18), dp_full = bar(19), p_ready = bar(20), ds_ready = bar(21), acc_full = bar(22), kv_ready = bar(23), own_full = bar(24);
+    auto q_full = [&](uint32_t n) { return bar(0 + (n & 1u)); };
+    auto o_full = [&](uint32_t n) { return bar(2 + o_place(n)); };
+    auto on_full = [&](uint32_t n) { return bar(4 + (n & 1u)); };
+    auto q_conv = [&](uint32_t n) { return bar(6 + (n & 1u)); };
+    // One barrier a product, in two turns: it tells the threads that the result is there, and the producers and the companion warps that what it read may go.
+    auto s_done = [&](uint32_t n) { return bar(8 + (n & 1u)); };
+    auto dp_done = [&](uint32_t n) { return bar(10 + (n & 1u)); };
+    auto dv_done = [&](uint32_t n) { return bar(12 + (n & 1u)); };
+    auto dk_done = [&](uint32_t n) { return bar(14 + (n & 1u)); };
+    const uint32_t qn_full = bar(16), o_conv = bar(17), p_ready = bar(18), ds_ready = bar(19), kv_ready = bar(20), own_full = bar(21);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 27; ++i) mbar_init(bar(i), i == 4 || i == 5 || i == 12 ? 8 : i == 20 || i == 21 || i == 23 ? 16 : i == 24 ? 2 : 1);  // own_full: two tiles
+        for (int i = 0; i < 22; ++i) mbar_init(bar(i), i == 6 || i == 7 || i == 17 ? 8 : i >= 18 && i <= 20 ? 16 : i == 21 ? 2 : 1);  // own_full: two tiles
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     const uint32_t tmem = tmem_take(bars + 8u * 28, reinterpret_cast<volatile uint32_t*>(gen + S::BAR + 8 * 28), warp);
@@ -548,15 +547,17 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
                 const AttnItem it = attn_item(p, w, true);
                 if (it.skip) continue;
                 const int n = steps(it);
-                auto load = [&](uint32_t free, uint32_t parity, int dst, const CUtensorMap* map, uint32_t landed, int i) {
-                    if (!mbar_wait(free, parity ^ 1u, p.status, 51)) return false;
+                // `back` blocks ago the place was last filled, and `done` is the product that read it
+                auto load = [&](auto done, uint32_t back, int dst, const CUtensorMap* map, uint32_t landed, int i) {
+                    const uint32_t at = n0 + i;
+                    if (at >= back && !mbar_wait(done(at - back), two(at - back), p.status, 51)) return false;
                     win_load<DP>(base + dst, map, landed, it.unit * AT_ROWS + i * AT_KEYS, it.h, it.b);
                     return true;
                 };
                 for (int i = 0; i < n && ok; ++i) {
                     const uint32_t at = n0 + i, place = (at & 1u) * T::RAW;
-                    if (warp == 0) ok = load(q_empty(at), two(at), S::Q_RAW + place, &map_qk, q_full(at), i) && load(o_empty(at), o_parity(at), S::O_RAW + o_place(at) * T::RAW, &map_ok, o_full(at), i);
-                    else ok = load(on_empty(at), two(at), S::O_MN + place, &map_on, on_full(at), i) && load(qn_empty, one(at), S::Q_MN, &map_qn, qn_full, i);
+                    if (warp == 0) ok = load(s_done, 2, S::Q_RAW + place, &map_qk, q_full(at), i) && load(dp_done, S::O_RAWS, S::O_RAW + o_place(at) * T::RAW, &map_ok, o_full(at), i);
+                    else ok = load(dv_done, 2, S::O_MN + place, &map_on, on_full(at), i) && load(dk_done, 1, S::Q_MN, &map_qn, qn_full, i);
                 }
                 n0 += n;
             }
@@ -575,43 +576,33 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
                     after_sync();
                     return r;
                 };
-                auto scores = [&](int i) {
-                    const uint32_t at = n0 + i;
-                    if (i >= n) return true;
+                auto scores = [&](uint32_t at) {
                     if (!landed(q_conv(at), two(at))) return false;
                     win_scores<DP>(tmem, tmem + 384, base16, base16 + (S::Q_RAW + (at & 1u) * T::RAW) / 16, base16 + (S::Q_TWIN + (at & 1u) * T::TWIN) / 16);
-                    umma_commit(q_empty(at));
-                    umma_commit(s_full);
+                    umma_commit(s_done(at));
                     return true;
                 };
-                auto dprobs = [&](int i) {
-                    const uint32_t at = n0 + i;
-                    if (i >= n) return true;
+                auto dprobs = [&](uint32_t at) {
                     if (!landed(o_conv, one(at))) return false;
                     win_scores<DP>(tmem + 64, tmem + 448, base16 + S::OWN / 16, base16 + (S::O_RAW + o_place(at) * T::RAW) / 16, base16 + S::O_TWIN / 16);
-                    umma_commit(o_empty(at));
-                    umma_commit(dp_full);
+                    umma_commit(dp_done(at));
                     return true;
                 };
-                ok = mbar_wait(kv_ready, items & 1u, p.status, 53);
-                if (!ok) break;
-                ok = scores(0) && dprobs(0);
+                ok = mbar_wait(kv_ready, items & 1u, p.status, 53) && scores(n0) && dprobs(n0);
                 for (int i = 0; i < n && ok; ++i) {
                     const uint32_t at = n0 + i;
+                    const bool more = i + 1 < n;
                     ok = mbar_wait(on_full(at), two(at), p.status, 54) && landed(p_ready, one(at));
                     if (!ok) break;
                     win_values<DP, 8>(tmem + 256, tmem, tmem + 128, tmem + 160, base16 + (S::O_MN + (at & 1u) * T::RAW) / 16, base16 + S::O_TWIN / 16, i % WT_FLUSH != 0);
-                    umma_commit(on_empty(at));
-                    umma_commit(o_free);
-                    ok = scores(i + 1) && mbar_wait(qn_full, one(at), p.status, 55) && landed(ds_ready, one(at));
+                    umma_commit(dv_done(at));
+                    ok = (!more || scores(at + 1)) && mbar_wait(qn_full, one(at), p.status, 55) && landed(ds_ready, one(at));
                     if (!ok) break;
                     win_values<DP, 8>(tmem + 320, tmem + 64, tmem + 192, tmem + 224, base16 + S::Q_MN / 16, base16 + (S::Q_TWIN + (at & 1u) * T::TWIN) / 16, i % WT_FLUSH != 0);
-                    umma_commit(qn_empty);
-                    umma_commit(q_free(at));
-                    ok = dprobs(i + 1);
+                    umma_commit(dk_done(at));
+                    ok = !more || dprobs(at + 1);
                 }
                 if (!ok) break;
-                umma_commit(acc_full);
                 n0 += n;
             }
         }
@@ -639,7 +630,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
             for (int i = 0; i < n && ok; ++i) {
                 const uint32_t at = n0 + i, place = (at & 1u) * T::RAW;
                 // dK of the block before last has read the companions that these replace; its statistics were used before that
-                ok = warp_wait(q_full(at), two(at), p.status, 56) && warp_wait(q_free(at), two(at) ^ 1u, p.status, 56);
+                ok = warp_wait(q_full(at), two(at), p.status, 56) && (at < 2u || warp_wait(dk_done(at - 2u), two(at - 2u), p.status, 56));
                 if (!ok) break;
                 if (t < AT_KEYS) {
                     float* slot = reinterpret_cast<float*>(gen + S::STATS + (at & 1u) * S::STATS_BLOCK) + t;
@@ -653,7 +644,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(q_conv(at));
-                ok = warp_wait(o_full(at), o_parity(at), p.status, 56) && warp_wait(o_free, one(at) ^ 1u, p.status, 56);
+                ok = warp_wait(o_full(at), S::O_RAWS == 2 ? two(at) : one(at), p.status, 56) && (at < 1u || warp_wait(dv_done(at - 1u), two(at - 1u), p.status, 56));
                 if (!ok) break;
                 win_split<DP, 256, false>(gen + S::O_RAW + o_place(at) * T::RAW, gen + S::O_TWIN, t);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -704,7 +695,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
             for (int i = 0; i < cnt; ++i, ++n) {
                 const float4* mp = reinterpret_cast<const float4*>(gen + S::STATS + (n & 1u) * S::STATS_BLOCK) + 4 * part;
                 const float4 *dp = mp + AT_KEYS / 4, *ip = dp + AT_KEYS / 4;
-                good = good && warp_wait(s_full, n & 1u, p.status, 57);
+                good = good && warp_wait(s_done(n), two(n), p.status, 57);
                 after_sync();
                 if (part >= 2 && i > 0 && i % WT_FLUSH == 0) move(i > WT_FLUSH);  // dV of the blocks before came before these scores
                 uint32_t u[16];
@@ -735,7 +726,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
                 tmem_stores_done();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_ready);
-                good = good && warp_wait(dp_full, n & 1u, p.status, 58);
+                good = good && warp_wait(dp_done(n), two(n), p.status, 58);
                 after_sync();
                 tmem_ld16(lanes + 64 + 16 * part, u);
 #pragma unroll
@@ -751,7 +742,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
                 __syncwarp();
                 if (lane == 0) mbar_arrive(ds_ready);
             }
-            good = good && warp_wait(acc_full, items & 1u, p.status, 59);
+            good = good && warp_wait(dk_done(n - 1u), two(n - 1u), p.status, 59);  // the last product of all
             after_sync();
             const float f = part < 2 ? p.scale : 1.0f;
 #pragma unroll
@@ -804,22 +795,20 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
     auto two = [](uint32_t n) { return (n >> 1) & 1u; };
     auto one = [](uint32_t n) { return n & 1u; };
     auto k_full = [&](uint32_t n) { return bar(0 + (n & 1u)); };
-    auto k_empty = [&](uint32_t n) { return bar(2 + (n & 1u)); };
+    auto v_full = [&](uint32_t n) { return bar(2 + (n & 1u)); };
+    auto kn_full = [&](uint32_t n) { return bar(4 + (n & 1u)); };
     auto twin = [](uint32_t n) { return n % S::TWINS; };
-    auto turn = [](uint32_t n) { return (n / S::TWINS) & 1u; };
-    auto k_conv = [&](uint32_t n) { return bar(4 + twin(n)); };
-    auto k_free = [&](uint32_t n) { return bar(7 + twin(n)); };  // companions: dQ has read them
-    auto v_full = [&](uint32_t n) { return bar(10 + (n & 1u)); };
-    auto v_empty = [&](uint32_t n) { return bar(12 + (n & 1u)); };
-    auto s_full = [&](uint32_t n) { return bar(14 + (n & 1u)); };
-    auto dp_full = [&](uint32_t n) { return bar(16 + (n & 1u)); };
-    auto ds_ready = [&](uint32_t n) { return bar(18 + (n & 1u)); };
-    auto kn_full = [&](uint32_t n) { return bar(20 + (n & 1u)); };
-    auto kn_empty = [&](uint32_t n) { return bar(22 + (n & 1u)); };
-    const uint32_t v_conv = bar(24), v_free = bar(25), own_full = bar(26), q_ready = bar(27), acc_full = bar(28);
+    auto k_conv = [&](uint32_t n) { return bar(6 + twin(n)); };
+    auto k_conv_turn = [](uint32_t n) { return (n / S::TWINS) & 1u; };
+    // one barrier a product, in two turns, as above
+    auto s_done = [&](uint32_t n) { return bar(9 + (n & 1u)); };
+    auto dp_done = [&](uint32_t n) { return bar(11 + (n & 1u)); };
+    auto dq_done = [&](uint32_t n) { return bar(13 + (n & 1u)); };
+    auto ds_ready = [&](uint32_t n) { return bar(15 + (n & 1u)); };
+    const uint32_t v_conv = bar(17), q_ready = bar(18), own_full = bar(19);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 29; ++i) mbar_init(bar(i), (i >= 4 && i < 7) || i == 24 ? 8 : i == 18 || i == 19 || i == 27 ? 16 : i == 26 ? 2 : 1);  // own_full: two tiles
+        for (int i = 0; i < 20; ++i) mbar_init(bar(i), (i >= 6 && i <= 8) || i == 17 ? 8 : i == 15 || i == 16 || i == 18 ? 16 : i == 19 ? 2 : 1);  // own_full: two tiles
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     const uint32_t tmem = tmem_take(bars + 8u * 30, reinterpret_cast<volatile uint32_t*>(gen + S::BAR + 8 * 30), warp);
@@ -836,15 +825,17 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
                 if (it.skip) continue;
                 const TileKeys keys(p, it.unit * AT_ROWS);
                 const int n = keys.count();
-                auto load = [&](uint32_t free, uint32_t parity, int dst, const CUtensorMap* map, uint32_t landed, int i) {
-                    if (!mbar_wait(free, parity ^ 1u, p.status, 61)) return false;
+                // the place was last filled two blocks ago, and `done` is the product that read it
+                auto load = [&](auto done, int dst, const CUtensorMap* map, uint32_t landed, int i) {
+                    const uint32_t at = n0 + i;
+                    if (at >= 2u && !mbar_wait(done(at - 2u), two(at - 2u), p.status, 61)) return false;
                     win_load<DP>(base + dst, map, landed, keys.block(i) * AT_KEYS, it.h, it.b);
                     return true;
                 };
                 for (int i = 0; i < n && ok; ++i) {
                     const uint32_t at = n0 + i, place = (at & 1u) * T::RAW;
-                    if (warp == 0) ok = load(k_empty(at), two(at), S::K_RAW + place, &map_kk, k_full(at), i) && load(v_empty(at), two(at), S::V_RAW + place, &map_vk, v_full(at), i);
-                    else ok = load(kn_empty(at), two(at), S::K_MN + place, &map_kn, kn_full(at), i);
+                    if (warp == 0) ok = load(s_done, S::K_RAW + place, &map_kk, k_full(at), i) && load(dp_done, S::V_RAW + place, &map_vk, v_full(at), i);
+                    else ok = load(dq_done, S::K_MN + place, &map_kn, kn_full(at), i);
                 }
                 n0 += n;
             }
@@ -858,36 +849,26 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
                 const AttnItem it = attn_item(p, w, false);
                 if (it.skip) break;  // only the last round has items left out
                 const int n = TileKeys(p, it.unit * AT_ROWS).count();
-                auto landed = [&](uint32_t b, uint32_t parity) {
-                    const bool r = mbar_wait(b, parity, p.status, 62);
+                auto products = [&](uint32_t at) {  // S and dP
+                    const uint32_t place = tmem + 128 * (at & 1u), raw = (at & 1u) * (T::RAW / 16);
+                    if (!mbar_wait(k_conv(at), k_conv_turn(at), p.status, 62) || !mbar_wait(v_conv, one(at), p.status, 62)) return false;
                     after_sync();
-                    return r;
-                };
-                auto products = [&](int i) {  // S and dP of block i
-                    const uint32_t at = n0 + i, place = tmem + 128 * (at & 1u), raw = (at & 1u) * (T::RAW / 16);
-                    if (i >= n) return true;
-                    if (!landed(k_conv(at), turn(at))) return false;
                     win_scores<DP>(place, tmem + 320, base16, base16 + S::K_RAW / 16 + raw, base16 + (S::K_TWIN + twin(at) * T::TWIN) / 16);
-                    umma_commit(k_empty(at));
-                    umma_commit(s_full(at));
-                    if (!landed(v_conv, one(at))) return false;
+                    umma_commit(s_done(at));
                     win_scores<DP>(place + 64, tmem + 384, base16 + S::OWN / 16, base16 + S::V_RAW / 16 + raw, base16 + S::V_TWIN / 16);
-                    umma_commit(v_empty(at));
-                    umma_commit(v_free);
-                    umma_commit(dp_full(at));
+                    umma_commit(dp_done(at));
                     return true;
                 };
                 ok = mbar_wait(q_ready, items & 1u, p.status, 63);
                 if (!ok) break;
-                ok = products(0);
+                ok = products(n0);
                 for (int i = 0; i < n && ok; ++i) {
                     const uint32_t at = n0 + i, place = tmem + 128 * (at & 1u);
-                    ok = products(i + 1) && mbar_wait(kn_full(at), two(at), p.status, 64) && landed(ds_ready(at), two(at));
+                    ok = (i + 1 == n || products(at + 1)) && mbar_wait(kn_full(at), two(at), p.status, 64) && mbar_wait(ds_ready(at), two(at), p.status, 64);
                     if (!ok) break;
+                    after_sync();
                     win_values<DP, 16>(tmem + 256, place + 64, place, place + 8, base16 + (S::K_MN + (at & 1u) * T::RAW) / 16, base16 + (S::K_TWIN + twin(at) * T::TWIN) / 16, i % WT_FLUSH != 0);
-                    umma_commit(kn_empty(at));
-                    umma_commit(k_free(at));
-                    if (i + 1 == n || (i + 1) % WT_FLUSH == 0) umma_commit(acc_full);
+                    umma_commit(dq_done(at));
                 }
                 if (!ok) break;
                 n0 += n;
@@ -910,7 +891,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
             for (int i = 0; i < n && ok; ++i) {
                 const uint32_t at = n0 + i, place = (at & 1u) * T::RAW;
                 // dQ has read the companions that these replace; that block's bias was used before
-                ok = warp_wait(k_full(at), two(at), p.status, 65) && warp_wait(k_free(at), turn(at) ^ 1u, p.status, 65);
+                ok = warp_wait(k_full(at), two(at), p.status, 65) && (at < S::TWINS || warp_wait(dq_done(at - S::TWINS), two(at - S::TWINS), p.status, 65));
                 if (!ok) break;
                 if (BIAS) {
                     if (t < WT_TAB) reinterpret_cast<float*>(gen + S::TABS)[(at & 1u) * WT_TAB + t] = nb;
@@ -920,7 +901,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(k_conv(at));
-                ok = warp_wait(v_full(at), two(at), p.status, 65) && warp_wait(v_free, one(at) ^ 1u, p.status, 65);
+                ok = warp_wait(v_full(at), two(at), p.status, 65) && (at < 1u || warp_wait(dp_done(at - 1u), two(at - 1u), p.status, 65));
                 if (!ok) break;
                 win_split<DP, 256, false>(gen + S::V_RAW + place, gen + S::V_TWIN, t);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -940,7 +921,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
         float* xch = reinterpret_cast<float*>(gen + S::XCH);  // dO . O of every row
         const float c = p.scale * kLog2e;
         const bool wants_dbias = BIAS && p.dbias_part != nullptr;
-        uint32_t n = 0, sums_out = 0, items = 0;
+        uint32_t n = 0, items = 0;
         bool good = true;
         uint8_t* own = gen + (part >> 1) * S::OWN;
         auto fetch = [&](int64_t w) {  // the rows of the item at w
@@ -1006,7 +987,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
             for (int i = 0; i < cnt; ++i, ++n) {
                 const uint32_t place = lanes + 128 * (n & 1u);
                 const int b = keys.block(i), j0 = b * AT_KEYS + 16 * part, room = r - j0;
-                good = good && warp_wait(s_full(n), (n >> 1) & 1u, p.status, 66);
+                good = good && warp_wait(s_done(n), two(n), p.status, 66);
                 after_sync();
                 uint32_t u[16];
                 float pr[16];
@@ -1029,15 +1010,14 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
 #pragma unroll
                     for (int e = 0; e < 16; ++e) pr[e] = keeps(e, room, from, to) ? pr[e] : 0.0f;
                 }
-                good = good && warp_wait(dp_full(n), (n >> 1) & 1u, p.status, 67);
+                good = good && warp_wait(dp_done(n), two(n), p.status, 67);
                 after_sync();
                 tmem_ld16(place + 64 + 16 * part, u);
 #pragma unroll
                 for (int e = 0; e < 16; ++e) pr[e] *= __uint_as_float(u[e]) - delta;  // a masked P is zero whatever dP holds
                 place_parts16(pr, place + 64 + 16 * part, place + 16 * part, place + 16 * part + 8);
                 if (i > 0 && i % WT_FLUSH == 0) {
-                    good = good && warp_wait(acc_full, sums_out & 1u, p.status, 68);
-                    ++sums_out;
+                    good = good && warp_wait(dq_done(n - 1u), two(n - 1u), p.status, 68);
                     after_sync();
                     if (16 * part < DP) move_sum(lanes + 256 + 16 * part, moved, i > WT_FLUSH, 1.0f);
                 }
@@ -1078,8 +1058,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
                     }
                 }
             }
-            good = good && warp_wait(acc_full, sums_out & 1u, p.status, 68);
-            ++sums_out;
+            good = good && warp_wait(dq_done(n - 1u), two(n - 1u), p.status, 68);  // the last product of all
             after_sync();
             if (wants_dbias) {
                 settle();
