@@ -768,16 +768,15 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
 // Roles as above.
 // Scores and dP alternate between two places, x = 0 and 1; dS takes the place of both, a thread's columns where it has read them.
 // Tensor memory: S / companions of dS [128 x, + 64) (of 16 keys: 8 columns bf16(dS), 8 bf16(dS - t)), dP / t of dS [128 x + 64, + 64), dQ [256, 320), t of q [320, 384), t of dO [384, 448).
-// Bias gradient: a warp adds up the dS of its 32 x 16 block along the diagonals, 47 of them, in sixteen shuffles, and lane n those
-// that belong to buckets n and n + 32; a block that lies in one bucket as a whole is added up row by row in registers instead.
+// Bias gradient: a warp adds up the dS of its 32 x 16 block along the diagonals, 47 of them, in sixteen shuffles; lane n keeps buckets n and n + 32, as
+// differences of running sums over the diagonals.  A block that lies in one bucket as a whole is added up row by row in registers instead.
 template <int DP, bool BIAS>
 struct DqSmem {
     using T = WinTile<DP>;
     static constexpr int OWN = AT_ROWS * DP * 4;
-    static constexpr uint32_t TWINS = BIAS ? 2 : 3;  // with a bias its table and sums take the place of the third one
+    static constexpr uint32_t TWINS = BIAS ? 2 : 3;  // with a bias its table takes the place of the third one
     static constexpr int K_RAW = 2 * OWN, V_RAW = K_RAW + 2 * T::RAW, K_MN = V_RAW + 2 * T::RAW, K_TWIN = K_MN + 2 * T::RAW, V_TWIN = K_TWIN + TWINS * T::TWIN;
-    static constexpr int XCH = V_TWIN + T::TWIN, TABS = XCH + AT_ROWS * 4;                                 // dO . O of every row; bias of a block's distances, two blocks
-    static constexpr int DIAG = TABS + (BIAS ? 2 * WT_TAB * 4 : 0), BAR = DIAG + (BIAS ? 16 * 64 * 4 : 0);  // [warp][64]: sums by diagonal, at an item's end by bucket
+    static constexpr int XCH = V_TWIN + T::TWIN, TABS = XCH + AT_ROWS * 4, BAR = TABS + (BIAS ? 2 * WT_TAB * 4 : 0);  // dO . O of every row; bias of a block's distances, two blocks
     static constexpr int TOTAL = BAR + 256 + 1024;
     static_assert(TOTAL <= 232448 && AW_MAX_BUCKETS == 64, "shared memory");
 };
@@ -916,8 +915,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
         constexpr int OC = DP / 2;                                       // and half of the columns of q (parts 0, 1) or dO (2, 3)
         const int half = part & 1;
         const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
-        float* sums = reinterpret_cast<float*>(gen + S::DIAG);  // [warp][64]
-        float* diag = sums + (warp - 12) * 64;
+        float* sums = reinterpret_cast<float*>(gen + S::OWN);  // [warp][bucket], at an item's end, when dO's companions have been read
         float* xch = reinterpret_cast<float*>(gen + S::XCH);  // dO . O of every row
         const float c = p.scale * kLog2e;
         const bool wants_dbias = BIAS && p.dbias_part != nullptr;
@@ -1042,19 +1040,20 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
                             if (lane - 15 + e >= 0) a += x;
                             else a2 += x;
                         }
-                        diag[lane] = a;
-                        diag[32 + lane] = a2;
-                        __syncwarp();
+                        // sums of the first x diagonals, in order; a bucket is a difference of two of them
 #pragma unroll
-                        for (int k = 0; k < 2; ++k) {
-                            const int bucket = lane + 32 * k;
-                            if (bucket > far_of || bucket < near_of) continue;
-                            const int from = max(0, p.rule.starts[bucket] - d0), to = bucket + 1 < p.rule.buckets ? min(47, p.rule.starts[bucket + 1] - d0) : 47;
-                            float t = 0.0f;
-                            for (int x = from; x < to; ++x) t += diag[x];
-                            (k ? sum1 : sum0) += t;
+                        for (int x = 1; x < 32; x <<= 1) {
+                            const float y = __shfl_up_sync(0xffffffffu, a, x), y2 = __shfl_up_sync(0xffffffffu, a2, x);
+                            if (lane >= x) { a += y; a2 += y2; }
                         }
-                        __syncwarp();
+                        a2 += __shfl_sync(0xffffffffu, a, 31);
+                        auto first = [&](int x) {  // x from 0 to 47
+                            const float y = __shfl_sync(0xffffffffu, a, (x - 1) & 31), y2 = __shfl_sync(0xffffffffu, a2, (x - 1) & 31);
+                            return x == 0 ? 0.0f : x <= 32 ? y : y2;
+                        };
+                        auto edge = [&](int bucket) { return bucket < p.rule.buckets ? max(0, min(47, p.rule.starts[bucket] - d0)) : 47; };
+                        sum0 += first(edge(lane + 1)) - first(edge(lane));
+                        if (p.rule.buckets > 32) sum1 += first(edge(lane + 33)) - first(edge(lane + 32));
                     }
                 }
             }
@@ -1062,24 +1061,28 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
             after_sync();
             if (wants_dbias) {
                 settle();
-                diag[lane] = sum0;
-                diag[32 + lane] = sum1;
+                sums[(warp - 12) * 64 + lane] = sum0;
+                sums[(warp - 12) * 64 + 32 + lane] = sum1;
             }
             if (16 * part < DP) place_result(gen, row, 16 * part, lanes + 256 + 16 * part, moved, cnt > WT_FLUSH, p.scale, p.scale);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             if (all_any(!good)) break;  // all of them leave together
+            if (wants_dbias && warp == 12) {  // before the next item's dO takes their place
+                float t[2] = {0.f, 0.f};
+#pragma unroll
+                for (int x = 0; x < 16; ++x) { t[0] += sums[x * 64 + lane]; t[1] += sums[x * 64 + 32 + lane]; }
+                float* part_out = p.dbias_part + (((int64_t)it.b * p.H + it.h) * p.units + it.unit) * p.rule.buckets;
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+                    if (lane + 32 * x < p.rule.buckets) part_out[lane + 32 * x] = t[x];
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+            }
             if (threadIdx.x == 384) {
                 own_store<DP>(&map_dq, base, p, r0, it.h, it.b);
                 tma_store_commit();
                 tma_store_wait_read<0>();
                 fetch(w + gridDim.x);
-            }
-            const int t = threadIdx.x - 384;
-            if (wants_dbias && t < p.rule.buckets) {
-                float a = 0.0f;
-#pragma unroll
-                for (int x = 0; x < 16; ++x) a += sums[x * 64 + t];
-                p.dbias_part[(((int64_t)it.b * p.H + it.h) * p.units + it.unit) * p.rule.buckets + t] = a;
             }
         }
         if (threadIdx.x == 384) tma_store_wait_all();
