@@ -774,9 +774,9 @@ template <int DP, bool BIAS>
 struct DqSmem {
     using T = WinTile<DP>;
     static constexpr int OWN = AT_ROWS * DP * 4;
-    static constexpr uint32_t TWINS = BIAS ? 2 : 3;  // with a bias its table takes the place of the third one
-    static constexpr int K_RAW = 2 * OWN, V_RAW = K_RAW + 2 * T::RAW, K_MN = V_RAW + 2 * T::RAW, K_TWIN = K_MN + 2 * T::RAW, V_TWIN = K_TWIN + TWINS * T::TWIN;
-    static constexpr int XCH = V_TWIN + T::TWIN, TABS = XCH + AT_ROWS * 4, BAR = TABS + (BIAS ? 2 * WT_TAB * 4 : 0);  // dO . O of every row; bias of a block's distances, two blocks
+    static constexpr uint32_t MNS = BIAS ? 1 : 2;  // with a bias its table takes the place of the second MN-major tile (a third place for companions is worth more: 264 us against 383)
+    static constexpr int K_RAW = 2 * OWN, V_RAW = K_RAW + 2 * T::RAW, K_MN = V_RAW + 2 * T::RAW, K_TWIN = K_MN + (int)MNS * T::RAW, V_TWIN = K_TWIN + 3 * T::TWIN;
+    static constexpr int XCH = V_TWIN + T::TWIN, TABS = XCH + AT_ROWS * 4, BAR = TABS + (BIAS ? 3 * WT_TAB * 4 : 0);  // dO . O of every row; bias of a block's distances, three blocks
     static constexpr int TOTAL = BAR + 256 + 1024;
     static_assert(TOTAL <= 232448 && AW_MAX_BUCKETS == 64, "shared memory");
 };
@@ -795,10 +795,9 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
     auto one = [](uint32_t n) { return n & 1u; };
     auto k_full = [&](uint32_t n) { return bar(0 + (n & 1u)); };
     auto v_full = [&](uint32_t n) { return bar(2 + (n & 1u)); };
-    auto kn_full = [&](uint32_t n) { return bar(4 + (n & 1u)); };
-    auto twin = [](uint32_t n) { return n % S::TWINS; };
-    auto k_conv = [&](uint32_t n) { return bar(6 + twin(n)); };
-    auto k_conv_turn = [](uint32_t n) { return (n / S::TWINS) & 1u; };
+    auto kn_place = [](uint32_t n) { return S::MNS == 2 ? n & 1u : 0u; };
+    auto kn_full = [&](uint32_t n) { return bar(4 + kn_place(n)); };
+    auto k_conv = [&](uint32_t n) { return bar(6 + n % 3u); };
     // one barrier a product, in two turns, as above
     auto s_done = [&](uint32_t n) { return bar(9 + (n & 1u)); };
     auto dp_done = [&](uint32_t n) { return bar(11 + (n & 1u)); };
@@ -824,17 +823,17 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
                 if (it.skip) continue;
                 const TileKeys keys(p, it.unit * AT_ROWS);
                 const int n = keys.count();
-                // the place was last filled two blocks ago, and `done` is the product that read it
-                auto load = [&](auto done, int dst, const CUtensorMap* map, uint32_t landed, int i) {
+                // `back` blocks ago the place was last filled, and `done` is the product that read it
+                auto load = [&](auto done, uint32_t back, int dst, const CUtensorMap* map, uint32_t landed, int i) {
                     const uint32_t at = n0 + i;
-                    if (at >= 2u && !mbar_wait(done(at - 2u), two(at - 2u), p.status, 61)) return false;
+                    if (at >= back && !mbar_wait(done(at - back), two(at - back), p.status, 61)) return false;
                     win_load<DP>(base + dst, map, landed, keys.block(i) * AT_KEYS, it.h, it.b);
                     return true;
                 };
                 for (int i = 0; i < n && ok; ++i) {
                     const uint32_t at = n0 + i, place = (at & 1u) * T::RAW;
-                    if (warp == 0) ok = load(s_done, S::K_RAW + place, &map_kk, k_full(at), i) && load(dp_done, S::V_RAW + place, &map_vk, v_full(at), i);
-                    else ok = load(dq_done, S::K_MN + place, &map_kn, kn_full(at), i);
+                    if (warp == 0) ok = load(s_done, 2, S::K_RAW + place, &map_kk, k_full(at), i) && load(dp_done, 2, S::V_RAW + place, &map_vk, v_full(at), i);
+                    else ok = load(dq_done, S::MNS, S::K_MN + kn_place(at) * T::RAW, &map_kn, kn_full(at), i);
                 }
                 n0 += n;
             }
@@ -850,9 +849,9 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
                 const int n = TileKeys(p, it.unit * AT_ROWS).count();
                 auto products = [&](uint32_t at) {  // S and dP
                     const uint32_t place = tmem + 128 * (at & 1u), raw = (at & 1u) * (T::RAW / 16);
-                    if (!mbar_wait(k_conv(at), k_conv_turn(at), p.status, 62) || !mbar_wait(v_conv, one(at), p.status, 62)) return false;
+                    if (!mbar_wait(k_conv(at), (at / 3u) & 1u, p.status, 62) || !mbar_wait(v_conv, one(at), p.status, 62)) return false;
                     after_sync();
-                    win_scores<DP>(place, tmem + 320, base16, base16 + S::K_RAW / 16 + raw, base16 + (S::K_TWIN + twin(at) * T::TWIN) / 16);
+                    win_scores<DP>(place, tmem + 320, base16, base16 + S::K_RAW / 16 + raw, base16 + (S::K_TWIN + at % 3u * T::TWIN) / 16);
                     umma_commit(s_done(at));
                     win_scores<DP>(place + 64, tmem + 384, base16 + S::OWN / 16, base16 + S::V_RAW / 16 + raw, base16 + S::V_TWIN / 16);
                     umma_commit(dp_done(at));
@@ -863,10 +862,10 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
                 ok = products(n0);
                 for (int i = 0; i < n && ok; ++i) {
                     const uint32_t at = n0 + i, place = tmem + 128 * (at & 1u);
-                    ok = (i + 1 == n || products(at + 1)) && mbar_wait(kn_full(at), two(at), p.status, 64) && mbar_wait(ds_ready(at), two(at), p.status, 64);
+                    ok = (i + 1 == n || products(at + 1)) && mbar_wait(kn_full(at), S::MNS == 2 ? two(at) : one(at), p.status, 64) && mbar_wait(ds_ready(at), two(at), p.status, 64);
                     if (!ok) break;
                     after_sync();
-                    win_values<DP, 16>(tmem + 256, place + 64, place, place + 8, base16 + (S::K_MN + (at & 1u) * T::RAW) / 16, base16 + (S::K_TWIN + twin(at) * T::TWIN) / 16, i % WT_FLUSH != 0);
+                    win_values<DP, 16>(tmem + 256, place + 64, place, place + 8, base16 + (S::K_MN + kn_place(at) * T::RAW) / 16, base16 + (S::K_TWIN + at % 3u * T::TWIN) / 16, i % WT_FLUSH != 0);
                     umma_commit(dq_done(at));
                 }
                 if (!ok) break;
@@ -890,13 +889,13 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
             for (int i = 0; i < n && ok; ++i) {
                 const uint32_t at = n0 + i, place = (at & 1u) * T::RAW;
                 // dQ has read the companions that these replace; that block's bias was used before
-                ok = warp_wait(k_full(at), two(at), p.status, 65) && (at < S::TWINS || warp_wait(dq_done(at - S::TWINS), two(at - S::TWINS), p.status, 65));
+                ok = warp_wait(k_full(at), two(at), p.status, 65) && (at < 3u || warp_wait(dq_done(at - 3u), two(at - 3u), p.status, 65));
                 if (!ok) break;
                 if (BIAS) {
-                    if (t < WT_TAB) reinterpret_cast<float*>(gen + S::TABS)[(at & 1u) * WT_TAB + t] = nb;
+                    if (t < WT_TAB) reinterpret_cast<float*>(gen + S::TABS)[at % 3u * WT_TAB + t] = nb;
                     if (i + 1 < n) request(i + 1);
                 }
-                win_split<DP, 256, false>(gen + S::K_RAW + place, gen + S::K_TWIN + twin(at) * T::TWIN, t);
+                win_split<DP, 256, false>(gen + S::K_RAW + place, gen + S::K_TWIN + at % 3u * T::TWIN, t);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(k_conv(at));
@@ -995,7 +994,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
 #pragma unroll
                         for (int e = 0; e < 16; ++e) pr[e] = ex2((fmaf(__uint_as_float(u[e]), p.scale, beyond) - m) * kLog2e) * inv;
                     } else {
-                        const float* mine = reinterpret_cast<const float*>(gen + S::TABS) + (n & 1u) * WT_TAB + row - 16 * part + AT_KEYS - 1;
+                        const float* mine = reinterpret_cast<const float*>(gen + S::TABS) + n % 3u * WT_TAB + row - 16 * part + AT_KEYS - 1;
 #pragma unroll
                         for (int e = 0; e < 16; ++e) pr[e] = ex2((fmaf(__uint_as_float(u[e]), p.scale, mine[-e]) - m) * kLog2e) * inv;
                     }
