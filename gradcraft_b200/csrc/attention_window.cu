@@ -7,6 +7,7 @@
 #include <algorithm>
 
 #include "attention_fma.cuh"
+#include "attention_tc.cuh"
 #include "attention_window.cuh"
 
 namespace gcb {
@@ -449,6 +450,8 @@ __global__ void __launch_bounds__(32 * ST_WARPS) window_attention_step_kernel(co
         }
     };
     rows(v0 + group, kk, vv);
+    int bucket = p.rule.buckets - 1;
+    float bias = p.rule.bias != nullptr ? p.rule.bias[h * p.rule.buckets + bucket] : 0.0f;
     for (int x0 = v0; x0 < v1; x0 += STEP) {  // the same trips for every lane
         const int x = x0 + group;
         rows(x + STEP, kn, vn);
@@ -463,7 +466,14 @@ __global__ void __launch_bounds__(32 * ST_WARPS) window_attention_step_kernel(co
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int y = x + u * GROUPS;
-            if (p.rule.bias != nullptr && y < v1) z[u] += p.rule.bias[h * p.rule.buckets + p.rule.bucket(last - key_of(y))];
+            if (p.rule.bias != nullptr && y < v1) {  // distances only go down along the walk, and so do buckets
+                const int d = last - key_of(y);
+                if (p.rule.starts[bucket] > d) {
+                    do --bucket; while (p.rule.starts[bucket] > d);
+                    bias = p.rule.bias[h * p.rule.buckets + bucket];
+                }
+                z[u] += bias;
+            }
             if (y >= v1) z[u] = -INFINITY;
             mx = fmaxf(mx, z[u]);
         }
@@ -514,10 +524,228 @@ __global__ void __launch_bounds__(32 * ST_WARPS) window_attention_step_kernel(co
     cluster_sync();  // nobody leaves while its shared memory is read
 }
 
+// Long caches: one CTA an SM, all of which share the tiles of all heads and sequences evenly, whatever their lengths.  A tile is 16 KB of keys and as
+// much of values, brought by TMA into a ring of six, so that 192 KB an SM are on their way; eight warps read it as above.  A head whose tiles
+// lie in several CTAs leaves partial results, which a second kernel joins in their order.
+// Bound by memory: 8 x 16 heads of 16384 keys x 64 (1.07 GB) 196 us after a flush of L2, 64 x 16 of 1028 (539 MB) 114, so that the second half of a long call passes
+// at 6.5 TB/s; the cluster kernel below took 137 for the latter.
+constexpr int SM_STAGES = 6, SM_TILE = 16384, SM_MAX_SEQ = 1024, SM_THREADS = 32 * ST_WARPS + 32;
+struct StreamAttn {
+    StepAttn a;
+    float* part;  // [CTA][head that began before it, head that goes on after it][D + 2]: o, maximum, sum
+    int* head;    // [CTA]: the head that its first tile continues, or -1
+    int n_seq;
+};
+struct StreamKeys {  // the keys of one sequence in tiles of R: the first s0 ones, then lo .. len - 1
+    int len, s0, lo, first_tiles, tiles;
+    __device__ __forceinline__ StreamKeys(const StepAttn& p, int b, int R) {
+        const int64_t n = p.lengths[b];
+        len = n < 0 || n > p.cache_len ? 0 : (int)n;
+        lo = p.rule.window_first(len - 1);
+        s0 = min(p.rule.S, lo);
+        first_tiles = (s0 + R - 1) / R;
+        tiles = len > 0 ? first_tiles + (len - lo + R - 1) / R : 0;
+    }
+    __device__ __forceinline__ int row(int t, int R) const { return t < first_tiles ? t * R : lo + (t - first_tiles) * R; }
+    __device__ __forceinline__ int rows(int t, int R) const { return min(R, (t < first_tiles ? s0 : len) - row(t, R)); }
+};
+__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
+template <int LPR>
+__global__ void __launch_bounds__(SM_THREADS, 1) window_attention_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ StreamAttn g) {
+    constexpr int RPW = 32 / LPR, U = 4, GROUPS = ST_WARPS * RPW, R = GROUPS * U, DP = 4 * LPR;
+    static_assert(R * DP * 4 == SM_TILE, "a tile is 16 KB");
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_u32(smem_raw) + 127u) & ~127u;
+    uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
+    __shared__ __align__(8) uint64_t bars[2 * SM_STAGES];
+    __shared__ float g_m[GROUPS], g_sum[GROUPS], g_o[GROUPS][DP + 4];
+    __shared__ int pre[SM_MAX_SEQ + 1];  // tiles of the sequences before, of one head
+    const StepAttn& p = g.a;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = p.D, H = p.H;
+    auto full = [&](int s) { return smem_u32(bars + s); };
+    auto empty = [&](int s) { return smem_u32(bars + SM_STAGES + s); };
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < SM_STAGES; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), ST_WARPS); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    pdl_trigger();
+    pdl_wait();
+    for (int b = threadIdx.x; b < g.n_seq; b += SM_THREADS) {
+        pre[b + 1] = StreamKeys(p, b, R).tiles;
+        if (blockIdx.x == 0 && (p.lengths[b] < 0 || p.lengths[b] > p.cache_len)) { atomicExch(&p.status[0], 2); atomicExch(&p.status[1], b); }
+    }
+    __syncthreads();
+    if (warp == 0) {
+        int run = 0;
+        for (int b0 = 0; b0 < g.n_seq; b0 += 32) {
+            int x = b0 + lane < g.n_seq ? pre[b0 + lane + 1] : 0;
+#pragma unroll
+            for (int s = 1; s < 32; s <<= 1) { const int y = __shfl_up_sync(0xffffffffu, x, s); if (lane >= s) x += y; }
+            if (b0 + lane < g.n_seq) pre[b0 + lane + 1] = run + x;
+            run += __shfl_sync(0xffffffffu, x, 31);
+        }
+        if (lane == 0) pre[0] = 0;
+    }
+    __syncthreads();
+    const int64_t total = (int64_t)pre[g.n_seq] * H, begin = total * blockIdx.x / gridDim.x, end = total * (blockIdx.x + 1) / gridDim.x;
+    for (int b = blockIdx.x; b < g.n_seq; b += gridDim.x)  // sequences without a key
+        if (pre[b] == pre[b + 1])
+            for (int i = threadIdx.x; i < H * D; i += SM_THREADS) p.out[b * p.o_so + i / D * p.o_si + i % D] = 0.0f;
+    // where the first tile lies: sequence, head, tile
+    int b = 0;
+    for (int step = SM_MAX_SEQ / 2; step > 0; step >>= 1)
+        if (b + step < g.n_seq && (int64_t)pre[b + step] * H <= begin) b += step;
+    StreamKeys keys(p, b, R);
+    int h = 0, t = 0;
+    if (begin < total) {
+        const int64_t at = begin - (int64_t)pre[b] * H;
+        h = (int)(at / keys.tiles);
+        t = (int)(at - (int64_t)h * keys.tiles);
+    }
+    auto next_unit = [&]() {
+        t = 0;
+        if (++h < H) return;
+        h = 0;
+        do { ++b; } while (b < g.n_seq && pre[b] == pre[b + 1]);
+        if (b < g.n_seq) keys = StreamKeys(p, b, R);
+    };
+    if (threadIdx.x == 0) g.head[blockIdx.x] = begin < total && t > 0 ? b * H + h : -1;
+    if (begin == end && begin < total && t > 0 && threadIdx.x < D + 2) {  // fewer tiles than CTAs, and none for this one in the middle of a head: an empty part
+        g.part[(int64_t)blockIdx.x * 2 * (D + 2) + threadIdx.x] = threadIdx.x == D ? -INFINITY : 0.0f;
+    }
+
+    if (warp == ST_WARPS) {
+        if (lane == 0) {
+            bool ok = true;
+            for (int64_t i = begin; i < end && ok; ++i) {
+                const uint32_t n = (uint32_t)(i - begin), s = n % SM_STAGES;
+                ok = mbar_wait(empty(s), ((n / SM_STAGES) & 1u) ^ 1u, p.status, 71);
+                if (!ok) break;
+                mbar_expect_tx(full(s), 2 * R * D * 4);
+                tma_load_4d(base + s * 2 * SM_TILE, &map_k, full(s), 0, keys.row(t, R), h, b);
+                tma_load_4d(base + s * 2 * SM_TILE + SM_TILE, &map_v, full(s), 0, keys.row(t, R), h, b);
+                if (++t == keys.tiles) next_unit();
+            }
+        }
+        return;
+    }
+    const int col = 4 * (lane % LPR), group = warp * RPW + lane / LPR;
+    const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+    bool good = true;
+    for (int64_t i = begin; i < end;) {
+        const bool continues = t > 0;  // only the first one of this CTA
+        const int last = keys.len - 1;
+        float4 q = col < D ? ld4(p.q + b * p.q_so + h * p.q_si + col) : zero, o = zero;
+        q.x *= p.scale; q.y *= p.scale; q.z *= p.scale; q.w *= p.scale;
+        float m = -INFINITY, sum = 0.0f;
+        int bucket = p.rule.buckets - 1;
+        float bias = p.rule.bias != nullptr ? p.rule.bias[(int64_t)h * p.rule.buckets + bucket] : 0.0f;
+        for (; t < keys.tiles && i < end; ++t, ++i) {
+            const uint32_t n = (uint32_t)(i - begin), s = n % SM_STAGES;
+            const int rows = keys.rows(t, R), r0 = keys.row(t, R);
+            good = good && __all_sync(0xffffffffu, mbar_wait(full(s), (n / SM_STAGES) & 1u, p.status, 72));
+            const float* kt = reinterpret_cast<const float*>(gen + s * 2 * SM_TILE);
+            const float* vt = kt + SM_TILE / 4;
+            float z[U];
+            float4 vv[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {  // rows that are not there hold anything and are not looked at
+                const int y = u * GROUPS + group;
+                const bool live = y < rows && col < D;
+                const float4 kk = live ? ld4(kt + y * D + col) : zero;
+                vv[u] = live ? ld4(vt + y * D + col) : zero;
+                z[u] = fmaf(q.x, kk.x, fmaf(q.y, kk.y, fmaf(q.z, kk.z, q.w * kk.w)));
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty(s));  // everything of this warp's is in registers
+#pragma unroll
+            for (int x = LPR / 2; x > 0; x >>= 1)
+#pragma unroll
+                for (int u = 0; u < U; ++u) z[u] += __shfl_xor_sync(0xffffffffu, z[u], x);
+            float mx = m;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int y = u * GROUPS + group;
+                if (p.rule.bias != nullptr && y < rows) {  // distances only go down along the walk, and so do buckets
+                    const int d = last - (r0 + y);
+                    if (p.rule.starts[bucket] > d) {
+                        do --bucket; while (p.rule.starts[bucket] > d);
+                        bias = p.rule.bias[(int64_t)h * p.rule.buckets + bucket];
+                    }
+                    z[u] += bias;
+                }
+                if (y >= rows) z[u] = -INFINITY;
+                mx = fmaxf(mx, z[u]);
+            }
+            const float rel = mx == -INFINITY ? 0.0f : mx, f = __expf(m - rel);
+            m = mx;
+            sum *= f;
+            o.x *= f; o.y *= f; o.z *= f; o.w *= f;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const float e = __expf(z[u] - rel);
+                sum += e;
+                o.x = fmaf(e, vv[u].x, o.x); o.y = fmaf(e, vv[u].y, o.y); o.z = fmaf(e, vv[u].z, o.z); o.w = fmaf(e, vv[u].w, o.w);
+            }
+        }
+        // this CTA's tiles of the head: its groups in their order
+        consumers_sync();  // the head before has been written
+        if (lane % LPR == 0) { g_m[group] = m; g_sum[group] = sum; }
+        st4(&g_o[group][col], o);
+        consumers_sync();
+        const int c = threadIdx.x;
+        if (c < D) {
+            float mx = -INFINITY;
+#pragma unroll
+            for (int x = 0; x < GROUPS; ++x) mx = fmaxf(mx, g_m[x]);
+            const float rel = mx == -INFINITY ? 0.0f : mx;
+            float a = 0.0f, all = 0.0f;
+#pragma unroll
+            for (int x = 0; x < GROUPS; ++x) {
+                const float f = __expf(g_m[x] - rel);
+                a = fmaf(f, g_o[x][c], a);
+                all = fmaf(f, g_sum[x], all);
+            }
+            const bool whole = !continues && t == keys.tiles;
+            if (whole) {
+                p.out[b * p.o_so + h * p.o_si + c] = mx == -INFINITY ? 0.0f : a / all;
+            } else {
+                float* part = g.part + ((int64_t)blockIdx.x * 2 + (continues ? 0 : 1)) * (D + 2);
+                part[c] = a;
+                if (c == 0) { part[D] = mx; part[D + 1] = all; }
+            }
+        }
+        if (t == keys.tiles) next_unit();
+    }
+}
+// Joins the parts of the heads that lie in several CTAs: the block of the second of them does it.
+__global__ void __launch_bounds__(128) window_attention_join_kernel(const __grid_constant__ StreamAttn g) {
+    pdl_trigger();
+    pdl_wait();
+    const int i = blockIdx.x + 1, ctas = gridDim.x + 1, unit = g.head[i], c = threadIdx.x, D = g.a.D;
+    if (unit < 0 || g.head[i - 1] == unit || c >= D) return;
+    auto part = [&](int cta, int which) { return g.part + ((int64_t)cta * 2 + which) * (D + 2); };
+    int end = i;
+    while (end < ctas && g.head[end] == unit) ++end;
+    float mx = part(i - 1, 1)[D];
+    for (int x = i; x < end; ++x) mx = fmaxf(mx, part(x, 0)[D]);
+    const float rel = mx == -INFINITY ? 0.0f : mx;
+    float f = __expf(part(i - 1, 1)[D] - rel), a = f * part(i - 1, 1)[c], all = f * part(i - 1, 1)[D + 1];
+    for (int x = i; x < end; ++x) {
+        f = __expf(part(x, 0)[D] - rel);
+        a = fmaf(f, part(x, 0)[c], a);
+        all = fmaf(f, part(x, 0)[D + 1], all);
+    }
+    g.a.out[unit / g.a.H * g.a.o_so + unit % g.a.H * g.a.o_si + c] = mx == -INFINITY ? 0.0f : a / all;
+}
+
 // ---- host side ----------------------------------------------------------------------------------------------------------------
 static bool vec_rows(const float* p, int64_t ld, int64_t so, int64_t si) { return aligned16(p) && ld % 4 == 0 && so % 4 == 0 && si % 4 == 0; }
 static bool own_rows(int64_t B, int64_t H, int64_t T, int64_t D, int64_t ld, int64_t so, int64_t si) { return (T <= 1 || ld >= D) && (H <= 1 || si > 0) && (B <= 1 || so > 0); }
-static size_t span_bytes(int64_t B, int64_t H, int64_t T, int64_t D, int64_t ld, int64_t so, int64_t si) { return sizeof(float) * (size_t)((B - 1) * so + (H - 1) * si + (T - 1) * ld + D); }
+// Floats of keys in sight from which the streaming kernel and its join are taken instead of the one launch of clusters (either, us, after a flush of L2:
+// 1 x 16 heads of 2048 x 64 16.4 clusters, 19.5 streamed; 8 x 16 of 512 20.5, 21.5; 4 x 16 of 2048 30.8, 29.7; 1 x 16 of 8192 36.9, 29.7; 32 x 16 of 512 47.1, 42.0).
+constexpr int64_t ST_STREAM = int64_t(1) << 22;
 constexpr int64_t AW_MAX_T = int64_t(1) << 24, AW_MAX_D = 128, AW_MAX_H = 65535;
 
 template <class K>
@@ -577,6 +805,25 @@ static int make_table(gcb_ctx* ctx, WindowAttn& p, Scratch& mem) {
     p.tab = mem.as<float>();
     GCB_CHECK_CUDA(launch_next(ctx->stream, dim3((unsigned)((p.tab_len + 255) / 256), (unsigned)p.H), 256, 0, window_attention_table_kernel, mem.as<float>(), p.tab_len, p.rule));
     return after_launch(ctx, "window_attention_table");
+}
+
+template <int LPR>
+static int stream_launch(gcb_ctx* ctx, const StreamAttn& g, const float* k, const float* v, int ctas) {
+    const StepAttn& p = g.a;
+    const int rows = SM_TILE / (16 * LPR);
+    CUtensorMap mk, mv;
+    auto rows_of = [&](CUtensorMap& map, const float* x, int64_t ld, int64_t so, int64_t si) {
+        return encode_rows(tma_encode(ctx), &map, x, p.D, p.cache_len, ld, si, so, p.H, g.n_seq, p.D, rows, CU_TENSOR_MAP_SWIZZLE_NONE);
+    };
+    GCB_REQUIRE(rows_of(mk, k, p.k_ld, p.k_so, p.k_si) && rows_of(mv, v, p.v_ld, p.v_so, p.v_si), "window attention: strides beyond what TMA can address");
+    constexpr size_t smem = 2 * SM_STAGES * SM_TILE + 128;
+    static bool done[kMaxDevices] = {};
+    if (!done[ctx->device]) { GCB_CHECK_CUDA(cudaFuncSetAttribute(window_attention_stream_kernel<LPR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)); done[ctx->device] = true; }
+    GCB_CHECK_CUDA(launch_chained(ctx->stream, dim3((unsigned)ctas), SM_THREADS, smem, window_attention_stream_kernel<LPR>, mk, mv, g));
+    const int rc = after_launch(ctx, "window_attention_stream");
+    if (rc) return rc;
+    GCB_CHECK_CUDA(launch_chained(ctx->stream, dim3((unsigned)ctas - 1), 128, 0, window_attention_join_kernel, g));
+    return after_launch(ctx, "window_attention_join");
 }
 
 }  // namespace gcb
@@ -716,8 +963,18 @@ int gcb_window_attention_step_f32(gcb_ctx* ctx, int64_t n_seq, int64_t H, int64_
     p.out = out; p.o_so = o_so; p.o_si = o_si;
     p.lengths = lengths; p.status = ctx->d_status; p.cache_len = cache_len; p.D = (int)D; p.H = (int)H; p.scale = scale;
     const bool vec = D % 4 == 0 && vec_rows(q, 0, q_so, q_si) && vec_rows(k, k_ld, k_so, k_si) && vec_rows(v, v_ld, v_so, v_si);
-    // As many stretches as fill the SMs about twice over, none shorter than 64 keys.
     const int64_t seen = p.rule.W ? std::min<int64_t>(cache_len, (int64_t)p.rule.W + p.rule.S) : cache_len;
+    if (vec && n_seq <= SM_MAX_SEQ && n_seq * H * seen * D >= ST_STREAM && rows_ok(k, k_ld, k_so, k_si, n_seq, H) && rows_ok(v, v_ld, v_so, v_si, n_seq, H) && tma_encode(ctx) != nullptr) {
+        StreamAttn g = {p, nullptr, nullptr, (int)n_seq};
+        Scratch mem(ctx);
+        if ((rc = mem.get(sizeof(float) * (size_t)kSMs * (2 * (D + 2) + 1)))) return rc;
+        g.part = mem.as<float>();
+        g.head = reinterpret_cast<int*>(g.part + kSMs * 2 * (D + 2));
+        rc = D <= 32 ? stream_launch<8>(ctx, g, k, v, kSMs) : D <= 64 ? stream_launch<16>(ctx, g, k, v, kSMs) : stream_launch<32>(ctx, g, k, v, kSMs);
+        if (!rc) note_write(ctx, out, span_bytes(n_seq, H, 1, D, 0, o_so, o_si));
+        return rc;
+    }
+    // As many stretches as fill the SMs about twice over, none shorter than 64 keys.
     int64_t split = 1;
     while (split < ST_MAX_SPLIT && n_seq * H * split < 2 * kSMs && seen / (2 * split) >= 64) split *= 2;
     GCB_REQUIRE(n_seq * H * split < (int64_t(1) << 31), "gcb_window_attention_step_f32: more heads than a grid holds");

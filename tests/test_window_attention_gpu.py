@@ -324,6 +324,13 @@ STEPS = [
     (2, 1, 128, 3001, 0, 0, 8, 2000),
     (3, 2, 7, 130, 50, 3, 3, 60),  # rows off 16-byte boundaries
     (1, 2, 32, 9000, 8000, 2, 0, 0),
+    # enough keys for the streaming kernel
+    (6, 4, 64, 3000, 0, 0, 32, 512),
+    (9, 8, 40, 2000, 1500, 64, 16, 128),
+    (6, 8, 128, 1200, 700, 4, 0, 0),
+    (150, 7, 32, 333, 100, 33, 8, 64),
+    (600, 1, 64, 129, 0, 0, 0, 0),
+    (5, 1, 64, 16384, 0, 0, 0, 0),
 ]
 
 
@@ -352,6 +359,29 @@ def test_single_positions(env, size):
     assert max_abs_rel(out.cpu().numpy(), R.step(q, k, v, lengths, D**-0.5, window, sinks, bias, starts)) < TOL
 
 
+@pytest.mark.parametrize("lengths", [[5, 0, 0, 130, 0], [0] * 7, [1] * 9, [64, 65, 63, 1, 0, 4096], [70, 4096], [4096, 0, 3]], ids=lambda x: "-".join(map(str, x)))
+def test_streamed_positions_of_uneven_lengths(env, lengths):
+    """Few tiles, or all of them in one sequence: heads that lie in several CTAs, CTAs without a tile."""
+    ctx, torch, capi = env
+    B, H, D, cap = len(lengths), 12, 64, 4096  # so many heads that two sequences reach the streaming kernel
+    rng = np.random.default_rng(4)
+    q, k, v = rng.standard_normal((B, H, D), dtype=np.float32), rng.standard_normal((B, H, cap, D), dtype=np.float32), rng.standard_normal((B, H, cap, D), dtype=np.float32)
+    out, kd, vd = torch.full((B, H, D), float("nan"), device="cuda"), torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda()
+    for b, n in enumerate(lengths):
+        kd[b, :, n:] = float("nan")
+        vd[b, :, n:] = float("nan")
+    before = ctx.ctx_launch_count_named(b"window_attention_stream")
+    at = (D, H * cap * D, cap * D)
+    got = []
+    for _ in range(2):
+        ctx.window_attention_step_f32(B, H, D, out, H * D, D, torch.from_numpy(q).cuda(), H * D, D, kd, *at, vd, *at, cap, torch.tensor(lengths, device="cuda"), 0.125, 3000, 5, None, 0, None)
+        ctx.sync()
+        got.append(out.clone())
+    assert ctx.ctx_launch_count_named(b"window_attention_stream") == before + 2
+    assert torch.equal(*got)
+    assert max_abs_rel(out.cpu().numpy(), R.step(q, k, v, lengths, 0.125, 3000, 5)) < TOL
+
+
 def test_a_cache_beyond_32_bits_of_offsets(env):
     """The last sequence's rows lie more than 2^32 elements behind the first one's."""
     ctx, torch, capi = env
@@ -370,6 +400,12 @@ def test_a_cache_beyond_32_bits_of_offsets(env):
 def test_a_length_outside_its_cache_is_reported(env):
     ctx, torch, capi = env
     x, out = torch.ones(2, 4, 1, 8, device="cuda"), torch.full((2, 1, 8), 5.0, device="cuda")
+    big, big_out, at = torch.ones(2, 40000, 1, 64, device="cuda"), torch.full((2, 1, 64), 5.0, device="cuda"), (64, 40000 * 64, 64)
+    ctx.window_attention_step_f32(2, 1, 64, big_out, 64, 64, big_out, 64, 64, big, *at, big, *at, 40000, torch.tensor([40001, 4000], device="cuda"), 1.0, 0, 0, None, 0, None)
+    with pytest.raises(capi.GcbError) as e:
+        ctx.sync()
+    assert e.value.status == capi.INVALID_ARG
+    assert (big_out[0] == 0).all() and ((big_out[1] - 1).abs() < 1e-6).all()
     for bad in (5, -1, 1 << 40):
         ctx.window_attention_step_f32(2, 1, 8, out, 8, 8, x, 8, 8, x, 8, 32, 8, x, 8, 32, 8, 4, torch.tensor([3, bad], device="cuda"), 1.0, 0, 0, None, 0, None)
         with pytest.raises(capi.GcbError) as e:
