@@ -21,6 +21,7 @@ struct gct_trainer {
     std::unique_ptr<GlobalNormClipper<float>> clipper;
     std::vector<std::pair<std::string, Parameter<float>*>> ordered;  // arena order
     std::unordered_map<std::string, Parameter<float>*> named;
+    DropoutCounter* dropout_counter = nullptr;
     float ce_eps = 1e-5f, clip = 0.0f;
     cudaStream_t copy_stream = nullptr;
     cudaEvent_t copy_event = nullptr;
@@ -46,6 +47,7 @@ static Tensor<int64_t> wrap_i64(const int64_t* p, int64_t B, int64_t T, Device d
 
 template <class Model>
 static void use_model(gct_trainer& tr, Model* model) {
+    tr.dropout_counter = &model->dropout_counter();
     tr.forward = [model](Tensor<int64_t> x) { return model->forward(std::move(x)); };
     tr.generate = [model, gpu = tr.gpu](const std::vector<int64_t>& start, int64_t context_length, int64_t max_tokens, int64_t num_sequences, std::optional<float> temperature, int64_t top_k) {
         return generate_tokens_incremental(*model, start, context_length, max_tokens, num_sequences, gpu, temperature, top_k);
@@ -58,7 +60,18 @@ const char* gct_last_error(void) { return g_err.c_str(); }
 
 int gct_create(const char* arch, int64_t V, int64_t T, int64_t C, int64_t H, int64_t L, int64_t F, float lr, float beta1, float beta2, float wd, float adam_eps, float norm_eps,
                float ce_eps, float clip, int device, gct_trainer** out) {
+    return gct_create_with(arch, V, T, C, H, L, F, lr, beta1, beta2, wd, adam_eps, norm_eps, ce_eps, clip, nullptr, device, out);
+}
+
+int gct_create_with(const char* arch, int64_t V, int64_t T, int64_t C, int64_t H, int64_t L, int64_t F, float lr, float beta1, float beta2, float wd, float adam_eps, float norm_eps,
+                    float ce_eps, float clip, const gct_block_options* options, int device, gct_trainer** out) {
     return guarded([&] {
+        BlockOptions opt;
+        if (options) {
+            opt.window = options->window; opt.sinks = options->sinks; opt.rel_buckets = options->rel_buckets; opt.rel_reach = options->rel_reach;
+            opt.dropout = options->dropout; opt.dropout_seed = options->dropout_seed;
+            if (opt.window < 0 || opt.sinks < 0 || opt.sinks > 64 || opt.rel_buckets < 0) throw std::runtime_error("gct_create_with: window, sinks (up to 64) and buckets are counts");
+        }
         if (!arch || !out) throw std::runtime_error("gct_create: NULL argument");
         auto tr = std::make_unique<gct_trainer>();
         tr->gpu = Device(DeviceType::CUDA, device);
@@ -67,12 +80,12 @@ int gct_create(const char* arch, int64_t V, int64_t T, int64_t C, int64_t H, int
         ZerosInit<float> z;
         const std::string a = arch;
         if (a == "lngelu") {
-            auto m = std::make_unique<LayerNormGPT<float>>(V, T, C, H, L, F, z, z, norm_eps);
+            auto m = std::make_unique<LayerNormGPT<float>>(V, T, C, H, L, F, z, z, norm_eps, opt);
             auto* raw = m.get();
             use_model(*tr, raw);
             tr->model = std::move(m);
         } else if (a == "rmsswiglu") {
-            auto m = std::make_unique<GPT<float>>(V, T, C, H, L, z, z, norm_eps);
+            auto m = std::make_unique<GPT<float>>(V, T, C, H, L, z, z, norm_eps, opt);
             auto* raw = m.get();
             use_model(*tr, raw);
             tr->model = std::move(m);
@@ -100,6 +113,14 @@ int gct_destroy(gct_trainer* tr) {
         if (tr->copy_stream) cudaStreamDestroy(tr->copy_stream);
         if (tr->copy_event) cudaEventDestroy(tr->copy_event);
         delete tr;
+    });
+}
+
+int64_t gct_dropout_counter(gct_trainer* tr) { return tr ? tr->dropout_counter->next : 0; }
+int gct_set_dropout_counter(gct_trainer* tr, int64_t counter) {
+    return guarded([&] {
+        if (!tr) throw std::runtime_error("gct_set_dropout_counter: NULL argument");
+        tr->dropout_counter->next = counter;
     });
 }
 

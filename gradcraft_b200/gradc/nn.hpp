@@ -313,20 +313,60 @@ public:
     Tensor<T> forward(Tensor<T> x) { return linear(std::move(x), m_weight.tensor(), m_bias.tensor()); }
 };
 
+// What a block may have besides the plain causal attention: a window with first positions that stay visible, a learned bias by distance bucket
+// (a table of heads x rel_buckets a layer, the last bucket reaching from about rel_reach on), dropout on both residual branches.
+struct BlockOptions {
+    int64_t window = 0, sinks = 0, rel_buckets = 0, rel_reach = 128;
+    float dropout = 0.0f;
+    int64_t dropout_seed = 0;
+    AttentionRule rule() const {
+        AttentionRule r{window, sinks, {}};
+        if (rel_buckets > 0) r.bucket_starts = AttentionRule::relative_buckets(rel_buckets, rel_reach);
+        return r;
+    }
+};
+
+// Elements are dropped while training, with masks from a counter that all layers of a model share.
+template <typename T>
+requires std::is_floating_point_v<T>
+class Dropout : public Module<T> {
+    float m_p;
+    std::shared_ptr<DropoutCounter> m_counter;
+
+public:
+    Dropout(float p, std::shared_ptr<DropoutCounter> counter) : m_p(p), m_counter(std::move(counter)) {
+        if (!(p >= 0.0f && p <= 1.0f)) throw std::runtime_error("Dropout: the probability must lie between 0 and 1");
+        if (!m_counter) throw std::runtime_error("Dropout: a counter to draw masks from is needed");
+    }
+    float p() const { return m_p; }
+    bool active() const { return this->is_training() && m_p > 0.0f; }
+    Tensor<T> forward(Tensor<T> x) { return active() ? dropout(std::move(x), m_p, *m_counter) : x; }
+    Tensor<T> add(Tensor<T> residual, Tensor<T> x) { return active() ? dropout(std::move(x), m_p, *m_counter, std::move(residual)) : std::move(residual) + std::move(x); }
+};
+
 template <typename T>
 requires std::is_floating_point_v<T>
 class MultiHeadAttention : public Module<T> {
     Linear<T> m_q_proj, m_k_proj, m_v_proj, m_out_proj;
     int64_t m_num_heads, m_head_dim;
     bool m_is_causal;
+    AttentionRule m_rule;
+    Parameter<T> m_rel_bias;  // (heads, buckets), where the rule has buckets
 
 public:
-    MultiHeadAttention(int64_t embed_dim, int64_t num_heads, bool is_causal, int64_t /*max_seq_len*/, const Initializer<T>& proj_w_init, const Initializer<T>& residual_w_init, const Initializer<T>& proj_b_init)
+    MultiHeadAttention(int64_t embed_dim, int64_t num_heads, bool is_causal, int64_t /*max_seq_len*/, const Initializer<T>& proj_w_init, const Initializer<T>& residual_w_init, const Initializer<T>& proj_b_init,
+                       const AttentionRule& rule = {})
         : m_q_proj(embed_dim, embed_dim, proj_w_init, proj_b_init), m_k_proj(embed_dim, embed_dim, proj_w_init, proj_b_init), m_v_proj(embed_dim, embed_dim, proj_w_init, proj_b_init),
-          m_out_proj(embed_dim, embed_dim, residual_w_init, proj_b_init), m_is_causal(is_causal) {
+          m_out_proj(embed_dim, embed_dim, residual_w_init, proj_b_init), m_is_causal(is_causal), m_rule(rule) {
         if (embed_dim % num_heads != 0) throw std::runtime_error("embed_dim modulo num_heads must = 0 in MHA.");
         m_num_heads = num_heads;
         m_head_dim = embed_dim / num_heads;
+        if (!m_rule.causal_only() && (!is_causal || m_head_dim > 128)) throw std::runtime_error("MHA: a window or a bias by distance takes causal attention with heads of up to 128 columns.");
+        if (m_rule.buckets() > 0) {
+            m_rel_bias = Parameter<T>(Tensor<T>::zeros({num_heads, m_rule.buckets()}));
+            m_rel_bias.set_no_decay(true);
+            this->register_parameter("rel_bias", &m_rel_bias);
+        }
         this->register_module("q_proj", &m_q_proj);
         this->register_module("k_proj", &m_k_proj);
         this->register_module("v_proj", &m_v_proj);
@@ -334,6 +374,8 @@ public:
     }
     int64_t num_heads() const { return m_num_heads; }
     bool is_causal() const { return m_is_causal; }
+    const AttentionRule& rule() const { return m_rule; }
+    const T* rel_bias() const { return m_rule.buckets() > 0 ? m_rel_bias.tensor().data_ptr() : nullptr; }
     void describe(gcb_gpt_layer& d) const {
         d.wq = m_q_proj.weight().data_ptr(); d.bq = m_q_proj.bias().data_ptr();
         d.wk = m_k_proj.weight().data_ptr(); d.bk = m_k_proj.bias().data_ptr();
@@ -345,7 +387,7 @@ public:
         auto heads = [&](Tensor<T> t) { return t.reshape({B, S, m_num_heads, m_head_dim}).permute({0, 2, 1, 3}); };  // views only
         std::vector<Tensor<T>> qkv = linear_group(std::move(x), {{m_q_proj.weight(), m_q_proj.bias()}, {m_k_proj.weight(), m_k_proj.bias()}, {m_v_proj.weight(), m_v_proj.bias()}});
         Tensor<T> Q = heads(qkv[0]), K = heads(qkv[1]), V = heads(qkv[2]);
-        Tensor<T> attn = sdpa(Q, K, V, m_is_causal);
+        Tensor<T> attn = m_rule.causal_only() ? sdpa(Q, K, V, m_is_causal) : window_attention(Q, K, V, m_rule, m_rule.buckets() > 0 ? std::optional<Tensor<T>>(m_rel_bias.tensor()) : std::nullopt);
         attn = attn.permute({0, 2, 1, 3}).reshape({B, S, m_num_heads * m_head_dim});  // a view: sdpa lays its output out (B, T, H, D)
         return m_out_proj.forward(attn);
     }
@@ -481,15 +523,18 @@ class BlockT : public Module<T> {
     MultiHeadAttention<T> m_attn;
     Norm m_norm2;
     MLP m_mlp;
+    Dropout<T> m_dropout;
 
 public:
     template <class NormMaker>
-    BlockT(int64_t C, int64_t H, int64_t max_seq, int64_t hidden, const Initializer<T>& base_init, const Initializer<T>& residual_init, NormMaker mk)
-        : m_norm1(mk()), m_attn(C, H, true, max_seq, base_init, residual_init, ZerosInit<T>()), m_norm2(mk()), m_mlp(C, hidden, base_init, residual_init) {
+    BlockT(int64_t C, int64_t H, int64_t max_seq, int64_t hidden, const Initializer<T>& base_init, const Initializer<T>& residual_init, NormMaker mk, const BlockOptions& opt = {}, std::shared_ptr<DropoutCounter> counter = nullptr)
+        : m_norm1(mk()), m_attn(C, H, true, max_seq, base_init, residual_init, ZerosInit<T>(), opt.rule()), m_norm2(mk()), m_mlp(C, hidden, base_init, residual_init),
+          m_dropout(opt.dropout, counter ? counter : std::make_shared<DropoutCounter>(opt.dropout_seed)) {
         this->register_module("norm1", &m_norm1);
         this->register_module("attn", &m_attn);
         this->register_module("norm2", &m_norm2);
         this->register_module("mlp", &m_mlp);
+        this->register_module("dropout", &m_dropout);
     }
     const MultiHeadAttention<T>& attn() const { return m_attn; }
     const MLP& mlp() const { return m_mlp; }
@@ -500,8 +545,8 @@ public:
         m_mlp.describe(d);
     }
     Tensor<T> forward(Tensor<T> x) {
-        x = x + m_attn.forward(m_norm1.forward(x));
-        x = x + m_mlp.forward(m_norm2.forward(x));
+        x = m_dropout.add(x, m_attn.forward(m_norm1.forward(x)));
+        x = m_dropout.add(x, m_mlp.forward(m_norm2.forward(x)));
         return x;
     }
 };
@@ -510,8 +555,9 @@ template <typename T>
 requires std::is_floating_point_v<T>
 class TransformerBlock : public BlockT<T, RMSNorm<T>, SwiGLUMLP<T>> {
 public:
-    TransformerBlock(int64_t C, int64_t H, int64_t max_seq, const Initializer<T>& base_init, const Initializer<T>& residual_init, T eps = static_cast<T>(1e-5))
-        : BlockT<T, RMSNorm<T>, SwiGLUMLP<T>>(C, H, max_seq, 3 * C, base_init, residual_init, [&] { return RMSNorm<T>({C}, {-1}, OnesInit<T>(), eps); }) {}
+    TransformerBlock(int64_t C, int64_t H, int64_t max_seq, const Initializer<T>& base_init, const Initializer<T>& residual_init, T eps = static_cast<T>(1e-5), const BlockOptions& opt = {},
+                     std::shared_ptr<DropoutCounter> counter = nullptr)
+        : BlockT<T, RMSNorm<T>, SwiGLUMLP<T>>(C, H, max_seq, 3 * C, base_init, residual_init, [&] { return RMSNorm<T>({C}, {-1}, OnesInit<T>(), eps); }, opt, std::move(counter)) {}
 };
 
 template <typename T, class Norm, class Block>
@@ -521,16 +567,25 @@ protected:
     PosEncoding<T> m_pos_embed;
     std::vector<std::unique_ptr<Block>> m_blocks;
     Norm m_final_norm;
+    std::shared_ptr<DropoutCounter> m_counter;  // one for all blocks: masks follow from the seed and the order of calls
 
     template <class NormMaker>
-    GPTBase(int64_t V, int64_t max_seq, int64_t C, const Initializer<T>& base_init, NormMaker mk)
-        : m_token_embed(V, {C}, NormalInit<T>(0, static_cast<T>(0.02))), m_pos_embed(max_seq, {C}, base_init), m_final_norm(mk()) {
+    GPTBase(int64_t V, int64_t max_seq, int64_t C, const Initializer<T>& base_init, NormMaker mk, int64_t dropout_seed = 0)
+        : m_token_embed(V, {C}, NormalInit<T>(0, static_cast<T>(0.02))), m_pos_embed(max_seq, {C}, base_init), m_final_norm(mk()), m_counter(std::make_shared<DropoutCounter>(dropout_seed)) {
         this->register_module("token_embed", &m_token_embed);
         this->register_module("pos_embed", &m_pos_embed);
     }
     void finish_registration() { this->register_module("final_norm", &m_final_norm); }
 
 public:
+    DropoutCounter& dropout_counter() { return *m_counter; }  // where masks go on; to be kept with a checkpoint and set again for the same ones
+    // What the blocks' attention has besides being causal: the rule, which they share, and every layer's bias table (NULL: none).
+    AttentionRule attention_rule() const { return m_blocks.empty() ? AttentionRule{} : m_blocks[0]->attn().rule(); }
+    std::vector<const T*> bias_tables() const {
+        std::vector<const T*> t;
+        for (const auto& b : m_blocks) t.push_back(b->attn().rel_bias());
+        return t;
+    }
     // The weights as the decoding kernel takes them; valid while the parameters stay where they are.
     gcb_gpt_model describe(std::vector<gcb_gpt_layer>& layers) const {
         layers.assign(m_blocks.size(), gcb_gpt_layer{});
@@ -560,16 +615,16 @@ template <typename T>
 requires std::is_floating_point_v<T>
 class GPT : public GPTBase<T, RMSNorm<T>, TransformerBlock<T>> {
 public:
-    GPT(int64_t V, int64_t max_seq, int64_t C, int64_t H, int64_t L, const Initializer<T>& base_init, const Initializer<T>& residual_init, T eps = static_cast<T>(1e-5))
-        : GPTBase<T, RMSNorm<T>, TransformerBlock<T>>(V, max_seq, C, base_init, [&] { return RMSNorm<T>({C}, {-1}, OnesInit<T>(), eps); }) {
+    GPT(int64_t V, int64_t max_seq, int64_t C, int64_t H, int64_t L, const Initializer<T>& base_init, const Initializer<T>& residual_init, T eps = static_cast<T>(1e-5), const BlockOptions& opt = {})
+        : GPTBase<T, RMSNorm<T>, TransformerBlock<T>>(V, max_seq, C, base_init, [&] { return RMSNorm<T>({C}, {-1}, OnesInit<T>(), eps); }, opt.dropout_seed) {
         for (int64_t i = 0; i < L; ++i) {
-            this->m_blocks.push_back(std::make_unique<TransformerBlock<T>>(C, H, max_seq, base_init, residual_init, eps));
+            this->m_blocks.push_back(std::make_unique<TransformerBlock<T>>(C, H, max_seq, base_init, residual_init, eps, opt, this->m_counter));
             this->register_module("block_" + std::to_string(i), this->m_blocks.back().get());
         }
         this->finish_registration();
     }
-    GPT(const GPTConfig& cfg, const Initializer<T>& base_init, const Initializer<T>& residual_init)
-        : GPT(cfg.vocab_size, cfg.max_seq_len, cfg.embed_dim, cfg.num_heads, cfg.num_layers, base_init, residual_init, cfg.calc_eps) {}
+    GPT(const GPTConfig& cfg, const Initializer<T>& base_init, const Initializer<T>& residual_init, const BlockOptions& opt = {})
+        : GPT(cfg.vocab_size, cfg.max_seq_len, cfg.embed_dim, cfg.num_heads, cfg.num_layers, base_init, residual_init, cfg.calc_eps, opt) {}
 };
 
 // The LayerNorm + GELU(d_ff) transformer assembled from the reference's primitives layernorm() and Tensor::gelu().
@@ -579,10 +634,10 @@ class LayerNormGPT : public GPTBase<T, LayerNorm<T>, BlockT<T, LayerNorm<T>, Gel
     using Block = BlockT<T, LayerNorm<T>, GeluMLP<T>>;
 
 public:
-    LayerNormGPT(int64_t V, int64_t max_seq, int64_t C, int64_t H, int64_t L, int64_t d_ff, const Initializer<T>& base_init, const Initializer<T>& residual_init, T eps = static_cast<T>(1e-5))
-        : GPTBase<T, LayerNorm<T>, Block>(V, max_seq, C, base_init, [&] { return LayerNorm<T>({C}, {-1}, OnesInit<T>(), ZerosInit<T>(), eps); }) {
+    LayerNormGPT(int64_t V, int64_t max_seq, int64_t C, int64_t H, int64_t L, int64_t d_ff, const Initializer<T>& base_init, const Initializer<T>& residual_init, T eps = static_cast<T>(1e-5), const BlockOptions& opt = {})
+        : GPTBase<T, LayerNorm<T>, Block>(V, max_seq, C, base_init, [&] { return LayerNorm<T>({C}, {-1}, OnesInit<T>(), ZerosInit<T>(), eps); }, opt.dropout_seed) {
         for (int64_t i = 0; i < L; ++i) {
-            this->m_blocks.push_back(std::make_unique<Block>(C, H, max_seq, d_ff, base_init, residual_init, [&] { return LayerNorm<T>({C}, {-1}, OnesInit<T>(), ZerosInit<T>(), eps); }));
+            this->m_blocks.push_back(std::make_unique<Block>(C, H, max_seq, d_ff, base_init, residual_init, [&] { return LayerNorm<T>({C}, {-1}, OnesInit<T>(), ZerosInit<T>(), eps); }, opt, this->m_counter));
             this->register_module("block_" + std::to_string(i), this->m_blocks.back().get());
         }
         this->finish_registration();
@@ -947,10 +1002,13 @@ class IncrementalGPT {
     Device m_device;
     std::vector<gcb_gpt_layer> m_layers;
     gcb_gpt_model m_model;
+    AttentionRule m_rule;                 // with one, positions go through the layers' operators one by one instead of the decoding kernel
+    std::vector<const float*> m_tables;   // its bias tables
     std::unique_ptr<gcb_gpt_decoder, int (*)(gcb_gpt_decoder*)> m_decoder{nullptr, gcb_gpt_decoder_destroy};
     int64_t m_cap = 0, m_seqs = 0;  // positions per sequence and sequences the cache holds
     Tensor<float> m_cache, m_x, m_a, m_q, m_o, m_scores, m_stats, m_h0, m_h1;
-    Tensor<int64_t> m_ids;
+    Tensor<int64_t> m_ids, m_now, m_lengths;
+    bool ruled() const { return !m_rule.causal_only(); }
 
     float* cache(int64_t layer, int which) { return m_cache.data_ptr() + (2 * layer + which) * m_seqs * m_cap * m_model.C; }
     static void at_least(Tensor<float>& t, int64_t n, Device d) {
@@ -972,6 +1030,25 @@ class IncrementalGPT {
             project(y1, x, w1, b1, rows, K, N);
         }
     }
+    // What a layer does after its attention: x + wo o, then the MLP.  x and a change places twice.
+    void after_attention(const gcb_gpt_layer& w, int64_t rows, float*& x, float*& a, const float* o, float* h0, float* h1) {
+        const gcb_gpt_model& m = m_model;
+        const int64_t C = m.C, F = m.F;
+        gcb_check(gcb_linear_residual_f32(m_ctx, GCB_OP_N, rows, C, C, o, C, w.wo, C, w.bo, x, a), "linear + residual");
+        std::swap(x, a);
+        norm(a, x, w.norm2_gamma, w.norm2_beta, rows);
+        const float *w_out, *b_out;
+        if (w.w3 != nullptr) {
+            project_two(h1, h0, a, w.w2, w.w1, w.b2, w.b1, rows, C, F);
+            gcb_check(gcb_swiglu_fwd_f32(m_ctx, h1, h0, h1, rows * F), "swiglu");
+            w_out = w.w3; b_out = w.b3;
+        } else {
+            gcb_check(gcb_linear_gelu_fwd_f32(m_ctx, GCB_OP_N, rows, F, C, a, C, w.w1, F, w.b1, h0, h1), "linear + gelu");
+            w_out = w.w2; b_out = w.b2;
+        }
+        gcb_check(gcb_linear_residual_f32(m_ctx, GCB_OP_N, rows, C, F, h1, F, w_out, C, b_out, x, a), "linear + residual");
+        std::swap(x, a);
+    }
     // Keys and values of the positions 0 .. n - 1 of `seqs` sequences, token ids on the device (seqs x n, dense).
     void forward_window(const int64_t* ids, int64_t seqs, int64_t n) {
         const gcb_gpt_model& m = m_model;
@@ -991,7 +1068,11 @@ class IncrementalGPT {
             project_two(v, k, a, w.wv, w.wk, w.bv, w.bk, rows, C, C);
             if (l + 1 == m.L) break;
             project(q, a, w.wq, w.bq, rows, C, C);
-            if (gcb_attention_preferred(m_ctx, seqs, H, n, D) && gcb_attention_supported(m_ctx, seqs, H, n, D, q, C, n * C, D, k, C, m_cap * C, D, v, C, m_cap * C, D, scale)) {
+            if (ruled()) {
+                at_least(m_stats, gcb_attention_stats_floats(seqs, H, n), m_device);
+                gcb_check(gcb_window_attention_fwd_f32(m_ctx, seqs, H, n, D, o, C, n * C, D, m_stats.data_ptr(), q, C, n * C, D, k, C, m_cap * C, D, v, C, m_cap * C, D, scale, m_rule.window, m_rule.sinks, m_tables[(size_t)l],
+                                                       m_rule.buckets(), m_rule.bucket_starts.data()), "window attention");
+            } else if (gcb_attention_preferred(m_ctx, seqs, H, n, D) && gcb_attention_supported(m_ctx, seqs, H, n, D, q, C, n * C, D, k, C, m_cap * C, D, v, C, m_cap * C, D, scale)) {
                 at_least(m_stats, gcb_attention_stats_floats(seqs, H, n), m_device);
                 gcb_check(gcb_attention_fwd_f32(m_ctx, seqs, H, n, D, o, C, n * C, D, m_stats.data_ptr(), q, C, n * C, D, k, C, m_cap * C, D, v, C, m_cap * C, D, scale), "attention");
             } else {
@@ -1001,37 +1082,80 @@ class IncrementalGPT {
                 gcb_check(gcb_causal_softmax_fwd_band_ld_f32(m_ctx, s, s, scale, seqs * H * n, n, ld, 128), "causal softmax");
                 gcb_check(gcb_gemm_batched_causal_f32(m_ctx, GCB_OP_N, GCB_OP_N, n, D, n, 1.0f, s, ld, H * n * ld, n * ld, v, C, m_cap * C, D, 0.0f, o, C, n * C, D, seqs, H, 2), "attention output");
             }
-            gcb_check(gcb_linear_residual_f32(m_ctx, GCB_OP_N, rows, C, C, o, C, w.wo, C, w.bo, x, a), "linear + residual");
-            std::swap(x, a);
-            norm(a, x, w.norm2_gamma, w.norm2_beta, rows);
-            const float *w_out, *b_out;
-            if (w.w3 != nullptr) {
-                project_two(h1, h0, a, w.w2, w.w1, w.b2, w.b1, rows, C, F);
-                gcb_check(gcb_swiglu_fwd_f32(m_ctx, h1, h0, h1, rows * F), "swiglu");
-                w_out = w.w3; b_out = w.b3;
-            } else {
-                gcb_check(gcb_linear_gelu_fwd_f32(m_ctx, GCB_OP_N, rows, F, C, a, C, w.w1, F, w.b1, h0, h1), "linear + gelu");
-                w_out = w.w2; b_out = w.b2;
+            after_attention(w, rows, x, a, o, h0, h1);
+        }
+    }
+    // One position of every sequence through the layers' operators; `logits` (n_seq x V, or NULL) where the next token hangs on it.
+    void step(const int64_t* ids, int64_t ids_ld, int64_t pos, float* logits) {
+        const gcb_gpt_model& m = m_model;
+        const int64_t C = m.C, H = m.H, D = C / H, rows = m_seqs;
+        const float scale = static_cast<float>(1.0 / std::sqrt((double)D));
+        for (Tensor<float>* t : {&m_x, &m_a, &m_q, &m_o}) at_least(*t, rows * C, m_device);
+        at_least(m_h0, rows * m.F, m_device);
+        at_least(m_h1, rows * m.F, m_device);
+        if (m_now._get_state() == nullptr) {
+            m_now = Tensor<int64_t>({rows}, m_device, uninitialized);
+            m_lengths = Tensor<int64_t>({rows}, m_device, uninitialized);
+        }
+        float *x = m_x.data_ptr(), *a = m_a.data_ptr();
+        const int64_t shape[2] = {rows, 2}, to[2] = {2, 1}, from[2] = {2 * ids_ld, 1};  // ids as pairs of floats, which a copy does not look into
+        gcb_check(gcb_copy_strided_f32(m_ctx, 2, shape, reinterpret_cast<float*>(m_now.data_ptr()), to, reinterpret_cast<const float*>(ids + pos), from, 0), "token ids of a position");
+        gcb_check(gcb_fill_arange_i64(m_ctx, m_lengths.data_ptr(), pos + 1, 0, rows), "lengths");
+        gcb_check(gcb_embed_f32(m_ctx, x, m_now.data_ptr(), GCB_IDX_I64, m.token_embed, rows, C, m.V), "embedding gather");
+        gcb_check(gcb_binary_rowvec_f32(m_ctx, GCB_B_ADD, x, x, m.pos_embed + pos * C, rows, C), "positions");
+        for (int64_t l = 0; l < m.L; ++l) {
+            const gcb_gpt_layer& w = m_layers[(size_t)l];
+            float *k = cache(l, 0), *v = cache(l, 1);
+            norm(a, x, w.norm1_gamma, w.norm1_beta, rows);
+            project(m_q.data_ptr(), a, w.wq, w.bq, rows, C, C);
+            gcb_check(gcb_gemm_f32(m_ctx, GCB_OP_N, GCB_OP_N, rows, C, C, 1.0f, a, C, w.wk, C, 0.0f, k + pos * C, m_cap * C, w.bk), "projection");  // into the cache
+            gcb_check(gcb_gemm_f32(m_ctx, GCB_OP_N, GCB_OP_N, rows, C, C, 1.0f, a, C, w.wv, C, 0.0f, v + pos * C, m_cap * C, w.bv), "projection");
+            gcb_check(gcb_window_attention_step_f32(m_ctx, rows, H, D, m_o.data_ptr(), C, D, m_q.data_ptr(), C, D, k, C, m_cap * C, D, v, C, m_cap * C, D, m_cap, m_lengths.data_ptr(), scale, m_rule.window, m_rule.sinks,
+                                                    m_tables[(size_t)l], m_rule.buckets(), m_rule.bucket_starts.data()), "window attention of a position");
+            after_attention(w, rows, x, a, m_o.data_ptr(), m_h0.data_ptr(), m_h1.data_ptr());
+        }
+        if (logits == nullptr) return;
+        norm(a, x, m.final_gamma, m.final_beta, rows);
+        gcb_check(gcb_gemm_f32(m_ctx, GCB_OP_N, GCB_OP_T, rows, m.V, C, 1.0f, a, C, m.token_embed, C, 0.0f, logits, m.V, nullptr), "logits");
+    }
+    void step_through(int64_t* ids, int64_t ids_ld, int64_t pos0, int64_t n_pos, int64_t n_known, float* logits) {
+        Tensor<float> own;
+        std::vector<float> host;
+        for (int64_t pos = pos0; pos < pos0 + n_pos; ++pos) {
+            const bool picks = logits == nullptr && pos + 1 >= n_known;
+            if (picks && host.empty()) {
+                own = Tensor<float>({m_seqs, m_model.V}, m_device, uninitialized);
+                host.resize((size_t)(m_seqs * m_model.V));
             }
-            gcb_check(gcb_linear_residual_f32(m_ctx, GCB_OP_N, rows, C, F, h1, F, w_out, C, b_out, x, a), "linear + residual");
-            std::swap(x, a);
+            step(ids, ids_ld, pos, picks ? own.data_ptr() : pos + 1 == pos0 + n_pos ? logits : nullptr);
+            if (!picks) continue;
+            gcb_check(gcb_copy_d2h(m_ctx, host.data(), own.data_ptr(), sizeof(float) * host.size()), "logits download");
+            for (int64_t b = 0; b < m_seqs; ++b) {
+                const auto row = host.begin() + b * m_model.V;
+                const int64_t token = std::max_element(row, row + m_model.V) - row;
+                gcb_check(gcb_copy_h2d(m_ctx, ids + b * ids_ld + pos + 1, &token, sizeof(token)), "token upload");
+            }
         }
     }
     void decode(int64_t* ids, int64_t ids_ld, int64_t pos0, int64_t n_pos, int64_t n_known, float* logits) {
+        if (ruled()) return step_through(ids, ids_ld, pos0, n_pos, n_known, logits);
         gcb_check(gcb_gpt_decode_f32(m_decoder.get(), m_seqs, m_cache.data_ptr(), m_cap, ids, ids_ld, pos0, n_pos, n_known, logits), "decoding");
     }
 
 public:
     template <class Model>
-    IncrementalGPT(const Model& model, Device device) : m_ctx(Backend::get().ctx(device)), m_device(device), m_model(model.describe(m_layers)) {}
-    bool takes(int64_t positions) const { return positions <= m_model.T && gcb_gpt_decode_supported(m_ctx, &m_model) == 1; }
+    IncrementalGPT(const Model& model, Device device)
+        : m_ctx(Backend::get().ctx(device)), m_device(device), m_model(model.describe(m_layers)), m_rule(model.attention_rule()), m_tables(model.bias_tables()) {}
+    bool takes(int64_t positions) const { return positions <= m_model.T && (ruled() || gcb_gpt_decode_supported(m_ctx, &m_model) == 1); }
 
     std::vector<int64_t> generate(const std::vector<int64_t>& start_tokens, int64_t context_length, int64_t max_tokens, int64_t num_sequences, std::optional<float> temperature, int64_t top_k) {
         const int64_t start = (int64_t)start_tokens.size(), C = m_model.C, V = m_model.V;
         const bool greedy = !temperature.has_value();
-        gcb_gpt_decoder* decoder = nullptr;
-        gcb_check(gcb_gpt_decoder_create(m_ctx, &m_model, &decoder), "decoder");
-        m_decoder.reset(decoder);
+        if (!ruled()) {
+            gcb_gpt_decoder* decoder = nullptr;
+            gcb_check(gcb_gpt_decoder_create(m_ctx, &m_model, &decoder), "decoder");
+            m_decoder.reset(decoder);
+        }
         m_seqs = greedy ? 1 : num_sequences;
         m_cap = std::min(context_length, max_tokens - 1);
         m_cache = Tensor<float>({2 * m_model.L * m_seqs * m_cap * C}, m_device, uninitialized);
@@ -1104,6 +1228,12 @@ template <class Model>
 std::vector<int64_t> generate_tokens_incremental(Model& model, const std::vector<int64_t>& start_tokens, int64_t context_length, int64_t max_tokens, int64_t num_sequences, Device infer_device,
                                                  std::optional<float> temperature = std::nullopt, int64_t top_k = 30) {
     check_generation((int64_t)start_tokens.size(), max_tokens, infer_device);
+    struct Evaluating {  // nothing is dropped while tokens are generated
+        Model& m;
+        bool was;
+        explicit Evaluating(Model& x) : m(x), was(x.is_training()) { if (was) m.eval(); }
+        ~Evaluating() { if (was) m.train(); }
+    } evaluating(model);
     bool here = true;  // a model elsewhere is refused by its own forward
     for (auto* p : model.parameters()) here = here && p->device() == infer_device;
     if (here && num_sequences > 0 && context_length > 0) {

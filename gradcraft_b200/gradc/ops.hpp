@@ -973,6 +973,149 @@ inline Tensor<float> sdpa(Tensor<float> q, Tensor<float> k, Tensor<float> v, boo
     return out;
 }
 
+// ---- attention under a visibility rule, dropout (the reference has the causal form of the one, and the other with a stored mask) ------------
+// What a query sees: itself and the window - 1 positions before it (0: all), and the first `sinks` ones; the first distances of the buckets that a
+// bias table has a column for.
+struct AttentionRule {
+    int64_t window = 0, sinks = 0;
+    std::vector<int64_t> bucket_starts;
+    int64_t buckets() const { return (int64_t)bucket_starts.size(); }
+    bool causal_only() const { return window == 0 && bucket_starts.empty(); }
+    static std::vector<int64_t> relative_buckets(int64_t buckets, int64_t reach) {
+        std::vector<int64_t> s((size_t)std::max<int64_t>(buckets, 0));
+        gcb_check(gcb_relative_bucket_starts(buckets, reach, s.data()), "relative position buckets");
+        return s;
+    }
+};
+
+class WindowAttentionNode : public Node<float> {
+    Tensor<float> m_q, m_k, m_v, m_bias;  // m_bias: (heads, buckets), or empty
+    AttentionRule m_rule;
+    float m_scale;
+    int64_t m_B, m_H, m_T, m_D;
+    Tensor<float> m_stats;
+    std::shared_ptr<Storage<float>> m_out_storage;  // O: the storage object of the tensor this node creates
+
+    struct At { int64_t ld, so, si; };
+    static At at(const Tensor<float>& t) { return {t.strides()[2], t.strides()[0], t.strides()[1]}; }
+    bool biased() const { return m_bias._get_state() != nullptr; }
+
+public:
+    WindowAttentionNode(Tensor<float> q, Tensor<float> k, Tensor<float> v, Tensor<float> bias, AttentionRule rule, float scale)
+        : m_q(std::move(q)), m_k(std::move(k)), m_v(std::move(v)), m_bias(std::move(bias)), m_rule(std::move(rule)), m_scale(scale) {
+        m_B = m_q.shape()[0]; m_H = m_q.shape()[1]; m_T = m_q.shape()[2]; m_D = m_q.shape()[3];
+    }
+    Tensor<float> realize() override {
+        m_q.realize(); m_k.realize(); m_v.realize();
+        if (biased()) m_bias.realize();
+        const At q = at(m_q), k = at(m_k), v = at(m_v);
+        m_stats = Tensor<float>({gcb_attention_stats_floats(m_B, m_H, m_T)}, m_q.device(), uninitialized);
+        Tensor<float> mem({m_B, m_T, m_H, m_D}, m_q.device(), uninitialized);
+        gcb_check(gcb_window_attention_fwd_f32(ctx_of(m_q), m_B, m_H, m_T, m_D, mem.data_ptr(), m_H * m_D, m_T * m_H * m_D, m_D, m_stats.data_ptr(), m_q.data_ptr(), q.ld, q.so, q.si, m_k.data_ptr(), k.ld, k.so, k.si,
+                                               m_v.data_ptr(), v.ld, v.so, v.si, m_scale, m_rule.window, m_rule.sinks, biased() ? m_bias.data_ptr() : nullptr, m_rule.buckets(), m_rule.bucket_starts.data()), "window attention");
+        return Tensor<float>({m_B, m_H, m_T, m_D}, SDPANode::out_strides(m_H, m_T, m_D), 0, mem._get_storage(), false);
+    }
+    void backward(const Tensor<float>& g_in, bool retain_graph) override {
+        Tensor<float> gc = g_in;
+        if (gc.strides()[3] != 1 && m_D != 1) gc = make_contiguous(gc);
+        const At g = at(gc), q = at(m_q), k = at(m_k), v = at(m_v);
+        // one block in the order of the projections' parameters in their arena, so that the projections' backward can take them together
+        const int64_t each = (m_B * m_T * m_H * m_D + 3) / 4 * 4;
+        Tensor<float> block({3 * each}, gc.device(), uninitialized);
+        auto part = [&](int64_t i) { return Tensor<float>({m_B, m_H, m_T, m_D}, SDPANode::out_strides(m_H, m_T, m_D), i * each, block._get_storage(), false); };
+        Tensor<float> dq = part(2), dk = part(1), dv = part(0);
+        float* dbias = nullptr;
+        bool acc = false;
+        if (biased() && m_bias.requires_grad()) { auto [t, a] = m_bias.grad_target(); dbias = t.data_ptr(); acc = a; }
+        gcb_check(gcb_window_attention_bwd_f32(ctx_of(gc), m_B, m_H, m_T, m_D, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), m_H * m_D, m_T * m_H * m_D, m_D, dbias, acc ? 1 : 0, gc.data_ptr(), g.ld, g.so, g.si,
+                                               m_out_storage->data(), m_H * m_D, m_T * m_H * m_D, m_D, m_stats.data_ptr(), m_q.data_ptr(), q.ld, q.so, q.si, m_k.data_ptr(), k.ld, k.so, k.si, m_v.data_ptr(), v.ld, v.so,
+                                               v.si, m_scale, m_rule.window, m_rule.sinks, biased() ? m_bias.data_ptr() : nullptr, m_rule.buckets(), m_rule.bucket_starts.data()), "window attention backward");
+        if (m_v.requires_grad()) push_grad(m_v, dv);
+        if (m_q.requires_grad()) push_grad(m_q, dq);
+        if (m_k.requires_grad()) push_grad(m_k, dk);
+        if (!retain_graph) { m_stats = Tensor<float>(); m_out_storage.reset(); }
+    }
+    std::vector<TensorStateBase*> get_input_states() override {
+        std::vector<TensorStateBase*> s{m_q._get_state_base(), m_k._get_state_base(), m_v._get_state_base()};
+        if (biased()) s.push_back(m_bias._get_state_base());
+        return s;
+    }
+    void set_output_storage(std::shared_ptr<Storage<float>> s) { m_out_storage = std::move(s); }
+};
+
+// Causal attention of (B, H, T, D) operands under `rule`; `bias` (heads, buckets) where the rule has buckets.
+inline Tensor<float> window_attention(Tensor<float> q, Tensor<float> k, Tensor<float> v, AttentionRule rule, std::optional<Tensor<float>> bias = std::nullopt, std::optional<float> scale = std::nullopt) {
+    Device d = infer_assert_device(q, k, v);
+    if (q.shape().size() != 4 || k.shape().size() != 4 || v.shape().size() != 4) throw std::runtime_error("window_attention expects 4D tensors.");
+    if (q.shape() != k.shape() || q.shape() != v.shape()) throw std::runtime_error("window_attention: q, k and v must have the same shape");
+    const int64_t B = q.shape()[0], H = q.shape()[1], T = q.shape()[2], D = q.shape()[3];
+    if (bias.has_value() != (rule.buckets() > 0)) throw std::runtime_error("window_attention: a bias table and buckets go together");
+    if (bias.has_value()) {
+        infer_assert_device(q, *bias);
+        if (bias->shape() != std::vector<int64_t>{H, rule.buckets()} || !bias->is_contiguous()) throw std::runtime_error("window_attention: the bias table must be (heads, buckets) and contiguous");
+    }
+    auto row_major_rows = [](Tensor<float>& t) { if (t.strides()[3] != 1 && t.shape()[3] != 1) t = t.contiguous(); };
+    row_major_rows(q); row_major_rows(k); row_major_rows(v);
+    const float s = scale.value_or(static_cast<float>(1.0 / std::sqrt((double)D)));
+    Tensor<float> out({B, H, T, D}, q.requires_grad() || k.requires_grad() || v.requires_grad() || (bias.has_value() && bias->requires_grad()), lazy, d);
+    out.m_strides = SDPANode::out_strides(H, T, D);
+    auto node = std::make_unique<WindowAttentionNode>(std::move(q), std::move(k), std::move(v), bias.value_or(Tensor<float>()), std::move(rule), s);
+    node->set_output_storage(out._get_storage());
+    out._get_state()->m_creation_op = std::move(node);
+    return out;
+}
+
+// Counters of the generator that dropout masks are drawn from: every call of a layer takes its own stretch, so that (seed, order of calls)
+// fixes all masks.
+struct DropoutCounter {
+    int64_t seed = 0, next = 0;
+    int64_t take(int64_t elements) {
+        const int64_t at = next;
+        next += (elements + 3) / 4;
+        return at;
+    }
+};
+
+class DropoutNode : public Node<float> {
+    Tensor<float> m_x, m_residual;  // m_residual may be empty
+    float m_p;
+    int64_t m_seed, m_offset;
+
+public:
+    DropoutNode(Tensor<float> x, Tensor<float> residual, float p, int64_t seed, int64_t offset) : m_x(std::move(x)), m_residual(std::move(residual)), m_p(p), m_seed(seed), m_offset(offset) {}
+    Tensor<float> realize() override {
+        m_x.realize();
+        Tensor<float> x = make_contiguous(m_x), r, out(m_x.shape(), m_x.device(), uninitialized);
+        if (m_residual._get_state() != nullptr) { m_residual.realize(); r = make_contiguous(m_residual); }
+        gcb_check(gcb_dropout_fwd_f32(ctx_of(out), out.data_ptr(), x.data_ptr(), r._get_state() != nullptr ? r.data_ptr() : nullptr, out.volume(), m_p, m_seed, m_offset), "dropout");
+        return out;
+    }
+    void backward(const Tensor<float>& g, bool) override {
+        Tensor<float> gc = make_contiguous(g);
+        if (m_residual._get_state() != nullptr) push_grad(m_residual, gc);
+        if (!m_x.requires_grad()) return;
+        auto [dx, acc] = m_x.grad_target();
+        gcb_check(gcb_dropout_bwd_f32(ctx_of(gc), dx.data_ptr(), gc.data_ptr(), gc.volume(), m_p, m_seed, m_offset, acc ? 1 : 0), "dropout backward");
+    }
+    std::vector<TensorStateBase*> get_input_states() override {
+        if (m_residual._get_state() != nullptr) return {m_x._get_state_base(), m_residual._get_state_base()};
+        return {m_x._get_state_base()};
+    }
+};
+// residual + dropout(x), or dropout(x): elements are dropped with probability p, the others divided by 1 - p
+inline Tensor<float> dropout(Tensor<float> x, float p, DropoutCounter& counter, std::optional<Tensor<float>> residual = std::nullopt) {
+    if (!(p >= 0.0f && p <= 1.0f)) throw std::runtime_error("dropout: the probability must lie between 0 and 1");
+    Device d = x.device();
+    if (residual.has_value()) {
+        infer_assert_device(x, *residual);
+        if (residual->shape() != x.shape()) throw std::runtime_error("dropout: the residual must have the shape of what is added to it");
+    }
+    Tensor<float> out(x.shape(), x.requires_grad() || (residual.has_value() && residual->requires_grad()), lazy, d);
+    const int64_t at = counter.take(x.volume());
+    out._get_state()->m_creation_op = std::make_unique<DropoutNode>(std::move(x), residual.value_or(Tensor<float>()), p, counter.seed, at);
+    return out;
+}
+
 // ---- embedding ------------------------------------------------------------------------------------------------------
 class EmbedNode : public Node<float> {
     Tensor<int64_t> m_idx;

@@ -21,8 +21,10 @@ def _lib():
         L.gct_last_error.restype = ctypes.c_char_p
         vp, i64, f32, ci = ctypes.c_void_p, ctypes.c_int64, ctypes.c_float, ctypes.c_int
         L.gct_create.argtypes = [ctypes.c_char_p] + [i64] * 6 + [f32] * 8 + [ci, ctypes.POINTER(vp)]
+        L.gct_create_with.argtypes = [ctypes.c_char_p] + [i64] * 6 + [f32] * 8 + [ctypes.POINTER(BlockOptions), ci, ctypes.POINTER(vp)]
+        L.gct_set_dropout_counter.argtypes = [vp, i64]
         L.gct_destroy.argtypes = [vp]
-        for n in ("gct_num_tensors", "gct_num_params", "gct_launch_count", "gct_arena_high_water_bytes", "gct_num_buckets"):
+        for n in ("gct_num_tensors", "gct_num_params", "gct_launch_count", "gct_arena_high_water_bytes", "gct_num_buckets", "gct_dropout_counter"):
             getattr(L, n).argtypes, getattr(L, n).restype = [vp], i64
         L.gct_param_info.argtypes = [vp, i64, ctypes.c_char_p, i64, ctypes.POINTER(i64), ctypes.POINTER(ci)]
         for n in ("gct_set_param", "gct_get_param", "gct_get_grad"):
@@ -42,6 +44,12 @@ def _lib():
     return _LIB
 
 
+class BlockOptions(ctypes.Structure):
+    """gct_block_options: attention over a window with first positions that stay visible, a learned bias by distance bucket, dropout."""
+
+    _fields_ = [(n, ctypes.c_int64) for n in ("window", "sinks", "rel_buckets", "rel_reach", "dropout_seed")] + [("dropout", ctypes.c_float)]
+
+
 class TrainerError(RuntimeError):
     pass
 
@@ -53,11 +61,13 @@ def _ptr(a):
 
 
 class Trainer:
-    def __init__(self, arch, V, T, C, H, L, F, lr=3e-4, beta1=0.9, beta2=0.95, wd=0.1, eps=1e-5, norm_eps=1e-5, ce_eps=1e-5, clip=0.0, device=0):
+    def __init__(self, arch, V, T, C, H, L, F, lr=3e-4, beta1=0.9, beta2=0.95, wd=0.1, eps=1e-5, norm_eps=1e-5, ce_eps=1e-5, clip=0.0, device=0, options=None):
+        """options: what a block has besides plain causal attention, as fields of BlockOptions (window, sinks, rel_buckets, rel_reach, dropout, dropout_seed)."""
         self.L = _lib()
         self.h = ctypes.c_void_p()
         self.shape = dict(arch=arch, V=V, T=T, C=C, H=H, L=L, F=F)
-        self._ok(self.L.gct_create(arch.encode(), V, T, C, H, L, F, lr, beta1, beta2, wd, eps, norm_eps, ce_eps, clip, device, ctypes.byref(self.h)))
+        opt = BlockOptions(**dict(dict(rel_reach=128), **options)) if options else None
+        self._ok(self.L.gct_create_with(arch.encode(), V, T, C, H, L, F, lr, beta1, beta2, wd, eps, norm_eps, ce_eps, clip, opt, device, ctypes.byref(self.h)))
 
     def _ok(self, rc):
         if rc != 0:
@@ -134,6 +144,13 @@ class Trainer:
 
     def load_checkpoint(self, model_path, optim_path):
         self._ok(self.L.gct_load_checkpoint(self.h, str(model_path).encode(), str(optim_path).encode()))
+
+    def dropout_counter(self):
+        """Where the next dropout mask starts; a run that goes on from a checkpoint sets it again for the same masks."""
+        return self.L.gct_dropout_counter(self.h)
+
+    def set_dropout_counter(self, counter):
+        self._ok(self.L.gct_set_dropout_counter(self.h, counter))
 
     def sync(self):
         self._ok(self.L.gct_sync(self.h))

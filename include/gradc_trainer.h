@@ -19,6 +19,19 @@ GCT_API const char* gct_last_error(void);
  * clip <= 0 disables GlobalNormClipper.  Weights start at zero (biases 0, gamma 1); load them with gct_set_param. */
 GCT_API int gct_create(const char* arch, int64_t V, int64_t T, int64_t C, int64_t H, int64_t L, int64_t F, float lr, float beta1, float beta2, float weight_decay, float adam_eps,
                        float norm_eps, float ce_eps, float clip, int device, gct_trainer** out);
+/* The same with options of the blocks: attention over a window of positions (0: all) with `sinks` first ones that stay visible, a learned bias by
+ * distance bucket (rel_buckets columns a head, parameters block_i.attn.rel_bias; 0: none; the last bucket from about rel_reach on), and
+ * dropout on both residual branches while training, with masks from dropout_seed and a counter (gct_dropout_counter).  NULL: none of them.
+ * Ranks of a data-parallel run take a seed each. */
+typedef struct gct_block_options {
+    int64_t window, sinks, rel_buckets, rel_reach, dropout_seed;
+    float dropout;
+} gct_block_options;
+GCT_API int gct_create_with(const char* arch, int64_t V, int64_t T, int64_t C, int64_t H, int64_t L, int64_t F, float lr, float beta1, float beta2, float weight_decay, float adam_eps,
+                            float norm_eps, float ce_eps, float clip, const gct_block_options* options, int device, gct_trainer** out);
+/* The counter that the next dropout mask starts at: a training run that goes on from a checkpoint sets it to what it was for the same masks. */
+GCT_API int64_t gct_dropout_counter(gct_trainer* tr);
+GCT_API int gct_set_dropout_counter(gct_trainer* tr, int64_t counter);
 GCT_API int gct_destroy(gct_trainer* tr);
 GCT_API int64_t gct_num_tensors(gct_trainer* tr);
 GCT_API int64_t gct_num_params(gct_trainer* tr);
