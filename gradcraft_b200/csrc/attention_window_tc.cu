@@ -186,6 +186,7 @@ __device__ __forceinline__ void place_result(uint8_t* tile, int row, int col, ui
 }
 __device__ __forceinline__ float* moved_at(const WindowTc& p, int which, int col, int row) { return p.moved + ((int64_t)blockIdx.x * 2 + which) * 64 * AT_ROWS + (col * AT_ROWS + row * 4); }
 
+__device__ __forceinline__ bool ready_wait(uint32_t bar, uint32_t parity, int* status, int where) { return __all_sync(0xffffffffu, mbar_test(bar, parity) || mbar_wait(bar, parity, status, where)) != 0; }
 // The issuing thread's waits are mostly over before they begin, and it is the one that everybody waits for: a plain test first (dQ 264 -> 247 us, dK and dV 363 -> 345).
 __device__ __forceinline__ bool issuer_wait(uint32_t bar, uint32_t parity, int* status, int where) { return mbar_test(bar, parity) || mbar_wait(bar, parity, status, where); }
 
@@ -320,7 +321,7 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 1) window_attention_tc_fwd_ker
 #pragma unroll
                 for (int kind = 0; kind < 2; ++kind) {
                     const int b = slot(kind, n);
-                    ok = warp_wait(full(b), (n >> 1) & 1u, p.status, 46);
+                    ok = ready_wait(full(b), (n >> 1) & 1u, p.status, 46);
                     if (!ok) break;
                     uint8_t* raw = gen + S::BLOCKS_OFF + b * S::BLOCK;
                     if (kind == 0) win_split<DP, 128, false>(raw, raw + S::RAW, t);
@@ -362,7 +363,7 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 1) window_attention_tc_fwd_ker
             if (!blocks) continue;
             const int r = r0 + row;
             const bool live = r < p.T;
-            bool good = warp_wait(own_full(q), items & 1u, p.status, 49);  // every thread keeps step with the barriers below, whatever a wait says
+            bool good = ready_wait(own_full(q), items & 1u, p.status, 49);  // every thread keeps step with the barriers below, whatever a wait says
             ++items;
             {
                 float x[OC];
@@ -389,7 +390,7 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 1) window_attention_tc_fwd_ker
                 const int b = keys.block(j);
                 float ahead = 0.0f;
                 if (BIAS && j + 1 < blocks) ahead = request(keys.block(j + 1));
-                good = good && warp_wait(s_full(q), s_phase & 1u, p.status, 47);
+                good = good && ready_wait(s_full(q), s_phase & 1u, p.status, 47);
                 ++s_phase;
                 after_sync();
                 if (j > 0 && j % WT_FLUSH == 0) {  // the products of the blocks before came before these scores
@@ -453,7 +454,7 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 1) window_attention_tc_fwd_ker
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_ready(q));
             }
-            good = good && warp_wait(o_full(q), o_phase & 1u, p.status, 48);
+            good = good && ready_wait(o_full(q), o_phase & 1u, p.status, 48);
             ++o_phase;
             after_sync();
             xch[half * 128 + row] = sum;
@@ -633,7 +634,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
             for (int i = 0; i < n && ok; ++i) {
                 const uint32_t at = n0 + i, place = (at & 1u) * T::RAW;
                 // dK of the block before last has read the companions that these replace; its statistics were used before that
-                ok = warp_wait(q_full(at), two(at), p.status, 56) && (at < 2u || warp_wait(dk_done(at - 2u), two(at - 2u), p.status, 56));
+                ok = ready_wait(q_full(at), two(at), p.status, 56) && (at < 2u || ready_wait(dk_done(at - 2u), two(at - 2u), p.status, 56));
                 if (!ok) break;
                 if (t < AT_KEYS) {
                     float* slot = reinterpret_cast<float*>(gen + S::STATS + (at & 1u) * S::STATS_BLOCK) + t;
@@ -647,7 +648,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(q_conv(at));
-                ok = warp_wait(o_full(at), S::O_RAWS == 2 ? two(at) : one(at), p.status, 56) && (at < 1u || warp_wait(dv_done(at - 1u), two(at - 1u), p.status, 56));
+                ok = ready_wait(o_full(at), S::O_RAWS == 2 ? two(at) : one(at), p.status, 56) && (at < 1u || ready_wait(dv_done(at - 1u), two(at - 1u), p.status, 56));
                 if (!ok) break;
                 win_split<DP, 256, false>(gen + S::O_RAW + o_place(at) * T::RAW, gen + S::O_TWIN, t);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -677,7 +678,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
         for (int64_t w = blockIdx.x; w < p.loop_end; w += gridDim.x, ++items) {
             const AttnItem it = attn_item(p, w, true);
             if (it.skip) break;
-            good = good && warp_wait(own_full, items & 1u, p.status, 50);  // every thread keeps step with the barriers of the items, whatever a wait says
+            good = good && ready_wait(own_full, items & 1u, p.status, 50);  // every thread keeps step with the barriers of the items, whatever a wait says
             {
                 float x[OC];
                 own_read(x, own, row, half * OC);
@@ -698,7 +699,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
             for (int i = 0; i < cnt; ++i, ++n) {
                 const float4* mp = reinterpret_cast<const float4*>(gen + S::STATS + (n & 1u) * S::STATS_BLOCK) + 4 * part;
                 const float4 *dp = mp + AT_KEYS / 4, *ip = dp + AT_KEYS / 4;
-                good = good && warp_wait(s_done(n), two(n), p.status, 57);
+                good = good && ready_wait(s_done(n), two(n), p.status, 57);
                 after_sync();
                 if (part >= 2 && i > 0 && i % WT_FLUSH == 0) move(i > WT_FLUSH);  // dV of the blocks before came before these scores
                 uint32_t u[16];
@@ -729,7 +730,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
                 tmem_stores_done();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_ready);
-                good = good && warp_wait(dp_done(n), two(n), p.status, 58);
+                good = good && ready_wait(dp_done(n), two(n), p.status, 58);
                 after_sync();
                 tmem_ld16(lanes + 64 + 16 * part, u);
 #pragma unroll
@@ -745,7 +746,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
                 __syncwarp();
                 if (lane == 0) mbar_arrive(ds_ready);
             }
-            good = good && warp_wait(dk_done(n - 1u), two(n - 1u), p.status, 59);  // the last product of all
+            good = good && ready_wait(dk_done(n - 1u), two(n - 1u), p.status, 59);  // the last product of all
             after_sync();
             const float f = part < 2 ? p.scale : 1.0f;
 #pragma unroll
@@ -892,7 +893,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
             for (int i = 0; i < n && ok; ++i) {
                 const uint32_t at = n0 + i, place = (at & 1u) * T::RAW;
                 // dQ has read the companions that these replace; that block's bias was used before
-                ok = warp_wait(k_full(at), two(at), p.status, 65) && (at < 3u || warp_wait(dq_done(at - 3u), two(at - 3u), p.status, 65));
+                ok = ready_wait(k_full(at), two(at), p.status, 65) && (at < 3u || ready_wait(dq_done(at - 3u), two(at - 3u), p.status, 65));
                 if (!ok) break;
                 if (BIAS) {
                     if (t < WT_TAB) reinterpret_cast<float*>(gen + S::TABS)[at % 3u * WT_TAB + t] = nb;
@@ -902,7 +903,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(k_conv(at));
-                ok = warp_wait(v_full(at), two(at), p.status, 65) && (at < 1u || warp_wait(dp_done(at - 1u), two(at - 1u), p.status, 65));
+                ok = ready_wait(v_full(at), two(at), p.status, 65) && (at < 1u || ready_wait(dp_done(at - 1u), two(at - 1u), p.status, 65));
                 if (!ok) break;
                 win_split<DP, 256, false>(gen + S::V_RAW + place, gen + S::V_TWIN, t);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -956,7 +957,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
             if (lane % LANES == 0)
 #pragma unroll
                 for (int x = 0; x < 8 / STEP; ++x) xch[8 * (warp - 12) + x * STEP + lane / LANES] = a[x];
-            good = good && warp_wait(own_full, items & 1u, p.status, 60);  // every thread keeps step with the barriers of the items, whatever a wait says
+            good = good && ready_wait(own_full, items & 1u, p.status, 60);  // every thread keeps step with the barriers of the items, whatever a wait says
             {
                 float x[OC];
                 own_read(x, own, row, half * OC);
@@ -987,7 +988,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
             for (int i = 0; i < cnt; ++i, ++n) {
                 const uint32_t place = lanes + 128 * (n & 1u);
                 const int b = keys.block(i), j0 = b * AT_KEYS + 16 * part, room = r - j0;
-                good = good && warp_wait(s_done(n), two(n), p.status, 66);
+                good = good && ready_wait(s_done(n), two(n), p.status, 66);
                 after_sync();
                 uint32_t u[16];
                 float pr[16];
@@ -1010,14 +1011,14 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
 #pragma unroll
                     for (int e = 0; e < 16; ++e) pr[e] = keeps(e, room, from, to) ? pr[e] : 0.0f;
                 }
-                good = good && warp_wait(dp_done(n), two(n), p.status, 67);
+                good = good && ready_wait(dp_done(n), two(n), p.status, 67);
                 after_sync();
                 tmem_ld16(place + 64 + 16 * part, u);
 #pragma unroll
                 for (int e = 0; e < 16; ++e) pr[e] *= __uint_as_float(u[e]) - delta;  // a masked P is zero whatever dP holds
                 place_parts16(pr, place + 64 + 16 * part, place + 16 * part, place + 16 * part + 8);
                 if (i > 0 && i % WT_FLUSH == 0) {
-                    good = good && warp_wait(dq_done(n - 1u), two(n - 1u), p.status, 68);
+                    good = good && ready_wait(dq_done(n - 1u), two(n - 1u), p.status, 68);
                     after_sync();
                     if (16 * part < DP) move_sum(lanes + 256 + 16 * part, moved, i > WT_FLUSH, 1.0f);
                 }
@@ -1059,7 +1060,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
                     }
                 }
             }
-            good = good && warp_wait(dq_done(n - 1u), two(n - 1u), p.status, 68);  // the last product of all
+            good = good && ready_wait(dq_done(n - 1u), two(n - 1u), p.status, 68);  // the last product of all
             after_sync();
             if (wants_dbias) {
                 settle();
