@@ -1,5 +1,5 @@
-// Tiles of fp32 FMA attention: 32 rows of a CTA's own against 64 of the other side, 256 threads as 16 x 16, rows of D + 4 floats (D a multiple
-// of four) in shared memory.
+// Tiles of fp32 FMA attention: 16 R rows of a CTA's own (R 2, or 4) against 64 of the other side, 256 threads as 16 x 16, rows of D + 4 floats
+// (D a multiple of four) in shared memory.
 #pragma once
 #include "common.cuh"
 
@@ -43,14 +43,14 @@ __device__ __forceinline__ void as_abt(float (&c)[R][C], const float* a, const f
     }
 }
 // acc[i][4 n + e] += sum_k p[ty + 16 i][k] b[k][64 n + 4 tx + e], k < 64
-template <int NC>
-__device__ __forceinline__ void as_ab(float (&acc)[2][4 * NC], const float* p, const float* b, int D, int ty, int tx) {
+template <int NC, int R>
+__device__ __forceinline__ void as_ab(float (&acc)[R][4 * NC], const float* p, const float* b, int D, int ty, int tx) {
     const int P = D + 4;
 #pragma unroll 4
     for (int k = 0; k < AS_T; k += 4) {
-        float a[2][4];
+        float a[R][4];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) { const float4 x = ld4(p + (ty + 16 * i) * (AS_T + 4) + k); a[i][0] = x.x; a[i][1] = x.y; a[i][2] = x.z; a[i][3] = x.w; }
+        for (int i = 0; i < R; ++i) { const float4 x = ld4(p + (ty + 16 * i) * (AS_T + 4) + k); a[i][0] = x.x; a[i][1] = x.y; a[i][2] = x.z; a[i][3] = x.w; }
 #pragma unroll
         for (int n = 0; n < NC; ++n) {
             const int c = 64 * n + 4 * tx;
@@ -59,7 +59,7 @@ __device__ __forceinline__ void as_ab(float (&acc)[2][4 * NC], const float* p, c
             for (int q = 0; q < 4; ++q) {
                 const float4 y = ld4(b + (k + q) * P + c);
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
+                for (int i = 0; i < R; ++i) {
                     acc[i][4 * n] = fmaf(a[i][q], y.x, acc[i][4 * n]); acc[i][4 * n + 1] = fmaf(a[i][q], y.y, acc[i][4 * n + 1]);
                     acc[i][4 * n + 2] = fmaf(a[i][q], y.z, acc[i][4 * n + 2]); acc[i][4 * n + 3] = fmaf(a[i][q], y.w, acc[i][4 * n + 3]);
                 }
@@ -67,22 +67,27 @@ __device__ __forceinline__ void as_ab(float (&acc)[2][4 * NC], const float* p, c
         }
     }
 }
-// acc[i][4 n + e] += sum_r p[r][2 ty + i] b[r][64 n + 4 tx + e], r < 64
-template <int NC>
-__device__ __forceinline__ void as_atb(float (&acc)[2][4 * NC], const float* p, const float* b, int D, int ty, int tx) {
+// acc[i][4 n + e] += sum_r p[r][R ty + i] b[r][64 n + 4 tx + e], r < 64
+template <int NC, int R>
+__device__ __forceinline__ void as_atb(float (&acc)[R][4 * NC], const float* p, const float* b, int D, int ty, int tx) {
+    static_assert(R == 2 || R == 4, "a thread's rows are one load");
     const int P = D + 4;
 #pragma unroll 8
     for (int r = 0; r < AS_T; ++r) {
-        const float2 a = *reinterpret_cast<const float2*>(p + r * (AS_OWN + 4) + 2 * ty);
+        float a[R];
+        const float* row = p + r * (16 * R + 4) + R * ty;
+        if (R == 2) { const float2 x = *reinterpret_cast<const float2*>(row); a[0] = x.x; a[1] = x.y; }
+        else { const float4 x = ld4(row); a[0] = x.x; a[1] = x.y; a[R - 2] = x.z; a[R - 1] = x.w; }
 #pragma unroll
         for (int n = 0; n < NC; ++n) {
             const int c = 64 * n + 4 * tx;
             if (c >= D) break;
             const float4 y = ld4(b + r * P + c);
-            acc[0][4 * n] = fmaf(a.x, y.x, acc[0][4 * n]); acc[0][4 * n + 1] = fmaf(a.x, y.y, acc[0][4 * n + 1]);
-            acc[0][4 * n + 2] = fmaf(a.x, y.z, acc[0][4 * n + 2]); acc[0][4 * n + 3] = fmaf(a.x, y.w, acc[0][4 * n + 3]);
-            acc[1][4 * n] = fmaf(a.y, y.x, acc[1][4 * n]); acc[1][4 * n + 1] = fmaf(a.y, y.y, acc[1][4 * n + 1]);
-            acc[1][4 * n + 2] = fmaf(a.y, y.z, acc[1][4 * n + 2]); acc[1][4 * n + 3] = fmaf(a.y, y.w, acc[1][4 * n + 3]);
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                acc[i][4 * n] = fmaf(a[i], y.x, acc[i][4 * n]); acc[i][4 * n + 1] = fmaf(a[i], y.y, acc[i][4 * n + 1]);
+                acc[i][4 * n + 2] = fmaf(a[i], y.z, acc[i][4 * n + 2]); acc[i][4 * n + 3] = fmaf(a[i], y.w, acc[i][4 * n + 3]);
+            }
         }
     }
 }

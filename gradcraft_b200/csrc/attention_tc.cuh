@@ -234,7 +234,8 @@ static bool encode_rows(TmaEncodeFn enc, CUtensorMap* map, const float* ptr, int
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 static bool rows_ok(const float* p, int64_t ld, int64_t so, int64_t si, int64_t B, int64_t H) {
-    return p && aligned16(p) && ld > 0 && ld % 4 == 0 && (H == 1 || (si > 0 && si % 4 == 0)) && (B == 1 || (so > 0 && so % 4 == 0));
+    constexpr int64_t reach = int64_t(1) << 38;  // a tensor map's strides stay below 2^40 bytes
+    return p && aligned16(p) && ld > 0 && ld < reach && ld % 4 == 0 && (H == 1 || (si > 0 && si < reach && si % 4 == 0)) && (B == 1 || (so > 0 && so < reach && so % 4 == 0));
 }
 static size_t span_bytes(int64_t B, int64_t H, int64_t T, int64_t D, int64_t ld, int64_t so, int64_t si) { return sizeof(float) * (size_t)((B - 1) * so + (H - 1) * si + (T - 1) * ld + D); }
 static int64_t padded(int64_t T) { return (T + AT_ROWS - 1) / AT_ROWS * AT_ROWS; }

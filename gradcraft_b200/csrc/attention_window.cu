@@ -13,9 +13,9 @@
 namespace gcb {
 
 // ---- fp32 FMA kernels ----------------------------------------------------------------------------------------------------------
-// A CTA owns 32 queries (forward, dQ) or 32 keys (dK, dV) of a head and walks over tiles of 64 of the other side, skipping those that the
-// rule hides as a whole.  The bias of a tile is looked up once per distance (95 of them) and read from shared memory.
-constexpr int AW_DIAG = AS_OWN + AS_T - 1;
+// A CTA owns 16 R queries (forward, dQ) or keys (dK, dV) of a head, R 2 or 4, and walks over tiles of 64 of the other side, skipping those that the
+// rule hides as a whole.  The bias of a tile is looked up once per distance and read from shared memory.
+__host__ __device__ constexpr int aw_diag(int R) { return 16 * R + AS_T - 1; }
 
 // ROWS rows of D columns from row r0 into [row][Dp + 4], zero beyond T and D.  VEC: rows start on 16 bytes and D is a multiple of four.
 template <int ROWS, bool VEC>
@@ -39,39 +39,43 @@ __device__ __forceinline__ void aw_st4(float* p, int c, int D, float4 x) {
     if (c + 2 < D) p[c + 2] = x.z;
     if (c + 3 < D) p[c + 3] = x.w;
 }
-// bias of the distances d0 .. d0 + 94 of a tile
+// bias of a tile's distances, the first of which is d0
+template <int R>
 __device__ __forceinline__ void aw_tab(float* sm, const WindowAttn& p, int64_t h, int d0) {
-    if (p.tab != nullptr && threadIdx.x < AW_DIAG) sm[threadIdx.x] = p.tab[h * p.tab_len + clamp_distance(d0 + (int)threadIdx.x, p.tab_len)];
+    if (p.tab != nullptr && threadIdx.x < aw_diag(R)) sm[threadIdx.x] = p.tab[h * p.tab_len + clamp_distance(d0 + (int)threadIdx.x, p.tab_len)];
 }
-// the tile of keys after k0 that queries q0 .. q0 + 31 look at
+// the tile of keys after k0 that the queries from q0 on look at
 __device__ __forceinline__ int aw_first_tile(const WindowRule& r, int q0) { return r.S > 0 ? 0 : r.window_first(q0) / AS_T * AS_T; }
 __device__ __forceinline__ int aw_next_tile(const WindowRule& r, int q0, int k0) {
     const int k1 = k0 + AS_T, lo = r.window_first(q0) / AS_T * AS_T;
     return k1 >= r.S && k1 < lo ? lo : k1;
 }
-static size_t aw_floats(int own, int other, int blocks, int64_t Dp) { return (size_t)(own * AS_OWN + other * AS_T) * (Dp + 4) + (size_t)blocks * AS_T * (AS_OWN + 4) + 2 * (AW_DIAG + 1); }
+static size_t aw_floats(int R, int own, int other, int blocks, int64_t Dp) { return (size_t)(own * 16 * R + other * AS_T) * (Dp + 4) + (size_t)blocks * AS_T * (16 * R + 4) + 2 * (aw_diag(R) + 1); }
 
-template <int NC, bool VEC>
+template <int R, int NC, bool VEC>
 __global__ void __launch_bounds__(256) window_attention_fwd_kernel(const __grid_constant__ WindowAttn p) {
+    constexpr int OWN = 16 * R;
     extern __shared__ __align__(16) float aw_sm[];
     pdl_trigger();
     pdl_wait();
-    const int D = p.D, Dp = (D + 3) / 4 * 4, tx = threadIdx.x & 15, ty = threadIdx.x >> 4, head = blockIdx.x / p.tiles, q0 = (blockIdx.x - head * p.tiles) * AS_OWN, last = min(q0 + AS_OWN, p.T);
+    const int D = p.D, Dp = (D + 3) / 4 * 4, tx = threadIdx.x & 15, ty = threadIdx.x >> 4, head = blockIdx.x / p.tiles, q0 = (blockIdx.x - head * p.tiles) * OWN, last = min(q0 + OWN, p.T);
     const int64_t b = head / p.H, h = head - b * p.H;
-    float *sq = aw_sm, *sk = sq + AS_OWN * (Dp + 4), *sv = sk + AS_T * (Dp + 4), *sp = sv + AS_T * (Dp + 4), *tab = sp + AS_T * (AS_OWN + 4);
+    float *sq = aw_sm, *sk = sq + OWN * (Dp + 4), *sv = sk + AS_T * (Dp + 4), *sp = sv + AS_T * (Dp + 4), *tab = sp + AS_T * (OWN + 4);
     const float *k = p.k + b * p.k_so + h * p.k_si, *v = p.v + b * p.v_so + h * p.v_si;
-    aw_load<AS_OWN, VEC>(sq, p.q + b * p.q_so + h * p.q_si, p.q_ld, q0, p.T, D, Dp);
-    float acc[2][4 * NC] = {}, m[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+    aw_load<OWN, VEC>(sq, p.q + b * p.q_so + h * p.q_si, p.q_ld, q0, p.T, D, Dp);
+    float acc[R][4 * NC] = {}, m[R], sum[R] = {};
+#pragma unroll
+    for (int i = 0; i < R; ++i) m[i] = -INFINITY;
     for (int k0 = aw_first_tile(p.rule, q0); k0 < last; k0 = aw_next_tile(p.rule, q0, k0)) {
         __syncthreads();
         aw_load<AS_T, VEC>(sk, k, p.k_ld, k0, p.T, D, Dp);
         aw_load<AS_T, VEC>(sv, v, p.v_ld, k0, p.T, D, Dp);
-        aw_tab(tab, p, h, q0 - k0 - (AS_T - 1));
+        aw_tab<R>(tab, p, h, q0 - k0 - (AS_T - 1));
         as_landed();
-        float s[2][4];
+        float s[R][4];
         as_abt(s, sq, sk, Dp, ty, tx);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < R; ++i) {
             const int row = q0 + ty + 16 * i;
             float mx = m[i];
 #pragma unroll
@@ -95,7 +99,7 @@ __global__ void __launch_bounds__(256) window_attention_fwd_kernel(const __grid_
     }
     float* out = p.out + b * p.o_so + h * p.o_si;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < R; ++i) {
         const int row = q0 + ty + 16 * i;
         if (row >= p.T) continue;
         const bool empty = m[i] == -INFINITY;
@@ -138,42 +142,40 @@ struct AwRows {
     }
 };
 
-// dQ of 32 queries; with a bias table also its gradient over them: thread n < buckets keeps bucket n, dbias_part is [head][tile][buckets].
+// dQ of 16 R queries; with a bias table also its gradient over them: thread n < buckets keeps bucket n, dbias_part is [head][tile][buckets].
 // Sums of a bucket go along the tile's diagonals, in a fixed order.
-template <int NC, bool VEC>
-__global__ void __launch_bounds__(256) window_attention_dq_kernel(const __grid_constant__ WindowAttn p) {
-    extern __shared__ __align__(16) float aw_sm[];
-    pdl_trigger();
-    pdl_wait();
-    const int D = p.D, Dp = (D + 3) / 4 * 4, tx = threadIdx.x & 15, ty = threadIdx.x >> 4, head = blockIdx.x / p.tiles, tile = blockIdx.x - head * p.tiles, q0 = tile * AS_OWN;
+template <int R, int NC, bool VEC>
+__device__ __forceinline__ void aw_dq(const WindowAttn& p, float* aw_sm, int item) {
+    constexpr int OWN = 16 * R;
+    const int D = p.D, Dp = (D + 3) / 4 * 4, tx = threadIdx.x & 15, ty = threadIdx.x >> 4, head = item / p.tiles, tile = item - head * p.tiles, q0 = tile * OWN;
     const int64_t b = head / p.H, h = head - b * p.H;
-    float *s0 = aw_sm, *s1 = s0 + AS_OWN * (Dp + 4), *s2 = s1 + AS_OWN * (Dp + 4), *s3 = s2 + AS_T * (Dp + 4), *ss = s3 + AS_T * (Dp + 4), *tab = ss + AS_T * (AS_OWN + 4), *diag = tab + AW_DIAG + 1;
+    float *s0 = aw_sm, *s1 = s0 + OWN * (Dp + 4), *s2 = s1 + OWN * (Dp + 4), *s3 = s2 + AS_T * (Dp + 4), *ss = s3 + AS_T * (Dp + 4), *tab = ss + AS_T * (OWN + 4), *diag = tab + aw_diag(R) + 1;
     const float *k = p.k + b * p.k_so + h * p.k_si, *v = p.v + b * p.v_so + h * p.v_si;
-    float dq[2][4 * NC] = {}, db = 0.0f;
-    AwRows<2, NC, VEC> rows;
-    aw_load<AS_OWN, VEC>(s0, p.q + b * p.q_so + h * p.q_si, p.q_ld, q0, p.T, D, Dp);
-    aw_load<AS_OWN, VEC>(s1, p.g + b * p.g_so + h * p.g_si, p.g_ld, q0, p.T, D, Dp);
+    float dq[R][4 * NC] = {}, db = 0.0f;
+    AwRows<R, NC, VEC> rows;
+    aw_load<OWN, VEC>(s0, p.q + b * p.q_so + h * p.q_si, p.q_ld, q0, p.T, D, Dp);
+    aw_load<OWN, VEC>(s1, p.g + b * p.g_so + h * p.g_si, p.g_ld, q0, p.T, D, Dp);
     rows.request(p, head, p.o + b * p.o_so + h * p.o_si, q0, ty, tx);
     bool first = true;
-    for (int k0 = aw_first_tile(p.rule, q0); k0 < min(q0 + AS_OWN, p.T); k0 = aw_next_tile(p.rule, q0, k0)) {
+    for (int k0 = aw_first_tile(p.rule, q0); k0 < min(q0 + OWN, p.T); k0 = aw_next_tile(p.rule, q0, k0)) {
         const int d0 = q0 - k0 - (AS_T - 1);
         __syncthreads();
         aw_load<AS_T, VEC>(s2, k, p.k_ld, k0, p.T, D, Dp);
         aw_load<AS_T, VEC>(s3, v, p.v_ld, k0, p.T, D, Dp);
-        aw_tab(tab, p, h, d0);
+        aw_tab<R>(tab, p, h, d0);
         as_landed();
         if (first) {
             rows.finish(s1, Dp, ty, tx);
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < R; ++i)
                 if (tx == 0 && q0 + ty + 16 * i < p.T) p.delta[head * p.Tp + q0 + ty + 16 * i] = rows.delta[i];
         }
         first = false;
-        float s[2][4], dp[2][4];
+        float s[R][4], dp[R][4];
         as_abt(s, s0, s2, Dp, ty, tx);
         as_abt(dp, s1, s3, Dp, ty, tx);
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < R; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const int r = ty + 16 * i, c = tx + 16 * j;
@@ -185,22 +187,22 @@ __global__ void __launch_bounds__(256) window_attention_dq_kernel(const __grid_c
         as_ab<NC>(dq, ss, s2, Dp, ty, tx);
         if (p.dbias_part) {
             const int t = threadIdx.x;
-            if (t < AW_DIAG) {
+            if (t < aw_diag(R)) {
                 float a = 0.0f;
-                for (int r = max(0, t - (AS_T - 1)); r <= min(AS_OWN - 1, t); ++r) a += ss[r * (AS_T + 4) + r - t + AS_T - 1];
+                for (int r = max(0, t - (AS_T - 1)); r <= min(OWN - 1, t); ++r) a += ss[r * (AS_T + 4) + r - t + AS_T - 1];
                 diag[t] = a;
             }
             __syncthreads();
             if (t < p.rule.buckets) {
-                const int end = t + 1 < p.rule.buckets ? p.rule.starts[t + 1] - d0 : AW_DIAG;
+                const int end = t + 1 < p.rule.buckets ? p.rule.starts[t + 1] - d0 : aw_diag(R);
                 float a = 0.0f;
-                for (int i = max(0, p.rule.starts[t] - d0); i < min(end, AW_DIAG); ++i) a += diag[i];
+                for (int i = max(0, p.rule.starts[t] - d0); i < min(end, aw_diag(R)); ++i) a += diag[i];
                 db += a;
             }
         }
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < R; ++i) {
         const int r = q0 + ty + 16 * i;
         if (r >= p.T) continue;
 #pragma unroll
@@ -208,56 +210,54 @@ __global__ void __launch_bounds__(256) window_attention_dq_kernel(const __grid_c
             aw_st4<VEC>(p.dq + b * p.d_so + h * p.d_si + r * p.d_ld, 64 * n + 4 * tx, D,
                         make_float4(p.scale * dq[i][4 * n], p.scale * dq[i][4 * n + 1], p.scale * dq[i][4 * n + 2], p.scale * dq[i][4 * n + 3]));
     }
-    if (p.dbias_part && threadIdx.x < p.rule.buckets) p.dbias_part[(int64_t)blockIdx.x * p.rule.buckets + threadIdx.x] = db;
+    if (p.dbias_part && threadIdx.x < p.rule.buckets) p.dbias_part[(int64_t)item * p.rule.buckets + threadIdx.x] = db;
 }
 
-// dK and dV of 32 keys from the queries that see them through the window.
-template <int NC, bool VEC>
-__global__ void __launch_bounds__(256) window_attention_dkv_kernel(const __grid_constant__ WindowAttn p) {
-    extern __shared__ __align__(16) float aw_sm[];
-    pdl_trigger();
-    pdl_wait();
-    const int D = p.D, Dp = (D + 3) / 4 * 4, tx = threadIdx.x & 15, ty = threadIdx.x >> 4, head = blockIdx.x / p.tiles, t0 = (blockIdx.x - head * p.tiles) * AS_OWN;
+// dK and dV of 16 R keys from the queries that see them through the window, and with far_inside from those beyond that still see the first keys.
+template <int R, int NC, bool VEC>
+__device__ __forceinline__ void aw_dkv(const WindowAttn& p, float* aw_sm, int item) {
+    constexpr int OWN = 16 * R;
+    const int D = p.D, Dp = (D + 3) / 4 * 4, tx = threadIdx.x & 15, ty = threadIdx.x >> 4, head = item / p.tiles, t0 = (item - head * p.tiles) * OWN;
     const int64_t b = head / p.H, h = head - b * p.H;
-    float *s0 = aw_sm, *s1 = s0 + AS_OWN * (Dp + 4), *s2 = s1 + AS_OWN * (Dp + 4), *s3 = s2 + AS_T * (Dp + 4), *sp = s3 + AS_T * (Dp + 4), *ss = sp + AS_T * (AS_OWN + 4), *tab = ss + AS_T * (AS_OWN + 4);
+    float *s0 = aw_sm, *s1 = s0 + OWN * (Dp + 4), *s2 = s1 + OWN * (Dp + 4), *s3 = s2 + AS_T * (Dp + 4), *sp = s3 + AS_T * (Dp + 4), *ss = sp + AS_T * (OWN + 4), *tab = ss + AS_T * (OWN + 4);
     const float *q = p.q + b * p.q_so + h * p.q_si, *g = p.g + b * p.g_so + h * p.g_si, *o = p.o + b * p.o_so + h * p.o_si;
-    float dk[2][4 * NC] = {}, dv[2][4 * NC] = {};
-    aw_load<AS_OWN, VEC>(s0, p.k + b * p.k_so + h * p.k_si, p.k_ld, t0, p.T, D, Dp);
-    aw_load<AS_OWN, VEC>(s1, p.v + b * p.v_so + h * p.v_si, p.v_ld, t0, p.T, D, Dp);
-    const int W = p.rule.W, keys_end = min(t0 + AS_OWN, p.T);
-    const int r_end = W > 0 && W < p.T - keys_end ? keys_end - 1 + W : p.T;
+    float dk[R][4 * NC] = {}, dv[R][4 * NC] = {};
+    aw_load<OWN, VEC>(s0, p.k + b * p.k_so + h * p.k_si, p.k_ld, t0, p.T, D, Dp);
+    aw_load<OWN, VEC>(s1, p.v + b * p.v_so + h * p.v_si, p.v_ld, t0, p.T, D, Dp);
+    const int W = p.rule.W, keys_end = min(t0 + OWN, p.T), always = p.far_inside ? p.rule.S : 0;
+    const int r_end = t0 >= always && W > 0 && W < p.T - keys_end ? keys_end - 1 + W : p.T;
     for (int r0 = t0 / AS_T * AS_T; r0 < r_end; r0 += AS_T) {
         __syncthreads();
         AwRows<4, NC, VEC> rows;
         aw_load<AS_T, VEC>(s2, q, p.q_ld, r0, p.T, D, Dp);
         aw_load<AS_T, VEC>(s3, g, p.g_ld, r0, p.T, D, Dp);
-        aw_tab(tab, p, h, r0 - t0 - (AS_OWN - 1));
+        aw_tab<R>(tab, p, h, r0 - t0 - (OWN - 1));
         rows.request(p, head, o, r0, ty, tx);
         as_landed();
         rows.finish(s3, Dp, ty, tx);
-        float s[4][2], dp[4][2];
+        float s[4][R], dp[4][R];
         as_abt(s, s2, s0, Dp, ty, tx);
         as_abt(dp, s3, s1, Dp, ty, tx);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
+            for (int j = 0; j < R; ++j) {
                 const int r = ty + 16 * i, c = tx + 16 * j, d = r0 + r - (t0 + c);
-                const float z = p.tab ? fmaf(s[i][j], p.scale, tab[r - c + AS_OWN - 1]) : s[i][j] * p.scale;
-                const bool seen = d >= 0 && (W == 0 || d < W);
+                const float z = p.tab ? fmaf(s[i][j], p.scale, tab[r - c + OWN - 1]) : s[i][j] * p.scale;
+                const bool seen = d >= 0 && (W == 0 || d < W || t0 + c < always);
                 const float pr = seen ? __expf(z - rows.m[i]) * rows.inv[i] : 0.0f;
-                sp[r * (AS_OWN + 4) + c] = pr;
-                ss[r * (AS_OWN + 4) + c] = pr * (dp[i][j] - rows.delta[i]);
+                sp[r * (OWN + 4) + c] = pr;
+                ss[r * (OWN + 4) + c] = pr * (dp[i][j] - rows.delta[i]);
             }
         __syncthreads();
         as_atb<NC>(dv, sp, s3, Dp, ty, tx);
         as_atb<NC>(dk, ss, s2, Dp, ty, tx);
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < R; ++i)
 #pragma unroll
         for (int n = 0; n < NC; ++n) {
-            const int c = 64 * n + 4 * tx, r = t0 + 2 * ty + i;
+            const int c = 64 * n + 4 * tx, r = t0 + R * ty + i;
             const float4 a = make_float4(p.scale * dk[i][4 * n], p.scale * dk[i][4 * n + 1], p.scale * dk[i][4 * n + 2], p.scale * dk[i][4 * n + 3]);
             const float4 e = make_float4(dv[i][4 * n], dv[i][4 * n + 1], dv[i][4 * n + 2], dv[i][4 * n + 3]);
             if (r < p.T) {
@@ -266,6 +266,16 @@ __global__ void __launch_bounds__(256) window_attention_dkv_kernel(const __grid_
                 aw_st4<VEC>(p.dv + at, c, D, e);
             }
         }
+}
+// One launch for both sides: they share nothing that one would have to wait for, since each takes dO . O for itself.  The CTAs of dK and dV come first:
+// theirs is the longer work.
+template <int R, int NC, bool VEC>
+__global__ void __launch_bounds__(256) window_attention_bwd_kernel(const __grid_constant__ WindowAttn p, int items) {
+    extern __shared__ __align__(16) float aw_sm[];
+    pdl_trigger();
+    pdl_wait();
+    if (blockIdx.x < items) aw_dkv<R, NC, VEC>(p, aw_sm, blockIdx.x);
+    else aw_dq<R, NC, VEC>(p, aw_sm, blockIdx.x - items);
 }
 // What the queries beyond the window, which see the first S keys alone, add to those keys' gradients.  Tiles of keys would spend most of their work on
 // keys that are not seen: here four keys lie in registers, a column quadruple a lane, and a warp passes over the rows of q and dO, 32 / LPR at a time.
@@ -748,27 +758,32 @@ static bool own_rows(int64_t B, int64_t H, int64_t T, int64_t D, int64_t ld, int
 constexpr int64_t ST_STREAM = int64_t(1) << 22;
 constexpr int64_t AW_MAX_T = int64_t(1) << 24, AW_MAX_D = 128, AW_MAX_H = 65535;
 
-template <class K>
-static int fma_launch(gcb_ctx* ctx, K kernel, bool* done, int64_t ctas, size_t floats, const WindowAttn& p) {
+template <class K, class... A>
+static int fma_launch(gcb_ctx* ctx, K kernel, bool* done, int64_t ctas, size_t floats, const char* name, const WindowAttn& p, A... more) {
     GCB_REQUIRE(ctas < (int64_t(1) << 31), "window attention: more tiles than a grid holds");
     if (!done[ctx->device]) { GCB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448 - 1024)); done[ctx->device] = true; }
-    GCB_CHECK_CUDA(launch_next(ctx->stream, dim3((unsigned)ctas), 256, sizeof(float) * floats, kernel, p));
-    return GCB_OK;
+    GCB_CHECK_CUDA(launch_next(ctx->stream, dim3((unsigned)ctas), 256, sizeof(float) * floats, kernel, p, more...));
+    return after_launch(ctx, name);
 }
-template <int NC, bool VEC>
+template <int R, int NC, bool VEC>
 static int fma_fwd(gcb_ctx* ctx, int64_t heads, const WindowAttn& p) {
     static bool done[kMaxDevices] = {};
-    const int rc = fma_launch(ctx, window_attention_fwd_kernel<NC, VEC>, done, heads * p.tiles, aw_floats(1, 2, 1, (p.D + 3) / 4 * 4), p);
-    return rc ? rc : after_launch(ctx, "window_attention_fwd");
+    return fma_launch(ctx, window_attention_fwd_kernel<R, NC, VEC>, done, heads * p.tiles, aw_floats(R, 1, 2, 1, (p.D + 3) / 4 * 4), "window_attention_fwd", p);
 }
-template <int NC, bool VEC>
+template <int R, int NC, bool VEC>
 static int fma_bwd(gcb_ctx* ctx, int64_t heads, const WindowAttn& p) {
-    static bool done_q[kMaxDevices] = {}, done_kv[kMaxDevices] = {};
-    const int64_t Dp = (p.D + 3) / 4 * 4;
-    int rc = fma_launch(ctx, window_attention_dq_kernel<NC, VEC>, done_q, heads * p.tiles, aw_floats(2, 2, 1, Dp), p);
-    if (!rc) rc = after_launch(ctx, "window_attention_dq");
-    if (!rc) rc = fma_launch(ctx, window_attention_dkv_kernel<NC, VEC>, done_kv, heads * p.tiles, aw_floats(2, 2, 2, Dp), p);
-    return rc ? rc : after_launch(ctx, "window_attention_dkv");
+    static bool done[kMaxDevices] = {};
+    return fma_launch(ctx, window_attention_bwd_kernel<R, NC, VEC>, done, 2 * heads * p.tiles, aw_floats(R, 2, 2, 2, (p.D + 3) / 4 * 4), "window_attention_bwd", p, (int)(heads * p.tiles));
+}
+// R, with 16 R rows of a CTA's own: 64 rows take 8 reads of shared memory for 64 FMAs where 32 rows take 6 for 32, and it is those reads that bound the kernels;
+// 32 rows where 64 would leave a quarter of the SMs idle.  Either, us, forward and backward: 16 x 16 x 1024 x 128 with a window of 256 1859 and 7645 with 32,
+// 1696 and 5537 with 64; 4 x 8 x 256 x 128 55 and 158, 47 and 132; 4 x 4 x 256 x 128 42 and 97, 47 and 108; 1 x 4 x 256 x 128 35 and 72, 47 and 108.  Twice the
+// threads for 64 rows, which leaves the reads as they are, took 1908 and 6028 in the first of these.
+static int fma_rows(int64_t heads, int64_t T) { return T > 32 && 4 * heads * ((T + 63) / 64) >= 3 * kSMs ? 4 : 2; }
+template <int R>
+static int fma_run(gcb_ctx* ctx, int64_t heads, const WindowAttn& p, bool vec) {
+    if (p.dq) return p.D <= 64 ? (vec ? fma_bwd<R, 1, true>(ctx, heads, p) : fma_bwd<R, 1, false>(ctx, heads, p)) : (vec ? fma_bwd<R, 2, true>(ctx, heads, p) : fma_bwd<R, 2, false>(ctx, heads, p));
+    return p.D <= 64 ? (vec ? fma_fwd<R, 1, true>(ctx, heads, p) : fma_fwd<R, 1, false>(ctx, heads, p)) : (vec ? fma_fwd<R, 2, true>(ctx, heads, p) : fma_fwd<R, 2, false>(ctx, heads, p));
 }
 // What queries beyond the window add to the first keys' gradients; after dK and dV have been written, and delta.
 static int far_gradients(gcb_ctx* ctx, int64_t heads, WindowAttn& p, bool vec, Scratch& mem) {
@@ -888,12 +903,13 @@ int gcb_window_attention_fwd_f32(gcb_ctx* ctx, int64_t B, int64_t H, int64_t T, 
     p.out = out; p.o_ld = o_ld; p.o_so = o_so; p.o_si = o_si;
     p.Tp = gcb_attention_stats_floats(1, 1, T) / 2; p.T = (int)T; p.D = (int)D; p.H = (int)H; p.scale = scale;
     p.row_max = stats; p.row_inv = stats + B * H * p.Tp;
-    p.tiles = (int)((T + AS_OWN - 1) / AS_OWN);
+    const int R = fma_rows(B * H, T);
+    p.tiles = (int)((T + 16 * R - 1) / (16 * R));
     const bool vec = D % 4 == 0 && vec_rows(q, q_ld, q_so, q_si) && vec_rows(k, k_ld, k_so, k_si) && vec_rows(v, v_ld, v_so, v_si) && vec_rows(out, o_ld, o_so, o_si);
     Scratch tab(ctx);
     if ((rc = make_table(ctx, p, tab))) return rc;
     if (window_tc_takes(ctx, B, p)) rc = window_tc_fwd(ctx, B, p);
-    else rc = D <= 64 ? (vec ? fma_fwd<1, true>(ctx, B * H, p) : fma_fwd<1, false>(ctx, B * H, p)) : (vec ? fma_fwd<2, true>(ctx, B * H, p) : fma_fwd<2, false>(ctx, B * H, p));
+    else rc = R == 4 ? fma_run<4>(ctx, B * H, p, vec) : fma_run<2>(ctx, B * H, p, vec);
     if (rc) return rc;
     note_write(ctx, out, span_bytes(B, H, T, D, o_ld, o_so, o_si));
     return GCB_OK;
@@ -920,7 +936,8 @@ int gcb_window_attention_bwd_f32(gcb_ctx* ctx, int64_t B, int64_t H, int64_t T, 
     p.dq = dq; p.dk = dk; p.dv = dv; p.d_ld = d_ld; p.d_so = d_so; p.d_si = d_si;
     p.Tp = gcb_attention_stats_floats(1, 1, T) / 2; p.T = (int)T; p.D = (int)D; p.H = (int)H; p.scale = scale;
     p.row_max = const_cast<float*>(stats); p.row_inv = p.row_max + B * H * p.Tp;
-    p.tiles = (int)((T + AS_OWN - 1) / AS_OWN);
+    const int R = fma_rows(B * H, T);
+    p.tiles = (int)((T + 16 * R - 1) / (16 * R));
     const int64_t heads = B * H;
     const bool vec = D % 4 == 0 && vec_rows(q, q_ld, q_so, q_si) && vec_rows(k, k_ld, k_so, k_si) && vec_rows(v, v_ld, v_so, v_si) && vec_rows(dout, g_ld, g_so, g_si) && vec_rows(out, o_ld, o_so, o_si) &&
                      vec_rows(dq, d_ld, d_so, d_si) && vec_rows(dk, d_ld, d_so, d_si) && vec_rows(dv, d_ld, d_so, d_si);
@@ -933,10 +950,13 @@ int gcb_window_attention_bwd_f32(gcb_ctx* ctx, int64_t B, int64_t H, int64_t T, 
         if ((rc = part.get(sizeof(float) * (size_t)(heads * tiles * buckets)))) return rc;
         p.dbias_part = part.as<float>();
     }
+    // Few queries beyond the window: the tiles of the first keys go on to the last query, which saves two launches (4 x 4 x 64 13.2 us, 18.4 with them;
+    // 5 x 6 x 331, window 100, 134.8 and 135.6; 8 x 8 x 200, window 30, 121.7 and 116.8; 2 x 4 x 512, window 64, 90.6 and 54.2).
+    p.far_inside = !tc && T - p.rule.W <= 128;
     if (tc) rc = window_tc_bwd(ctx, B, p);
-    else rc = D <= 64 ? (vec ? fma_bwd<1, true>(ctx, heads, p) : fma_bwd<1, false>(ctx, heads, p)) : (vec ? fma_bwd<2, true>(ctx, heads, p) : fma_bwd<2, false>(ctx, heads, p));
+    else rc = R == 4 ? fma_run<4>(ctx, heads, p, vec) : fma_run<2>(ctx, heads, p, vec);
     if (rc) return rc;
-    if (p.rule.S > 0 && p.rule.W < T && (rc = far_gradients(ctx, heads, p, vec, far))) return rc;  // some query looks past its window
+    if (p.rule.S > 0 && p.rule.W < T && !p.far_inside && (rc = far_gradients(ctx, heads, p, vec, far))) return rc;  // some query looks past its window
     for (float* d : {dq, dk, dv}) note_write(ctx, d, span_bytes(B, H, T, D, d_ld, d_so, d_si));
     if (dbias) {
         GCB_CHECK_CUDA(launch_next(ctx->stream, dim3((unsigned)((H * buckets + 7) / 8)), 256, 0, window_attention_dbias_kernel, dbias, part.as<float>(), (int)H, (int)B, tiles, (int)buckets, accumulate_dbias));

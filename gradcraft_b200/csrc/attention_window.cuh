@@ -52,7 +52,7 @@ struct WindowAttn {
     float* delta;                                   // backward: dO . O per query, Tp a head, written with dQ
     const float* tab;                               // [H][tab_len]: bias by distance, the last one for all distances beyond; NULL: no bias
     int64_t q_ld, q_so, q_si, k_ld, k_so, k_si, v_ld, v_so, v_si, g_ld, g_so, g_si, o_ld, o_so, o_si, d_ld, d_so, d_si, Tp;
-    int T, D, H, tiles, tab_len, far_chunks, far_rows;
+    int T, D, H, tiles, tab_len, far_chunks, far_rows, far_inside;
     float scale;
     WindowRule rule;
 };

@@ -135,6 +135,45 @@ def test_forward_and_gradients(env, size, engine):
         ctx.ctx_set_gemm_engine(0)
 
 
+@pytest.mark.parametrize("size", [s for s in SIZES if s[2] <= 64], ids=lambda s: "x".join(map(str, s)))
+def test_short_sequences_on_the_tensor_cores(env, size):
+    """Where the choice between the kernels goes the other way by itself."""
+    ctx, torch, capi = env
+    B, H, T, D, window, sinks, buckets, reach = size
+    ctx.ctx_set_gemm_engine(2)
+    try:
+        before = ctx.ctx_launch_count_named(b"window_attention_tc")
+        Case(torch, B, H, T, D, buckets, reach).check(ctx, window, sinks, D**-0.5)
+        assert ctx.ctx_launch_count_named(b"window_attention_tc") == before + 3
+    finally:
+        ctx.ctx_set_gemm_engine(0)
+
+
+@pytest.mark.parametrize("D", [40, 33, 128])
+@pytest.mark.parametrize("T, window, sinks, buckets", [(65, 20, 3, 8), (64, 0, 0, 0), (300, 100, 5, 32), (129, 1, 1, 0)])
+def test_enough_heads_for_tiles_of_64_rows(env, T, window, sinks, buckets, D):
+    ctx, torch, capi = env
+    ctx.ctx_set_gemm_engine(1)
+    try:
+        Case(torch, 8, 14, T, D, buckets, 64).check(ctx, window, sinks, D**-0.5)
+    finally:
+        ctx.ctx_set_gemm_engine(0)
+
+
+@pytest.mark.parametrize("engine", [0, 2])
+def test_one_position_with_a_stride_that_no_tensor_map_holds(env, engine):
+    ctx, torch, capi = env
+    ctx.ctx_set_gemm_engine(engine)
+    try:
+        c = Case(torch, 1, 3, 1, 16)
+        for name in c.dev:
+            view, (_, so, si) = c.dev[name]
+            c.dev[name] = (view, (1 << 40, so, si))
+        c.check(ctx, 4, 1, 0.25)
+    finally:
+        ctx.ctx_set_gemm_engine(0)
+
+
 @pytest.mark.parametrize("D", [64, 20, 7])
 @pytest.mark.parametrize("layout", ["bhtd", "wide", "odd", "shared"])
 def test_layouts(env, layout, D):
