@@ -300,7 +300,7 @@ __device__ __forceinline__ void sum_eight(float (&v)[8], int lane) {  // every l
 template <int LPR, bool VEC>
 __global__ void __launch_bounds__(256, 2) window_attention_far_kernel(const __grid_constant__ WindowAttn p) {
     constexpr int RPW = 32 / LPR, U = 2, DP = 4 * LPR, STEP = 8 * RPW;
-    __shared__ float sums[8][2 * AW_KEYS][DP];
+    __shared__ __align__(16) float sums[8][2 * AW_KEYS][DP];
     pdl_trigger();
     pdl_wait();
     const int groups = (p.rule.S + AW_KEYS - 1) / AW_KEYS, per_head = groups * p.far_chunks, head = blockIdx.x / per_head, item = blockIdx.x - head * per_head, j0 = item / p.far_chunks * AW_KEYS, chunk = item % p.far_chunks;
@@ -430,7 +430,8 @@ __device__ __forceinline__ float peer_float(const float* p, uint32_t rank) {
 template <int LPR, bool VEC>  // lanes a row: 8, 16 or 32 of four columns each
 __global__ void __launch_bounds__(32 * ST_WARPS) window_attention_step_kernel(const __grid_constant__ StepAttn p) {
     constexpr int RPW = 32 / LPR, U = 4, GROUPS = ST_WARPS * RPW, STEP = GROUPS * U, DP = 4 * LPR;
-    __shared__ float g_m[GROUPS], g_sum[GROUPS], g_o[GROUPS][DP + 4], c_o[DP], c_m, c_sum;
+    __shared__ __align__(16) float g_o[GROUPS][DP + 4];
+    __shared__ float g_m[GROUPS], g_sum[GROUPS], c_o[DP], c_m, c_sum;
     pdl_trigger();
     pdl_wait();
     const int rank = (int)cluster_rank(), split = (int)cluster_size(), item = blockIdx.x / split, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -538,7 +539,7 @@ __global__ void __launch_bounds__(32 * ST_WARPS) window_attention_step_kernel(co
 // much of values, brought by TMA into a ring of six, so that 192 KB an SM are on their way; eight warps read it as above.  A head whose tiles
 // lie in several CTAs leaves partial results, which a second kernel joins in their order.
 // Bound by memory: 8 x 16 heads of 16384 keys x 64 (1.07 GB) 196 us after a flush of L2, 64 x 16 of 1028 (539 MB) 114, so that the second half of a long call passes
-// at 6.5 TB/s; the cluster kernel below took 137 for the latter.
+// at 6.5 TB/s; the cluster kernel above took 137 for the latter.
 constexpr int SM_STAGES = 6, SM_TILE = 16384, SM_MAX_SEQ = 1024, SM_THREADS = 32 * ST_WARPS + 32;
 struct StreamAttn {
     StepAttn a;
@@ -569,7 +570,8 @@ __global__ void __launch_bounds__(SM_THREADS, 1) window_attention_stream_kernel(
     const uint32_t base = (smem_u32(smem_raw) + 127u) & ~127u;
     uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
     __shared__ __align__(8) uint64_t bars[2 * SM_STAGES];
-    __shared__ float g_m[GROUPS], g_sum[GROUPS], g_o[GROUPS][DP + 4];
+    __shared__ __align__(16) float g_o[GROUPS][DP + 4];
+    __shared__ float g_m[GROUPS], g_sum[GROUPS];
     __shared__ int pre[SM_MAX_SEQ + 1];  // tiles of the sequences before, of one head
     const StepAttn& p = g.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = p.D, H = p.H;
@@ -984,7 +986,7 @@ int gcb_window_attention_step_f32(gcb_ctx* ctx, int64_t n_seq, int64_t H, int64_
     p.lengths = lengths; p.status = ctx->d_status; p.cache_len = cache_len; p.D = (int)D; p.H = (int)H; p.scale = scale;
     const bool vec = D % 4 == 0 && vec_rows(q, 0, q_so, q_si) && vec_rows(k, k_ld, k_so, k_si) && vec_rows(v, v_ld, v_so, v_si);
     const int64_t seen = p.rule.W ? std::min<int64_t>(cache_len, (int64_t)p.rule.W + p.rule.S) : cache_len;
-    if (vec && n_seq <= SM_MAX_SEQ && n_seq * H * seen * D >= ST_STREAM && rows_ok(k, k_ld, k_so, k_si, n_seq, H) && rows_ok(v, v_ld, v_so, v_si, n_seq, H) && tma_encode(ctx) != nullptr) {
+    if (vec && n_seq <= SM_MAX_SEQ && n_seq * H < (int64_t(1) << 31) && n_seq * cache_len < (int64_t(1) << 34) && n_seq * H * seen * D >= ST_STREAM && rows_ok(k, k_ld, k_so, k_si, n_seq, H) && rows_ok(v, v_ld, v_so, v_si, n_seq, H) && tma_encode(ctx) != nullptr) {
         StreamAttn g = {p, nullptr, nullptr, (int)n_seq};
         Scratch mem(ctx);
         if ((rc = mem.get(sizeof(float) * (size_t)kSMs * (2 * (D + 2) + 1)))) return rc;

@@ -123,6 +123,15 @@ public:
     bool is_training() const { return m_is_training; }
     void train() { m_is_training = true; for (auto& [n, m] : m_submodules) m->train(); }
     void eval() { m_is_training = false; for (auto& [n, m] : m_submodules) m->eval(); }
+    // this module's mode and its submodules', depth first, and their way back
+    void training_modes(std::vector<bool>& out) const {
+        out.push_back(m_is_training);
+        for (const auto& [n, m] : m_submodules) m->training_modes(out);
+    }
+    void set_training_modes(const std::vector<bool>& modes, size_t& at) {
+        m_is_training = modes[at++];
+        for (auto& [n, m] : m_submodules) m->set_training_modes(modes, at);
+    }
     void register_module(std::string prefix, Module<T>* module) { m_submodules.emplace_back(std::move(prefix), module); }
     void register_parameter(std::string prefix, Parameter<T>* param) { m_parameters.emplace_back(std::move(prefix), param); }
 
@@ -1093,7 +1102,7 @@ class IncrementalGPT {
         for (Tensor<float>* t : {&m_x, &m_a, &m_q, &m_o}) at_least(*t, rows * C, m_device);
         at_least(m_h0, rows * m.F, m_device);
         at_least(m_h1, rows * m.F, m_device);
-        if (m_now._get_state() == nullptr) {
+        if (m_now._get_state() == nullptr || m_now.volume() != rows) {
             m_now = Tensor<int64_t>({rows}, m_device, uninitialized);
             m_lengths = Tensor<int64_t>({rows}, m_device, uninitialized);
         }
@@ -1230,9 +1239,9 @@ std::vector<int64_t> generate_tokens_incremental(Model& model, const std::vector
     check_generation((int64_t)start_tokens.size(), max_tokens, infer_device);
     struct Evaluating {  // nothing is dropped while tokens are generated
         Model& m;
-        bool was;
-        explicit Evaluating(Model& x) : m(x), was(x.is_training()) { if (was) m.eval(); }
-        ~Evaluating() { if (was) m.train(); }
+        std::vector<bool> was;
+        explicit Evaluating(Model& x) : m(x) { m.training_modes(was); m.eval(); }
+        ~Evaluating() { size_t at = 0; m.set_training_modes(was, at); }
     } evaluating(model);
     bool here = true;  // a model elsewhere is refused by its own forward
     for (auto* p : model.parameters()) here = here && p->device() == infer_device;

@@ -71,7 +71,9 @@ GCB_API int gcb_selftest_bounded_wait(gcb_ctx* ctx, int max_polls);
 GCB_API int64_t gcb_ctx_launch_count(gcb_ctx* ctx);
 /* Launches whose kernel-family name starts with `prefix` (for tests and benches that assert which code path ran).  Families:
  * gemm_tc_pair[_gelu_fwd|_gelu_bwd], gemm_tc_256[_softmax_bwd], gemm_tc_128, gemm_tc_64, splitk_reduce, gemm_simt, gemm_simt_backward, gemm_pack,
- * attention_fwd, attention_delta, attention_bwd, attention_small_fwd, attention_small_bwd, gpt_decode,
+ * attention_fwd, attention_delta, attention_bwd, attention_small_fwd, attention_small_bwd, gpt_decode, window_attention_fwd, window_attention_bwd,
+ * window_attention_tc_fwd, window_attention_tc_dq, window_attention_tc_dkv, window_attention_table, window_attention_far, window_attention_far_sum,
+ * window_attention_dbias, window_attention_step, window_attention_stream, window_attention_join, dropout,
  * presplit_weight, layernorm_bwd_ring, layernorm_bwd_warp, rmsnorm_bwd_ring, ..., one per entry point otherwise. */
 GCB_API int64_t gcb_ctx_launch_count_named(gcb_ctx* ctx, const char* prefix);
 /* Which GEMM engine ran last: 0 none, 1 SIMT fp32, 2 tcgen05 (split fp32). */
@@ -250,7 +252,8 @@ GCB_API int gcb_attention_bwd_f32(gcb_ctx* ctx, int64_t batch, int64_t heads, in
                           const float* q, int64_t q_ld, int64_t q_so, int64_t q_si, const float* k, int64_t k_ld, int64_t k_so, int64_t k_si,
                           const float* v, int64_t v_ld, int64_t v_so, int64_t v_si, float scale);
 
-/* Causal attention under a visibility rule, over batch x heads sequences of seq_len rows and head_dim columns (head_dim <= 128):
+/* Causal attention under a visibility rule, over batch x heads sequences of seq_len rows and head_dim columns (head_dim <= 128,
+ * heads <= 65535, seq_len <= 2^24):
  *   query i sees key j   <=>   j <= i and (window == 0 or i - j < window or j < sinks)          sinks <= 64
  *   score(i, j) = scale q_i . k_j + bias[h, n],  n = the last bucket with bucket_starts[n] <= i - j
  * bias (optional): device, heads x buckets; bucket_starts: host, `buckets` (<= 64) first distances, ascending from 0 (several buckets may
@@ -271,7 +274,7 @@ GCB_API int gcb_window_attention_bwd_f32(gcb_ctx* ctx, int64_t batch, int64_t he
 /* The same for one new position of every sequence: q and out hold one row a head, k and v (caches of cache_len rows a sequence) the
  * positions so far, the new one's among them; lengths (device, n_seq) says how many those are, and the query is at the last of them.  A
  * length of 0 gives zeros; one outside 0 .. cache_len is reported like an index outside its table, and gives zeros.  Rows beyond a sequence's length,
- * and rows the rule hides, are not read. */
+ * and rows the rule hides, may hold anything. */
 GCB_API int gcb_window_attention_step_f32(gcb_ctx* ctx, int64_t n_seq, int64_t heads, int64_t head_dim, float* out, int64_t o_so, int64_t o_si, const float* q, int64_t q_so, int64_t q_si,
                                  const float* k, int64_t k_ld, int64_t k_so, int64_t k_si, const float* v, int64_t v_ld, int64_t v_so, int64_t v_si, int64_t cache_len, const int64_t* lengths,
                                  float scale, int64_t window, int64_t sinks, const float* bias /*opt*/, int64_t buckets, const int64_t* bucket_starts);
@@ -282,7 +285,8 @@ GCB_API int gcb_relative_bucket_starts(int64_t buckets, int64_t reach, int64_t* 
 /* Dropout with a mask that is drawn again wherever it is needed: element i takes word i % 4 of Philox4x32-10 at counter offset + i / 4
  * under the key seed (both as unsigned numbers), and is dropped when that word is below p 2^32 (p in 0 .. 1); what is kept is divided by 1 - p.
  * fwd: out = residual + dropout(x), residual optional; out may be x or residual.  bwd: dx (+)= the same mask and factor on dy.  A call uses up
- * (n + 3) / 4 counters: the next one with the same seed continues at offset + (n + 3) / 4.  A dropped value is not looked at. */
+ * (n + 3) / 4 counters: the next one with the same seed continues at offset + (n + 3) / 4.  A dropped value is not looked at.
+ * A captured call draws the mask it was captured with at every replay. */
 GCB_API int gcb_dropout_fwd_f32(gcb_ctx* ctx, float* out, const float* x, const float* residual /*opt*/, int64_t n, float p, int64_t seed, int64_t offset);
 GCB_API int gcb_dropout_bwd_f32(gcb_ctx* ctx, float* dx, const float* dy, int64_t n, float p, int64_t seed, int64_t offset, int accumulate);
 
