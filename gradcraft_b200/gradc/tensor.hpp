@@ -455,7 +455,11 @@ std::pair<Tensor<T>, bool> Tensor<T>::grad_target() {
         if (g.m_state->m_storage.use_count() > 1 && !g.m_state->m_storage->m_owner) {
             // the buffer is shared with another tensor's gradient (it was adopted by aliasing): copy before writing
             Tensor<T> own(m_shape, device(), uninitialized);
-            if constexpr (std::is_same_v<T, float>) gcb_check(gcb_copy_d2d(Backend::get().ctx(device()), own.data_ptr(), g.data_ptr(), sizeof(T) * (size_t)volume()), "gradient copy");
+            if constexpr (std::is_same_v<T, float>) {
+                gcb_ctx* c = Backend::get().ctx(device());
+                if (g.is_contiguous()) gcb_check(gcb_copy_d2d(c, own.data_ptr(), g.data_ptr(), sizeof(T) * (size_t)volume()), "gradient copy");
+                else gcb_check(gcb_copy_strided_f32(c, (int)m_shape.size(), m_shape.data(), own.data_ptr(), own.strides().data(), g.data_ptr(), g.strides().data(), 0), "gradient copy");
+            }
             st.m_grad = own;
         }
         return {st.m_grad.value(), true};
