@@ -42,6 +42,23 @@ __device__ __forceinline__ void as_abt(float (&c)[R][C], const float* a, const f
             for (int j = 0; j < C; ++j) c[i][j] = fmaf(x[i].x, y[j].x, fmaf(x[i].y, y[j].y, fmaf(x[i].z, y[j].z, fmaf(x[i].w, y[j].w, c[i][j]))));
     }
 }
+// two fused multiply-adds in one instruction
+union F4 { float4 f; unsigned long long d[2]; };
+__device__ __forceinline__ unsigned long long twice(float x) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %1};" : "=l"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c) : "l"(a), "l"(b));
+    return c;
+}
+__device__ __forceinline__ void fma2_to(float& x, float& y, unsigned long long a, unsigned long long b) {  // (x, y) += a b
+    unsigned long long c;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(c) : "f"(x), "f"(y));
+    c = fma2(a, b, c);
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(c));
+}
 // acc[i][4 n + e] += sum_k p[ty + 16 i][k] b[k][64 n + 4 tx + e], k < 64
 template <int NC, int R>
 __device__ __forceinline__ void as_ab(float (&acc)[R][4 * NC], const float* p, const float* b, int D, int ty, int tx) {
@@ -57,11 +74,13 @@ __device__ __forceinline__ void as_ab(float (&acc)[R][4 * NC], const float* p, c
             if (c >= D) break;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const float4 y = ld4(b + (k + q) * P + c);
+                F4 y;
+                y.f = ld4(b + (k + q) * P + c);
 #pragma unroll
                 for (int i = 0; i < R; ++i) {
-                    acc[i][4 * n] = fmaf(a[i][q], y.x, acc[i][4 * n]); acc[i][4 * n + 1] = fmaf(a[i][q], y.y, acc[i][4 * n + 1]);
-                    acc[i][4 * n + 2] = fmaf(a[i][q], y.z, acc[i][4 * n + 2]); acc[i][4 * n + 3] = fmaf(a[i][q], y.w, acc[i][4 * n + 3]);
+                    const unsigned long long w = twice(a[i][q]);
+                    fma2_to(acc[i][4 * n], acc[i][4 * n + 1], w, y.d[0]);
+                    fma2_to(acc[i][4 * n + 2], acc[i][4 * n + 3], w, y.d[1]);
                 }
             }
         }
@@ -82,11 +101,13 @@ __device__ __forceinline__ void as_atb(float (&acc)[R][4 * NC], const float* p, 
         for (int n = 0; n < NC; ++n) {
             const int c = 64 * n + 4 * tx;
             if (c >= D) break;
-            const float4 y = ld4(b + r * P + c);
+            F4 y;
+            y.f = ld4(b + r * P + c);
 #pragma unroll
             for (int i = 0; i < R; ++i) {
-                acc[i][4 * n] = fmaf(a[i], y.x, acc[i][4 * n]); acc[i][4 * n + 1] = fmaf(a[i], y.y, acc[i][4 * n + 1]);
-                acc[i][4 * n + 2] = fmaf(a[i], y.z, acc[i][4 * n + 2]); acc[i][4 * n + 3] = fmaf(a[i], y.w, acc[i][4 * n + 3]);
+                const unsigned long long w = twice(a[i]);
+                fma2_to(acc[i][4 * n], acc[i][4 * n + 1], w, y.d[0]);
+                fma2_to(acc[i][4 * n + 2], acc[i][4 * n + 3], w, y.d[1]);
             }
         }
     }

@@ -39,6 +39,32 @@ __device__ __forceinline__ void aw_st4(float* p, int c, int D, float4 x) {
     if (c + 2 < D) p[c + 2] = x.z;
     if (c + 3 < D) p[c + 3] = x.w;
 }
+// c[i][j] = a[ty + 16 i] . b[tx + 16 j], even and odd columns apart until the end
+template <int R, int C>
+__device__ __forceinline__ void aw_abt(float (&c)[R][C], const float* a, const float* b, int D, int ty, int tx) {
+    const int P = D + 4;
+    unsigned long long sum[R][C] = {};
+#pragma unroll 4
+    for (int d = 0; d < D; d += 4) {
+        F4 x[R], y[C];
+#pragma unroll
+        for (int i = 0; i < R; ++i) x[i].f = ld4(a + (ty + 16 * i) * P + d);
+#pragma unroll
+        for (int j = 0; j < C; ++j) y[j].f = ld4(b + (tx + 16 * j) * P + d);
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int j = 0; j < C; ++j) sum[i][j] = fma2(x[i].d[1], y[j].d[1], fma2(x[i].d[0], y[j].d[0], sum[i][j]));
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+            float even, odd;
+            asm("mov.b64 {%0, %1}, %2;" : "=f"(even), "=f"(odd) : "l"(sum[i][j]));
+            c[i][j] = even + odd;
+        }
+}
 // bias of a tile's distances, the first of which is d0
 template <int R>
 __device__ __forceinline__ void aw_tab(float* sm, const WindowAttn& p, int64_t h, int d0) {
@@ -53,7 +79,7 @@ __device__ __forceinline__ int aw_next_tile(const WindowRule& r, int q0, int k0)
 static size_t aw_floats(int R, int own, int other, int blocks, int64_t Dp) { return (size_t)(own * 16 * R + other * AS_T) * (Dp + 4) + (size_t)blocks * AS_T * (16 * R + 4) + 2 * (aw_diag(R) + 1); }
 
 template <int R, int NC, bool VEC>
-__global__ void __launch_bounds__(256) window_attention_fwd_kernel(const __grid_constant__ WindowAttn p) {
+__global__ void __launch_bounds__(256, 2) window_attention_fwd_kernel(const __grid_constant__ WindowAttn p) {
     constexpr int OWN = 16 * R;
     extern __shared__ __align__(16) float aw_sm[];
     pdl_trigger();
@@ -73,7 +99,7 @@ __global__ void __launch_bounds__(256) window_attention_fwd_kernel(const __grid_
         aw_tab<R>(tab, p, h, q0 - k0 - (AS_T - 1));
         as_landed();
         float s[R][4];
-        as_abt(s, sq, sk, Dp, ty, tx);
+        aw_abt(s, sq, sk, Dp, ty, tx);
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             const int row = q0 + ty + 16 * i;
@@ -172,8 +198,8 @@ __device__ __forceinline__ void aw_dq(const WindowAttn& p, float* aw_sm, int ite
         }
         first = false;
         float s[R][4], dp[R][4];
-        as_abt(s, s0, s2, Dp, ty, tx);
-        as_abt(dp, s1, s3, Dp, ty, tx);
+        aw_abt(s, s0, s2, Dp, ty, tx);
+        aw_abt(dp, s1, s3, Dp, ty, tx);
 #pragma unroll
         for (int i = 0; i < R; ++i)
 #pragma unroll
@@ -236,8 +262,8 @@ __device__ __forceinline__ void aw_dkv(const WindowAttn& p, float* aw_sm, int it
         as_landed();
         rows.finish(s3, Dp, ty, tx);
         float s[4][R], dp[4][R];
-        as_abt(s, s2, s0, Dp, ty, tx);
-        as_abt(dp, s3, s1, Dp, ty, tx);
+        aw_abt(s, s2, s0, Dp, ty, tx);
+        aw_abt(dp, s3, s1, Dp, ty, tx);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -777,10 +803,10 @@ static int fma_bwd(gcb_ctx* ctx, int64_t heads, const WindowAttn& p) {
     static bool done[kMaxDevices] = {};
     return fma_launch(ctx, window_attention_bwd_kernel<R, NC, VEC>, done, 2 * heads * p.tiles, aw_floats(R, 2, 2, 2, (p.D + 3) / 4 * 4), "window_attention_bwd", p, (int)(heads * p.tiles));
 }
-// R, with 16 R rows of a CTA's own: 64 rows take 8 reads of shared memory for 64 FMAs where 32 rows take 6 for 32, and it is those reads that bound the kernels;
-// 32 rows where 64 would leave a quarter of the SMs idle.  Either, us, forward and backward: 16 x 16 x 1024 x 128 with a window of 256 1859 and 7645 with 32,
-// 1696 and 5537 with 64; 4 x 8 x 256 x 128 55 and 158, 47 and 132; 4 x 4 x 256 x 128 42 and 97, 47 and 108; 1 x 4 x 256 x 128 35 and 72, 47 and 108.  Twice the
-// threads for 64 rows, which leaves the reads as they are, took 1908 and 6028 in the first of these.
+// R, with 16 R rows of a CTA's own: 64 rows take 8 reads of shared memory for 32 double FMAs where 32 rows take 6 for 16, and the kernels wait for those reads
+// most; 32 rows where 64 would leave a quarter of the SMs idle.  Either, us, forward and backward: 16 x 16 x 1024 x 128 with a window of 256 1794 and 6998 with
+// 32, 1656 and 5117 with 64; 4 x 8 x 256 x 128 54 and 147, 47 and 126; 4 x 4 x 256 x 128 40 and 92, 47 and 108; 1 x 4 x 256 x 128 33 and 62, 47 and 108.  Twice
+// the threads for 64 rows, which leaves the reads as they are, is slower than twice the rows a thread (6028 and 5537 in the first of these, with single FMAs).
 static int fma_rows(int64_t heads, int64_t T) { return T > 32 && 4 * heads * ((T + 63) / 64) >= 3 * kSMs ? 4 : 2; }
 template <int R>
 static int fma_run(gcb_ctx* ctx, int64_t heads, const WindowAttn& p, bool vec) {
@@ -952,8 +978,8 @@ int gcb_window_attention_bwd_f32(gcb_ctx* ctx, int64_t B, int64_t H, int64_t T, 
         if ((rc = part.get(sizeof(float) * (size_t)(heads * tiles * buckets)))) return rc;
         p.dbias_part = part.as<float>();
     }
-    // Few queries beyond the window: the tiles of the first keys go on to the last query, which saves two launches (4 x 4 x 64 13.2 us, 18.4 with them;
-    // 5 x 6 x 331, window 100, 134.8 and 135.6; 8 x 8 x 200, window 30, 121.7 and 116.8; 2 x 4 x 512, window 64, 90.6 and 54.2).
+    // Few queries beyond the window: the tiles of the first keys go on to the last query, which saves two launches (4 x 4 x 64 13 us, 18 with them;
+    // 5 x 6 x 331, window 100, 135 and 136; 8 x 8 x 200, window 30, 122 and 117; 2 x 4 x 512, window 64, 91 and 54).
     p.far_inside = !tc && T - p.rule.W <= 128;
     if (tc) rc = window_tc_bwd(ctx, B, p);
     else rc = R == 4 ? fma_run<4>(ctx, heads, p, vec) : fma_run<2>(ctx, heads, p, vec);

@@ -1137,14 +1137,14 @@ static int make_moved(WindowTc& p, Scratch& mem) {
     return rc;
 }
 
-// Short sequences that the FMA kernels do sooner (forward and backward, us, there and here): up to 64 positions while half the SMs hold their tiles of 32
-// (4 x 4 x 64 x 32, window 16 and 2 sinks, 6.2 and 13.2, 7.1 and 23.2; 1 x 4 x 64 x 64 7.3 and 13.6, 7.8 and 18.6; 16 x 4 x 64 x 64 11.3 and 21.8, 8.4 and 21.1;
-// 4 x 4 x 128 x 64 12.6 and 25.0, 10.8 and 24.0), and forward up to 32 positions however many there are (64 x 12 x 32 x 64 24.0, 42.1; backward 110, 94).
-static bool short_enough(int64_t heads, int T, bool backward) { return T <= 64 && (2 * heads * ((T + 31) / 32) <= kSMs || (T <= 32 && !backward)); }
+// Short sequences that the FMA kernels do sooner: up to 32 positions, and up to 64 where every SM has a tile of 32 at most (forward and backward, us, there and
+// here: 64 x 12 x 32 x 64 27 and 74, 42 and 95; 4 x 4 x 64 x 32, window 16 and 2 sinks, 6.3 and 13.1, 8.0 and 23.3; 1 x 4 x 64 x 64 7.0 and 13.7, 8.3 and 19.0;
+// 16 x 4 x 64 x 64 9.0 and 18.2, 9.1 and 21.1; 64 x 12 x 64 x 64 38 and 156, 42 and 108; 4 x 4 x 128 x 64 11.7 and 28.9, 11.4 and 24.6).
+static bool short_enough(int64_t heads, int T) { return T <= 32 || (T <= 64 && heads * ((T + 31) / 32) <= kSMs); }
 // Heads of up to 64 columns (tensor memory holds two query tiles of that width), the split arithmetic of mode 2, rows that TMA can address.
 bool window_tc_takes(gcb_ctx* ctx, int64_t B, const WindowAttn& a) {
     if (ctx->gemm_engine == 1 || ctx->gemm_split_mode != 2 || a.D > 64 || a.D % 4 != 0 || !(a.scale > 0.0f) || a.scale > 1e30f) return false;
-    if (ctx->gemm_engine == 0 && short_enough(B * a.H, a.T, a.g != nullptr)) return false;
+    if (ctx->gemm_engine == 0 && short_enough(B * a.H, a.T)) return false;
     if (!rows_ok(a.q, a.q_ld, a.q_so, a.q_si, B, a.H) || !rows_ok(a.k, a.k_ld, a.k_so, a.k_si, B, a.H) || !rows_ok(a.v, a.v_ld, a.v_so, a.v_si, B, a.H)) return false;
     if (a.out && !rows_ok(a.out, a.o_ld, a.o_so, a.o_si, B, a.H)) return false;
     if (a.g && (!rows_ok(a.g, a.g_ld, a.g_so, a.g_si, B, a.H) || !rows_ok(a.o, a.o_ld, a.o_so, a.o_si, B, a.H) || !rows_ok(a.dq, a.d_ld, a.d_so, a.d_si, B, a.H) || !rows_ok(a.dk, a.d_ld, a.d_so, a.d_si, B, a.H) ||
