@@ -70,8 +70,7 @@ __device__ __forceinline__ void as_ab(float (&acc)[R][4 * NC], const float* p, c
         for (int i = 0; i < R; ++i) { const float4 x = ld4(p + (ty + 16 * i) * (AS_T + 4) + k); a[i][0] = x.x; a[i][1] = x.y; a[i][2] = x.z; a[i][3] = x.w; }
 #pragma unroll
         for (int n = 0; n < NC; ++n) {
-            const int c = 64 * n + 4 * tx;
-            if (c >= D) break;
+            const int c = min(64 * n + 4 * tx, D - 4);  // what lies beyond D is not used, and a branch would keep the loads of several rows apart
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 F4 y;
@@ -99,8 +98,7 @@ __device__ __forceinline__ void as_atb(float (&acc)[R][4 * NC], const float* p, 
         else { const float4 x = ld4(row); a[0] = x.x; a[1] = x.y; a[R - 2] = x.z; a[R - 1] = x.w; }
 #pragma unroll
         for (int n = 0; n < NC; ++n) {
-            const int c = 64 * n + 4 * tx;
-            if (c >= D) break;
+            const int c = min(64 * n + 4 * tx, D - 4);  // what lies beyond D is not used, and a branch would keep the loads of several rows apart
             F4 y;
             y.f = ld4(b + r * P + c);
 #pragma unroll
