@@ -10,11 +10,15 @@ constexpr int AS_OWN = 32, AS_T = 64;
 // ROWS rows of D columns from row r0 into [row][D + 4], asynchronously; rows beyond T are zero
 template <int ROWS>
 __device__ __forceinline__ void as_load(float* sm, const float* p, int64_t ld, int r0, int T, int D) {
-    const int d4 = D >> 2;
-    for (int i = threadIdx.x; i < ROWS * d4; i += 256) {
-        const int r = i / d4, c = (i - r * d4) * 4;
+    const int d4 = D >> 2, down = 256 / d4, across = 256 - down * d4;
+    int r = threadIdx.x / d4, q = threadIdx.x - r * d4;
+    while (r < ROWS) {
+        const int c = 4 * q;
         const bool live = r0 + r < T;
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(sm + r * (D + 4) + c)), "l"(live ? p + (r0 + r) * ld + c : p), "r"(live ? 16 : 0) : "memory");
+        r += down;
+        q += across;
+        if (q >= d4) { q -= d4; ++r; }
     }
 }
 __device__ __forceinline__ void as_landed() {
