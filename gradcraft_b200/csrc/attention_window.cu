@@ -803,11 +803,11 @@ static int fma_bwd(gcb_ctx* ctx, int64_t heads, const WindowAttn& p) {
     static bool done[kMaxDevices] = {};
     return fma_launch(ctx, window_attention_bwd_kernel<R, NC, VEC>, done, 2 * heads * p.tiles, aw_floats(R, 2, 2, 2, (p.D + 3) / 4 * 4), "window_attention_bwd", p, (int)(heads * p.tiles));
 }
-// R, with 16 R rows of a CTA's own: 64 rows take 8 reads of shared memory for 32 double FMAs where 32 rows take 6 for 16, and the kernels wait for those reads
-// most; 32 rows where 64 would leave a quarter of the SMs idle.  Either, us, forward and backward: 16 x 16 x 1024 x 128 with a window of 256 1794 and 6998 with
-// 32, 1656 and 5117 with 64; 4 x 8 x 256 x 128 54 and 147, 47 and 126; 4 x 4 x 256 x 128 40 and 92, 47 and 108; 1 x 4 x 256 x 128 33 and 62, 47 and 108.  Twice
-// the threads for 64 rows, which leaves the reads as they are, is slower than twice the rows a thread (6028 and 5537 in the first of these, with single FMAs).
-static int fma_rows(int64_t heads, int64_t T) { return T > 32 && 4 * heads * ((T + 63) / 64) >= 3 * kSMs ? 4 : 2; }
+// R, with 16 R rows of a CTA's own: 64 rows take 8 reads of shared memory for 32 double FMAs where 32 rows take 6 for 16; 32 rows where 64 would leave three fifths
+// of the SMs idle.  Either, us, forward and backward: 16 x 16 x 1024 x 128 with a window of 256 1745 and 6371 with 32, 1542 and 4406 with 64; 4 x 8 x 256 x 128
+// 51 and 134, 42 and 115; 4 x 4 x 256 x 128 45 and 84, 42 and 74; 1 x 4 x 256 x 128 31 and 55, 42 and 73; 64 x 12 x 32 x 64 25 and 66, 33 and 116.  Twice the
+// threads for 64 rows, which leaves the reads as they are, was slower than twice the rows a thread (6028 and 5537 in the first of these, at an earlier step).
+static int fma_rows(int64_t heads, int64_t T) { return T > 32 && 5 * heads * ((T + 63) / 64) >= 2 * kSMs ? 4 : 2; }
 template <int R>
 static int fma_run(gcb_ctx* ctx, int64_t heads, const WindowAttn& p, bool vec) {
     if (p.dq) return p.D <= 64 ? (vec ? fma_bwd<R, 1, true>(ctx, heads, p) : fma_bwd<R, 1, false>(ctx, heads, p)) : (vec ? fma_bwd<R, 2, true>(ctx, heads, p) : fma_bwd<R, 2, false>(ctx, heads, p));

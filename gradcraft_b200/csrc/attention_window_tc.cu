@@ -1139,10 +1139,14 @@ static int make_moved(WindowTc& p, Scratch& mem) {
     return rc;
 }
 
-// Short sequences that the FMA kernels do sooner: up to 32 positions, and up to 64 where every SM has a tile of 32 at most (forward and backward, us, there and
-// here: 64 x 12 x 32 x 64 27 and 74, 42 and 95; 4 x 4 x 64 x 32, window 16 and 2 sinks, 6.3 and 13.1, 8.0 and 23.3; 1 x 4 x 64 x 64 7.0 and 13.7, 8.3 and 19.0;
-// 16 x 4 x 64 x 64 9.0 and 18.2, 9.1 and 21.1; 64 x 12 x 64 x 64 38 and 156, 42 and 108; 4 x 4 x 128 x 64 11.7 and 28.9, 11.4 and 24.6).
-static bool short_enough(int64_t heads, int T) { return T <= 32 || (T <= 64 && heads * ((T + 31) / 32) <= kSMs); }
+// Short sequences that the FMA kernels do sooner: up to 32 positions, up to 64 where every SM has a tile of 32 at most, up to 128 where a quarter of them has
+// (forward and backward, us, there and here: 64 x 12 x 32 x 64 25 and 66, 42 and 95; 4 x 4 x 64 x 32, window 16 and 2 sinks, 5.5 and 8.8, 7.3 and 23.1; 1 x 4 x 64 x 64
+// 6.2 and 9.7, 7.9 and 18.3; 16 x 4 x 64 x 64 8.8 and 13.5, 8.6 and 21.2; 32 x 4 x 64 x 64 11.7 and 23.8, 9.1 and 22.3; 64 x 12 x 64 x 64 35 and 125, 43 and 109;
+// 1 x 4 x 128 x 64 10.4 and 17.5, 10.7 and 22.4; 4 x 4 x 128 x 64 10.7 and 24.9, 10.8 and 24.2).
+static bool short_enough(int64_t heads, int T) {
+    const int64_t tiles = heads * ((T + 31) / 32);
+    return T <= 32 || (T <= 64 && tiles <= kSMs) || (T <= 128 && 4 * tiles <= kSMs);
+}
 // Heads of up to 64 columns (tensor memory holds two query tiles of that width), the split arithmetic of mode 2, rows that TMA can address.
 bool window_tc_takes(gcb_ctx* ctx, int64_t B, const WindowAttn& a) {
     if (ctx->gemm_engine == 1 || ctx->gemm_split_mode != 2 || a.D > 64 || a.D % 4 != 0 || !(a.scale > 0.0f) || a.scale > 1e30f) return false;

@@ -135,7 +135,7 @@ def test_forward_and_gradients(env, size, engine):
         ctx.ctx_set_gemm_engine(0)
 
 
-@pytest.mark.parametrize("size", [s for s in SIZES if s[2] <= 64], ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("size", [s for s in SIZES if s[2] <= 128], ids=lambda s: "x".join(map(str, s)))
 def test_short_sequences_on_the_tensor_cores(env, size):
     """Where the choice between the kernels goes the other way by itself."""
     ctx, torch, capi = env
