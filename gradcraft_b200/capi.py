@@ -52,10 +52,10 @@ def parse_header(path=HEADER):
 
 def _ptr(x):
     """Address of a torch tensor or numpy array; None, integers and ctypes values as they are (the prototype converts them)."""
-    try:
+    if hasattr(x, "data_ptr"):
         return x.data_ptr()
-    except AttributeError:
-        return x.ctypes.data if hasattr(x, "ctypes") else x
+    array = getattr(x, "__array_interface__", None)  # sooner had than x.ctypes
+    return x if array is None else array["data"][0]
 
 
 class Lib:

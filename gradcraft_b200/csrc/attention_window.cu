@@ -14,7 +14,8 @@ namespace gcb {
 
 // ---- fp32 FMA kernels ----------------------------------------------------------------------------------------------------------
 // A CTA owns 16 R queries (forward, dQ) or keys (dK, dV) of a head, R 2 or 4, and walks over tiles of 64 of the other side, skipping those that the
-// rule hides as a whole.  The bias of a tile is looked up once per distance and read from shared memory.
+// rule hides as a whole.  The bias of a tile is looked up once per distance and read from shared memory
+// (from the buckets themselves: a table by distance first would be a launch).
 __host__ __device__ constexpr int aw_diag(int R) { return 16 * R + AS_T - 1; }
 
 // ROWS rows of D columns from row r0 into [row][Dp + 4], zero beyond T and D.  VEC: rows start on 16 bytes and D is a multiple of four.
@@ -65,10 +66,24 @@ __device__ __forceinline__ void aw_abt(float (&c)[R][C], const float* a, const f
             c[i][j] = even + odd;
         }
 }
+// A head's row of the bias table and the buckets' first distances, kept by the CTA behind its other tables; ready after the next barrier.
+template <int R>
+__device__ __forceinline__ float* aw_lut(float* tab, const WindowAttn& p, int64_t h) {
+    float* lut = tab + 2 * (aw_diag(R) + 1);
+    const int t = threadIdx.x;
+    if (t < p.rule.buckets) { lut[t] = p.rule.bias[h * p.rule.buckets + t]; lut[AW_MAX_BUCKETS + t] = __int_as_float(p.rule.starts[t]); }
+    return lut;
+}
 // bias of a tile's distances, the first of which is d0
 template <int R>
-__device__ __forceinline__ void aw_tab(float* sm, const WindowAttn& p, int64_t h, int d0) {
-    if (p.tab != nullptr && threadIdx.x < aw_diag(R)) sm[threadIdx.x] = p.tab[h * p.tab_len + clamp_distance(d0 + (int)threadIdx.x, p.tab_len)];
+__device__ __forceinline__ void aw_tab(float* sm, const WindowAttn& p, const float* lut, int d0) {
+    if (p.rule.bias == nullptr || threadIdx.x >= aw_diag(R)) return;
+    const int d = max(0, d0 + (int)threadIdx.x);
+    int n = 0;
+#pragma unroll
+    for (int step = AW_MAX_BUCKETS / 2; step > 0; step >>= 1)
+        if (n + step < p.rule.buckets && __float_as_int(lut[AW_MAX_BUCKETS + n + step]) <= d) n += step;
+    sm[threadIdx.x] = lut[n];
 }
 // the tile of keys after k0 that the queries from q0 on look at
 __device__ __forceinline__ int aw_first_tile(const WindowRule& r, int q0) { return r.S > 0 ? 0 : r.window_first(q0) / AS_T * AS_T; }
@@ -76,7 +91,7 @@ __device__ __forceinline__ int aw_next_tile(const WindowRule& r, int q0, int k0)
     const int k1 = k0 + AS_T, lo = r.window_first(q0) / AS_T * AS_T;
     return k1 >= r.S && k1 < lo ? lo : k1;
 }
-static size_t aw_floats(int R, int own, int other, int blocks, int64_t Dp) { return (size_t)(own * 16 * R + other * AS_T) * (Dp + 4) + (size_t)blocks * AS_T * (16 * R + 4) + 2 * (aw_diag(R) + 1); }
+static size_t aw_floats(int R, int own, int other, int blocks, int64_t Dp) { return (size_t)(own * 16 * R + other * AS_T) * (Dp + 4) + (size_t)blocks * AS_T * (16 * R + 4) + 2 * (aw_diag(R) + 1) + 2 * AW_MAX_BUCKETS; }
 
 template <int R, int NC, bool VEC>
 __global__ void __launch_bounds__(256, 2) window_attention_fwd_kernel(const __grid_constant__ WindowAttn p) {
@@ -87,6 +102,7 @@ __global__ void __launch_bounds__(256, 2) window_attention_fwd_kernel(const __gr
     const int D = p.D, Dp = (D + 3) / 4 * 4, tx = threadIdx.x & 15, ty = threadIdx.x >> 4, head = blockIdx.x / p.tiles, q0 = (blockIdx.x - head * p.tiles) * OWN, last = min(q0 + OWN, p.T);
     const int64_t b = head / p.H, h = head - b * p.H;
     float *sq = aw_sm, *sk = sq + OWN * (Dp + 4), *sv = sk + AS_T * (Dp + 4), *sp = sv + AS_T * (Dp + 4), *tab = sp + AS_T * (OWN + 4);
+    const float* lut = aw_lut<R>(tab, p, h);
     const float *k = p.k + b * p.k_so + h * p.k_si, *v = p.v + b * p.v_so + h * p.v_si;
     aw_load<OWN, VEC>(sq, p.q + b * p.q_so + h * p.q_si, p.q_ld, q0, p.T, D, Dp);
     float acc[R][4 * NC] = {}, m[R], sum[R] = {};
@@ -96,7 +112,7 @@ __global__ void __launch_bounds__(256, 2) window_attention_fwd_kernel(const __gr
         __syncthreads();
         aw_load<AS_T, VEC>(sk, k, p.k_ld, k0, p.T, D, Dp);
         aw_load<AS_T, VEC>(sv, v, p.v_ld, k0, p.T, D, Dp);
-        aw_tab<R>(tab, p, h, q0 - k0 - (AS_T - 1));
+        aw_tab<R>(tab, p, lut, q0 - k0 - (AS_T - 1));
         as_landed();
         float s[R][4];
         aw_abt(s, sq, sk, Dp, ty, tx);
@@ -106,7 +122,7 @@ __global__ void __launch_bounds__(256, 2) window_attention_fwd_kernel(const __gr
             float mx = m[i];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float z = p.tab ? fmaf(s[i][j], p.scale, tab[ty + 16 * i - (tx + 16 * j) + AS_T - 1]) : s[i][j] * p.scale;
+                const float z = p.rule.bias ? fmaf(s[i][j], p.scale, tab[ty + 16 * i - (tx + 16 * j) + AS_T - 1]) : s[i][j] * p.scale;
                 s[i][j] = p.rule.sees(row, k0 + tx + 16 * j) ? z : -INFINITY;
                 mx = fmaxf(mx, s[i][j]);
             }
@@ -176,6 +192,7 @@ __device__ __forceinline__ void aw_dq(const WindowAttn& p, float* aw_sm, int ite
     const int D = p.D, Dp = (D + 3) / 4 * 4, tx = threadIdx.x & 15, ty = threadIdx.x >> 4, head = item / p.tiles, tile = item - head * p.tiles, q0 = tile * OWN;
     const int64_t b = head / p.H, h = head - b * p.H;
     float *s0 = aw_sm, *s1 = s0 + OWN * (Dp + 4), *s2 = s1 + OWN * (Dp + 4), *s3 = s2 + AS_T * (Dp + 4), *ss = s3 + AS_T * (Dp + 4), *tab = ss + AS_T * (OWN + 4), *diag = tab + aw_diag(R) + 1;
+    const float* lut = aw_lut<R>(tab, p, h);
     const float *k = p.k + b * p.k_so + h * p.k_si, *v = p.v + b * p.v_so + h * p.v_si;
     float dq[R][4 * NC] = {}, db = 0.0f;
     AwRows<R, NC, VEC> rows;
@@ -188,7 +205,7 @@ __device__ __forceinline__ void aw_dq(const WindowAttn& p, float* aw_sm, int ite
         __syncthreads();
         aw_load<AS_T, VEC>(s2, k, p.k_ld, k0, p.T, D, Dp);
         aw_load<AS_T, VEC>(s3, v, p.v_ld, k0, p.T, D, Dp);
-        aw_tab<R>(tab, p, h, d0);
+        aw_tab<R>(tab, p, lut, d0);
         as_landed();
         if (first) {
             rows.finish(s1, Dp, ty, tx);
@@ -205,7 +222,7 @@ __device__ __forceinline__ void aw_dq(const WindowAttn& p, float* aw_sm, int ite
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const int r = ty + 16 * i, c = tx + 16 * j;
-                const float z = p.tab ? fmaf(s[i][j], p.scale, tab[r - c + AS_T - 1]) : s[i][j] * p.scale;
+                const float z = p.rule.bias ? fmaf(s[i][j], p.scale, tab[r - c + AS_T - 1]) : s[i][j] * p.scale;
                 const float pr = p.rule.sees(q0 + r, k0 + c) ? __expf(z - rows.m[i]) * rows.inv[i] : 0.0f;
                 ss[r * (AS_T + 4) + c] = pr * (dp[i][j] - rows.delta[i]);
             }
@@ -246,6 +263,7 @@ __device__ __forceinline__ void aw_dkv(const WindowAttn& p, float* aw_sm, int it
     const int D = p.D, Dp = (D + 3) / 4 * 4, tx = threadIdx.x & 15, ty = threadIdx.x >> 4, head = item / p.tiles, t0 = (item - head * p.tiles) * OWN;
     const int64_t b = head / p.H, h = head - b * p.H;
     float *s0 = aw_sm, *s1 = s0 + OWN * (Dp + 4), *s2 = s1 + OWN * (Dp + 4), *s3 = s2 + AS_T * (Dp + 4), *sp = s3 + AS_T * (Dp + 4), *ss = sp + AS_T * (OWN + 4), *tab = ss + AS_T * (OWN + 4);
+    const float* lut = aw_lut<R>(tab, p, h);
     const float *q = p.q + b * p.q_so + h * p.q_si, *g = p.g + b * p.g_so + h * p.g_si, *o = p.o + b * p.o_so + h * p.o_si;
     float dk[R][4 * NC] = {}, dv[R][4 * NC] = {};
     aw_load<OWN, VEC>(s0, p.k + b * p.k_so + h * p.k_si, p.k_ld, t0, p.T, D, Dp);
@@ -257,7 +275,7 @@ __device__ __forceinline__ void aw_dkv(const WindowAttn& p, float* aw_sm, int it
         AwRows<4, NC, VEC> rows;
         aw_load<AS_T, VEC>(s2, q, p.q_ld, r0, p.T, D, Dp);
         aw_load<AS_T, VEC>(s3, g, p.g_ld, r0, p.T, D, Dp);
-        aw_tab<R>(tab, p, h, r0 - t0 - (OWN - 1));
+        aw_tab<R>(tab, p, lut, r0 - t0 - (OWN - 1));
         rows.request(p, head, o, r0, ty, tx);
         as_landed();
         rows.finish(s3, Dp, ty, tx);
@@ -269,7 +287,7 @@ __device__ __forceinline__ void aw_dkv(const WindowAttn& p, float* aw_sm, int it
 #pragma unroll
             for (int j = 0; j < R; ++j) {
                 const int r = ty + 16 * i, c = tx + 16 * j, d = r0 + r - (t0 + c);
-                const float z = p.tab ? fmaf(s[i][j], p.scale, tab[r - c + OWN - 1]) : s[i][j] * p.scale;
+                const float z = p.rule.bias ? fmaf(s[i][j], p.scale, tab[r - c + OWN - 1]) : s[i][j] * p.scale;
                 const bool seen = d >= 0 && (W == 0 || d < W || t0 + c < always);
                 const float pr = seen ? __expf(z - rows.m[i]) * rows.inv[i] : 0.0f;
                 sp[r * (OWN + 4) + c] = pr;
@@ -805,7 +823,7 @@ static int fma_bwd(gcb_ctx* ctx, int64_t heads, const WindowAttn& p) {
 }
 // R, with 16 R rows of a CTA's own: 64 rows take 8 reads of shared memory for 32 double FMAs where 32 rows take 6 for 16; 32 rows where 64 would leave three fifths
 // of the SMs idle.  Either, us, forward and backward: 16 x 16 x 1024 x 128 with a window of 256 1745 and 6371 with 32, 1542 and 4406 with 64; 4 x 8 x 256 x 128
-// 51 and 134, 42 and 115; 4 x 4 x 256 x 128 45 and 84, 42 and 74; 1 x 4 x 256 x 128 31 and 55, 42 and 73; 64 x 12 x 32 x 64 25 and 66, 33 and 116.  Twice the
+// 51 and 134, 42 and 115; 4 x 4 x 256 x 128 45 and 84, 43 and 74; 1 x 4 x 256 x 128 31 and 55, 42 and 73; 64 x 12 x 32 x 64 25 and 66, 33 and 116.  Twice the
 // threads for 64 rows, which leaves the reads as they are, was slower than twice the rows a thread (6028 and 5537 in the first of these, at an earlier step).
 static int fma_rows(int64_t heads, int64_t T) { return T > 32 && 5 * heads * ((T + 63) / 64) >= 2 * kSMs ? 4 : 2; }
 template <int R>
@@ -935,8 +953,9 @@ int gcb_window_attention_fwd_f32(gcb_ctx* ctx, int64_t B, int64_t H, int64_t T, 
     p.tiles = (int)((T + 16 * R - 1) / (16 * R));
     const bool vec = D % 4 == 0 && vec_rows(q, q_ld, q_so, q_si) && vec_rows(k, k_ld, k_so, k_si) && vec_rows(v, v_ld, v_so, v_si) && vec_rows(out, o_ld, o_so, o_si);
     Scratch tab(ctx);
-    if ((rc = make_table(ctx, p, tab))) return rc;
-    if (window_tc_takes(ctx, B, p)) rc = window_tc_fwd(ctx, B, p);
+    const bool tc = window_tc_takes(ctx, B, p);
+    if (tc && (rc = make_table(ctx, p, tab))) return rc;
+    if (tc) rc = window_tc_fwd(ctx, B, p);
     else rc = R == 4 ? fma_run<4>(ctx, B * H, p, vec) : fma_run<2>(ctx, B * H, p, vec);
     if (rc) return rc;
     note_write(ctx, out, span_bytes(B, H, T, D, o_ld, o_so, o_si));
@@ -972,19 +991,20 @@ int gcb_window_attention_bwd_f32(gcb_ctx* ctx, int64_t B, int64_t H, int64_t T, 
     const bool tc = window_tc_takes(ctx, B, p);
     const int tiles = tc ? (int)((T + AW_TC_TILE - 1) / AW_TC_TILE) : p.tiles;
     Scratch part(ctx), far(ctx), tab(ctx), delta(ctx);
-    if ((rc = make_table(ctx, p, tab)) || (rc = delta.get(sizeof(float) * (size_t)(heads * p.Tp)))) return rc;
+    // Few queries beyond the window: the tiles of the first keys go on to the last query, which saves two launches (4 x 4 x 64 13 us, 18 with them;
+    // 5 x 6 x 331, window 100, 135 and 136; 8 x 8 x 200, window 30, 122 and 117; 2 x 4 x 512, window 64, 91 and 54).
+    p.far_inside = !tc && T - p.rule.W <= 128;
+    const bool beyond = p.rule.S > 0 && p.rule.W < T && !p.far_inside;  // some query looks past its window
+    if (((tc || beyond) && (rc = make_table(ctx, p, tab))) || (rc = delta.get(sizeof(float) * (size_t)(heads * p.Tp)))) return rc;
     p.delta = delta.as<float>();
     if (dbias) {
         if ((rc = part.get(sizeof(float) * (size_t)(heads * tiles * buckets)))) return rc;
         p.dbias_part = part.as<float>();
     }
-    // Few queries beyond the window: the tiles of the first keys go on to the last query, which saves two launches (4 x 4 x 64 13 us, 18 with them;
-    // 5 x 6 x 331, window 100, 135 and 136; 8 x 8 x 200, window 30, 122 and 117; 2 x 4 x 512, window 64, 91 and 54).
-    p.far_inside = !tc && T - p.rule.W <= 128;
     if (tc) rc = window_tc_bwd(ctx, B, p);
     else rc = R == 4 ? fma_run<4>(ctx, heads, p, vec) : fma_run<2>(ctx, heads, p, vec);
     if (rc) return rc;
-    if (p.rule.S > 0 && p.rule.W < T && !p.far_inside && (rc = far_gradients(ctx, heads, p, vec, far))) return rc;  // some query looks past its window
+    if (beyond && (rc = far_gradients(ctx, heads, p, vec, far))) return rc;
     for (float* d : {dq, dk, dv}) note_write(ctx, d, span_bytes(B, H, T, D, d_ld, d_so, d_si));
     if (dbias) {
         GCB_CHECK_CUDA(launch_next(ctx->stream, dim3((unsigned)((H * buckets + 7) / 8)), 256, 0, window_attention_dbias_kernel, dbias, part.as<float>(), (int)H, (int)B, tiles, (int)buckets, accumulate_dbias));
