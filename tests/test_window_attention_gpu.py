@@ -468,3 +468,43 @@ def test_single_positions_continue_what_a_forward_pass_began(env):
         ctx.window_attention_step_f32(B, H, D, out, H * D, D, c.dev["q"][0][:, :, t].contiguous(), H * D, D, *c.arg("k"), *c.arg("v"), T, torch.full((B,), t + 1, device="cuda"), *c.rule)
         ctx.sync()
         assert max_abs_rel(out.cpu().numpy(), c.out[:, :, t].cpu().numpy()) < TOL
+
+
+def test_two_contexts_at_once(env):
+    """Calls of two contexts on streams of their own, queued in turn without waiting, give what each gives alone."""
+    _, torch, capi = env
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    ctxs = [capi.Context(0, s.cuda_stream) for s in streams]
+    sizes = [(4, 8, 700, 64), (2, 6, 300, 128)]
+    cases = [Case(torch, *size, 16, 64, seed=i) for i, size in enumerate(sizes)]
+    rng = np.random.default_rng(8)
+    n, H, cap, D = 8, 16, 4096, 64
+    lengths = torch.from_numpy(rng.integers(1, cap, n)).cuda()
+    caches = [torch.randn(2, n, cap, H, D, device="cuda") for _ in range(2)]
+    q = torch.randn(n, H, D, device="cuda")
+    outs = [torch.empty(n, H, D, device="cuda") for _ in range(2)]
+
+    def calls(i):
+        with torch.cuda.stream(streams[i]):
+            cases[i].forward(ctxs[i], 100, 3, 0.125)
+            cases[i].backward(ctxs[i])
+            at = (H * D, cap * H * D, D)
+            ctxs[i].window_attention_step_f32(n, H, D, outs[i], H * D, D, q, H * D, D, caches[i][0], *at, caches[i][1], *at, cap, lengths, 0.125, 0, 0, None, 0, None)
+
+    def results(i):
+        return [t.clone() for t in [cases[i].out, cases[i].dbias, outs[i]] + cases[i].grads]
+
+    torch.cuda.synchronize()
+    alone = []
+    for i in range(2):
+        calls(i)
+        torch.cuda.synchronize()
+        alone.append(results(i))
+    for _ in range(5):
+        for i in range(2):
+            calls(i)
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(a, b) for a, b in zip(results(i), alone[i]))
+        ctxs[i].sync()
+        ctxs[i].close()
