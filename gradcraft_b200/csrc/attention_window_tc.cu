@@ -12,8 +12,8 @@
 //     products and T^2 floats there, seven products here.
 // The gradients of the first S keys from queries beyond the window are left to the FMA kernel of attention_window.cu: 128-key tiles would
 // spend T / 64 blocks on a handful of keys.
-// 1 x 16 heads of 8192 x 64, window 1024, four first positions: forward 241 us, dQ 245, dK and dV 343 (with a bias of 32 buckets 265, 354, 405); 16 x 16 heads of
-// 1024, window 256: 204, 261, 327.  The tensor cores are at work for 45, 54 and 52 % of a call at 4096 positions, and 41, 51 and 42 % of the issue slots go to what
+// 1 x 16 heads of 8192 x 64, window 1024, four first positions: forward 231 us, dQ 246, dK and dV 324 (with a bias of 32 buckets 260, 351, 375); 16 x 16 heads of
+// 1024, window 256: 198, 244, 255.  The tensor cores are at work for 45, 54 and 52 % of a call at 4096 positions, and 41, 51 and 42 % of the issue slots go to what
 // turns scores into probabilities and rows into companions; what is left is the way of a block from role to role, a barrier each time.
 // Every wait is bounded, as in the GEMM kernels.
 #include "attention_tc.cuh"
@@ -1107,6 +1107,11 @@ static WindowTc operands(gcb_ctx* ctx, int64_t B, const WindowAttn& a, int tiles
     p.out = a.out; p.row_max = a.row_max; p.row_inv = a.row_inv; p.dbias_part = a.dbias_part;
     p.delta = a.delta; p.tab = a.tab; p.tab_len = a.tab_len; p.scale = a.scale; p.T = a.T; p.D = a.D; p.rule = a.rule; p.status = ctx->d_status;
     plan(p, B, a.H, a.T, tiles_per_unit);
+    // Heads are taken all together, the heaviest tiles of every one first, so that the lightest are left for the end; not where every tile goes back to the first keys
+    // and k and v of all heads are more than the L2 cache holds, 126 MB: groups of heads then stay in it (kernels as they are here and in groups, us: 16 x 16 x 1024 x 64,
+    // window 256, forward 197 and 204, dQ 245 and 263, dK and dV 256 and 332; 8 x 12 x 512, no window, 37, 50, 64 and 38, 53, 77; 16 x 16 x 1024, no window, 240, 294,
+    // 350 and 232, 293, 350).
+    if (a.rule.W > 0 || 2 * sizeof(float) * p.heads * (int64_t)a.T * a.D <= (int64_t(126) << 20)) p.group = p.heads;
     return p;
 }
 template <class K, class... Maps>
