@@ -1166,7 +1166,8 @@ bool window_tc_takes(gcb_ctx* ctx, int64_t B, const WindowAttn& a) {
 
 int window_tc_fwd(gcb_ctx* ctx, int64_t B, const WindowAttn& a) {
     TmaEncodeFn enc = tma_encode(ctx);
-    // two query tiles share their key blocks; one tile a CTA where pairs would leave SMs idle
+    // two query tiles share their key blocks; one tile a CTA where pairs would leave SMs idle (in pairs and one by one, us: 16 x 16 x 1024, window 256, 197 and 262;
+    // 1 x 12 x 4099, window 512, 86 and 95; 2 x 12 x 1024 45 and 43; 1 x 4 x 512 26 and 23; 3 x 12 x 700 34 and 34)
     WindowTc p = operands(ctx, B, a, B * a.H * ((a.T + 255) / 256) < kSMs ? 1 : 2);
     Scratch moved(ctx);
     int rc = make_moved(p, moved);
