@@ -13,7 +13,7 @@
 // The gradients of the first S keys from queries beyond the window are left to the FMA kernel of attention_window.cu: 128-key tiles would
 // spend T / 64 blocks on a handful of keys.
 // 1 x 16 heads of 8192 x 64, window 1024, four first positions: forward 231 us, dQ 246, dK and dV 324 (with a bias of 32 buckets 260, 351, 375); 16 x 16 heads of
-// 1024, window 256: 198, 244, 255.  The tensor cores are at work for 45, 54 and 52 % of a call at 4096 positions, and 41, 51 and 42 % of the issue slots go to what
+// 1024, window 256: 198, 244, 255.  The tensor cores are at work for 34, 43 and 46 % of a call at 4096 positions, and 43, 53 and 49 % of the issue slots go to what
 // turns scores into probabilities and rows into companions; what is left is the way of a block from role to role, a barrier each time.
 // Every wait is bounded, as in the GEMM kernels.
 #include "attention_tc.cuh"

@@ -595,7 +595,7 @@ public:
         for (const auto& b : m_blocks) t.push_back(b->attn().rel_bias());
         return t;
     }
-    // The weights as the decoding kernel takes them; valid while the parameters stay where they are.
+    // The weights as the decoding kernel takes them, which knows nothing of an attention rule; valid while the parameters stay where they are.
     gcb_gpt_model describe(std::vector<gcb_gpt_layer>& layers) const {
         layers.assign(m_blocks.size(), gcb_gpt_layer{});
         for (size_t i = 0; i < m_blocks.size(); ++i) m_blocks[i]->describe(layers[i]);
