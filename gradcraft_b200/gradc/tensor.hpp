@@ -452,8 +452,9 @@ std::pair<Tensor<T>, bool> Tensor<T>::grad_target() {
     TensorState<T>& st = *m_state;
     if (st.m_grad.has_value()) {
         Tensor<T>& g = st.m_grad.value();
-        if (g.m_state->m_storage.use_count() > 1 && !g.m_state->m_storage->m_owner) {
-            // the buffer is shared with another tensor's gradient (it was adopted by aliasing): copy before writing
+        if (!g.is_contiguous() || (g.m_state->m_storage.use_count() > 1 && !g.m_state->m_storage->m_owner)) {
+            // The buffer is shared with another tensor's gradient (it was adopted by aliasing), or it was adopted with strides while callers walk over
+            // the target row by row: copy before writing.
             Tensor<T> own(m_shape, device(), uninitialized);
             if constexpr (std::is_same_v<T, float>) {
                 gcb_ctx* c = Backend::get().ctx(device());
