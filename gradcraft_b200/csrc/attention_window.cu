@@ -574,7 +574,7 @@ __global__ void __launch_bounds__(32 * ST_WARPS) window_attention_step_kernel(co
             a = fmaf(f, peer_float(c_o + t, i), a);
             total = fmaf(f, peer_float(&c_sum, i), total);
         }
-        p.out[b * p.o_so + h * p.o_si + t] = mx == -INFINITY ? 0.0f : a / total;
+        p.out[b * p.o_so + h * p.o_si + t] = total == 0.0f ? 0.0f : a / total;  // nothing seen; scores that are not numbers leave no maximum either, but a sum that is none
     }
     cluster_sync();  // nobody leaves while its shared memory is read
 }
@@ -765,7 +765,7 @@ __global__ void __launch_bounds__(SM_THREADS, 1) window_attention_stream_kernel(
             }
             const bool whole = !continues && t == keys.tiles;
             if (whole) {
-                p.out[b * p.o_so + h * p.o_si + c] = mx == -INFINITY ? 0.0f : a / all;
+                p.out[b * p.o_so + h * p.o_si + c] = all == 0.0f ? 0.0f : a / all;
             } else {
                 float* part = g.part + ((int64_t)blockIdx.x * 2 + (continues ? 0 : 1)) * (D + 2);
                 part[c] = a;
@@ -793,7 +793,7 @@ __global__ void __launch_bounds__(128) window_attention_join_kernel(const __grid
         a = fmaf(f, part(x, 0)[c], a);
         all = fmaf(f, part(x, 0)[D + 1], all);
     }
-    g.a.out[unit / g.a.H * g.a.o_so + unit % g.a.H * g.a.o_si + c] = mx == -INFINITY ? 0.0f : a / all;
+    g.a.out[unit / g.a.H * g.a.o_so + unit % g.a.H * g.a.o_si + c] = all == 0.0f ? 0.0f : a / all;
 }
 
 // ---- host side ----------------------------------------------------------------------------------------------------------------
