@@ -527,7 +527,8 @@ __global__ void __launch_bounds__(32 * ST_WARPS) window_attention_step_kernel(co
                     do --bucket; while (p.rule.starts[bucket] > d);
                     bias = p.rule.bias[h * p.rule.buckets + bucket];
                 }
-                z[u] += bias;
+                if (bias == -INFINITY) { z[u] = -INFINITY; vv[u] = make_float4(0.f, 0.f, 0.f, 0.f); }  // hidden: may hold anything
+                else z[u] += bias;
             }
             if (y >= v1) z[u] = -INFINITY;
             mx = fmaxf(mx, z[u]);
@@ -729,7 +730,8 @@ __global__ void __launch_bounds__(SM_THREADS, 1) window_attention_stream_kernel(
                         do --bucket; while (p.rule.starts[bucket] > d);
                         bias = p.rule.bias[(int64_t)h * p.rule.buckets + bucket];
                     }
-                    z[u] += bias;
+                    if (bias == -INFINITY) { z[u] = -INFINITY; vv[u] = zero; }
+                    else z[u] += bias;
                 }
                 if (y >= rows) z[u] = -INFINITY;
                 mx = fmaxf(mx, z[u]);

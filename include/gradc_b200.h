@@ -275,7 +275,7 @@ GCB_API int gcb_window_attention_bwd_f32(gcb_ctx* ctx, int64_t batch, int64_t he
 /* The same for one new position of every sequence: q and out hold one row a head, k and v (caches of cache_len rows a sequence) the
  * positions so far, the new one's among them; lengths (device, n_seq) says how many those are, and the query is at the last of them.  A
  * length of 0 gives zeros; one outside 0 .. cache_len is reported like an index outside its table, and gives zeros.  Rows beyond a sequence's length,
- * and rows the rule hides, may hold anything. */
+ * rows that the rule hides and rows in a bucket that a bias of -inf hides may hold anything; a NaN in the query or in a key that it sees gives NaN. */
 GCB_API int gcb_window_attention_step_f32(gcb_ctx* ctx, int64_t n_seq, int64_t heads, int64_t head_dim, float* out, int64_t o_so, int64_t o_si, const float* q, int64_t q_so, int64_t q_si,
                                  const float* k, int64_t k_ld, int64_t k_so, int64_t k_si, const float* v, int64_t v_ld, int64_t v_so, int64_t v_si, int64_t cache_len, const int64_t* lengths,
                                  float scale, int64_t window, int64_t sinks, const float* bias /*opt*/, int64_t buckets, const int64_t* bucket_starts);

@@ -1,4 +1,4 @@
-"""Attention of single positions on values that are not finite: a query or a key that it sees passes them on.
+"""Attention of single positions on values that are not finite: a query or a key that it sees passes them on, what a bias of -inf hides does not.
 
 Tolerance as in test_window_attention_gpu.py: two products of up to 128 terms and an exponential, well below 2e-5 of the largest value."""
 import numpy as np
@@ -88,3 +88,25 @@ def test_keys_that_are_not_numbers(env, size):
     assert np.isnan(got[lost]).all() and np.isposinf(got[0, 1]).all()
     lost[0, 1] = True
     assert max_abs_rel(got[~lost], want[~lost]) < TOL
+
+
+@ids
+@pytest.mark.parametrize("hidden", [[0], [2], [7], [1, 3, 5], list(range(8))], ids=str)
+def test_what_a_bias_of_minus_infinity_hides_may_hold_anything(env, size, hidden):
+    B, H, D, cap, window, sinks, _ = size
+    q, k, v, lengths = data(size, 2)
+    starts = R.bucket_starts(8, 64)
+    bias = np.random.default_rng(6).standard_normal((H, 8), dtype=np.float32)
+    bias[:, hidden] = -np.inf
+    want = R.step(q, k, v, lengths, D**-0.5, window, sinks, bias, starts)
+    for b, n in enumerate(lengths):
+        j = np.arange(n)
+        j = j[np.isin(np.searchsorted(starts, n - 1 - j, side="right") - 1, hidden)]
+        k[b][:, j[::2]] = np.nan
+        k[b][:, j[1::2]] = np.inf
+        v[b][:, j[::3]] = np.nan
+        v[b][:, j[1::3]] = -np.inf
+    got = run(env, size, q, k, v, lengths, bias, starts)
+    assert max_abs_rel(got, want) < TOL
+    if len(hidden) == 8:
+        assert not got.any()
