@@ -7,6 +7,8 @@ import ctypes
 import os
 import re
 
+import numpy as np
+
 HERE = os.path.dirname(os.path.abspath(__file__))
 HEADER = os.path.join(HERE, "..", "include", "gradc_b200.h")
 LIB_PATH = os.path.join(HERE, "libgradc_b200.so")
@@ -51,11 +53,11 @@ def parse_header(path=HEADER):
 
 
 def _ptr(x):
-    """Address of a torch tensor or numpy array; None, integers and ctypes values as they are (the prototype converts them)."""
+    """Address of a torch tensor or numpy array; None, integers and ctypes values as they are.  The prototype converts those, and refuses whatever else
+    there is: numpy scalars too, which have an array interface, but to a copy that goes with it."""
     if hasattr(x, "data_ptr"):
         return x.data_ptr()
-    array = getattr(x, "__array_interface__", None)  # sooner had than x.ctypes
-    return x if array is None else array["data"][0]
+    return x.__array_interface__["data"][0] if isinstance(x, np.ndarray) else x  # sooner had than x.ctypes
 
 
 class Lib:
