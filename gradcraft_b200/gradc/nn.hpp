@@ -535,10 +535,12 @@ class BlockT : public Module<T> {
     Dropout<T> m_dropout;
 
 public:
+    // `counter`: what dropout's masks are drawn from, the same one for all blocks of a stack; with dropout it has to be given, since blocks with a
+    // counter of their own each would drop the same positions
     template <class NormMaker>
     BlockT(int64_t C, int64_t H, int64_t max_seq, int64_t hidden, const Initializer<T>& base_init, const Initializer<T>& residual_init, NormMaker mk, const BlockOptions& opt = {}, std::shared_ptr<DropoutCounter> counter = nullptr)
         : m_norm1(mk()), m_attn(C, H, true, max_seq, base_init, residual_init, ZerosInit<T>(), opt.rule()), m_norm2(mk()), m_mlp(C, hidden, base_init, residual_init),
-          m_dropout(opt.dropout, counter ? counter : std::make_shared<DropoutCounter>(opt.dropout_seed)) {
+          m_dropout(opt.dropout, counter || opt.dropout != 0.0f ? counter : std::make_shared<DropoutCounter>(opt.dropout_seed)) {
         this->register_module("norm1", &m_norm1);
         this->register_module("attn", &m_attn);
         this->register_module("norm2", &m_norm2);
