@@ -148,13 +148,15 @@ _contexts = {}
 
 
 def _context():
-    """One context for every stream a program launches on."""
+    """One context for every stream a program launches on.  The default stream's handle is 0 on every device, and a stream that is gone may leave its
+    handle to another one: contexts go by device and stream, and hold on to the stream."""
     from gradcraft_b200 import capi
 
-    stream = torch.cuda.current_stream().cuda_stream
-    if stream not in _contexts:
-        _contexts[stream] = capi.Context(torch.cuda.current_device(), stream)
-    return _contexts[stream]
+    device, stream = torch.cuda.current_device(), torch.cuda.current_stream()
+    key = device, stream.cuda_stream
+    if key not in _contexts:
+        _contexts[key] = capi.Context(device, stream.cuda_stream), stream
+    return _contexts[key][0]
 
 
 def _own_attention(s):
