@@ -5,6 +5,7 @@
 // This file holds the entry points, the fp32 FMA kernels, which take any strides and heads of up to 128 columns, and the kernel for single
 // positions.
 #include <algorithm>
+#include <utility>
 
 #include "attention_fma.cuh"
 #include "attention_tc.cuh"
@@ -800,7 +801,18 @@ __global__ void __launch_bounds__(128) window_attention_join_kernel(const __grid
 
 // ---- host side ----------------------------------------------------------------------------------------------------------------
 static bool vec_rows(const float* p, int64_t ld, int64_t so, int64_t si) { return aligned16(p) && ld % 4 == 0 && so % 4 == 0 && si % 4 == 0; }
-static bool own_rows(int64_t B, int64_t H, int64_t T, int64_t D, int64_t ld, int64_t so, int64_t si) { return (T <= 1 || ld >= D) && (H <= 1 || si > 0) && (B <= 1 || so > 0); }
+// Rows that are written lie apart: by ascending stride, each one reaches past the stretch that the smaller ones cover, as in a dense tensor or a slice of one.
+static bool own_rows(int64_t B, int64_t H, int64_t T, int64_t D, int64_t ld, int64_t so, int64_t si) {
+    std::pair<int64_t, int64_t> d[3] = {{ld, T}, {si, H}, {so, B}};
+    std::sort(d, d + 3);
+    double stretch = (double)D;
+    for (const auto& [stride, n] : d) {
+        if (n <= 1) continue;
+        if ((double)stride < stretch) return false;
+        stretch += (double)(n - 1) * (double)stride;
+    }
+    return true;
+}
 // Floats of keys in sight from which the streaming kernel and its join are taken instead of the one launch of clusters (either, us, after a flush of L2:
 // 1 x 16 heads of 2048 x 64 16.4 clusters, 19.5 streamed; 8 x 16 of 512 20.5, 21.5; 4 x 16 of 2048 30.8, 29.7; 1 x 16 of 8192 36.9, 29.7; 32 x 16 of 512 47.1, 42.0).
 constexpr int64_t ST_STREAM = int64_t(1) << 22;

@@ -259,7 +259,8 @@ GCB_API int gcb_attention_bwd_f32(gcb_ctx* ctx, int64_t batch, int64_t heads, in
  * bias (optional): device, heads x buckets; bucket_starts: host, `buckets` (<= 64) first distances, ascending from 0 (several buckets may
  * start at one distance; the last of them counts).  A bias of -inf hides a bucket; a query that then sees nothing gets zeros and gives no gradient.
  * q, k, v, out, dout and the gradients are addressed through row, sequence and head strides in elements, any strides for what is only read; columns
- * are contiguous.  out and the gradients must not overlap their inputs.  stats: gcb_attention_stats_floats floats that the forward
+ * are contiguous.  out and the gradients must not overlap their inputs, and their strides are those of a dense tensor or of a slice of one (rows that
+ * would lie on top of one another are refused).  stats: gcb_attention_stats_floats floats that the forward
  * fills and the backward reads.  dq, dk and dv share one layout and are overwritten; dbias (optional, heads x buckets) is overwritten or added
  * to.  Deterministic: every sum is taken in a fixed order.  The calls take workspace from the arena while they run;
  * captured ones go on using it, so that graphs of one context are replayed one after another, on its stream or behind it, and cached memory is not released
