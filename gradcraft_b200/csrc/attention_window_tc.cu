@@ -21,7 +21,7 @@
 
 namespace gcb {
 
-constexpr int WT_FLUSH = 8;                     // blocks whose products are added up in tensor memory before the sum moves on
+constexpr int WT_FLUSH = 4;                     // backward: blocks whose products are added up in tensor memory before the sum moves on
 constexpr int WT_DIAG = AT_ROWS + AT_KEYS - 1;  // distances in a block of scores
 constexpr int WT_TAB = 192;                     // their place in shared memory, in floats
 constexpr float kLog2e = 1.4426950408889634f;
@@ -30,7 +30,7 @@ struct WindowTc {
     int64_t q_ld, q_so, q_si, k_ld, k_so, k_si, v_ld, v_so, v_si, g_ld, g_so, g_si, o_ld, o_so, o_si, d_ld, d_so, d_si;
     const float *q, *k, *v, *g, *o;
     float *out, *dq, *dk, *dv, *row_max, *row_inv, *delta, *dbias_part;
-    float* moved;      // 64 KB a CTA, where an item may have more than WT_FLUSH blocks
+    float* moved;      // 64 KB a CTA, for what leaves tensor memory before an item's end
     const float* tab;  // [H][tab_len]: bias by distance, the last one for all distances beyond; NULL: no bias
     int tab_len;
     int64_t Tp;
@@ -102,6 +102,8 @@ __device__ __forceinline__ void win_split(const uint8_t* raw, uint8_t* twin, int
                                                                         pack_bf16(b.x - trunc_tf32(b.x), b.y - trunc_tf32(b.y)), pack_bf16(b.z - trunc_tf32(b.z), b.w - trunc_tf32(b.w)));
     }
 }
+// Every addition of the tensor core cuts off up to 2^-23 of the sum that it adds to, always towards zero.  Both products therefore begin with those of the remainders, while
+// the sum is still 2^-10 of what it will be.
 // D[128 x 64] = A[128 x DP] B[64 x DP]^T.  A: t in tensor memory, companions in shared memory (place_row); B: K-major raw tile and companions (addresses in 16-byte units).
 template <int DP>
 __device__ __forceinline__ void win_scores(uint32_t d, uint32_t a_t, uint32_t a_twin, uint32_t b_raw, uint32_t b_twin) {
@@ -111,11 +113,15 @@ __device__ __forceinline__ void win_scores(uint32_t d, uint32_t a_t, uint32_t a_
     asm volatile("" : "+r"(a_t), "+r"(a_twin), "+r"(b_raw), "+r"(b_twin));  // descriptors are made here, one addition each: kept across the loop they are spilled
 #pragma unroll
     for (int kb = 0; kb < DP / 16; ++kb) {
-        const uint32_t b = b_raw + (kb >> 1) * 512 + (kb & 1) * 4, tw = b_twin + kb * 16, a = a_twin + kb * 512;
-        umma_tf32_ts(d, a_t + 16 * kb, tile_desc<16, 1024, 2>(b), idesc, kb > 0 ? 1u : 0u);
-        umma_tf32_ts(d, a_t + 16 * kb + 8, tile_desc<16, 1024, 2>(b + 2), idesc, 1u);
-        umma_bf16(d, tile_desc<128, 256, 0>(a + 256), tile_desc<128, WinTile<DP>::ROWS8, 0>(tw), idesc_bf, 1u);
+        const uint32_t tw = b_twin + kb * 16, a = a_twin + kb * 512;
+        umma_bf16(d, tile_desc<128, 256, 0>(a + 256), tile_desc<128, WinTile<DP>::ROWS8, 0>(tw), idesc_bf, kb > 0 ? 1u : 0u);
         umma_bf16(d, tile_desc<128, 256, 0>(a), tile_desc<128, WinTile<DP>::ROWS8, 0>(tw + small), idesc_bf, 1u);
+    }
+#pragma unroll
+    for (int kb = 0; kb < DP / 16; ++kb) {
+        const uint32_t b = b_raw + (kb >> 1) * 512 + (kb & 1) * 4;
+        umma_tf32_ts(d, a_t + 16 * kb, tile_desc<16, 1024, 2>(b), idesc, 1u);
+        umma_tf32_ts(d, a_t + 16 * kb + 8, tile_desc<16, 1024, 2>(b + 2), idesc, 1u);
     }
 }
 // D[128 x DP] (+)= A[128 x 64] B[64 x DP].  A: its three parts in tensor memory, the companions of 16 columns STEP apart; B: MN-major raw tile and companions.
@@ -127,11 +133,15 @@ __device__ __forceinline__ void win_values(uint32_t d, uint32_t a_t, uint32_t a_
     asm volatile("" : "+r"(a_t), "+r"(a_big), "+r"(a_sml), "+r"(b_raw), "+r"(b_twin));
 #pragma unroll
     for (int kb = 0; kb < AT_KEYS / 16; ++kb) {
-        const uint32_t b = b_raw + kb * 128, tw = b_twin + kb * 2 * (WinTile<DP>::ROWS8 / 16);
-        umma_tf32_ts(d, a_t + 16 * kb, tile_desc<8192, 512, 1>(b), idesc, (kb > 0 || accumulate) ? 1u : 0u);
-        umma_tf32_ts(d, a_t + 16 * kb + 8, tile_desc<8192, 512, 1>(b + 64), idesc, 1u);
-        umma_bf16_ts(d, a_sml + STEP * kb, tile_desc<WinTile<DP>::ROWS8, 128, 0>(tw), idesc_bf, 1u);
+        const uint32_t tw = b_twin + kb * 2 * (WinTile<DP>::ROWS8 / 16);
+        umma_bf16_ts(d, a_sml + STEP * kb, tile_desc<WinTile<DP>::ROWS8, 128, 0>(tw), idesc_bf, (kb > 0 || accumulate) ? 1u : 0u);
         umma_bf16_ts(d, a_big + STEP * kb, tile_desc<WinTile<DP>::ROWS8, 128, 0>(tw + small), idesc_bf, 1u);
+    }
+#pragma unroll
+    for (int kb = 0; kb < AT_KEYS / 16; ++kb) {
+        const uint32_t b = b_raw + kb * 128;
+        umma_tf32_ts(d, a_t + 16 * kb, tile_desc<8192, 512, 1>(b), idesc, 1u);
+        umma_tf32_ts(d, a_t + 16 * kb + 8, tile_desc<8192, 512, 1>(b + 64), idesc, 1u);
     }
 }
 // The 128 rows a CTA owns of an operand or of a result pass through shared memory, as TMA moves them: [32 columns][128 rows][128 bytes], 128-byte swizzle.
@@ -162,29 +172,35 @@ __device__ __forceinline__ void own_read(float (&x)[N], uint8_t* tile, int row, 
         x[e] = f.x; x[e + 1] = f.y; x[e + 2] = f.z; x[e + 3] = f.w;
     }
 }
-// Moves 16 columns of a sum from tensor memory to a CTA's place in `moved`, [which][column / 4][row][4]: moved = (there ? moved * f : 0) + sum.
-// The tensor core truncates when it adds, so that a sum over hundreds of instructions comes out too small by half a unit for each (8192 keys in one
-// sum: 6e-5 of the result); one of WT_FLUSH blocks, 128 instructions, is off by 3e-6, and these are added here with rounding.
-__device__ __forceinline__ void move_sum(uint32_t taddr, float* moved, bool there, float f) {
+// Moves 16 columns of a sum from tensor memory to a CTA's place in `moved`, [which][column / 4][row][4]: moved = (there ? moved : 0) + sum.
+// A sum over hundreds of instructions comes out too small (8192 keys in one sum: 6e-5 of the result); one of WT_FLUSH blocks, 64 instructions, by at most 8e-6 where all terms have
+// one sign, and these are added here with rounding.  Every eight blocks instead: 2.5 % off the backward pass; every two: 5 % more.
+__device__ __forceinline__ void move_sum(uint32_t taddr, float* moved, bool there) {
     uint32_t x[16];
     tmem_ld16(taddr, x);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         float* at = moved + e * 4 * AT_ROWS;
         const float4 o = there ? ld4(at) : make_float4(0.f, 0.f, 0.f, 0.f);
-        st4(at, make_float4(fmaf(o.x, f, __uint_as_float(x[4 * e])), fmaf(o.y, f, __uint_as_float(x[4 * e + 1])), fmaf(o.z, f, __uint_as_float(x[4 * e + 2])), fmaf(o.w, f, __uint_as_float(x[4 * e + 3]))));
+        st4(at, make_float4(o.x + __uint_as_float(x[4 * e]), o.y + __uint_as_float(x[4 * e + 1]), o.z + __uint_as_float(x[4 * e + 2]), o.w + __uint_as_float(x[4 * e + 3])));
     }
 }
-// 16 columns of a result on their way out: a sum in tensor memory times f, plus what has moved times f_moved.
-__device__ __forceinline__ void place_result(uint8_t* tile, int row, int col, uint32_t taddr, const float* moved, bool there, float f, float f_moved) {
+// 16 columns of a result on their way out: f times a sum in tensor memory and what has moved.
+__device__ __forceinline__ void place_result(uint8_t* tile, int row, int col, uint32_t taddr, const float* moved, bool there, float f) {
     uint32_t x[16];
     tmem_ld16(taddr, x);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         const float4 o = there ? ld4(moved + e * 4 * AT_ROWS) : make_float4(0.f, 0.f, 0.f, 0.f);
-        *own_at(tile, row, col + 4 * e) = make_float4(fmaf(o.x, f_moved, __uint_as_float(x[4 * e]) * f), fmaf(o.y, f_moved, __uint_as_float(x[4 * e + 1]) * f), fmaf(o.z, f_moved, __uint_as_float(x[4 * e + 2]) * f),
-                                                      fmaf(o.w, f_moved, __uint_as_float(x[4 * e + 3]) * f));
+        *own_at(tile, row, col + 4 * e) = make_float4((o.x + __uint_as_float(x[4 * e])) * f, (o.y + __uint_as_float(x[4 * e + 1])) * f, (o.z + __uint_as_float(x[4 * e + 2])) * f, (o.w + __uint_as_float(x[4 * e + 3])) * f);
     }
+}
+__device__ __forceinline__ void tmem_read(uint32_t taddr, float (&x)[32]) { tmem_ld32(taddr, x); }
+__device__ __forceinline__ void tmem_read(uint32_t taddr, float (&x)[16]) {
+    uint32_t u[16];
+    tmem_ld16(taddr, u);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x[e] = __uint_as_float(u[e]);
 }
 __device__ __forceinline__ float* moved_at(const WindowTc& p, int which, int col, int row) { return p.moved + ((int64_t)blockIdx.x * 2 + which) * 64 * AT_ROWS + (col * AT_ROWS + row * 4); }
 
@@ -193,7 +209,11 @@ __device__ __forceinline__ bool ready_wait(uint32_t bar, uint32_t parity, int* s
 __device__ __forceinline__ bool issuer_wait(uint32_t bar, uint32_t parity, int* status, int where) { return mbar_test(bar, parity) || mbar_wait(bar, parity, status, where); }
 
 // ---- forward ------------------------------------------------------------------------------------------------------------------
-// Tensor memory of query tile q, from column 256 q: scores / t of P [0, 64), bf16(P) [64, 96), bf16(P - t) [96, 128), O [128, 192), t of q [192, 256).
+// Tensor memory of query tile q, from column 256 q: scores / t of P [0, 64), bf16(P) [64, 96), bf16(P - t) [96, 128), a block's share of O [128, 192), t of q [192, 256).
+// O itself is added up by the threads, with rounding: dO . O has to agree with the dP of the backward pass, or gradients that are small differences of the two are wrong
+// (2048 positions, window 1024, values whose common part is ten times as large as the rest: bias gradient off by 1e-2 of its largest with sums of eight blocks in tensor memory, 2e-4
+// so, 3e-5 by the FMA kernels; dQ 1e-3, 2e-4, 8e-5).  A thread's sums lie in shared memory as far as there is room, 12 of 32 columns, and the others in L2, requested before the wait
+// for the block: 214 us at 16 x 16 x 1024, window 256 (all of them in L2: 225; 20 in registers, 12 in shared memory: 262; sums of eight blocks in tensor memory: 206).
 template <int DP, bool BIAS>
 __global__ void __launch_bounds__(AT_FWD_THREADS, 1) window_attention_tc_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_q,
                                                                                     const __grid_constant__ CUtensorMap map_o, const __grid_constant__ WindowTc p) {
@@ -229,7 +249,7 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 1) window_attention_tc_fwd_ker
     };
     auto slot = [&](int kind, uint32_t n) { return (int)(2 * kind + (n & 1u)); };  // kind 0: k, 1: v; n: running block number
 
-    if (warp < 4) regs_give<56>();
+    if (warp < 4) regs_give<40>();
     if (warp == 0) {
         if (lane == 0) {
             uint32_t n = 0;
@@ -260,7 +280,6 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 1) window_attention_tc_fwd_ker
                 if (it.skip) continue;
                 const Union u(TileKeys(p, tile_row(it, 0)), TileKeys(p, tile_row(it, 1)));
                 const int blocks = u.blocks;
-                int done[2] = {0, 0};  // blocks of each tile
                 auto scores = [&](int q, int j) {
                     const uint32_t raw = base16 + S::BLOCKS_OFF / 16 + slot(0, n + j) * (S::BLOCK / 16);
                     win_scores<DP>(tmem + 256 * q, tmem + 256 * q + 192, base16 + q * (S::TWIN / 16), raw, raw + S::RAW / 16);
@@ -294,7 +313,7 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 1) window_attention_tc_fwd_ker
                             if (ok) {
                                 after_sync();
                                 const uint32_t t0 = tmem + 256 * q;
-                                win_values<DP, 8>(t0 + 128, t0, t0 + 64, t0 + 96, v_raw, v_raw + S::RAW / 16, (done[q]++ % WT_FLUSH) != 0);
+                                win_values<DP, 8>(t0 + 128, t0, t0 + 64, t0 + 96, v_raw, v_raw + S::RAW / 16, false);
                                 if (now == t.last) umma_commit(o_full(q));
                             }
                         }
@@ -311,7 +330,7 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 1) window_attention_tc_fwd_ker
             }
         }
     } else if (warp >= 4 && warp < 8) {
-        regs_give<72>();
+        regs_give<56>();
         const int t = threadIdx.x - 128;
         uint32_t n = 0;
         bool ok = true;
@@ -335,13 +354,15 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 1) window_attention_tc_fwd_ker
             }
         }
     } else if (warp >= 8) {
-        regs_take<88>();
+        regs_take<96>();
         // two threads a query: each has 32 of a block's 64 keys, and half of the columns of q and O
         const int q = (warp - 8) >> 3, half = ((warp - 8) >> 2) & 1, row = 32 * (warp & 3) + lane, bar = 1 + q, at_tile = (threadIdx.x - 256) & 255;
         const uint32_t t0 = tmem + 256 * q + ((uint32_t)(32 * (warp & 3)) << 16);
         float* xch = reinterpret_cast<float*>(gen + S::STAGE_OFF) + q * 256;  // [half][row]
         float* tabs = reinterpret_cast<float*>(gen + S::STAGE_OFF + 2048) + q * 2 * WT_TAB;
-        constexpr int OC = DP / 2;
+        constexpr int OC = DP / 2, NEAR = 12;  // columns of a thread, and how many of their sums lie in shared memory
+        float4* near_by = reinterpret_cast<float4*>(gen + S::STAGE_OFF + 2048 + 4 * WT_TAB * 4) + (threadIdx.x - 256);
+        static_assert(2048 + 4 * WT_TAB * 4 + NEAR * 4 * 512 <= 8 * 4096, "shared memory");
         const float c = BIAS ? kLog2e : p.scale * kLog2e;  // scores, or scores before the scale, to log2 units
         uint32_t s_phase = 0, o_phase = 0, items = 0;
         bool ok = true;
@@ -387,18 +408,29 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 1) window_attention_tc_fwd_ker
                 pair_sync(bar);
             }
             float* moved = moved_at(p, q, half * OC, row);
-            float m = -INFINITY, sum = 0.0f, m_out = -INFINITY;  // m: the maximum the probabilities are relative to; m_out: the one what has moved to `out` is
+            float m = -INFINITY, sum = 0.0f, m_out = -INFINITY;  // m: the maximum the probabilities are relative to; m_out: the one the sums are
+            auto sums = [&](int e) { return e < NEAR / 4 ? near_by[512 * e] : __ldcg(reinterpret_cast<const float4*>(moved + e * 4 * AT_ROWS)); };
             for (int j = 0; j < blocks; ++j) {
                 const int b = keys.block(j);
                 float ahead = 0.0f;
                 if (BIAS && j + 1 < blocks) ahead = request(keys.block(j + 1));
+                float4 was[OC / 4];
+#pragma unroll
+                for (int e = NEAR / 4; e < OC / 4; ++e) was[e] = j > 1 ? sums(e) : make_float4(0.f, 0.f, 0.f, 0.f);
                 good = good && ready_wait(s_full(q), s_phase & 1u, p.status, 47);
                 ++s_phase;
                 after_sync();
-                if (j > 0 && j % WT_FLUSH == 0) {  // the products of the blocks before came before these scores
+                if (j > 0) {  // the products of the block before came before these scores
                     const float f = m_out == m ? 1.0f : ex2((m_out - m) * c);
+                    float x[OC];
+                    tmem_read(t0 + 128 + half * OC, x);
 #pragma unroll
-                    for (int g = 0; g < OC / 16; ++g) move_sum(t0 + 128 + half * OC + 16 * g, moved + 16 * g * AT_ROWS, j > WT_FLUSH, f);
+                    for (int e = 0; e < OC / 4; ++e) {
+                        if (e < NEAR / 4) was[e] = j > 1 ? sums(e) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        const float4 now = make_float4(fmaf(was[e].x, f, x[4 * e]), fmaf(was[e].y, f, x[4 * e + 1]), fmaf(was[e].z, f, x[4 * e + 2]), fmaf(was[e].w, f, x[4 * e + 3]));
+                        if (e < NEAR / 4) near_by[512 * e] = now;
+                        else __stcg(reinterpret_cast<float4*>(moved + e * 4 * AT_ROWS), now);
+                    }
                     m_out = m;
                 }
                 float v[32];
@@ -428,18 +460,9 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 1) window_attention_tc_fwd_ker
                     mx = fmaxf(mx, xch[(half ^ 1) * 128 + row]);
                     if (j == 0) {
                         m = mx;
-                    } else {  // O holds the previous blocks' sums: their products came before these scores
-                        const float f = mx > m ? ex2((m - mx) * c) : 1.0f;
+                    } else {
+                        sum *= mx > m ? ex2((m - mx) * c) : 1.0f;
                         m = fmaxf(m, mx);
-                        sum *= f;
-#pragma unroll
-                        for (int g = 0; g < OC / 16; ++g) {
-                            uint32_t x[16];
-                            tmem_ld16(t0 + 128 + half * OC + 16 * g, x);
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * f);
-                            tmem_st16(t0 + 128 + half * OC + 16 * g, x);
-                        }
                     }
                     pair_sync(bar);  // both have read before either writes again
                 }
@@ -465,9 +488,14 @@ __global__ void __launch_bounds__(AT_FWD_THREADS, 1) window_attention_tc_fwd_ker
             const float inv = empty_row ? 0.0f : 1.0f / (sum + xch[(half ^ 1) * 128 + row]);
             pair_sync(bar);
             if (!ok) break;
-            const float inv_moved = inv * (m_out == m ? 1.0f : ex2((m_out - m) * c));
+            const float inv_sums = inv * (m_out == m ? 1.0f : ex2((m_out - m) * c));
+            float x[OC];
+            tmem_read(t0 + 128 + half * OC, x);
 #pragma unroll
-            for (int g = 0; g < OC / 16; ++g) place_result(own, row, half * OC + 16 * g, t0 + 128 + half * OC + 16 * g, moved + 16 * g * AT_ROWS, blocks > WT_FLUSH, inv, inv_moved);
+            for (int e = 0; e < OC / 4; ++e) {
+                const float4 o = blocks > 1 ? sums(e) : make_float4(0.f, 0.f, 0.f, 0.f);
+                *own_at(own, row, half * OC + 4 * e) = make_float4(fmaf(o.x, inv_sums, x[4 * e] * inv), fmaf(o.y, inv_sums, x[4 * e + 1] * inv), fmaf(o.z, inv_sums, x[4 * e + 2] * inv), fmaf(o.w, inv_sums, x[4 * e + 3] * inv));
+            }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             pair_sync(bar);
             if (at_tile == 0) {
@@ -695,7 +723,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
             float* moved = moved_at(p, part >> 1, half * OC, row);
             auto move = [&](bool there) {
 #pragma unroll
-                for (int g = 0; g < OC / 16; ++g) move_sum(lanes + (part < 2 ? 320 : 256) + half * OC + 16 * g, moved + 16 * g * AT_ROWS, there, 1.0f);
+                for (int g = 0; g < OC / 16; ++g) move_sum(lanes + (part < 2 ? 320 : 256) + half * OC + 16 * g, moved + 16 * g * AT_ROWS, there);
             };
 #pragma unroll 1
             for (int i = 0; i < cnt; ++i, ++n) {
@@ -752,7 +780,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dkv_ker
             after_sync();
             const float f = part < 2 ? p.scale : 1.0f;
 #pragma unroll
-            for (int g = 0; g < OC / 16; ++g) place_result(own, row, half * OC + 16 * g, lanes + (part < 2 ? 320 : 256) + half * OC + 16 * g, moved + 16 * g * AT_ROWS, cnt > WT_FLUSH, f, f);
+            for (int g = 0; g < OC / 16; ++g) place_result(own, row, half * OC + 16 * g, lanes + (part < 2 ? 320 : 256) + half * OC + 16 * g, moved + 16 * g * AT_ROWS, cnt > WT_FLUSH, f);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             if (all_any(!good)) break;  // all of them leave together
             if (threadIdx.x == 384) {
@@ -1022,7 +1050,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
                 if (i > 0 && i % WT_FLUSH == 0) {
                     good = good && ready_wait(dq_done(n - 1u), two(n - 1u), p.status, 68);
                     after_sync();
-                    if (16 * part < DP) move_sum(lanes + 256 + 16 * part, moved, i > WT_FLUSH, 1.0f);
+                    if (16 * part < DP) move_sum(lanes + 256 + 16 * part, moved, i > WT_FLUSH);
                 }
                 tmem_stores_done();
                 __syncwarp();
@@ -1069,7 +1097,7 @@ __global__ void __launch_bounds__(AT_BWD_THREADS, 1) window_attention_tc_dq_kern
                 sums[(warp - 12) * 64 + lane] = sum0;
                 sums[(warp - 12) * 64 + 32 + lane] = sum1;
             }
-            if (16 * part < DP) place_result(gen, row, 16 * part, lanes + 256 + 16 * part, moved, cnt > WT_FLUSH, p.scale, p.scale);
+            if (16 * part < DP) place_result(gen, row, 16 * part, lanes + 256 + 16 * part, moved, cnt > WT_FLUSH, p.scale);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             if (all_any(!good)) break;  // all of them leave together
             if (wants_dbias && warp == 12) {  // before the next item's dO takes their place
@@ -1136,9 +1164,9 @@ static int run_bwd(gcb_ctx* ctx, const WindowTc& p, const BwdMaps& m) {
     if (!rc) rc = tc_launch(ctx, window_attention_tc_dkv_kernel<DP, BIAS>, done_kv, AT_BWD_THREADS, DkvSmem<DP, BIAS>::TOTAL, p, m.qk, m.qn, m.ok, m.on, m.kk, m.vk, m.dk, m.dv);
     return rc ? rc : after_launch(ctx, "window_attention_tc_dkv");
 }
-// Room for the sums that leave tensor memory before an item's end.
-static int make_moved(WindowTc& p, Scratch& mem) {
-    if (p.T <= WT_FLUSH * AT_KEYS) return GCB_OK;
+// Room for the sums that leave tensor memory before an item's end, where an item may have more than `blocks` blocks.
+static int make_moved(WindowTc& p, Scratch& mem, int blocks) {
+    if (p.T <= blocks * AT_KEYS) return GCB_OK;
     const int rc = mem.get((size_t)std::min<int64_t>(p.items, kSMs) * 2 * 64 * AT_ROWS * sizeof(float));
     p.moved = mem.as<float>();
     return rc;
@@ -1170,7 +1198,7 @@ int window_tc_fwd(gcb_ctx* ctx, int64_t B, const WindowAttn& a) {
     // 1 x 12 x 4099, window 512, 86 and 95; 2 x 12 x 1024 45 and 43; 1 x 4 x 512 26 and 23; 3 x 12 x 700 34 and 34)
     WindowTc p = operands(ctx, B, a, B * a.H * ((a.T + 255) / 256) < kSMs ? 1 : 2);
     Scratch moved(ctx);
-    int rc = make_moved(p, moved);
+    int rc = make_moved(p, moved, 1);
     if (rc) return rc;
     CUtensorMap k, v, q, o;
     GCB_REQUIRE(encode_rows(enc, &k, a.k, a.D, a.T, a.k_ld, a.k_si, a.k_so, a.H, B, 32, AT_KEYS, CU_TENSOR_MAP_SWIZZLE_128B) &&
@@ -1187,7 +1215,7 @@ int window_tc_bwd(gcb_ctx* ctx, int64_t B, const WindowAttn& a) {
     TmaEncodeFn enc = tma_encode(ctx);
     WindowTc p = operands(ctx, B, a, 1);
     Scratch moved(ctx);
-    const int rc = make_moved(p, moved);
+    const int rc = make_moved(p, moved, WT_FLUSH);
     if (rc) return rc;
     BwdMaps m;
     auto rows = [&](CUtensorMap& map, const float* x, int64_t ld, int64_t so, int64_t si, bool k_major) {
