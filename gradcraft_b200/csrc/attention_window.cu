@@ -327,7 +327,8 @@ __global__ void __launch_bounds__(256) window_attention_bwd_kernel(const __grid_
 // keys that are not seen: here four keys lie in registers, a column quadruple a lane, and a warp passes over the rows of q and dO, 32 / LPR at a time.
 // A CTA takes far_rows queries of a head and four of the keys, and leaves its sums in far_part, [head][chunk][S][dk, dv][Dp].
 // Bound by memory (q and dO once for every four keys) and, about as much, by the eight sums over a row's lanes.
-// 256 heads of 768 queries beyond a window, four keys: 228 us as tiles of 32 keys.
+// 256 heads of 768 queries beyond a window: 54 us with four keys, 228 as tiles of 32 keys.  Its time grows with the number of keys: a backward pass of 16 x 16 x 1024 x 64, window 256, takes
+// 490 us without first keys, 569 with four, 687 with sixteen and 1148 with 64; of 1 x 16 x 8192 x 64, window 1024, 559, 616, 685 and 948.
 constexpr int AW_KEYS = 4;
 template <int LPR>
 __device__ __forceinline__ void sum_eight(float (&v)[8], int lane) {  // every lane gets all eight sums over its LPR lanes: halves change hands until each lane has one
@@ -849,8 +850,8 @@ static int fma_bwd(gcb_ctx* ctx, int64_t heads, const WindowAttn& p) {
     return fma_launch(ctx, window_attention_bwd_kernel<R, NC, VEC>, done, 2 * heads * p.tiles, aw_floats(R, 2, 2, 2, (p.D + 3) / 4 * 4), "window_attention_bwd", p, (int)(heads * p.tiles));
 }
 // R, with 16 R rows of a CTA's own: 64 rows take 8 reads of shared memory for 32 double FMAs where 32 rows take 6 for 16; 32 rows where 64 would leave three fifths
-// of the SMs idle.  Either, us, forward and backward: 16 x 16 x 1024 x 128 with a window of 256 1745 and 6371 with 32, 1542 and 4406 with 64; 4 x 8 x 256 x 128
-// 51 and 134, 42 and 115; 4 x 4 x 256 x 128 45 and 84, 43 and 74; 1 x 4 x 256 x 128 31 and 55, 42 and 73; 64 x 12 x 32 x 64 25 and 66, 33 and 116.  Twice the
+// of the SMs idle.  Either, us, forward and backward: 16 x 16 x 1024 x 128 with a window of 256 1508 and 5898 with 32, 1339 and 4006 with 64; 4 x 8 x 256 x 128
+// 51 and 134, 42 and 114; 4 x 4 x 256 x 128 47 and 84, 42 and 73; 1 x 4 x 256 x 128 31 and 55, 41 and 73; 64 x 12 x 32 x 64 25 and 86, 33 and 116.  Twice the
 // threads for 64 rows, which leaves the reads as they are, was slower than twice the rows a thread (6028 and 5537 in the first of these, at an earlier step).
 static int fma_rows(int64_t heads, int64_t T) { return T > 32 && 5 * heads * ((T + 63) / 64) >= 2 * kSMs ? 4 : 2; }
 template <int R>

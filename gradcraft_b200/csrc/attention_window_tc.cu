@@ -12,9 +12,9 @@
 //     products and T^2 floats there, seven products here.
 // The gradients of the first S keys from queries beyond the window are left to the FMA kernel of attention_window.cu: 128-key tiles would
 // spend T / 64 blocks on a handful of keys.
-// 1 x 16 heads of 8192 x 64, window 1024, four first positions: forward 231 us, dQ 246, dK and dV 324 (with a bias of 32 buckets 260, 351, 375); 16 x 16 heads of
-// 1024, window 256: 198, 244, 255.  The tensor cores are at work for 34, 43 and 46 % of a call at 4096 positions, and 43, 53 and 49 % of the issue slots go to what
-// turns scores into probabilities and rows into companions; what is left is the way of a block from role to role, a barrier each time.
+// 1 x 16 heads of 8192 x 64, window 1024, four first positions: forward 252 us, dQ 261, dK and dV 346 (with a bias of 32 buckets 288, 342, 386); 16 x 16 heads of
+// 1024, window 256: 212, 252, 266; each after a flush of the L2 cache.  The tensor cores are at work for 31, 42 and 44 % of a call at 4096 positions, and 45, 52 and 48 % of the issue
+// slots go to what turns scores into probabilities and rows into companions; what is left is the way of a block from role to role, a barrier each time.
 // Every wait is bounded, as in the GEMM kernels.
 #include "attention_tc.cuh"
 #include "attention_window.cuh"
@@ -1137,8 +1137,8 @@ static WindowTc operands(gcb_ctx* ctx, int64_t B, const WindowAttn& a, int tiles
     plan(p, B, a.H, a.T, tiles_per_unit);
     // Heads are taken all together, the heaviest tiles of every one first, so that the lightest are left for the end; not where every tile goes back to the first keys
     // and k and v of all heads are more than the L2 cache holds, 126 MB: groups of heads then stay in it (kernels as they are here and in groups, us: 16 x 16 x 1024 x 64,
-    // window 256, forward 197 and 204, dQ 245 and 263, dK and dV 256 and 332; 8 x 12 x 512, no window, 37, 50, 64 and 38, 53, 77; 16 x 16 x 1024, no window, 240, 294,
-    // 350 and 232, 293, 350).
+    // window 256, forward 212 and 220, dQ 252 and 274, dK and dV 266 and 350; 8 x 12 x 512, no window, 45, 56, 68 and 45, 60, 83; 16 x 16 x 1024, no window, 254, 305,
+    // 373 and 248, 303, 372).
     if (a.rule.W > 0 || 2 * sizeof(float) * p.heads * (int64_t)a.T * a.D <= (int64_t(126) << 20)) p.group = p.heads;
     return p;
 }
@@ -1173,14 +1173,15 @@ static int make_moved(WindowTc& p, Scratch& mem, int blocks) {
 }
 
 // Short sequences that the FMA kernels do sooner: up to 32 positions, up to 64 where every SM has a tile of 32 at most, up to 128 where a quarter of them has
-// (forward and backward, us, there and here: 64 x 12 x 32 x 64 25 and 66, 42 and 95; 4 x 4 x 64 x 32, window 16 and 2 sinks, 5.5 and 8.8, 7.3 and 23.1; 1 x 4 x 64 x 64
-// 6.2 and 9.7, 7.9 and 18.3; 16 x 4 x 64 x 64 8.8 and 13.5, 8.6 and 21.2; 32 x 4 x 64 x 64 11.7 and 23.8, 9.1 and 22.3; 64 x 12 x 64 x 64 35 and 125, 43 and 109;
-// 1 x 4 x 128 x 64 10.4 and 17.5, 10.7 and 22.4; 4 x 4 x 128 x 64 10.7 and 24.9, 10.8 and 24.2).
+// (forward and backward, us, there and here: 64 x 12 x 32 x 64 25 and 86, 41 and 94; 4 x 4 x 64 x 32, window 16 and 2 sinks, 5.2 and 8.0, 7.1 and 22.7; 1 x 4 x 64 x 64
+// 5.9 and 9.5, 7.7 and 18.4; 16 x 4 x 64 x 64 9.9 and 13.3, 8.2 and 20.8; 32 x 4 x 64 x 64 11.7 and 23.3, 8.8 and 21.8; 64 x 12 x 64 x 64 34 and 125, 41 and 106;
+// 1 x 4 x 128 x 64 10.3 and 16.8, 10.7 and 22.5; 4 x 4 x 128 x 64 12.5 and 17.1, 10.9 and 23.8; 4 x 12 x 128 x 64 18.4 and 31.1, 10.9 and 24.0).
 static bool short_enough(int64_t heads, int T) {
     const int64_t tiles = heads * ((T + 31) / 32);
     return T <= 32 || (T <= 64 && tiles <= kSMs) || (T <= 128 && 4 * tiles <= kSMs);
 }
-// Heads of up to 64 columns (tensor memory holds two query tiles of that width), the split arithmetic of mode 2, rows that TMA can address.
+// Heads of up to 64 columns (tensor memory holds two query tiles of that width), the split arithmetic of mode 2, rows that TMA can address: strides that grow, so that one k and v for
+// all heads or sequences (a stride of 0), or rows backwards, go to the FMA kernels.
 bool window_tc_takes(gcb_ctx* ctx, int64_t B, const WindowAttn& a) {
     if (ctx->gemm_engine == 1 || ctx->gemm_split_mode != 2 || a.D > 64 || a.D % 4 != 0 || !(a.scale > 0.0f) || a.scale > 1e30f) return false;
     if (ctx->gemm_engine == 0 && short_enough(B * a.H, a.T)) return false;
@@ -1194,8 +1195,8 @@ bool window_tc_takes(gcb_ctx* ctx, int64_t B, const WindowAttn& a) {
 
 int window_tc_fwd(gcb_ctx* ctx, int64_t B, const WindowAttn& a) {
     TmaEncodeFn enc = tma_encode(ctx);
-    // two query tiles share their key blocks; one tile a CTA where pairs would leave SMs idle (in pairs and one by one, us: 16 x 16 x 1024, window 256, 197 and 262;
-    // 1 x 12 x 4099, window 512, 86 and 95; 2 x 12 x 1024 45 and 43; 1 x 4 x 512 26 and 23; 3 x 12 x 700 34 and 34)
+    // two query tiles share their key blocks; one tile a CTA where pairs would leave SMs idle (in pairs and one by one, us: 16 x 16 x 1024, window 256, 205 and 273;
+    // 1 x 12 x 4099, window 512, 89 and 99; 2 x 12 x 1024 48 and 46; 1 x 4 x 512 27 and 25; 3 x 12 x 700 36 and 36)
     WindowTc p = operands(ctx, B, a, B * a.H * ((a.T + 255) / 256) < kSMs ? 1 : 2);
     Scratch moved(ctx);
     int rc = make_moved(p, moved, 1);

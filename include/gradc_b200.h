@@ -265,7 +265,7 @@ GCB_API int gcb_attention_bwd_f32(gcb_ctx* ctx, int64_t batch, int64_t heads, in
  * to.  Deterministic: every sum is taken in a fixed order.  The calls take workspace from the arena while they run;
  * captured ones go on using it, so that graphs of one context are replayed one after another, on its stream or behind it, and cached memory is not released
  * while they live.  A value that is not finite in a row of k or v reaches, besides the queries that see it, others whose tile holds that row;
- * one in a row of q or dout its own rows of out and dq, and dk and dv of all keys whose tile meets that row.
+ * one in a row of q or dout its own rows of out and dq, dbias, and dk and dv of all keys whose tile meets that row.
  * The reference has the causal form (frontend/tensor_other.hpp:53-93). */
 GCB_API int gcb_window_attention_fwd_f32(gcb_ctx* ctx, int64_t batch, int64_t heads, int64_t seq_len, int64_t head_dim, float* out, int64_t o_ld, int64_t o_so, int64_t o_si, float* stats,
                                  const float* q, int64_t q_ld, int64_t q_so, int64_t q_si, const float* k, int64_t k_ld, int64_t k_so, int64_t k_si,

@@ -44,7 +44,8 @@ GCT_API int gct_set_lr(gct_trainer* tr, float lr);
 GCT_API int gct_zero_grad(gct_trainer* tr);
 /* One micro-batch: tokens/targets are [B, T] int64.  on_device != 0: pointers are device memory already (no copy);
  * otherwise they are host memory (pinned for an asynchronous copy) and are uploaded inside the call.
- * The loss is divided by `accum` before backward.  loss_out may be NULL (no device-to-host read, no sync). */
+ * The loss is divided by `accum` before backward.  loss_out may be NULL (no device-to-host read, no sync).
+ * Always in training mode: a loss without dropout comes from a trainer without it that was given the same weights. */
 GCT_API int gct_forward_backward(gct_trainer* tr, const int64_t* tokens, const int64_t* targets, int on_device, int64_t B, int64_t T, int64_t accum, float* loss_out);
 /* clip (if enabled) + AdamW.  norm_out may be NULL. */
 GCT_API int gct_optimizer_step(gct_trainer* tr, float* norm_out);
